@@ -1,0 +1,260 @@
+"""linear = act(x w^T + bias) + residual and its gradients against the formula in 64 bits on the same bf16 values.
+
+Tolerances, element by element.  u = 2^-8: a rounding to bf16, relative.  A sum of K products on the tensor core, K/16 steps of 16 with fp32 rounding
+or cutting (2^-22 of the running magnitude, two steps more for bias and residual): acc(K) = (K/16 + 2) 2^-22 of the sum of the products' magnitudes.
+Activations are formed with errors of a few 2^-21 of max(|value|, |argument|) (hardware exponential and reciprocal): 2^-18 is allowed.
+  y:  |act'| <= L times the error of z, the activation's own, u |y| for its rounding (fp32 y: 2^-22 |y|)
+  dz: |dy| times the error of act': L2 >= |act''| times that of z (bf16 z: u |z| more), from y (relu2): 2 sqrt(y (1 + u)), i.e. u/2 relative;
+      u |dz| for its rounding to bf16
+  dx, dw: the sums of the bounds on dz times the other operand's magnitudes, acc of the sum, u of the result;  dbias: dz's without its rounding
+"""
+import pytest
+import torch as th
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -8
+L1 = {None: 1, 'relu': 1, 'tanh': 1, 'sigmoid': 0.25, 'silu': 1.1, 'gelu': 1.13}
+L2 = {None: 0, 'relu': 0, 'tanh': 0.77, 'sigmoid': 0.1, 'silu': 0.5, 'gelu': 1.13}
+F64 = {None: lambda z: z, 'relu': th.relu, 'relu2': lambda z: th.relu(z).square(), 'tanh': th.tanh, 'sigmoid': th.sigmoid,
+       'silu': th.nn.functional.silu, 'gelu': lambda z: th.nn.functional.gelu(z, approximate='tanh')}
+
+
+def acc(K):
+    return (K / 16 + 2) * 2.0 ** -22
+
+
+def inputs(M, N, K, bias, residual, out, seed):
+    g = th.Generator(device='cuda').manual_seed(seed)
+
+    def rn(*s):
+        return th.randn(*s, generator=g, device='cuda')
+
+    x, w = rn(M, K).bfloat16(), (rn(N, K) / K ** 0.5).bfloat16()
+    return x, w, rn(N).to(bias) if bias else None, rn(M, N).to(out) if residual else None, rn(M, N).to(out)
+
+
+def check(name, got, want, bound):
+    assert got.shape == want.shape, name
+    e = (got.double() - want).abs() - bound
+    assert bool((e <= 0).all()), f'{name}: {int((e > 0).sum())} of {e.numel()} beyond the bound, the worst by {float(e.max()):.2e}'
+
+
+def compare(x, w, b, r, dy, act, out=th.bfloat16, call=None):
+    """One call with its backward against the formula."""
+    from wind_rwkv.rwkv7 import linear
+    K = w.shape[1]
+    leaves = [None if t is None else t.detach().requires_grad_() for t in (x, w, b, r)]
+    y = (call or linear)(leaves[0], leaves[1], leaves[2], act=act, residual=leaves[3], out_dtype=out)
+    assert y.dtype == out
+    grads = iter(th.autograd.grad(y, [t for t in leaves if t is not None], dy))
+    X, W = x.detach().double().reshape(-1, K), w.detach().double()
+    N = W.shape[0]
+    Z = X @ W.T + (0 if b is None else b.detach().double())
+    mag = X.abs() @ W.abs().T + (0 if b is None else b.detach().double().abs())
+    Zr = Z.clone().requires_grad_()
+    A = F64[act](Zr)
+    R = 0 if r is None else r.detach().double().reshape(-1, N)
+    Y = A.detach() + R
+    D, = th.autograd.grad(A.sum(), Zr)
+    ez = acc(K) * mag
+    l1 = 2 * (Z.abs() + ez) if act == 'relu2' else L1[act]
+    own = 0 if act is None else 2.0 ** -18 * (A.detach().abs() + (0 if act in ('relu', 'relu2') else Z.abs()))
+    e = l1 * ez + own
+    round_y = U if out == th.bfloat16 else 2.0 ** -22
+    check('y', y.reshape(-1, N), Y, e + round_y * (Y.abs() + e) + (0 if r is None else 2.0 ** -22 * R.abs()))
+    DY = dy.double().reshape(-1, N)
+    DZ = DY * D
+    if act == 'relu2':
+        ed = 2 * ez + D * U + 2 * (Z.abs() <= ez) * ez
+    elif act == 'relu':
+        ed = (Z.abs() <= ez).double()
+    else:
+        ed = L2[act] * (ez + U * Z.abs()) + (0 if act is None else 2.0 ** -18 * (1 + Z.abs()))
+    edz = DY.abs() * ed
+    edzr = edz + U * (DZ.abs() + edz)
+    M = X.shape[0]
+    dx = next(grads)
+    check('dx', dx.reshape(-1, K), DZ @ W, (edzr @ W.abs()) * (1 + U) + acc(N) * (DZ.abs() @ W.abs()) + U * (DZ @ W).abs())
+    check('dw', next(grads), DZ.T @ X, (edzr.T @ X.abs()) * (1 + U) + acc(M) * (DZ.abs().T @ X.abs()) + U * (DZ.T @ X).abs())
+    if b is not None:
+        s = DZ.sum(0)
+        round_b = U if b.dtype == th.bfloat16 else 0
+        check('dbias', next(grads), s, edz.sum(0) * (1 + U) + (M + 8) * 2.0 ** -24 * DZ.abs().sum(0) + round_b * s.abs())
+    if r is not None:
+        assert th.equal(next(grads), dy)
+    return y
+
+
+SHAPES = [  # rows, columns, k
+    (1, 1, 8), (1, 8192, 2048), (3, 77, 200), (16, 129, 1024), (17, 2048, 8192), (33, 1000, 64), (64, 257, 4104),   # few rows
+    (65, 64, 64), (100, 130, 72), (333, 77, 200), (513, 200, 768), (700, 1000, 136),                                # tiles
+    (1300, 4096, 72), (1283, 4001, 200), (2500, 2053, 1032), (5000, 96, 2048), (20000, 40, 24)]                     # pairs, and mixtures in the backward
+
+
+@pytest.mark.parametrize('M,N,K', SHAPES)
+def test_shapes(M, N, K):
+    compare(*inputs(M, N, K, None, False, th.bfloat16, M + N + K), 'relu2')
+    compare(*inputs(M, N, K, th.float32, True, th.bfloat16, M + N + K + 1), None)
+
+
+@pytest.mark.parametrize('act', list(F64))
+@pytest.mark.parametrize('M,N,K', [(5, 100, 128), (200, 264, 128), (1400, 3333, 128)])
+@pytest.mark.parametrize('residual', [False, True])
+def test_activations(act, M, N, K, residual):
+    compare(*inputs(M, N, K, th.bfloat16, residual, th.bfloat16, 7), act)
+
+
+@pytest.mark.parametrize('act', [None, 'relu2', 'tanh'])
+@pytest.mark.parametrize('M,N,K', [(7, 50001, 64), (300, 203, 256), (1400, 3333, 64), (1536, 4096, 64)])
+def test_fp32_output(act, M, N, K):
+    compare(*inputs(M, N, K, th.float32, True, th.float32, 9), act, out=th.float32)
+
+
+def test_large_arguments():
+    """Activations far out on both sides: exponentials that overflow and vanish."""
+    x, w, _, _, dy = inputs(70, 96, 64, None, False, th.bfloat16, 3)
+    for act in F64:
+        compare(x * 64, w, None, None, dy, act)
+
+
+def test_layouts():
+    """Rows that lie in wider tensors, batch dimensions, orders and alignments that are copied."""
+    x, w, b, r, dy = inputs(60, 72, 64, th.float32, True, th.bfloat16, 5)
+    wide = th.zeros(60, 160, dtype=th.bfloat16, device='cuda')
+    wide[:, 8:72] = x
+    off = th.zeros(60, 160, dtype=th.bfloat16, device='cuda')
+    off[:, 1:65] = x
+    ww = th.zeros(72, 96, dtype=th.bfloat16, device='cuda')
+    ww[:, :64] = w
+    rr = th.zeros(60, 75, dtype=th.bfloat16, device='cuda')
+    rr[:, 3:] = r
+    first = compare(x, w, b, r, dy, 'silu')
+    for xs in (wide[:, 8:72], off[:, 1:65], x.t().contiguous().t()):
+        for ws in (ww[:, :64], w.t().contiguous().t()):
+            assert th.equal(compare(xs, ws, b, rr[:, 3:], dy, 'silu'), first)
+    assert th.equal(compare(x, w, b, r.t().contiguous().t(), dy.t().contiguous().t(), 'silu'), first)
+    y3 = compare(x.view(3, 20, 64), w, b, r.view(3, 20, 72), dy.view(3, 20, 72), 'silu')
+    assert y3.shape == (3, 20, 72) and th.equal(y3.view(60, 72), first)
+    x4 = x.view(3, 20, 64).transpose(0, 1)
+    y4 = compare(x4, w, b, r.view(3, 20, 72).transpose(0, 1), dy.view(3, 20, 72).transpose(0, 1), 'silu')
+    assert th.equal(y4.transpose(0, 1).reshape(60, 72), first)
+    one = compare(x[0], w, b, r[0], dy[0], 'silu')
+    assert one.shape == (72,)
+    bb = th.zeros(144, device='cuda')
+    bb[::2] = b
+    assert th.equal(compare(x, w, bb[::2], r, dy, 'silu'), first)
+
+
+def test_empty():
+    from wind_rwkv.rwkv7 import linear
+    x = th.zeros(0, 64, dtype=th.bfloat16, device='cuda', requires_grad=True)
+    w = th.ones(9, 64, dtype=th.bfloat16, device='cuda', requires_grad=True)
+    b = th.ones(9, device='cuda', requires_grad=True)
+    y = linear(x, w, b, act='gelu')
+    assert y.shape == (0, 9)
+    dx, dw, db = th.autograd.grad(y, (x, w, b), th.zeros_like(y))
+    assert dx.shape == (0, 64) and not dw.any() and not db.any()
+
+
+def test_only_what_is_wanted():
+    from wind_rwkv.rwkv7 import linear
+    x, w, b, r, dy = inputs(40, 24, 64, th.float32, True, th.bfloat16, 5)
+    full = [t.clone().requires_grad_() for t in (x, w, b, r)]
+    want = th.autograd.grad(linear(full[0], full[1], full[2], act='tanh', residual=full[3]), full, dy)
+    for i in range(4):
+        ins = [t.clone() for t in (x, w, b, r)]
+        ins[i].requires_grad_()
+        got, = th.autograd.grad(linear(ins[0], ins[1], ins[2], act='tanh', residual=ins[3]), ins[i], dy)
+        assert th.equal(got, want[i])
+    ins = [t.clone() for t in (x, w, r)]
+    ins[2].requires_grad_()
+    got, = th.autograd.grad(linear(ins[0], ins[1], act='tanh', residual=ins[2]), ins[2], dy)
+    assert th.equal(got, dy)
+
+
+def test_gradient_against_differences():
+    """The derivative along one direction of all inputs: a central difference of the 64-bit formula against the gradients.  Each gradient is off by
+    at most the bounds above, of which the largest part, a few u relative to the sum of the terms' magnitudes, is allowed here."""
+    x, w, b, r, dy = inputs(48, 40, 64, th.float32, True, th.bfloat16, 11)
+    from wind_rwkv.rwkv7 import linear
+    for act in F64:
+        leaves = [t.clone().requires_grad_() for t in (x, w, b, r)]
+        grads = th.autograd.grad(linear(leaves[0], leaves[1], leaves[2], act=act, residual=leaves[3]), leaves, dy)
+        g = th.Generator(device='cuda').manual_seed(1)
+        dirs = [th.randn(t.shape, generator=g, device='cuda', dtype=th.float64) for t in leaves]
+
+        def f(h):
+            X, W, B, R = [t.detach().double() + h * d for t, d in zip(leaves, dirs)]
+            return ((F64[act](X @ W.T + B) + R) * dy.double()).sum()
+
+        num = (f(1e-5) - f(-1e-5)) / 2e-5
+        got = sum((a.double() * d).sum() for a, d in zip(grads, dirs))
+        scale = sum((a.double() * d).abs().sum() for a, d in zip(grads, dirs))
+        assert abs(float(got - num)) <= 4 * U * float(scale)
+
+
+def test_same_results_every_time_and_in_a_graph():
+    from wind_rwkv.rwkv7 import linear
+    for M, N, K in ((1, 2048, 2048), (300, 96, 2048), (1400, 3328, 512)):
+        x, w, b, r, dy = inputs(M, N, K, th.float32, True, th.bfloat16, 5)
+        first = linear(x, w, b, act='gelu', residual=r)
+        for _ in range(3):
+            assert th.equal(linear(x, w, b, act='gelu', residual=r), first)
+        graph = th.cuda.CUDAGraph()
+        with th.cuda.graph(graph):
+            again = linear(x, w, b, act='gelu', residual=r)
+        again.zero_()
+        graph.replay()
+        assert th.equal(again, first)
+        x.copy_(x.flip(0))
+        graph.replay()
+        assert th.equal(again, linear(x, w, b, act='gelu', residual=r))
+
+
+def test_streams_and_calls_that_follow_one_another():
+    """Two streams at once, and a call that reads what the one ahead of it writes."""
+    from wind_rwkv.rwkv7 import linear
+    x, w, b, r, _ = inputs(400, 512, 512, th.float32, True, th.bfloat16, 5)
+    want = x
+    for _ in range(6):
+        want = linear(want, w, b, act='tanh', residual=r)
+        th.cuda.synchronize()
+    side = th.cuda.Stream()
+    side.wait_stream(th.cuda.current_stream())
+    a = c = x
+    for _ in range(6):
+        a = linear(a, w, b, act='tanh', residual=r)
+        with th.cuda.stream(side):
+            c = linear(c, w, b, act='tanh', residual=r)
+    th.cuda.synchronize()
+    assert th.equal(a, want) and th.equal(c, want)
+
+
+def test_python_form_agrees():
+    """The form that torch.compile traces, called directly."""
+    from wind_rwkv.rwkv7.rwkv7_linear import ACTS, Linear
+    for act, residual, out in (('relu2', False, th.bfloat16), ('relu2', True, th.bfloat16), ('gelu', True, th.float32), (None, True, th.bfloat16)):
+        x, w, b, r, dy = inputs(90, 51, 72, th.bfloat16, residual, out, 5)
+        compare(x, w, b, r, dy, act, out, call=lambda x, w, b, act, residual, out_dtype: Linear.apply(x, w, b, residual, ACTS[act], out_dtype == th.float32))
+
+
+def test_compiles():
+    from wind_rwkv.rwkv7 import linear
+    x, w, b, r, dy = inputs(90, 56, 72, th.float32, True, th.bfloat16, 5)
+
+    def f(x, w, b, r):
+        return linear(linear(x, w, b, act='relu2'), w.t(), act=None).float().sum() + linear(x, w, b, act='gelu', residual=r).float().sum()
+
+    grads = []
+    for g in (f, th.compile(f, fullgraph=True)):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b, r)]
+        g(*leaves).backward()
+        grads.append([t.grad for t in leaves])
+    for a, c in zip(*grads):
+        assert th.allclose(a.float(), c.float(), rtol=2 * U, atol=2 * U * float(a.float().abs().max()))
+
+
+def test_device_status_is_clean():
+    from wind_rwkv.rwkv7 import _lib
+    assert _lib.device_status() == 0

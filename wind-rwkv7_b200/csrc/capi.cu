@@ -6,6 +6,7 @@
 #include "wkv7_kernels.h"
 #include "ddlerp.h"
 #include "expand_loras.h"
+#include "linear.h"
 
 #include <mutex>
 
@@ -426,6 +427,85 @@ int wkv7_proj_gemm(const void* A, const void* W, void* C, int64_t M, int64_t N, 
 }
 
 static_assert(WKV7_PROJ_LD_MAX == wkv7::PROJ_MAX && WKV7_PROJ_MAX <= wkv7::PROJ_MAX, "mirrored constants");
+
+static_assert(WKV7_ACT_NONE == wkv7::kActNone && WKV7_ACT_RELU == wkv7::kActRelu && WKV7_ACT_RELU2 == wkv7::kActRelu2 && WKV7_ACT_TANH == wkv7::kActTanh &&
+              WKV7_ACT_SIGMOID == wkv7::kActSigmoid && WKV7_ACT_SILU == wkv7::kActSilu && WKV7_ACT_GELU == wkv7::kActGelu, "mirrored constants");
+
+static int linear_check(const void* x, const void* w, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int act, int flags, int known_flags) {
+    if (M < 0 || N <= 0 || K <= 0 || ldx < K || ldw < K || act < 0 || act >= wkv7::kActs || (flags & ~known_flags)) return WKV7_ERR_SHAPE;
+    if (K % 8 != 0 || ldx % 8 != 0 || ldw % 8 != 0) return WKV7_ERR_ALIGN;  // 16-byte rows for the bulk tensor copies
+    // coordinates of the copies are 32 bits wide (tiles overhang by up to 255), strides of the maps 40
+    constexpr int64_t most = 0x7fffffffLL - 256;
+    if (M > most || N > most || K > most || ldx > most || ldw > most) return WKV7_ERR_TOO_LARGE;
+    if (M == 0) return WKV7_OK;
+    if (!x || !w) return WKV7_ERR_NULL;
+    return aligned16(x) && aligned16(w) ? WKV7_OK : WKV7_ERR_ALIGN;
+}
+
+int wkv7_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, int64_t M, int64_t N, int64_t K,
+                    int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int64_t ldz, int act, int flags, void* stream) {
+    int rc = linear_check(x, w, M, N, K, ldx, ldw, act, flags, WKV7_LINEAR_F32_OUT | WKV7_LINEAR_F32_BIAS);
+    if (rc) return rc;
+    const int64_t n8 = (N + 7) / 8 * 8;
+    if (ldy < N || (residual && ldr < N) || (z && ldz < n8)) return WKV7_ERR_SHAPE;
+    if (z && (ldz % 8 != 0 || !aligned16(z))) return WKV7_ERR_ALIGN;
+    if (M == 0) return WKV7_OK;
+    if (!y) return WKV7_ERR_NULL;
+    const uintptr_t ysize = flags & WKV7_LINEAR_F32_OUT ? 4 : 2, bsize = flags & WKV7_LINEAR_F32_BIAS ? 4 : 2;
+    if ((uintptr_t)y % ysize || (uintptr_t)residual % ysize || (uintptr_t)bias % bsize) return WKV7_ERR_ALIGN;
+    int* status = status_ptr();
+    if (!status) return WKV7_ERR_LAUNCH;
+    const wkv7::LinearEpilogue e{bias, residual, y, z, ldr, ldy, ldz, M, N, act, bsize == 4, ysize == 4};
+    return wkv7::launch_linear({x, ldx, false}, {w, ldw, false}, K, e, status, (cudaStream_t)stream);
+}
+
+static int64_t linear_dz_bytes(int64_t M, int64_t N) { return (M * ((N + 7) / 8 * 8) * 2 + 15) / 16 * 16; }
+
+int64_t wkv7_linear_bwd_workspace_bytes(int64_t M, int64_t N) {
+    if (M <= 0 || N <= 0) return 0;
+    return linear_dz_bytes(M, N) + (int64_t)wkv7::linear_dz_chunks(M, N) * N * 4;
+}
+
+int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void* dy, void* dx, void* dw, float* dbias, int64_t M, int64_t N, int64_t K,
+                    int64_t ldx, int64_t ldw, int64_t lds, int64_t lddy, int act, int flags, void* workspace, void* stream) {
+    int rc = linear_check(x, w, M, N, K, ldx, ldw, act, flags, WKV7_LINEAR_F32_OUT | WKV7_LINEAR_FROM_Y);
+    if (rc) return rc;
+    const bool from_y = flags & WKV7_LINEAR_FROM_Y, f32 = flags & WKV7_LINEAR_F32_OUT;
+    if (from_y && ((act != WKV7_ACT_RELU && act != WKV7_ACT_RELU2) || f32)) return WKV7_ERR_SHAPE;
+    if (lddy < N || (act && lds < N)) return WKV7_ERR_SHAPE;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (M == 0) {  // sums over nothing
+        if ((dw && cudaMemsetAsync(dw, 0, (size_t)N * K * 2, s) != cudaSuccess) || (dbias && cudaMemsetAsync(dbias, 0, (size_t)N * 4, s) != cudaSuccess)) return WKV7_ERR_LAUNCH;
+        return WKV7_OK;
+    }
+    if (!dy || !workspace || (act && !saved)) return WKV7_ERR_NULL;
+    if (!aligned16(workspace) || (dx && !aligned16(dx)) || (dw && !aligned16(dw)) || (uintptr_t)dbias % 4 || (uintptr_t)dy % (f32 ? 4 : 2) || (act && (uintptr_t)saved % 2))
+        return WKV7_ERR_ALIGN;
+    int* status = status_ptr();
+    if (!status) return WKV7_ERR_LAUNCH;
+    // without an activation a bf16 dy whose rows the bulk copies can read is dz
+    const bool as_is = !act && !f32 && aligned16(dy) && lddy % 8 == 0;
+    wkv7::LinearOperand dz{dy, lddy, false};
+    if (!as_is || dbias) {
+        if (!as_is) dz = wkv7::LinearOperand{workspace, (N + 7) / 8 * 8, false};
+        if (dbias || ((dx || dw) && !as_is)) {
+            const wkv7::LinearDz d{dy, saved, as_is || !(dx || dw) ? nullptr : workspace, dbias, (float*)((char*)workspace + linear_dz_bytes(M, N)), M, N, lddy, lds,
+                                   (N + 7) / 8 * 8, act, f32, from_y};
+            rc = wkv7::launch_linear_dz(d, s);
+            if (rc) return rc;
+        }
+    }
+    if (dx) {
+        const wkv7::LinearEpilogue e{nullptr, nullptr, dx, nullptr, 0, K, 0, M, K, 0, false, false};
+        rc = wkv7::launch_linear(dz, {w, ldw, true}, N, e, status, s);
+        if (rc) return rc;
+    }
+    if (dw) {
+        const wkv7::LinearEpilogue e{nullptr, nullptr, dw, nullptr, 0, K, 0, N, K, 0, false, false};
+        rc = wkv7::launch_linear({dz.p, dz.ld, true}, {x, ldx, true}, M, e, status, s);
+    }
+    return rc;
+}
 
 static int ddlerp_check(int64_t B, int64_t T, int64_t C, int64_t D) {
     if (B < 0 || T < 0 || C <= 0 || D <= 0) return WKV7_ERR_SHAPE;

@@ -1,0 +1,722 @@
+// Dense products with their epilogue:  y = act(x w^T + bias) + residual, and the products of its backward.
+//     x [M, K], w [N, K] (an nn.Linear weight), bf16;  fp32 accumulation in tensor memory;  y bf16 or fp32
+//     dz = dy act'(z),  dx = dz w,  dw = dz^T x,  dbias = sum of dz over the rows
+// All three are one form, out[i, j] = sum_k P[i, k] Q[j, k]: an operand whose k is contiguous in memory is read K-major, one whose index is (w in
+// dx; dz and x in dw) as it lies, MN-major, so that nothing is transposed in memory.
+//
+// linear_pair_kernel, for large products: persistent pairs of CTAs, a tile of 256 x BN per pair (each CTA holds 128 rows of P and half of the
+// tile's Q rows; one thread of the pair issues tcgen05.mma.cta_group::2), two accumulators, so that eight warps empty one while the
+// other is filled.
+// linear_tile_kernel, for the rest: one tile of 128 x NT a CTA, the sum over k split over a cluster of up to eight CTAs, which add their
+// parts through distributed shared memory in a fixed order.  Few rows (decoding): the weight is P and the rows of x are Q, so that a CTA
+// streams 128 weight rows against all of x.
+#include <cuda.h>
+#include <cstring>
+
+#include "linear.h"
+#include "mma_bf16.cuh"
+#include "wkv7_kernels.h"
+
+namespace wkv7 {
+namespace lin {
+
+constexpr int BM = 128, BK = 64;
+constexpr int MAXSTAGES = 12;
+
+// ---- activations -----------------------------------------------------------------------------------------
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float sigmoid_f(float x) { return rcp_mufu(1.f + ex2_approx(-LOG2E * x)); }
+__device__ __forceinline__ float tanh_f(float x) {
+    // (1 - e) / (1 + e), e = exp(-2 |x|): relative error 2e-6 from |x| = 0.1 on; the series' first four terms below (next one: 2e-10)
+    const float t = fabsf(x), e = ex2_approx(-2.f * LOG2E * t), x2 = x * x;
+    const float big = copysignf((1.f - e) * rcp_mufu(1.f + e), x);
+    const float small = x * (1.f + x2 * (-1.f / 3.f + x2 * (2.f / 15.f - x2 * (17.f / 315.f))));
+    return t < 0.1f ? small : big;
+}
+constexpr float GELU_C = 1.5957691216057308f;  // 2 sqrt(2 / pi): gelu(x) = x sigmoid(GELU_C (x + 0.044715 x^3))
+__device__ __forceinline__ float gelu_s(float x) { return sigmoid_f(GELU_C * x * (1.f + 0.044715f * x * x)); }
+__device__ __forceinline__ float relu_f(float x) { return x < 0.f ? 0.f : x; }  // (a NaN stays one)
+
+__device__ __forceinline__ void act8(int act, float (&f)[8]) {
+    switch (act) {
+        case kActRelu:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = relu_f(f[i]);
+            break;
+        case kActRelu2:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { f[i] = relu_f(f[i]); f[i] *= f[i]; }
+            break;
+        case kActTanh:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = tanh_f(f[i]);
+            break;
+        case kActSigmoid:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = sigmoid_f(f[i]);
+            break;
+        case kActSilu:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] *= sigmoid_f(f[i]);
+            break;
+        case kActGelu:
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] *= gelu_s(f[i]);
+            break;
+        default: break;
+    }
+}
+// act'(z); from_y: of relu and relu2 from their values, 2 sqrt(y) for 2 relu(z)
+__device__ __forceinline__ float act_grad(int act, bool from_y, float z) {
+    switch (act) {
+        case kActRelu: return z > 0.f ? 1.f : 0.f;
+        case kActRelu2: return from_y ? 2.f * sqrtf(z) : 2.f * relu_f(z);
+        case kActTanh: { const float t = tanh_f(z); return 1.f - t * t; }
+        case kActSigmoid: { const float s = sigmoid_f(z); return s * (1.f - s); }
+        case kActSilu: { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }
+        case kActGelu: {
+            const float s = gelu_s(z);
+            return s + z * s * (1.f - s) * GELU_C * (1.f + 3.f * 0.044715f * z * z);
+        }
+        default: return 1.f;
+    }
+}
+
+// ---- epilogue --------------------------------------------------------------------------------------------
+struct Epi : LinearEpilogue {
+    bool vec;  // rows of y and of the residual start on 16-byte boundaries
+};
+__device__ __forceinline__ void load8g(const void* base, bool f32, long long at, float (&f)[8]) {
+    if (f32) {
+        const float4 a = *reinterpret_cast<const float4*>((const float*)base + at), b = *reinterpret_cast<const float4*>((const float*)base + at + 4);
+        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    } else {
+        unpack8(*reinterpret_cast<const uint4*>((const bf16*)base + at), f);
+    }
+}
+__device__ __forceinline__ float load1g(const void* base, bool f32, long long at) {
+    return f32 ? ((const float*)base)[at] : __bfloat162float(((const bf16*)base)[at]);
+}
+// eight adjacent columns of a row, from the accumulator to memory; bias already added
+__device__ __forceinline__ void finish8(const Epi& e, long long row, long long col, float (&f)[8]) {
+    const int live = (int)(e.cols - col < 8 ? e.cols - col : 8);
+    if (e.z) *reinterpret_cast<uint4*>((bf16*)e.z + row * e.ldz + col) = pack8(f);  // (ldz is a multiple of 8: room for all eight)
+    act8(e.act, f);
+    if (e.vec && live == 8) {
+        if (e.residual) {
+            float r[8];
+            load8g(e.residual, e.y_f32, row * e.ldr + col, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] += r[i];
+        }
+        if (e.y_f32) {
+            float* y = (float*)e.y + row * e.ldy + col;
+            *reinterpret_cast<float4*>(y) = make_float4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<float4*>(y + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+            *reinterpret_cast<uint4*>((bf16*)e.y + row * e.ldy + col) = pack8(f);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < live) {
+            float v = f[i];
+            if (e.residual) v += load1g(e.residual, e.y_f32, row * e.ldr + col + i);
+            if (e.y_f32) ((float*)e.y)[row * e.ldy + col + i] = v;
+            else ((bf16*)e.y)[row * e.ldy + col + i] = __float2bfloat16_rn(v);
+        }
+}
+
+// ---- tensor core and copy helpers --------------------------------------------------------------------------
+// shared-memory descriptors of 128-byte-swizzled operands.  K-major: 128-byte rows of 64 k, groups of 8 rows 1024 bytes apart.  MN-major: [k][64
+// indices] boxes, 8 k rows = 1024 bytes, the next 64 indices in the next box of 64 k (8192 bytes).
+__device__ __forceinline__ uint64_t desc_of(uint32_t saddr, bool mn) {
+    const uint64_t lbo = mn ? (8192 >> 4) : 1;
+    return (uint64_t)((saddr >> 4) & 0x3fff) | (lbo << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// fp32 accumulate, bf16 operands
+__host__ __device__ constexpr uint32_t idesc_of(int m, int n, bool p_mn, bool q_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((p_mn ? 1u : 0u) << 15) | ((q_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t ta, uint32_t (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(v[0]),"=r"(v[1]),"=r"(v[2]),"=r"(v[3]),"=r"(v[4]),"=r"(v[5]),"=r"(v[6]),"=r"(v[7]),"=r"(v[8]),"=r"(v[9]),"=r"(v[10]),"=r"(v[11]),"=r"(v[12]),"=r"(v[13]),"=r"(v[14]),"=r"(v[15]),
+                   "=r"(v[16]),"=r"(v[17]),"=r"(v[18]),"=r"(v[19]),"=r"(v[20]),"=r"(v[21]),"=r"(v[22]),"=r"(v[23]),"=r"(v[24]),"=r"(v[25]),"=r"(v[26]),"=r"(v[27]),"=r"(v[28]),"=r"(v[29]),"=r"(v[30]),"=r"(v[31])
+                 : "r"(ta));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t ta, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]),"=r"(v[1]),"=r"(v[2]),"=r"(v[3]),"=r"(v[4]),"=r"(v[5]),"=r"(v[6]),"=r"(v[7]),"=r"(v[8]),"=r"(v[9]),"=r"(v[10]),"=r"(v[11]),"=r"(v[12]),"=r"(v[13]),"=r"(v[14]),"=r"(v[15])
+                 : "r"(ta));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
+// ---- tiles of 128 x NT, k split over a cluster ---------------------------------------------------------------
+struct TileParams {
+    CUtensorMap P, Q;
+    Epi e;
+    int p_mn, q_mn, nt, kblocks, splits, stages, swap, p_tiles;  // swap: P runs over the columns of y, Q over its rows
+    uint32_t tmem_cols;
+};
+struct TileCtrl {
+    uint64_t full[MAXSTAGES], empty[MAXSTAGES], accum, drain;
+    uint32_t tmem_base;
+    volatile int abort, zero;
+};
+static_assert(sizeof(TileCtrl) <= 1024, "the KB ahead of the ring");
+constexpr int TILE_THREADS = 192;  // warps 0-3: accumulator rows, warp 4: copies, warp 5: products; all six: the result
+__host__ __device__ constexpr int p_bytes() { return BM * 128; }
+__host__ __device__ constexpr int q_bytes(int nt) { return nt * 128; }  // a multiple of 1024 from 8 rows on
+__host__ __device__ constexpr int tile_pitch(int nt, int swap) { return swap ? nt + 1 : nt + 4; }
+
+__global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_constant__ TileParams p, int* status) {
+    extern __shared__ unsigned char smem_dyn[];
+    TileCtrl* ctrl = reinterpret_cast<TileCtrl*>(smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u));
+    unsigned char* sm = reinterpret_cast<unsigned char*>(ctrl) + 1024;
+    const int stage_bytes = p_bytes() + q_bytes(p.nt);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const int rank = blockIdx.x % p.splits;
+    const long long tile = blockIdx.x / p.splits;
+    const int p0 = (int)(tile % p.p_tiles) * BM, q0 = (int)(tile / p.p_tiles) * p.nt;
+    const int lo = (int)((long long)p.kblocks * rank / p.splits), hi = (int)((long long)p.kblocks * (rank + 1) / p.splits);
+
+    if (tid == 0) {
+        for (int s = 0; s < p.stages; ++s) { mbar_init(&ctrl->full[s], 1); mbar_init(&ctrl->empty[s], 1); }
+        mbar_init(&ctrl->accum, 1); mbar_init(&ctrl->drain, 1);
+        ctrl->abort = 0; ctrl->zero = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctrl->tmem_base)), "r"(p.tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = ctrl->tmem_base;
+    stream_order();
+
+    if (warp == 4) {
+        if (elect_one()) {
+            int s = 0, round = 0, issued = 0;
+            for (int kb = lo; kb < hi; ++kb) {
+                if (round > 0 && !mbar_wait_bounded<true>(&ctrl->empty[s], (round - 1) & 1, &ctrl->abort, status)) break;
+                const uint32_t bar = smem_u32(&ctrl->full[s]), dst = smem_u32(sm + s * stage_bytes);
+                expect_tx(&ctrl->full[s], (uint32_t)stage_bytes);
+                auto load = [&](const CUtensorMap* m, uint32_t to, int x, int y) {
+                    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                                 ::"r"(to), "l"(m), "r"(bar), "r"(x), "r"(y) : "memory");
+                };
+                if (p.p_mn) { load(&p.P, dst, p0, kb * BK); load(&p.P, dst + 8192, p0 + 64, kb * BK); }
+                else load(&p.P, dst, kb * BK, p0);
+                if (p.q_mn) for (int b = 0; b < p.nt; b += 64) load(&p.Q, dst + p_bytes() + b * 128, q0 + b, kb * BK);
+                else load(&p.Q, dst + p_bytes(), kb * BK, q0);
+                ++issued;
+                if (++s == p.stages) { s = 0; ++round; }
+            }
+            for (int i = 0; i < p.stages; ++i) mbar_landed(&ctrl->full[i], (issued + p.stages - 1 - i) / p.stages, &ctrl->zero, status);
+        }
+        __syncwarp();
+    } else if (warp == 5) {
+        if (elect_one()) {
+            const uint32_t idesc = idesc_of(BM, p.nt, p.p_mn, p.q_mn);
+            const uint64_t step_p = p.p_mn ? 2048 >> 4 : 2, step_q = p.q_mn ? 2048 >> 4 : 2;  // 16 k
+            int s = 0, round = 0;
+            for (int kb = lo; kb < hi; ++kb) {
+                mbar_wait_bounded<false>(&ctrl->full[s], round & 1, &ctrl->abort, status);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t da = desc_of(smem_u32(sm + s * stage_bytes), p.p_mn), db = desc_of(smem_u32(sm + s * stage_bytes + p_bytes()), p.q_mn);
+#pragma unroll
+                for (int ks = 0; ks < BK / 16; ++ks)
+                    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                                 ::"r"(tmem), "l"(da + ks * step_p), "l"(db + ks * step_q), "r"(idesc), "r"((kb > lo || ks > 0) ? 1u : 0u) : "memory");
+                asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&ctrl->empty[s])) : "memory");
+                if (++s == p.stages) { s = 0; ++round; }
+            }
+            asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&ctrl->accum)) : "memory");
+            if (ctrl->abort) {  // the later waits fell through: wait for what was issued before tensor memory is released
+                asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&ctrl->drain)) : "memory");
+                mbar_wait_bounded<false>(&ctrl->drain, 0, &ctrl->zero, status);
+            }
+        }
+        __syncwarp();
+    }
+    __syncwarp();
+    // the accumulator to shared memory, in the place of the operands (all products have read theirs, and nothing is in flight)
+    const int pitch = tile_pitch(p.nt, p.swap);
+    float* part = reinterpret_cast<float*>(sm);
+    if (warp < 4) {
+        mbar_wait_bounded<true>(&ctrl->accum, 0, &ctrl->abort, status);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    }
+    __syncthreads();  // (the copying thread has seen its last copies land)
+    if (warp < 4) {
+        float* row = part + (32 * warp + lane) * pitch;
+#pragma unroll 1
+        for (int c = 0; c < p.nt; c += 16) {
+            uint32_t v[16];
+            tmem_ld16(tmem + ((uint32_t)(32 * warp) << 16) + c, v);
+            if (p.swap) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) row[c + i] = __uint_as_float(v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<float4*>(row + c + i) = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+            }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    if (p.splits > 1) cluster_sync();
+    else __syncthreads();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+
+    // this CTA's share of the tile: the parts are added in the order of their ranks
+    const uint32_t mine = smem_u32(part);
+    const bool ok = !ctrl->abort;
+    const Epi& e = p.e;
+    if (p.swap) {  // lanes along P, i.e. along a row of y
+        const int units = BM * p.nt, from = (int)((long long)units * rank / p.splits), to = (int)((long long)units * (rank + 1) / p.splits);
+        for (int u = from + tid; u < to && ok; u += TILE_THREADS) {
+            const int i = u & (BM - 1), j = u / BM;
+            const long long row = q0 + j, col = p0 + i;
+            if (row >= e.rows || col >= e.cols) continue;
+            float v = 0.f;
+            for (int r = 0; r < p.splits; ++r) {
+                float x;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(map_rank(mine + (i * pitch + j) * 4, r)) : "memory");
+                v += x;
+            }
+            if (e.bias) v += load1g(e.bias, e.bias_f32, col);
+            if (e.z) ((bf16*)e.z)[row * e.ldz + col] = __float2bfloat16_rn(v);
+            float f[8] = {v};
+            act8(e.act, f);
+            v = f[0];
+            if (e.residual) v += load1g(e.residual, e.y_f32, row * e.ldr + col);
+            if (e.y_f32) ((float*)e.y)[row * e.ldy + col] = v;
+            else ((bf16*)e.y)[row * e.ldy + col] = __float2bfloat16_rn(v);
+        }
+    } else {
+        const int per_row = p.nt / 8, units = BM * per_row, from = (int)((long long)units * rank / p.splits), to = (int)((long long)units * (rank + 1) / p.splits);
+        for (int u = from + tid; u < to && ok; u += TILE_THREADS) {
+            const int i = u / per_row, j = 8 * (u % per_row);
+            const long long row = p0 + i, col = q0 + j;
+            if (row >= e.rows || col >= e.cols) continue;
+            float f[8] = {};
+            for (int r = 0; r < p.splits; ++r) {
+                float x[8];
+                const uint32_t a = map_rank(mine + (i * pitch + j) * 4, r);
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(a) : "memory");
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]) : "r"(a + 16) : "memory");
+#pragma unroll
+                for (int q = 0; q < 8; ++q) f[q] += x[q];
+            }
+            if (e.bias) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (col + q < e.cols) f[q] += load1g(e.bias, e.bias_f32, col + q);
+            }
+            finish8(e, row, col, f);
+        }
+    }
+    if (p.splits > 1) cluster_sync();  // nobody leaves while its part is read
+}
+
+// ---- pairs of CTAs, persistent ------------------------------------------------------------------------------------
+struct PairParams {
+    CUtensorMap P, Q;
+    Epi e;
+    int p_mn, q_mn, bn, kblocks, p_tiles, q_tiles;
+    long long tiles;
+};
+constexpr int PAIR_STAGES = 6, PAIR_THREADS = 384;  // warp 0: copies, 1: products, 4-11: epilogue
+constexpr int PAIR_P = BM * 128, PAIR_Q = 128 * 128, PAIR_STAGE = PAIR_P + PAIR_Q;
+constexpr int PAIR_STAGING = 32 * 32 * 4;  // a block of 32 x 32 per epilogue warp
+constexpr int BAND = 8;                    // tile rows of 256 that are walked together, column by column, so that concurrent tiles share operands in L2
+struct PairCtrl {
+    uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], accum_full[2], accum_empty[2], drain;
+    uint32_t tmem_base;
+    volatile int abort, zero;
+};
+constexpr int PAIR_SMEM = 1024 + PAIR_STAGES * PAIR_STAGE + 8 * PAIR_STAGING + (int)sizeof(PairCtrl);
+static_assert(PAIR_SMEM <= 232448, "shared memory of a CTA");
+
+__device__ __forceinline__ void pair_tile(const PairParams& p, long long t, int& pi, int& qi) {
+    const long long per_band = (long long)BAND * p.q_tiles;
+    const int band = (int)(t / per_band), rows = min(BAND, p.p_tiles - band * BAND);
+    const int r = (int)(t - band * per_band);
+    pi = band * BAND + r % rows;
+    qi = r / rows;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) linear_pair_kernel(const __grid_constant__ PairParams p, int* status) {
+    extern __shared__ unsigned char smem_dyn[];
+    unsigned char* sm = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
+    unsigned char* staging = sm + PAIR_STAGES * PAIR_STAGE;
+    PairCtrl* ctrl = reinterpret_cast<PairCtrl*>(staging + 8 * PAIR_STAGING);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    const uint32_t rank = cluster_rank();
+    const long long first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+    if (tid == 0) {
+        for (int s = 0; s < PAIR_STAGES; ++s) { mbar_init(&ctrl->full[s], 1); mbar_init(&ctrl->empty[s], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&ctrl->accum_full[i], 1); mbar_init(&ctrl->accum_empty[i], 16); }
+        mbar_init(&ctrl->drain, 1);
+        ctrl->abort = 0; ctrl->zero = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctrl->tmem_base)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();  // the other CTA's barriers are set up
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = ctrl->tmem_base;
+    stream_wait();
+
+    if (warp == 0) {
+        if (elect_one()) {
+            const int half = p.bn / 2;
+            const uint32_t q_tx = p.q_mn ? (uint32_t)((half + 63) / 64) * 8192u : (uint32_t)half * 128u;
+            int s = 0, round = 0;
+            long long issued = 0;
+            bool going = true;
+            for (long long t = first; t < p.tiles && going; t += step) {
+                int pi, qi;
+                pair_tile(p, t, pi, qi);
+                const int p0 = pi * 2 * BM + (int)rank * BM, q0 = qi * p.bn + (int)rank * half;
+                for (int kb = 0; kb < p.kblocks; ++kb) {
+                    if (round > 0 && !mbar_wait_bounded<true>(&ctrl->empty[s], (round - 1) & 1, &ctrl->abort, status)) { going = false; break; }
+                    // both CTAs' copies count at the first CTA's barrier, whose thread issues the products
+                    if (rank == 0) expect_tx(&ctrl->full[s], 2 * (PAIR_P + q_tx));
+                    const uint32_t bar = map_rank(smem_u32(&ctrl->full[s]), 0), dst = smem_u32(sm + s * PAIR_STAGE);
+                    auto load = [&](const CUtensorMap* m, uint32_t to, int x, int y) {
+                        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
+                                     ::"r"(to), "l"(m), "r"(bar), "r"(x), "r"(y) : "memory");
+                    };
+                    if (p.p_mn) { load(&p.P, dst, p0, kb * BK); load(&p.P, dst + 8192, p0 + 64, kb * BK); }
+                    else load(&p.P, dst, kb * BK, p0);
+                    if (p.q_mn) for (int b = 0; b < half; b += 64) load(&p.Q, dst + PAIR_P + b * 128, q0 + b, kb * BK);
+                    else load(&p.Q, dst + PAIR_P, kb * BK, q0);
+                    ++issued;
+                    if (++s == PAIR_STAGES) { s = 0; ++round; }
+                }
+            }
+            stream_release();
+            // this CTA's copies have landed when the products that read them are done, of which both CTAs hear
+            for (int i = 0; i < PAIR_STAGES; ++i) {
+                const long long n = (issued + PAIR_STAGES - 1 - i) / PAIR_STAGES;
+                if (n > 0) mbar_wait_bounded<true>(&ctrl->empty[i], (uint32_t)(n - 1) & 1, &ctrl->zero, status);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1 && rank == 0) {
+        if (elect_one()) {
+            const uint32_t idesc = idesc_of(2 * BM, p.bn, p.p_mn, p.q_mn);
+            const uint64_t step_p = p.p_mn ? 2048 >> 4 : 2, step_q = p.q_mn ? 2048 >> 4 : 2;
+            auto commit = [](uint64_t* bar) {
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+            };
+            int s = 0, round = 0, n = 0;
+            for (long long t = first; t < p.tiles; t += step, ++n) {
+                const int buf = n & 1;
+                if (n >= 2) mbar_wait_bounded<false>(&ctrl->accum_empty[buf], ((n >> 1) - 1) & 1, &ctrl->abort, status);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t acc = tmem + buf * 256;
+                for (int kb = 0; kb < p.kblocks; ++kb) {
+                    mbar_wait_bounded<false>(&ctrl->full[s], round & 1, &ctrl->abort, status);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t da = desc_of(smem_u32(sm + s * PAIR_STAGE), p.p_mn), db = desc_of(smem_u32(sm + s * PAIR_STAGE + PAIR_P), p.q_mn);
+#pragma unroll
+                    for (int ks = 0; ks < BK / 16; ++ks)
+                        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                                     ::"r"(acc), "l"(da + ks * step_p), "l"(db + ks * step_q), "r"(idesc), "r"((kb > 0 || ks > 0) ? 1u : 0u) : "memory");
+                    commit(&ctrl->empty[s]);
+                    if (++s == PAIR_STAGES) { s = 0; ++round; }
+                }
+                commit(&ctrl->accum_full[buf]);
+            }
+            if (ctrl->abort) {
+                commit(&ctrl->drain);
+                mbar_wait_bounded<false>(&ctrl->drain, 0, &ctrl->zero, status);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // warps 4-7 take the first half of the tile's columns, 8-11 the second; a warp reads the 32 accumulator rows that it may, 32 columns at a time, and
+        // turns the block in shared memory (16-byte units, unit u of row r at u ^ (r % 8): no conflicts either way), so that four lanes have
+        // 32 adjacent columns of a row: 64 bytes of bf16, two whole sectors a row and instruction
+        const int quarter = warp & 3, side = (warp - 4) >> 2;
+        unsigned char* mine = staging + (warp - 4) * PAIR_STAGING;
+        const Epi& e = p.e;
+        int n = 0;
+        for (long long t = first; t < p.tiles; t += step, ++n) {
+            int pi, qi;
+            pair_tile(p, t, pi, qi);
+            const int buf = n & 1;
+            mbar_wait_bounded<true>(&ctrl->accum_full[buf], (n >> 1) & 1, &ctrl->abort, status);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const bool ok = !ctrl->abort;
+            const long long row0 = (long long)pi * 2 * BM + rank * BM + 32 * quarter;
+            const int blocks = p.bn / 32, b0 = side ? (blocks + 1) / 2 : 0, b1 = side ? blocks : (blocks + 1) / 2;
+#pragma unroll 1
+            for (int b = b0; b < b1; ++b) {
+                uint32_t v[32];
+                tmem_ld32(tmem + buf * 256 + ((uint32_t)(32 * quarter) << 16) + 32 * b, v);
+                if (b == b1 - 1) {  // the accumulator may be filled again
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_rank(smem_u32(&ctrl->accum_empty[buf]), 0)) : "memory");
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    *reinterpret_cast<uint4*>(mine + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+                __syncwarp();
+                const int g = lane & 3;
+                const long long col = (long long)qi * p.bn + 32 * b + 8 * g;
+                float bias[8] = {};
+                if (e.bias && col < e.cols) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (col + i < e.cols) bias[i] = load1g(e.bias, e.bias_f32, col + i);
+                }
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const int r = 8 * it + (lane >> 2);
+                    const float4 x = *reinterpret_cast<const float4*>(mine + r * 128 + (((2 * g) ^ (r & 7)) << 4));
+                    const float4 y = *reinterpret_cast<const float4*>(mine + r * 128 + (((2 * g + 1) ^ (r & 7)) << 4));
+                    float f[8] = {x.x + bias[0], x.y + bias[1], x.z + bias[2], x.w + bias[3], y.x + bias[4], y.y + bias[5], y.z + bias[6], y.w + bias[7]};
+                    if (ok && row0 + r < e.rows && col < e.cols) finish8(e, row0 + r, col, f);
+                }
+                __syncwarp();
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();  // all that arrives at the other CTA's barriers has arrived, and neither reads the accumulators any more
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// ---- dz and the bias' gradient ---------------------------------------------------------------------------------
+// A CTA has 256 columns (8 adjacent ones a thread) of a chunk of rows, 8 rows at a time.  Bound by DRAM.
+constexpr int DZ_COLS = 256, DZ_THREADS = 256;
+struct DzParams : LinearDz {
+    long long rows_per;
+    bool vec;  // rows of dy and saved start on 16-byte boundaries
+};
+__global__ void __launch_bounds__(DZ_THREADS) linear_dz_kernel(const __grid_constant__ DzParams p) {
+    stream_order();
+    __shared__ float sums[8][DZ_COLS + 4];
+    const int g = threadIdx.x & 31, r = threadIdx.x >> 5;
+    const long long col = (long long)blockIdx.x * DZ_COLS + 8 * g;
+    const long long lo = blockIdx.y * p.rows_per, hi = lo + p.rows_per < p.M ? lo + p.rows_per : p.M;
+    float acc[8] = {};
+    if (col < p.N) {
+        const bool whole = p.vec && col + 8 <= p.N;
+#pragma unroll 2
+        for (long long m = lo + r; m < hi; m += 8) {
+            float d[8], z[8] = {};
+            if (whole) {
+                load8g(p.dy, p.dy_f32, m * p.lddy + col, d);
+                if (p.act) load8g(p.saved, false, m * p.lds + col, z);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const bool in = col + i < p.N;
+                    d[i] = in ? load1g(p.dy, p.dy_f32, m * p.lddy + col + i) : 0.f;
+                    z[i] = in && p.act ? load1g(p.saved, false, m * p.lds + col + i) : 0.f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (p.act) d[i] *= act_grad(p.act, p.from_y, z[i]);
+                acc[i] += d[i];
+            }
+            if (p.dz) *reinterpret_cast<uint4*>((bf16*)p.dz + m * p.ldz + col) = pack8(d);  // (ldz is a multiple of 8)
+        }
+    }
+    if (!p.dbias) return;
+    *reinterpret_cast<float4*>(&sums[r][8 * g]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    *reinterpret_cast<float4*>(&sums[r][8 * g + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    __syncthreads();
+    const long long c = (long long)blockIdx.x * DZ_COLS + threadIdx.x;
+    if (c < p.N) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += sums[i][threadIdx.x];
+        p.partial[blockIdx.y * p.N + c] = s;
+    }
+}
+__global__ void __launch_bounds__(256) linear_dbias_kernel(const float* partial, float* dbias, long long N, int chunks) {
+    stream_order();
+    __shared__ float sums[8][33];
+    const int x = threadIdx.x & 31, r = threadIdx.x >> 5;
+    const long long c = (long long)blockIdx.x * 32 + x;
+    float s = 0.f;
+    if (c < N)
+        for (int i = r; i < chunks; i += 8) s += partial[i * N + c];
+    sums[r][x] = s;
+    __syncthreads();
+    if (r == 0 && c < N) {
+        for (int i = 1; i < 8; ++i) s += sums[i][x];
+        dbias[c] = s;
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(f);
+    }();
+    return fn;
+}
+// box_rows: indices of a K-major box; an MN-major one is 64 indices x 64 k
+static bool encode(CUtensorMap* m, const LinearOperand& o, long long n, long long k, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)(o.mn ? n : k), (cuuint64_t)(o.mn ? k : n)};
+    const cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)(o.mn ? BK : box_rows)};
+    const cuuint32_t es[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(o.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+static bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename P> static bool launch_cluster(void (*kern)(P, int*), unsigned grid, unsigned threads, int smem, int cluster, cudaStream_t stream, const P& p, int* status) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(grid); c.blockDim = dim3(threads); c.dynamicSmemBytes = smem; c.stream = stream;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = attr; c.numAttrs = 1;
+    if (cluster > 1) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+        c.numAttrs = 2;
+    }
+    if (cudaLaunchKernelEx(&c, kern, p, status) == cudaSuccess) return true;
+    cudaGetLastError();
+    return false;
+}
+
+static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb, long long k, const Epi& e, bool swap, int nt, int splits, int* status, cudaStream_t stream) {
+    TileParams p;
+    memset(&p, 0, sizeof(p));
+    if (!encode(&p.P, a, na, k, BM) || !encode(&p.Q, b, nb, k, nt)) return kLaunchFailed;
+    p.e = e;
+    p.p_mn = a.mn; p.q_mn = b.mn; p.nt = nt; p.swap = swap;
+    p.kblocks = (int)((k + BK - 1) / BK);
+    p.splits = splits;
+    p.p_tiles = (int)((na + BM - 1) / BM);
+    p.tmem_cols = 32;
+    while ((int)p.tmem_cols < nt) p.tmem_cols *= 2;
+    const long long tiles = p.p_tiles * ((nb + nt - 1) / nt), grid = tiles * splits;
+    if (grid > 0x7fffffffLL) return kTooLarge;
+    const int stage = p_bytes() + q_bytes(nt), part = BM * tile_pitch(nt, swap) * 4;
+    // a CTA of a full grid shares its SM with another one
+    const int room = (grid > sm_count() ? 113 : 226) * 1024 - 2048, most = (p.kblocks + splits - 1) / splits;
+    p.stages = room / stage;
+    if (p.stages > MAXSTAGES) p.stages = MAXSTAGES;
+    if (p.stages > most) p.stages = most;
+    const int ring = p.stages * stage > part ? p.stages * stage : part;
+    const int smem = 2048 + ring;
+    if (cudaFuncSetAttribute(linear_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return kLaunchFailed;
+    return launch_cluster(linear_tile_kernel, (unsigned)grid, TILE_THREADS, smem, splits, stream, p, status) ? kOk : kLaunchFailed;
+}
+
+static int run_pair(LinearOperand a, LinearOperand b, long long na, long long nb, long long k, const Epi& e, int bn, int* status, cudaStream_t stream) {
+    PairParams p;
+    memset(&p, 0, sizeof(p));
+    if (!encode(&p.P, a, na, k, BM) || !encode(&p.Q, b, nb, k, bn / 2)) return kLaunchFailed;
+    p.e = e;
+    p.p_mn = a.mn; p.q_mn = b.mn; p.bn = bn;
+    p.kblocks = (int)((k + BK - 1) / BK);
+    p.p_tiles = (int)((na + 2 * BM - 1) / (2 * BM));
+    p.q_tiles = (int)((nb + bn - 1) / bn);
+    p.tiles = (long long)p.p_tiles * p.q_tiles;
+    const long long pairs = sm_count() / 2;
+    const unsigned grid = 2 * (unsigned)(p.tiles < pairs ? p.tiles : pairs);
+    if (cudaFuncSetAttribute(linear_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return kLaunchFailed;
+    return launch_cluster(linear_pair_kernel, grid, PAIR_THREADS, PAIR_SMEM, 1, stream, p, status) ? kOk : kLaunchFailed;
+}
+
+}  // namespace lin
+
+int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const LinearEpilogue& ep, int* status, cudaStream_t stream) {
+    using namespace lin;
+    Epi e;
+    static_cast<LinearEpilogue&>(e) = ep;
+    const int per16 = ep.y_f32 ? 4 : 8;
+    e.vec = al16(ep.y) && ep.ldy % per16 == 0 && (!ep.residual || (al16(ep.residual) && ep.ldr % per16 == 0));
+    const int kblocks = (int)((k + BK - 1) / BK), sms = sm_count();
+    auto split = [&](long long tiles) {  // CTAs of one tile: as many as fill the SMs
+        int s = 1;
+        while (s < 8 && 2 * s <= kblocks && tiles * s * 2 <= sms) s *= 2;
+        return s;
+    };
+    if (ep.rows <= 64 && !rows.mn) {
+        const int nt = ep.rows <= 16 ? 16 : ep.rows <= 32 ? 32 : 64;
+        return run_tile(cols, rows, ep.cols, ep.rows, k, e, true, nt, split((ep.cols + BM - 1) / BM), status, stream);
+    }
+    const long long pair_tiles = ((ep.rows + 255) / 256) * ((ep.cols + 255) / 256);
+    if (2 * pair_tiles >= sms) return run_pair(rows, cols, ep.rows, ep.cols, k, e, 256, status, stream);
+    const long long tiles = ((ep.rows + BM - 1) / BM) * ((ep.cols + 127) / 128);
+    return run_tile(rows, cols, ep.rows, ep.cols, k, e, false, 128, split(tiles), status, stream);
+}
+
+int linear_dz_chunks(long long M, long long N) {
+    // CTAs of at least 64 rows, some four an SM
+    const long long cols = (N + lin::DZ_COLS - 1) / lin::DZ_COLS;
+    long long c = (4 * 148 + cols - 1) / cols;
+    const long long most = (M + 63) / 64;
+    if (c > most) c = most;
+    return (int)(c < 1 ? 1 : c);
+}
+
+int launch_linear_dz(const LinearDz& d, cudaStream_t stream) {
+    using namespace lin;
+    DzParams p;
+    static_cast<LinearDz&>(p) = d;
+    const int chunks = linear_dz_chunks(d.M, d.N);
+    p.rows_per = (d.M + chunks - 1) / chunks;
+    p.vec = al16(d.dy) && d.lddy % (d.dy_f32 ? 4 : 8) == 0 && (!d.act || (al16(d.saved) && d.lds % 8 == 0));
+    const int cols = (int)((d.N + DZ_COLS - 1) / DZ_COLS);
+    if (!launch(linear_dz_kernel, dim3(cols, chunks), DZ_THREADS, 0, stream, p)) return kLaunchFailed;
+    if (d.dbias && !launch(linear_dbias_kernel, dim3((unsigned)((d.N + 31) / 32)), 256, 0, stream, (const float*)d.partial, d.dbias, d.N, chunks)) return kLaunchFailed;
+    return kOk;
+}
+
+}  // namespace wkv7

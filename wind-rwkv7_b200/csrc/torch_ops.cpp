@@ -456,6 +456,122 @@ py::object expand_loras(const variable_list& in) {
 }
 
 
+// ---- linear -----------------------------------------------------------------------------------------------
+// t [..., n] as rows of n adjacent elements, one pitch apart
+bool pitched_rows(const Tensor& t, int64_t* ld) {
+    const int64_t n = t.size(-1);
+    if (!plain(t) || t.numel() == 0 || (n > 1 && t.stride(-1) != 1)) return false;
+    int64_t pitch = 0, rows = 1;
+    for (int64_t i = t.dim() - 2; i >= 0; --i) {
+        if (t.size(i) == 1) continue;
+        if (!pitch) pitch = t.stride(i);
+        if (t.stride(i) != pitch * rows || pitch < n) return false;
+        rows *= t.size(i);
+    }
+    *ld = pitch ? pitch : n;
+    return true;
+}
+// an operand of the products: rows on 16-byte boundaries
+bool operand_rows(const Tensor& t, int64_t* ld) {
+    return pitched_rows(t, ld) && t.scalar_type() == at::kBFloat16 && *ld % 8 == 0 && !(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15);
+}
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// y, z (z undefined unless save_z)
+std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& residual, int64_t act, bool out_f32, bool save_z) {
+    const int64_t K = x.size(-1), N = w.size(0), M = x.numel() / K, n8 = (N + 7) / 8 * 8;
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = N;
+    Tensor y = at::empty(shape, x.options().dtype(out_f32 ? at::kFloat : at::kBFloat16)), z;
+    if (save_z) z = at::empty({M, n8}, x.options());
+    int64_t ldx = K, ldw = K, ldr = N;
+    operand_rows(x, &ldx);
+    operand_rows(w, &ldw);
+    if (residual.defined()) pitched_rows(residual, &ldr);
+    const int flags = (out_f32 ? WKV7_LINEAR_F32_OUT : 0) | (bias.defined() && bias.scalar_type() == at::kFloat ? WKV7_LINEAR_F32_BIAS : 0);
+    check(wkv7_linear_fwd(x.data_ptr(), w.data_ptr(), ptr(bias), ptr(residual), y.data_ptr(), ptr(z), M, N, K, ldx, ldw, ldr, N, n8, (int)act, flags, stream()),
+          "wkv7_linear_fwd");
+    return {y, z};
+}
+struct LinearFn : public Function<LinearFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias_, const OptTensor& residual_, int64_t act, bool out_f32, bool grad) {
+        const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
+        // relu and relu2 have their derivative in their value; of the others it is formed from the argument
+        const bool from_y = (act == WKV7_ACT_RELU || act == WKV7_ACT_RELU2) && !out_f32 && !residual.defined();
+        const auto [y, z] = linear_forward(x, w, bias, residual, act, out_f32, grad && act && !from_y);
+        if (grad) ctx->save_for_backward({x, w, from_y ? y : z});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["f32"] = out_f32;
+        ctx->saved_data["from_y"] = from_y;
+        ctx->saved_data["grad"] = grad;
+        ctx->saved_data["bias"] = bias.defined() ? (int64_t)bias.scalar_type() : (int64_t)-1;
+        ctx->saved_data["residual"] = residual.defined();
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list go) {
+        variable_list g(7);
+        Tensor dy = go[0];
+        if (!dy.defined()) return g;
+        const int64_t bias = ctx->saved_data["bias"].toInt(), act = ctx->saved_data["act"].toInt();
+        const bool out_f32 = ctx->saved_data["f32"].toBool(), from_y = ctx->saved_data["from_y"].toBool();
+        // (edges are counted over the arguments that are tensors)
+        const bool want_db = bias >= 0 && ctx->needs_input_grad(2), want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1);
+        if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(bias >= 0 ? 3 : 2)) g[3] = dy;
+        if (!ctx->saved_data["grad"].toBool() || !(want_dx || want_dw || want_db)) return g;
+        const variable_list s = ctx->get_saved_variables();
+        const c10::cuda::CUDAGuard guard(s[0].device());
+        at::NoGradGuard ng;
+        // (hooks on saved tensors may hand back other layouts)
+        int64_t ldx, ldw, lds = 1, lddy;
+        Tensor x = s[0], w = s[1], saved = s[2];
+        if (!operand_rows(x, &ldx)) { x = dense(x); ldx = x.size(-1); }
+        if (!operand_rows(w, &ldw)) { w = dense(w); ldw = w.size(-1); }
+        const int64_t K = x.size(-1), N = w.size(0), M = x.numel() / K;
+        if (act && !pitched_rows(saved, &lds)) { saved = dense(saved); lds = saved.size(-1); }
+        if (!pitched_rows(dy, &lddy)) { dy = dy.contiguous(); lddy = N; }
+        Tensor db;
+        if (want_dx) g[0] = at::empty(x.sizes(), x.options());
+        if (want_dw) g[1] = at::empty(w.sizes(), w.options());
+        if (want_db) db = at::empty({N}, x.options().dtype(at::kFloat));
+        Tensor ws = at::empty({wkv7_linear_bwd_workspace_bytes(M, N)}, x.options().dtype(at::kByte));
+        check(wkv7_linear_bwd(x.data_ptr(), w.data_ptr(), act ? ptr(saved) : nullptr, dy.data_ptr(), ptr(g[0]), ptr(g[1]), f32(db),
+                              M, N, K, ldx, ldw, act ? lds : N, lddy, (int)act, (out_f32 ? WKV7_LINEAR_F32_OUT : 0) | (from_y ? WKV7_LINEAR_FROM_Y : 0), ws.data_ptr(), stream()),
+              "wkv7_linear_bwd");
+        if (want_db) g[2] = db.to((at::ScalarType)bias);
+        return g;
+    }
+};
+py::object linear(const Tensor& x, const Tensor& w, const OptTensor& bias_, const OptTensor& residual_, int64_t act, bool out_f32) {
+    const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
+    int64_t ld;
+    if (!eager({&x, &w, &bias, &residual}) || x.dim() < 1 || w.dim() != 2 || !operand_rows(x, &ld) || !operand_rows(w, &ld) || w.device() != x.device()) return py::none();
+    const int64_t K = x.size(-1), N = w.size(0);
+    if (w.size(1) != K || K % 8 != 0) return py::none();
+    if (bias.defined() && (!plain(bias) || bias.dim() != 1 || bias.size(0) != N || !bias.is_contiguous() || bias.device() != x.device() ||
+                           (bias.scalar_type() != at::kFloat && bias.scalar_type() != at::kBFloat16)))
+        return py::none();
+    if (residual.defined()) {
+        std::vector<int64_t> shape = x.sizes().vec();
+        shape.back() = N;
+        if (residual.sizes() != at::IntArrayRef(shape) || residual.scalar_type() != (out_f32 ? at::kFloat : at::kBFloat16) || residual.device() != x.device() ||
+            !pitched_rows(residual, &ld))
+            return py::none();
+    }
+    Tensor y;
+    {
+        py::gil_scoped_release nogil;
+        const c10::cuda::CUDAGuard guard(x.device());
+        const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+        if (grad_wanted({&x, &w, &bias, &residual})) {
+            y = LinearFn::apply(x, w, opt(bias), opt(residual), act, out_f32, grad_wanted({&x, &w, &bias}));
+        } else {
+            at::NoGradGuard ng;
+            y = linear_forward(x, w, bias, residual, act, out_f32, false).first;
+        }
+    }
+    return py::cast(y);
+}
+
 // ---- TimeMixer --------------------------------------------------------------------------------------------
 // One autograd node for the whole layer: the ops above, the projection kernel and plain matrix products, in the order of
 // time_mixer.py.  All parameters are converted by one launch, and first-stage weights that share an input lie next to each other
@@ -691,4 +807,5 @@ PYBIND11_MODULE(_wkv7_torch, mod) {
     mod.def("ddlerp", ddlerp);
     mod.def("expand_loras", expand_loras);
     mod.def("mixer", mixer);
+    mod.def("linear", linear);
 }

@@ -62,6 +62,9 @@ _SIGNATURES = {
     'wkv7_ddlerp_bwd': (_int, [_vp] * 16 + [_i64] * 4 + [_vp]),
     'wkv7_ddlerp_bwd_tc': (_int, [_vp] * 17 + [_i64] * 4 + [_vp]),
     'wkv7_ddlerp_bwd_tc_workspace_bytes': (ctypes.c_size_t, [_i64] * 2),
+    'wkv7_linear_fwd': (_int, [_vp] * 6 + [_i64] * 8 + [_int] * 2 + [_vp]),
+    'wkv7_linear_bwd_workspace_bytes': (_i64, [_i64] * 2),
+    'wkv7_linear_bwd': (_int, [_vp] * 7 + [_i64] * 7 + [_int] * 2 + [_vp] * 2),
     'wkv7_expand_loras_fwd': (_int, [_vp] * 18 + [_i64] * 4 + [_vp]),
     'wkv7_expand_loras_fwd_ld': (_int, [_vp] * 19 + [_i64] * 4 + [_vp]),
     'wkv7_expand_loras_bwd_ld': (_int, [_vp] * 35 + [_i64] * 4 + [_vp]),
