@@ -231,6 +231,19 @@ def test_streams_and_calls_that_follow_one_another():
     assert th.equal(a, want) and th.equal(c, want)
 
 
+@pytest.mark.parametrize('M', [4, 100, 3000])
+def test_in_a_thread_that_has_made_no_call_yet(M):
+    """Such a thread has no current context; the tensor maps' encoding needs one."""
+    import threading
+    from wind_rwkv.rwkv7 import linear
+    x, w, b, r, _ = inputs(M, 3328, 64, th.float32, True, th.bfloat16, 5)
+    want, got = linear(x, w, b, residual=r), []
+    t = threading.Thread(target=lambda: got.append(linear(x, w, b, residual=r)))
+    t.start()
+    t.join()
+    assert th.equal(got[0], want)
+
+
 def test_python_form_agrees():
     """The form that torch.compile traces, called directly."""
     from wind_rwkv.rwkv7.rwkv7_linear import ACTS, Linear

@@ -633,6 +633,8 @@ template <typename P> static bool launch_cluster(void (*kern)(P, int*), unsigned
 }
 
 static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb, long long k, const Epi& e, bool swap, int nt, int splits, int* status, cudaStream_t stream) {
+    // (first of all: it gives a thread that has made no other call yet, one of autograd's, the context that encoding a tensor map needs)
+    if (cudaFuncSetAttribute(linear_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return kLaunchFailed;
     TileParams p;
     memset(&p, 0, sizeof(p));
     if (!encode(&p.P, a, na, k, BM) || !encode(&p.Q, b, nb, k, nt)) return kLaunchFailed;
@@ -653,11 +655,11 @@ static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb
     if (p.stages > most) p.stages = most;
     const int ring = p.stages * stage > part ? p.stages * stage : part;
     const int smem = 2048 + ring;
-    if (cudaFuncSetAttribute(linear_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return kLaunchFailed;
     return launch_cluster(linear_tile_kernel, (unsigned)grid, TILE_THREADS, smem, splits, stream, p, status) ? kOk : kLaunchFailed;
 }
 
 static int run_pair(LinearOperand a, LinearOperand b, long long na, long long nb, long long k, const Epi& e, int bn, int* status, cudaStream_t stream) {
+    if (cudaFuncSetAttribute(linear_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return kLaunchFailed;
     PairParams p;
     memset(&p, 0, sizeof(p));
     if (!encode(&p.P, a, na, k, BM) || !encode(&p.Q, b, nb, k, bn / 2)) return kLaunchFailed;
@@ -669,7 +671,6 @@ static int run_pair(LinearOperand a, LinearOperand b, long long na, long long nb
     p.tiles = (long long)p.p_tiles * p.q_tiles;
     const long long pairs = sm_count() / 2;
     const unsigned grid = 2 * (unsigned)(p.tiles < pairs ? p.tiles : pairs);
-    if (cudaFuncSetAttribute(linear_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return kLaunchFailed;
     return launch_cluster(linear_pair_kernel, grid, PAIR_THREADS, PAIR_SMEM, 1, stream, p, status) ? kOk : kLaunchFailed;
 }
 
