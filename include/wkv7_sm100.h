@@ -47,6 +47,7 @@ extern "C" {
 #define WKV7_ERR_LAUNCH (-7)         /* the CUDA launch failed */
 #define WKV7_ERR_TOO_LARGE (-8)
 #define WKV7_ERR_DEVICE_TIMEOUT (-9) /* reported by wkv7_device_status() */
+#define WKV7_ERR_INDEX (-11)         /* reported by wkv7_device_status(): wkv7_reorder was given a parent that does not exist */
 #define WKV7_ERR_STATIC_SCRATCH (-10) /* problem too large for wkv7_attn_ln_bwd_static's built-in scratch */
 
 /* Size of the scratch array compiled into the library for wkv7_attn_ln_bwd_static. */
@@ -311,6 +312,29 @@ int wkv7_linear_fwd(const void* x, const void* w, const void* bias, const void* 
 int64_t wkv7_linear_bwd_workspace_bytes(int64_t M, int64_t N);
 int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void* dy, void* dx, void* dw, float* dbias, int64_t M, int64_t N, int64_t K,
                     int64_t ldx, int64_t ldw, int64_t lds, int64_t lddy, int act, int flags, void* workspace, void* stream);
+
+/*
+ * Beam search's selection (no reference counterpart).  For each of B sequences with W beams over a vocabulary of V: the k best of the W V
+ * candidates by scores[b][w] + logits[b][w][v] - log sum_v' exp(logits[b][w][v']), best first, equal ones by the lowest w V + v.
+ * logits [B,W,V] bf16, or fp32 with logits_f32, strides (stride_b, stride_w, 1) in elements; scores fp32 [B,W], the beams' sums of log-probabilities.
+ * -inf, +inf and NaN rule a logit out (score -inf), and a beam whose score they are; a candidate whose score is below fp32's range counts as -inf; where
+ * fewer than k candidates are above -inf the rest are the lowest at -inf.  Comparisons are made in 64 bits.
+ * finished (1 byte each, [B,W], or null): such a beam goes on with token eos alone, its score unchanged; out_finished [B,k] then receives whether the
+ * beam had ended or ends with this token.  Outputs: out_scores fp32, parents and tokens int64, [B,k].  1 <= k <= 64, W <= 64, k <= W V < 2^31,
+ * V <= 2^30, 0 <= eos < V where finished is given.  workspace: wkv7_beam_select_workspace_bytes(B, W, V) bytes, 16-byte aligned.
+ */
+int64_t wkv7_beam_select_workspace_bytes(int64_t B, int64_t W, int64_t V);
+int wkv7_beam_select(const void* logits, const float* scores, const void* finished, float* out_scores, int64_t* parents, int64_t* tokens,
+                     void* out_finished, int64_t B, int64_t W, int64_t V, int64_t k, int64_t eos, int64_t stride_b, int64_t stride_w, int logits_f32,
+                     void* workspace, void* stream);
+/*
+ * The beams' states follow their parents: row b k + j of dst[i] := row b W + parents[b][j] of src[i], for `count` tensors whose rows are row_bytes[i] adjacent
+ * bytes, src_pitch[i] and dst_pitch[i] bytes apart (the arrays are host memory; any count).  dst[i] == src[i] with equal pitches and k == W: in place, rows that
+ * stay are not touched; otherwise dst must not overlap any src, and no dst another.  parents [B,k] int64, or int32 with parents_i32, device
+ * memory.  A parent outside 0 .. W-1 leaves its row as it is (in place) or zero, and WKV7_ERR_INDEX in the status word.  W, k <= 64.
+ */
+int wkv7_reorder(int count, const void* const* src, void* const* dst, const int64_t* row_bytes, const int64_t* src_pitch, const int64_t* dst_pitch,
+                 const void* parents, int parents_i32, int64_t B, int64_t W, int64_t k, void* stream);
 
 /*
  * expand_loras: second-stage LoRA expansion producing (w, k, kk, b) for the mixer.  Replaces

@@ -7,6 +7,7 @@
 #include "ddlerp.h"
 #include "expand_loras.h"
 #include "linear.h"
+#include "beam.h"
 
 #include <mutex>
 
@@ -126,6 +127,7 @@ const char* wkv7_status_string(int status) {
         case WKV7_ERR_TOO_LARGE: return "B*H exceeds the grid limit, or B*H*ceil(T/16) checkpoint records exceed 32-bit row addressing";
         case WKV7_ERR_DEVICE_TIMEOUT: return "a bounded device-side wait ran out";
         case WKV7_ERR_STATIC_SCRATCH: return "problem needs more than WKV7_STATIC_SCRATCH_BYTES of built-in scratch (B*3*H*N*4 bytes); use wkv7_attn_ln_bwd with a caller-provided workspace";
+        case WKV7_ERR_INDEX: return "wkv7_reorder: a parent beam that does not exist";
         default: return "unknown status";
     }
 }
@@ -505,6 +507,67 @@ int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void*
         rc = wkv7::launch_linear({dz.p, dz.ld, true}, {x, ldx, true}, M, e, status, s);
     }
     return rc;
+}
+
+static_assert(WKV7_ERR_INDEX == wkv7::kBadIndex, "mirrored constants");
+
+static int beam_check(int64_t B, int64_t W, int64_t V, int64_t k) {
+    if (B < 0 || W < 1 || V < 1 || k < 1 || W > wkv7::BEAM_MAX_W || k > wkv7::BEAM_MAX_K) return WKV7_ERR_SHAPE;
+    if (V > 1 << 30 || W * V > 0x7fffffffLL || B > 0x7fffffffLL / wkv7::BEAM_MAX_W) return WKV7_ERR_TOO_LARGE;
+    return k <= W * V ? WKV7_OK : WKV7_ERR_SHAPE;
+}
+
+int64_t wkv7_beam_select_workspace_bytes(int64_t B, int64_t W, int64_t V) {
+    return beam_check(B, W, V, 1) || B == 0 ? 0 : (int64_t)wkv7::beam_workspace_bytes(B, W, V);
+}
+
+int wkv7_beam_select(const void* logits, const float* scores, const void* finished, float* out_scores, int64_t* parents, int64_t* tokens,
+                     void* out_finished, int64_t B, int64_t W, int64_t V, int64_t k, int64_t eos, int64_t stride_b, int64_t stride_w, int logits_f32,
+                     void* workspace, void* stream) {
+    int rc = beam_check(B, W, V, k);
+    if (rc) return rc;
+    if (stride_b < 0 || stride_w < 0 || (finished && (eos < 0 || eos >= V))) return WKV7_ERR_SHAPE;
+    if (B == 0) return WKV7_OK;
+    if (!logits || !scores || !out_scores || !parents || !tokens || !workspace || (finished && !out_finished)) return WKV7_ERR_NULL;
+    if ((uintptr_t)logits % (logits_f32 ? 4 : 2) || (uintptr_t)scores % 4 || (uintptr_t)out_scores % 4 || (uintptr_t)parents % 8 || (uintptr_t)tokens % 8 || !aligned16(workspace))
+        return WKV7_ERR_ALIGN;
+    wkv7::BeamParams p{};
+    p.logits = logits; p.scores = scores; p.finished = (const unsigned char*)finished;
+    p.out_scores = out_scores; p.parents = parents; p.tokens = tokens; p.out_finished = (unsigned char*)out_finished;
+    p.sb = stride_b; p.sw = stride_w;
+    p.B = (int)B; p.W = (int)W; p.V = (int)V; p.k = (int)k; p.eos = (int)eos; p.f32 = logits_f32 != 0;
+    return wkv7::launch_beam_select(p, workspace, (cudaStream_t)stream);
+}
+
+int wkv7_reorder(int count, const void* const* src, void* const* dst, const int64_t* row_bytes, const int64_t* src_pitch, const int64_t* dst_pitch,
+                 const void* parents, int parents_i32, int64_t B, int64_t W, int64_t k, void* stream) {
+    if (count < 0 || B < 0 || W < 1 || k < 1 || W > wkv7::BEAM_MAX_W || k > wkv7::BEAM_MAX_K) return WKV7_ERR_SHAPE;
+    if (B > 0x7fffffffLL / wkv7::BEAM_MAX_W) return WKV7_ERR_TOO_LARGE;
+    for (int i = 0; i < count; ++i) {
+        if (row_bytes[i] < 0 || src_pitch[i] < row_bytes[i] || dst_pitch[i] < row_bytes[i]) return WKV7_ERR_SHAPE;
+        if (B == 0 || row_bytes[i] == 0) continue;
+        if (!src[i] || !dst[i]) return WKV7_ERR_NULL;
+        if (src[i] == dst[i] && (k != W || src_pitch[i] != dst_pitch[i])) return WKV7_ERR_SHAPE;
+    }
+    if (B == 0 || count == 0) return WKV7_OK;
+    if (!parents) return WKV7_ERR_NULL;
+    if ((uintptr_t)parents % (parents_i32 ? 4 : 8)) return WKV7_ERR_ALIGN;
+    int* status = status_ptr();
+    if (!status) return WKV7_ERR_LAUNCH;
+    for (int from = 0; from < count; from += wkv7::REORDER_MAX) {
+        wkv7::ReorderParams p{};
+        p.parents = parents; p.idx64 = !parents_i32;
+        p.B = (int)B; p.W = (int)W; p.k = (int)k; p.status = status;
+        for (int i = from; i < count && i < from + wkv7::REORDER_MAX; ++i) {
+            if (row_bytes[i] == 0) continue;
+            const int j = p.count++;
+            p.src[j] = src[i]; p.dst[j] = dst[i];
+            p.row_bytes[j] = row_bytes[i]; p.src_pitch[j] = src_pitch[i]; p.dst_pitch[j] = dst_pitch[i];
+        }
+        const int rc = p.count ? wkv7::launch_reorder(p, (cudaStream_t)stream) : WKV7_OK;
+        if (rc) return rc;
+    }
+    return WKV7_OK;
 }
 
 static int ddlerp_check(int64_t B, int64_t T, int64_t C, int64_t D) {

@@ -34,6 +34,7 @@ void check(int rc, const char* what) {
                                  "); its results are invalid.  wkv7_device_status() reads and clears the error.");
 }
 void* stream() { return (void*)at::cuda::getCurrentCUDAStream().stream(); }
+float* f32_of(const Tensor& t) { return t.data_ptr<float>(); }
 float* f32(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 Tensor scratch(const Tensor& like) {
     static const int64_t bytes = (int64_t)wkv7_workspace_bytes();
@@ -572,6 +573,98 @@ py::object linear(const Tensor& x, const Tensor& w, const OptTensor& bias_, cons
     return py::cast(y);
 }
 
+// ---- beam search --------------------------------------------------------------------------------------------
+py::object beam_select(const Tensor& logits, const Tensor& scores, int64_t k, const OptTensor& finished_, int64_t eos) {
+    const Tensor finished = finished_.value_or(Tensor());
+    if (!eager({&logits, &scores, &finished}, false) || !plain(logits) || !plain(scores) || logits.dim() != 3 || scores.dim() != 2 || logits.numel() == 0) return py::none();
+    const bool f32 = logits.scalar_type() == at::kFloat;
+    const int64_t B = logits.size(0), W = logits.size(1), V = logits.size(2);
+    if ((!f32 && logits.scalar_type() != at::kBFloat16) || (V > 1 && logits.stride(2) != 1) || scores.scalar_type() != at::kFloat || !scores.is_contiguous() ||
+        scores.device() != logits.device() || scores.size(0) != B || scores.size(1) != W || W > 64 || k < 1 || k > 64 || k > W * V)
+        return py::none();
+    if (finished.defined() != (eos >= 0) || eos >= V) return py::none();
+    if (finished.defined() && (!plain(finished) || finished.scalar_type() != at::kBool || !finished.is_contiguous() || finished.device() != logits.device() ||
+                               finished.dim() != 2 || finished.size(0) != B || finished.size(1) != W))
+        return py::none();
+    Tensor out, parents, tokens, fin;
+    {
+        py::gil_scoped_release nogil;
+        const c10::cuda::CUDAGuard guard(logits.device());
+        at::NoGradGuard ng;
+        out = at::empty({B, k}, scores.options());
+        parents = at::empty({B, k}, scores.options().dtype(at::kLong));
+        tokens = at::empty({B, k}, scores.options().dtype(at::kLong));
+        if (finished.defined()) fin = at::empty({B, k}, finished.options());
+        Tensor ws = at::empty({wkv7_beam_select_workspace_bytes(B, W, V)}, scores.options().dtype(at::kByte));
+        check(wkv7_beam_select(logits.data_ptr(), f32_of(scores), ptr(finished), f32_of(out), parents.data_ptr<int64_t>(), tokens.data_ptr<int64_t>(), ptr(fin), B, W, V, k,
+                               eos, logits.stride(0), logits.stride(1), f32, ws.data_ptr(), stream()), "wkv7_beam_select");
+    }
+    return finished.defined() ? py::make_tuple(out, parents, tokens, fin) : py::make_tuple(out, parents, tokens);
+}
+
+// [rows, ...] as rows of adjacent bytes, `pitch` apart
+bool row_layout(const Tensor& t, int64_t* bytes, int64_t* pitch) {
+    int64_t n = 1;
+    for (int64_t i = t.dim() - 1; i > 0; --i) {
+        if (t.size(i) != 1 && t.stride(i) != n) return false;
+        n *= t.size(i);
+    }
+    const int64_t ld = t.size(0) <= 1 ? n : t.stride(0);
+    *bytes = n * t.element_size();
+    *pitch = ld * t.element_size();
+    return ld >= n;
+}
+py::object reorder_states(const variable_list& states, const Tensor& parents, bool inplace) {
+    if (states.empty() || !eager({&parents}, false) || !plain(parents) || parents.dim() != 2 || parents.numel() == 0 || !parents.is_contiguous() ||
+        (parents.scalar_type() != at::kLong && parents.scalar_type() != at::kInt) || at::tracer::impl::is_dispatch_enabled())
+        return py::none();
+    const int64_t B = parents.size(0), k = parents.size(1), count = (int64_t)states.size();
+    const int64_t rows = states[0].dim() ? states[0].size(0) : 0, W = rows / B;
+    if (k > 64 || rows == 0 || rows % B != 0 || W > 64 || (inplace && W != k)) return py::none();
+    const Eager ok(false);
+    std::vector<int64_t> bytes(count), sp(count), dp(count);
+    std::vector<const void*> src(count);
+    std::vector<void*> dst(count);
+    const bool grad_mode = at::GradMode::is_enabled();
+    for (int64_t i = 0; i < count; ++i) {
+        const Tensor& t = states[i];
+        if (!ok(t) || !plain(t) || (t.is_conj() && !inplace) || t.device() != parents.device() || t.dim() == 0 || t.size(0) != rows || t.numel() == 0 || !row_layout(t, &bytes[i], &sp[i])) return py::none();
+        if (inplace && grad_mode && t.requires_grad()) return py::none();
+        src[i] = t.data_ptr();
+    }
+    if (inplace && count > 1) {  // rows that share memory are refused by the Python path; so, to be looked at there, are tensors within one another's extent
+        std::vector<std::pair<uintptr_t, uintptr_t>> at(count);
+        for (int64_t i = 0; i < count; ++i) at[i] = {(uintptr_t)src[i], (uintptr_t)src[i] + (rows - 1) * sp[i] + bytes[i]};
+        std::sort(at.begin(), at.end());
+        for (int64_t i = 1; i < count; ++i)
+            if (at[i].first < at[i - 1].second) return py::none();
+    }
+    variable_list out;
+    {
+        py::gil_scoped_release nogil;
+        const c10::cuda::CUDAGuard guard(parents.device());
+        at::NoGradGuard ng;
+        for (int64_t i = 0; i < count; ++i) {
+            if (inplace) {
+                out.push_back(states[i]);
+                dp[i] = sp[i];
+            } else {
+                std::vector<int64_t> shape = states[i].sizes().vec();
+                shape[0] = B * k;
+                out.push_back(at::empty(shape, states[i].options()));
+                dp[i] = bytes[i];
+            }
+            dst[i] = out[i].data_ptr();
+        }
+        check(wkv7_reorder((int)count, src.data(), dst.data(), bytes.data(), sp.data(), dp.data(), parents.data_ptr(), parents.scalar_type() == at::kInt, B, W, k, stream()),
+              "wkv7_reorder");
+        if (inplace)
+            for (const Tensor& t : out)
+                if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+    return py::cast(out);
+}
+
 // ---- TimeMixer --------------------------------------------------------------------------------------------
 // One autograd node for the whole layer: the ops above, the projection kernel and plain matrix products, in the order of
 // time_mixer.py.  All parameters are converted by one launch, and first-stage weights that share an input lie next to each other
@@ -808,4 +901,6 @@ PYBIND11_MODULE(_wkv7_torch, mod) {
     mod.def("expand_loras", expand_loras);
     mod.def("mixer", mixer);
     mod.def("linear", linear);
+    mod.def("beam_select", beam_select);
+    mod.def("reorder_states", reorder_states);
 }

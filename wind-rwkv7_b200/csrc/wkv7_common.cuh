@@ -55,6 +55,7 @@ enum Status : int {
     kLaunchFailed = -7,    // cudaGetLastError() after launch was not cudaSuccess
     kTooLarge = -8,
     kDeviceTimeout = -9,   // a bounded device-side wait (mbar_wait_bounded) gave up
+    kBadIndex = -11,       // reorder: a parent beam that does not exist (-10 is the C ABI's WKV7_ERR_STATIC_SCRATCH)
 };
 
 // ---- IO element access ----------------------------------------------------------------------

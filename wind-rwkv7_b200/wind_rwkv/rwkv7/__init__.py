@@ -5,6 +5,7 @@ from .rwkv7_attn import attn, attn_step, load_attn
 from .rwkv7_attn_ln import attn_ln, load_attn_ln
 from .rwkv7_proj import proj
 from .rwkv7_linear import linear
+from .rwkv7_beam import beam_select, reorder_states
 
 from .time_mixer import TimeMixer
 

@@ -65,6 +65,9 @@ _SIGNATURES = {
     'wkv7_linear_fwd': (_int, [_vp] * 6 + [_i64] * 8 + [_int] * 2 + [_vp]),
     'wkv7_linear_bwd_workspace_bytes': (_i64, [_i64] * 2),
     'wkv7_linear_bwd': (_int, [_vp] * 7 + [_i64] * 7 + [_int] * 2 + [_vp] * 2),
+    'wkv7_beam_select_workspace_bytes': (_i64, [_i64] * 3),
+    'wkv7_beam_select': (_int, [_vp] * 7 + [_i64] * 7 + [_int] + [_vp] * 2),
+    'wkv7_reorder': (_int, [_int] + [_vp] * 6 + [_int] + [_i64] * 3 + [_vp]),
     'wkv7_expand_loras_fwd': (_int, [_vp] * 18 + [_i64] * 4 + [_vp]),
     'wkv7_expand_loras_fwd_ld': (_int, [_vp] * 19 + [_i64] * 4 + [_vp]),
     'wkv7_expand_loras_bwd_ld': (_int, [_vp] * 35 + [_i64] * 4 + [_vp]),
