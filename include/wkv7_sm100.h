@@ -286,9 +286,9 @@ int wkv7_proj_gemm_group_ld(int count, const void* const* A, const void* const* 
  *   y = act(x w^T + bias) + residual
  * x [M,K], w [N,K] (an nn.Linear weight) bf16, rows ldx, ldw elements apart; y [M,N] bf16, or fp32 with WKV7_LINEAR_F32_OUT; bias [N] bf16, or fp32
  * with WKV7_LINEAR_F32_BIAS, or null; residual [M,N] of y's type, or null (may be y itself).  K, ldx and ldw multiples of 8, x and w 16-byte
- * aligned (bulk tensor copies); any M >= 0, N > 0, any ldr, ldy >= N.  z: null, or [M,N] bf16 with rows ldz apart (a multiple of 8, 16-byte
- * aligned), where the activation's argument goes for the backward; the columns between N and the next multiple of 8 may be written.
- * tcgen05 products, fp32 accumulation; results do not depend on the number of SMs' load, and are the same from call to call.  May report
+ * aligned (bulk tensor copies); any M >= 0, N > 0, any ldr, ldy >= N.  z: null, or [M,N] bf16, fp32 with
+ * WKV7_LINEAR_F32_Z, with rows ldz apart (a multiple of 8, 16-byte aligned), where the activation's argument goes for the backward; the columns between N and the next multiple of 8 may be written.
+ * tcgen05 products, fp32 accumulation; Results are the same from call to call.  May report
  * WKV7_ERR_DEVICE_TIMEOUT through the status word (bounded waits).
  */
 #define WKV7_ACT_NONE 0
@@ -301,11 +301,12 @@ int wkv7_proj_gemm_group_ld(int count, const void* const* A, const void* const* 
 #define WKV7_LINEAR_F32_OUT 1
 #define WKV7_LINEAR_F32_BIAS 2
 #define WKV7_LINEAR_FROM_Y 4
+#define WKV7_LINEAR_F32_Z 8
 int wkv7_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, int64_t M, int64_t N, int64_t K,
                     int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int64_t ldz, int act, int flags, void* stream);
 /*
  * Its backward: dz = dy act'(z), dx = dz w [M,K] bf16, dw = dz^T x [N,K] bf16, dbias = column sums of dz [N] fp32; each of the three may be null.
- * (The residual's gradient is dy.)  dy [M,N] of y's type, rows lddy apart.  saved: z as wkv7_linear_fwd wrote it, rows lds apart; with
+ * (The residual's gradient is dy.)  dy [M,N] of y's type, rows lddy apart.  saved: z as wkv7_linear_fwd wrote it (WKV7_LINEAR_F32_Z: fp32), rows lds apart; with
  * WKV7_LINEAR_FROM_Y (WKV7_ACT_RELU and _RELU2, bf16 y, no residual) y itself; not read with WKV7_ACT_NONE.  dz is rounded to bf16 for the
  * products, not for dbias.  No atomics: results are the same from call to call.  workspace: wkv7_linear_bwd_workspace_bytes(M, N) bytes, 16-byte aligned.
  */

@@ -6,7 +6,7 @@ Activations are formed with errors of a few 2^-21 of max(|value|, |argument|) (h
   y:  |act'| <= L times the error of z, the activation's own, u |y| for its rounding (fp32 y: 2^-22 |y|)
   dz: |dy| times the error of act': L2 >= |act''| times that of z (bf16 z: u |z| more), from y (relu2): 2 sqrt(y (1 + u)), i.e. u/2 relative;
       u |dz| for its rounding to bf16
-  dx, dw: the sums of the bounds on dz times the other operand's magnitudes, acc of the sum, u of the result;  dbias: dz's without its rounding
+  dx, dw: the sums of the bounds on dz times the other operand's magnitudes, acc of the sum, u of the result;  dbias: dz's without its rounding, fp32 with z in fp32
 """
 import pytest
 import torch as th
@@ -71,6 +71,9 @@ def compare(x, w, b, r, dy, act, out=th.bfloat16, call=None):
         ed = (Z.abs() <= ez).double()
     else:
         ed = L2[act] * (ez + U * Z.abs()) + (0 if act is None else 2.0 ** -18 * (1 + Z.abs()))
+    # a bias in fp32: its gradient's terms from an argument in fp32
+    edb = 2 * ez + 2.0 ** -22 * Z.abs() if act == 'relu2' else (ed if act == 'relu' else L2[act] * ez + (0 if act is None else 2.0 ** -18 * (1 + Z.abs())))
+    edb = DY.abs() * (edb if b is not None and b.dtype == th.float32 else ed)
     edz = DY.abs() * ed
     edzr = edz + U * (DZ.abs() + edz)
     M = X.shape[0]
@@ -80,7 +83,7 @@ def compare(x, w, b, r, dy, act, out=th.bfloat16, call=None):
     if b is not None:
         s = DZ.sum(0)
         round_b = U if b.dtype == th.bfloat16 else 0
-        check('dbias', next(grads), s, edz.sum(0) * (1 + U) + (M + 8) * 2.0 ** -24 * DZ.abs().sum(0) + round_b * s.abs())
+        check('dbias', next(grads), s, edb.sum(0) * (1 + U) + (M + 8) * 2.0 ** -24 * DZ.abs().sum(0) + round_b * s.abs())
     if r is not None:
         assert th.equal(next(grads), dy)
     return y

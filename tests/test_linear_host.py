@@ -23,7 +23,7 @@ def bwd(lib, M=4, N=16, K=64, lds=16, lddy=16, act=2, flags=0, saved=0x1000, dy=
 
 def test_forward_checks(lib):
     assert fwd(lib, M=-1) == fwd(lib, N=0) == fwd(lib, K=0) == -1
-    assert fwd(lib, act=7) == fwd(lib, act=-1) == fwd(lib, flags=8) == fwd(lib, flags=4) == -1
+    assert fwd(lib, act=7) == fwd(lib, act=-1) == fwd(lib, flags=16) == fwd(lib, flags=4) == -1
     assert fwd(lib, ldx=56) == fwd(lib, ldw=56) == fwd(lib, ldy=15) == fwd(lib, r=0x1000, ldr=15) == -1
     assert fwd(lib, N=17, ldy=17, z=0x1000, ldz=17) == -1                     # z's rows hold the next multiple of 8
     assert fwd(lib, K=60) == fwd(lib, ldx=68) == fwd(lib, ldw=68) == -4
@@ -35,7 +35,7 @@ def test_forward_checks(lib):
 
 
 def test_backward_checks(lib):
-    assert bwd(lib, flags=4, act=3) == bwd(lib, flags=5, act=2) == bwd(lib, flags=2) == -1   # a derivative from y: relu and relu2, bf16
+    assert bwd(lib, flags=4, act=3) == bwd(lib, flags=5, act=2) == bwd(lib, flags=2) == bwd(lib, flags=12) == -1   # a derivative from y: relu and relu2, bf16
     assert bwd(lib, lds=15) == bwd(lib, lddy=15) == -1
     assert bwd(lib, dy=None) == bwd(lib, saved=None) == bwd(lib, ws=None) == -6
     assert bwd(lib, dx=0x1008) == bwd(lib, dw=0x1008) == bwd(lib, ws=0x1008) == bwd(lib, db=0x1002) == bwd(lib, saved=0x1001) == -4

@@ -446,7 +446,7 @@ static int linear_check(const void* x, const void* w, int64_t M, int64_t N, int6
 
 int wkv7_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, int64_t M, int64_t N, int64_t K,
                     int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int64_t ldz, int act, int flags, void* stream) {
-    int rc = linear_check(x, w, M, N, K, ldx, ldw, act, flags, WKV7_LINEAR_F32_OUT | WKV7_LINEAR_F32_BIAS);
+    int rc = linear_check(x, w, M, N, K, ldx, ldw, act, flags, WKV7_LINEAR_F32_OUT | WKV7_LINEAR_F32_BIAS | WKV7_LINEAR_F32_Z);
     if (rc) return rc;
     const int64_t n8 = (N + 7) / 8 * 8;
     if (ldy < N || (residual && ldr < N) || (z && ldz < n8)) return WKV7_ERR_SHAPE;
@@ -457,7 +457,7 @@ int wkv7_linear_fwd(const void* x, const void* w, const void* bias, const void* 
     if ((uintptr_t)y % ysize || (uintptr_t)residual % ysize || (uintptr_t)bias % bsize) return WKV7_ERR_ALIGN;
     int* status = status_ptr();
     if (!status) return WKV7_ERR_LAUNCH;
-    const wkv7::LinearEpilogue e{bias, residual, y, z, ldr, ldy, ldz, M, N, act, bsize == 4, ysize == 4};
+    const wkv7::LinearEpilogue e{bias, residual, y, z, ldr, ldy, ldz, M, N, act, bsize == 4, ysize == 4, (flags & WKV7_LINEAR_F32_Z) != 0};
     return wkv7::launch_linear({x, ldx, false}, {w, ldw, false}, K, e, status, (cudaStream_t)stream);
 }
 
@@ -470,10 +470,10 @@ int64_t wkv7_linear_bwd_workspace_bytes(int64_t M, int64_t N) {
 
 int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void* dy, void* dx, void* dw, float* dbias, int64_t M, int64_t N, int64_t K,
                     int64_t ldx, int64_t ldw, int64_t lds, int64_t lddy, int act, int flags, void* workspace, void* stream) {
-    int rc = linear_check(x, w, M, N, K, ldx, ldw, act, flags, WKV7_LINEAR_F32_OUT | WKV7_LINEAR_FROM_Y);
+    int rc = linear_check(x, w, M, N, K, ldx, ldw, act, flags, WKV7_LINEAR_F32_OUT | WKV7_LINEAR_FROM_Y | WKV7_LINEAR_F32_Z);
     if (rc) return rc;
-    const bool from_y = flags & WKV7_LINEAR_FROM_Y, f32 = flags & WKV7_LINEAR_F32_OUT;
-    if (from_y && ((act != WKV7_ACT_RELU && act != WKV7_ACT_RELU2) || f32)) return WKV7_ERR_SHAPE;
+    const bool from_y = flags & WKV7_LINEAR_FROM_Y, f32 = flags & WKV7_LINEAR_F32_OUT, z32 = flags & WKV7_LINEAR_F32_Z;
+    if (from_y && ((act != WKV7_ACT_RELU && act != WKV7_ACT_RELU2) || f32 || z32)) return WKV7_ERR_SHAPE;
     if (lddy < N || (act && lds < N)) return WKV7_ERR_SHAPE;
     cudaStream_t s = (cudaStream_t)stream;
     if (M == 0) {  // sums over nothing
@@ -481,7 +481,7 @@ int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void*
         return WKV7_OK;
     }
     if (!dy || !workspace || (act && !saved)) return WKV7_ERR_NULL;
-    if (!aligned16(workspace) || (dx && !aligned16(dx)) || (dw && !aligned16(dw)) || (uintptr_t)dbias % 4 || (uintptr_t)dy % (f32 ? 4 : 2) || (act && (uintptr_t)saved % 2))
+    if (!aligned16(workspace) || (dx && !aligned16(dx)) || (dw && !aligned16(dw)) || (uintptr_t)dbias % 4 || (uintptr_t)dy % (f32 ? 4 : 2) || (act && (uintptr_t)saved % (z32 ? 4 : 2)))
         return WKV7_ERR_ALIGN;
     int* status = status_ptr();
     if (!status) return WKV7_ERR_LAUNCH;
@@ -492,18 +492,18 @@ int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void*
         if (!as_is) dz = wkv7::LinearOperand{workspace, (N + 7) / 8 * 8, false};
         if (dbias || ((dx || dw) && !as_is)) {
             const wkv7::LinearDz d{dy, saved, as_is || !(dx || dw) ? nullptr : workspace, dbias, (float*)((char*)workspace + linear_dz_bytes(M, N)), M, N, lddy, lds,
-                                   (N + 7) / 8 * 8, act, f32, from_y};
+                                   (N + 7) / 8 * 8, act, f32, z32, from_y};
             rc = wkv7::launch_linear_dz(d, s);
             if (rc) return rc;
         }
     }
     if (dx) {
-        const wkv7::LinearEpilogue e{nullptr, nullptr, dx, nullptr, 0, K, 0, M, K, 0, false, false};
+        const wkv7::LinearEpilogue e{nullptr, nullptr, dx, nullptr, 0, K, 0, M, K, 0, false, false, false};
         rc = wkv7::launch_linear(dz, {w, ldw, true}, N, e, status, s);
         if (rc) return rc;
     }
     if (dw) {
-        const wkv7::LinearEpilogue e{nullptr, nullptr, dw, nullptr, 0, K, 0, N, K, 0, false, false};
+        const wkv7::LinearEpilogue e{nullptr, nullptr, dw, nullptr, 0, K, 0, N, K, 0, false, false, false};
         rc = wkv7::launch_linear({dz.p, dz.ld, true}, {x, ldx, true}, M, e, status, s);
     }
     return rc;

@@ -66,12 +66,12 @@ __device__ __forceinline__ void act8(int act, float (&f)[8]) {
         default: break;
     }
 }
-// act'(z); from_y: of relu and relu2 from their values, 2 sqrt(y) for 2 relu(z)
-__device__ __forceinline__ float act_grad(int act, bool from_y, float z) {
-    switch (act) {
+// act'(z); FROM_Y: of relu and relu2 from their values, 2 sqrt(y) for 2 relu(z)
+template <int ACT, bool FROM_Y> __device__ __forceinline__ float act_grad(float z) {
+    switch (ACT) {
         case kActRelu: return z > 0.f ? 1.f : 0.f;
-        case kActRelu2: return from_y ? 2.f * sqrtf(z) : 2.f * relu_f(z);
-        case kActTanh: { const float t = tanh_f(z); return 1.f - t * t; }
+        case kActRelu2: return FROM_Y ? 2.f * sqrtf(z) : 2.f * relu_f(z);
+        case kActTanh: { const float e = ex2_approx(-2.f * LOG2E * fabsf(z)), r = rcp_mufu(1.f + e); return 4.f * e * r * r; }
         case kActSigmoid: { const float s = sigmoid_f(z); return s * (1.f - s); }
         case kActSilu: { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }
         case kActGelu: {
@@ -97,10 +97,22 @@ __device__ __forceinline__ void load8g(const void* base, bool f32, long long at,
 __device__ __forceinline__ float load1g(const void* base, bool f32, long long at) {
     return f32 ? ((const float*)base)[at] : __bfloat162float(((const bf16*)base)[at]);
 }
+__device__ __forceinline__ void store_z1(const Epi& e, long long row, long long col, float v) {
+    if (e.z_f32) ((float*)e.z)[row * e.ldz + col] = v;
+    else ((bf16*)e.z)[row * e.ldz + col] = __float2bfloat16_rn(v);
+}
+__device__ __forceinline__ void store8g(void* base, bool f32, long long at, const float (&f)[8]) {
+    if (f32) {
+        *reinterpret_cast<float4*>((float*)base + at) = make_float4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<float4*>((float*)base + at + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+        *reinterpret_cast<uint4*>((bf16*)base + at) = pack8(f);
+    }
+}
 // eight adjacent columns of a row, from the accumulator to memory; bias already added
 __device__ __forceinline__ void finish8(const Epi& e, long long row, long long col, float (&f)[8]) {
     const int live = (int)(e.cols - col < 8 ? e.cols - col : 8);
-    if (e.z) *reinterpret_cast<uint4*>((bf16*)e.z + row * e.ldz + col) = pack8(f);  // (ldz is a multiple of 8: room for all eight)
+    if (e.z) store8g(e.z, e.z_f32, row * e.ldz + col, f);  // (ldz is a multiple of 8: room for all eight)
     act8(e.act, f);
     if (e.vec && live == 8) {
         if (e.residual) {
@@ -109,13 +121,7 @@ __device__ __forceinline__ void finish8(const Epi& e, long long row, long long c
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] += r[i];
         }
-        if (e.y_f32) {
-            float* y = (float*)e.y + row * e.ldy + col;
-            *reinterpret_cast<float4*>(y) = make_float4(f[0], f[1], f[2], f[3]);
-            *reinterpret_cast<float4*>(y + 4) = make_float4(f[4], f[5], f[6], f[7]);
-        } else {
-            *reinterpret_cast<uint4*>((bf16*)e.y + row * e.ldy + col) = pack8(f);
-        }
+        store8g(e.y, e.y_f32, row * e.ldy + col, f);
         return;
     }
 #pragma unroll
@@ -174,7 +180,7 @@ __device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
 struct TileParams {
     CUtensorMap P, Q;
     Epi e;
-    int p_mn, q_mn, nt, kblocks, splits, stages, swap, p_tiles;  // swap: P runs over the columns of y, Q over its rows
+    int p_mn, q_mn, nt, kblocks, splits, stages, accs, swap, p_tiles;  // swap: P runs over the columns of y, Q over its rows
     uint32_t tmem_cols;
 };
 struct TileCtrl {
@@ -184,15 +190,22 @@ struct TileCtrl {
 };
 static_assert(sizeof(TileCtrl) <= 1024, "the KB ahead of the ring");
 constexpr int TILE_THREADS = 192;  // warps 0-3: accumulator rows, warp 4: copies, warp 5: products; all six: the result
-__host__ __device__ constexpr int p_bytes() { return BM * 128; }
+constexpr int P_BYTES = BM * 128;
 __host__ __device__ constexpr int q_bytes(int nt) { return nt * 128; }  // a multiple of 1024 from 8 rows on
-__host__ __device__ constexpr int tile_pitch(int nt, int swap) { return swap ? nt + 1 : nt + 4; }
+// Accumulator rows in shared memory, nt + 4 floats apart: rows r .. r + 7 start on different groups of four banks.  Each CTA of a cluster has 128 / splits rows
+// of the tile to finish and a place for every CTA's part of them.
+__host__ __device__ constexpr int part_pitch(int nt) { return nt + 4; }
+__host__ __device__ constexpr int part_bytes(int nt) { return BM * part_pitch(nt) * 4; }
+
+__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
 __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_constant__ TileParams p, int* status) {
     extern __shared__ unsigned char smem_dyn[];
     TileCtrl* ctrl = reinterpret_cast<TileCtrl*>(smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u));
     unsigned char* sm = reinterpret_cast<unsigned char*>(ctrl) + 1024;
-    const int stage_bytes = p_bytes() + q_bytes(p.nt);
+    const int stage_bytes = P_BYTES + q_bytes(p.nt);
+    // the parts have a place of their own where other CTAs write to it, which may be done with their share of k before this one
+    float* parts = reinterpret_cast<float*>(p.splits > 1 ? sm + p.stages * stage_bytes : sm);
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int rank = blockIdx.x % p.splits;
@@ -215,6 +228,7 @@ __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = ctrl->tmem_base;
+    if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (waited for before the first write to another CTA)
     stream_order();
 
     if (warp == 4) {
@@ -230,8 +244,8 @@ __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_
                 };
                 if (p.p_mn) { load(&p.P, dst, p0, kb * BK); load(&p.P, dst + 8192, p0 + 64, kb * BK); }
                 else load(&p.P, dst, kb * BK, p0);
-                if (p.q_mn) for (int b = 0; b < p.nt; b += 64) load(&p.Q, dst + p_bytes() + b * 128, q0 + b, kb * BK);
-                else load(&p.Q, dst + p_bytes(), kb * BK, q0);
+                if (p.q_mn) for (int b = 0; b < p.nt; b += 64) load(&p.Q, dst + P_BYTES + b * 128, q0 + b, kb * BK);
+                else load(&p.Q, dst + P_BYTES, kb * BK, q0);
                 ++issued;
                 if (++s == p.stages) { s = 0; ++round; }
             }
@@ -242,17 +256,18 @@ __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_
         if (elect_one()) {
             const uint32_t idesc = idesc_of(BM, p.nt, p.p_mn, p.q_mn);
             const uint64_t step_p = p.p_mn ? 2048 >> 4 : 2, step_q = p.q_mn ? 2048 >> 4 : 2;  // 16 k
-            int s = 0, round = 0;
+            int s = 0, round = 0, a = 0;
             for (int kb = lo; kb < hi; ++kb) {
                 mbar_wait_bounded<false>(&ctrl->full[s], round & 1, &ctrl->abort, status);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t da = desc_of(smem_u32(sm + s * stage_bytes), p.p_mn), db = desc_of(smem_u32(sm + s * stage_bytes + p_bytes()), p.q_mn);
+                const uint64_t da = desc_of(smem_u32(sm + s * stage_bytes), p.p_mn), db = desc_of(smem_u32(sm + s * stage_bytes + P_BYTES), p.q_mn);
 #pragma unroll
                 for (int ks = 0; ks < BK / 16; ++ks)
                     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                                 ::"r"(tmem), "l"(da + ks * step_p), "l"(db + ks * step_q), "r"(idesc), "r"((kb > lo || ks > 0) ? 1u : 0u) : "memory");
+                                 ::"r"(tmem + a * p.nt), "l"(da + ks * step_p), "l"(db + ks * step_q), "r"(idesc), "r"((kb >= lo + p.accs || ks > 0) ? 1u : 0u) : "memory");
                 asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&ctrl->empty[s])) : "memory");
                 if (++s == p.stages) { s = 0; ++round; }
+                if (++a == p.accs) a = 0;
             }
             asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&ctrl->accum)) : "memory");
             if (ctrl->abort) {  // the later waits fell through: wait for what was issued before tensor memory is released
@@ -263,28 +278,30 @@ __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_
         __syncwarp();
     }
     __syncwarp();
-    // the accumulator to shared memory, in the place of the operands (all products have read theirs, and nothing is in flight)
-    const int pitch = tile_pitch(p.nt, p.swap);
-    float* part = reinterpret_cast<float*>(sm);
     if (warp < 4) {
         mbar_wait_bounded<true>(&ctrl->accum, 0, &ctrl->abort, status);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
-    __syncthreads();  // (the copying thread has seen its last copies land)
+    if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else __syncthreads();  // the ring, where the result goes, is read no more, and its last copies have landed
+    const int pitch = part_pitch(p.nt), rows = BM / p.splits;
     if (warp < 4) {
-        float* row = part + (32 * warp + lane) * pitch;
+        // a lane has a row of the accumulators and sends it to the CTA that finishes it
+        const int row = 32 * warp + lane;
+        const uint32_t to = map_rank(smem_u32(parts + (rank * rows + row % rows) * pitch), row / rows);
 #pragma unroll 1
         for (int c = 0; c < p.nt; c += 16) {
             uint32_t v[16];
             tmem_ld16(tmem + ((uint32_t)(32 * warp) << 16) + c, v);
-            if (p.swap) {
+            for (int a = 1; a < min(p.accs, hi - lo); ++a) {
+                uint32_t u[16];
+                tmem_ld16(tmem + ((uint32_t)(32 * warp) << 16) + a * p.nt + c, u);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) row[c + i] = __uint_as_float(v[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<float4*>(row + c + i) = make_float4(__uint_as_float(v[i]), __uint_as_float(v[i + 1]), __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(u[i]));
             }
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (c + i) * 4), "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]) : "memory");
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     }
@@ -292,45 +309,46 @@ __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_
     else __syncthreads();
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
 
-    // this CTA's share of the tile: the parts are added in the order of their ranks
-    const uint32_t mine = smem_u32(part);
-    const bool ok = !ctrl->abort;
+    // this CTA's rows of the tile: the parts are added in the order of their ranks
+    if (ctrl->abort) return;
     const Epi& e = p.e;
-    if (p.swap) {  // lanes along P, i.e. along a row of y
-        const int units = BM * p.nt, from = (int)((long long)units * rank / p.splits), to = (int)((long long)units * (rank + 1) / p.splits);
-        for (int u = from + tid; u < to && ok; u += TILE_THREADS) {
-            const int i = u & (BM - 1), j = u / BM;
-            const long long row = q0 + j, col = p0 + i;
-            if (row >= e.rows || col >= e.cols) continue;
-            float v = 0.f;
-            for (int r = 0; r < p.splits; ++r) {
-                float x;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(map_rank(mine + (i * pitch + j) * 4, r)) : "memory");
-                v += x;
+    const int r0 = rank * rows;
+    if (p.swap) {  // a thread has four of Q's indices, lanes run along P, i.e. along a row of y
+        for (int u = tid; u < rows * (p.nt / 4); u += TILE_THREADS) {
+            const int i = u % rows, j = u / rows * 4;
+            const long long col = p0 + r0 + i;
+            if (col >= e.cols || q0 + j >= e.rows) continue;
+            float4 x = ld4(parts + i * pitch + j);
+            for (int r = 1; r < p.splits; ++r) {
+                const float4 y = ld4(parts + (r * rows + i) * pitch + j);
+                x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
             }
-            if (e.bias) v += load1g(e.bias, e.bias_f32, col);
-            if (e.z) ((bf16*)e.z)[row * e.ldz + col] = __float2bfloat16_rn(v);
-            float f[8] = {v};
+            const float bias = e.bias ? load1g(e.bias, e.bias_f32, col) : 0.f;
+            float f[8] = {x.x + bias, x.y + bias, x.z + bias, x.w + bias};
+            for (int q = 0; q < 4; ++q)
+                if (e.z && q0 + j + q < e.rows) store_z1(e, q0 + j + q, col, f[q]);
             act8(e.act, f);
-            v = f[0];
-            if (e.residual) v += load1g(e.residual, e.y_f32, row * e.ldr + col);
-            if (e.y_f32) ((float*)e.y)[row * e.ldy + col] = v;
-            else ((bf16*)e.y)[row * e.ldy + col] = __float2bfloat16_rn(v);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const long long row = q0 + j + q;
+                if (row >= e.rows) break;
+                float v = f[q];
+                if (e.residual) v += load1g(e.residual, e.y_f32, row * e.ldr + col);
+                if (e.y_f32) ((float*)e.y)[row * e.ldy + col] = v;
+                else ((bf16*)e.y)[row * e.ldy + col] = __float2bfloat16_rn(v);
+            }
         }
     } else {
-        const int per_row = p.nt / 8, units = BM * per_row, from = (int)((long long)units * rank / p.splits), to = (int)((long long)units * (rank + 1) / p.splits);
-        for (int u = from + tid; u < to && ok; u += TILE_THREADS) {
+        const int per_row = p.nt / 8;
+        for (int u = tid; u < rows * per_row; u += TILE_THREADS) {
             const int i = u / per_row, j = 8 * (u % per_row);
-            const long long row = p0 + i, col = q0 + j;
+            const long long row = p0 + r0 + i, col = q0 + j;
             if (row >= e.rows || col >= e.cols) continue;
             float f[8] = {};
             for (int r = 0; r < p.splits; ++r) {
-                float x[8];
-                const uint32_t a = map_rank(mine + (i * pitch + j) * 4, r);
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(a) : "memory");
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]) : "r"(a + 16) : "memory");
-#pragma unroll
-                for (int q = 0; q < 8; ++q) f[q] += x[q];
+                const float* x = parts + (r * rows + i) * pitch + j;
+                const float4 a = ld4(x), b = ld4(x + 4);
+                f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
             }
             if (e.bias) {
 #pragma unroll
@@ -340,7 +358,6 @@ __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_
             finish8(e, row, col, f);
         }
     }
-    if (p.splits > 1) cluster_sync();  // nobody leaves while its part is read
 }
 
 // ---- pairs of CTAs, persistent ------------------------------------------------------------------------------------
@@ -530,7 +547,8 @@ struct DzParams : LinearDz {
     long long rows_per;
     bool vec;  // rows of dy and saved start on 16-byte boundaries
 };
-__global__ void __launch_bounds__(DZ_THREADS) linear_dz_kernel(const __grid_constant__ DzParams p) {
+constexpr int DZ_AHEAD = 4;  // rows a thread has requested at a time
+template <int ACT, bool FROM_Y> __global__ void __launch_bounds__(DZ_THREADS) linear_dz_kernel(const __grid_constant__ DzParams p) {
     stream_order();
     __shared__ float sums[8][DZ_COLS + 4];
     const int g = threadIdx.x & 31, r = threadIdx.x >> 5;
@@ -538,27 +556,35 @@ __global__ void __launch_bounds__(DZ_THREADS) linear_dz_kernel(const __grid_cons
     const long long lo = blockIdx.y * p.rows_per, hi = lo + p.rows_per < p.M ? lo + p.rows_per : p.M;
     float acc[8] = {};
     if (col < p.N) {
-        const bool whole = p.vec && col + 8 <= p.N;
-#pragma unroll 2
-        for (long long m = lo + r; m < hi; m += 8) {
-            float d[8], z[8] = {};
-            if (whole) {
-                load8g(p.dy, p.dy_f32, m * p.lddy + col, d);
-                if (p.act) load8g(p.saved, false, m * p.lds + col, z);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool in = col + i < p.N;
-                    d[i] = in ? load1g(p.dy, p.dy_f32, m * p.lddy + col + i) : 0.f;
-                    z[i] = in && p.act ? load1g(p.saved, false, m * p.lds + col + i) : 0.f;
-                }
-            }
+        auto row = [&](long long m, float (&d)[8], const float (&z)[8]) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                if (p.act) d[i] *= act_grad(p.act, p.from_y, z[i]);
+                if (ACT) d[i] = __fmul_rn(d[i], act_grad<ACT, FROM_Y>(z[i]));  // (not merged into the sum: dbias is the same whether dz is wanted or not)
                 acc[i] += d[i];
             }
             if (p.dz) *reinterpret_cast<uint4*>((bf16*)p.dz + m * p.ldz + col) = pack8(d);  // (ldz is a multiple of 8)
+        };
+        const bool whole = p.vec && col + 8 <= p.N;
+        long long m = lo + r;
+        for (; whole && m + 8 * (DZ_AHEAD - 1) < hi; m += 8 * DZ_AHEAD) {
+            float d[DZ_AHEAD][8], z[DZ_AHEAD][8];
+#pragma unroll
+            for (int a = 0; a < DZ_AHEAD; ++a) {
+                load8g(p.dy, p.dy_f32, (m + 8 * a) * p.lddy + col, d[a]);
+                if (ACT) load8g(p.saved, p.saved_f32, (m + 8 * a) * p.lds + col, z[a]);
+            }
+#pragma unroll
+            for (int a = 0; a < DZ_AHEAD; ++a) row(m + 8 * a, d[a], z[a]);
+        }
+        for (; m < hi; m += 8) {
+            float d[8], z[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool in = col + i < p.N;
+                d[i] = in ? load1g(p.dy, p.dy_f32, m * p.lddy + col + i) : 0.f;
+                z[i] = in && ACT ? load1g(p.saved, p.saved_f32, m * p.lds + col + i) : 0.f;
+            }
+            row(m, d, z);
         }
     }
     if (!p.dbias) return;
@@ -643,19 +669,27 @@ static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb
     p.kblocks = (int)((k + BK - 1) / BK);
     p.splits = splits;
     p.p_tiles = (int)((na + BM - 1) / BM);
-    p.tmem_cols = 32;
-    while ((int)p.tmem_cols < nt) p.tmem_cols *= 2;
     const long long tiles = p.p_tiles * ((nb + nt - 1) / nt), grid = tiles * splits;
     if (grid > 0x7fffffffLL) return kTooLarge;
-    const int stage = p_bytes() + q_bytes(nt), part = BM * tile_pitch(nt, swap) * 4;
-    // a CTA of a full grid shares its SM with another one
-    const int room = (grid > sm_count() ? 113 : 226) * 1024 - 2048, most = (p.kblocks + splits - 1) / splits;
+    const int stage = P_BYTES + q_bytes(nt), part = part_bytes(nt), most = (p.kblocks + splits - 1) / splits;
+    // CTAs that share an SM: as many as let the whole grid run at once, up to four; clusters of four and eight, two (they do not find whole free SMs everywhere)
+    int per_sm = (int)((grid + sm_count() - 1) / sm_count());
+    if (per_sm < 2 && splits > 2) per_sm = 2;
+    const int cap = nt > 64 ? 2 : 4;
+    if (per_sm > cap) per_sm = cap;
+    const int room = 227 * 1024 / per_sm - 1024 - 2048 - (splits > 1 ? part : 0);  // (the system has a KB of each CTA's)
     p.stages = room / stage;
+    if (p.stages < 2) p.stages = 2;
     if (p.stages > MAXSTAGES) p.stages = MAXSTAGES;
     if (p.stages > most) p.stages = most;
-    const int ring = p.stages * stage > part ? p.stages * stage : part;
-    const int smem = 2048 + ring;
-    return launch_cluster(linear_tile_kernel, (unsigned)grid, TILE_THREADS, smem, splits, stream, p, status) ? kOk : kLaunchFailed;
+    // Products of one accumulator follow one another with its rounding, which cuts: the error of a long sum grows with its length.  Where tensor memory has
+    // room k blocks go to several accumulators in turn, which are added in the end (16 rows, K = 2048, fp32 results: relative error 2.1e-6 -> 5e-7).
+    p.accs = 128 / nt;
+    if (p.accs > most) p.accs = most;
+    p.tmem_cols = 32;
+    while ((int)p.tmem_cols < nt * p.accs) p.tmem_cols *= 2;
+    const int ring = splits > 1 ? p.stages * stage + part : p.stages * stage > part ? p.stages * stage : part;
+    return launch_cluster(linear_tile_kernel, (unsigned)grid, TILE_THREADS, 2048 + ring, splits, stream, p, status) ? kOk : kLaunchFailed;
 }
 
 static int run_pair(LinearOperand a, LinearOperand b, long long na, long long nb, long long k, const Epi& e, int bn, int* status, cudaStream_t stream) {
@@ -713,9 +747,13 @@ int launch_linear_dz(const LinearDz& d, cudaStream_t stream) {
     static_cast<LinearDz&>(p) = d;
     const int chunks = linear_dz_chunks(d.M, d.N);
     p.rows_per = (d.M + chunks - 1) / chunks;
-    p.vec = al16(d.dy) && d.lddy % (d.dy_f32 ? 4 : 8) == 0 && (!d.act || (al16(d.saved) && d.lds % 8 == 0));
+    p.vec = al16(d.dy) && d.lddy % (d.dy_f32 ? 4 : 8) == 0 && (!d.act || (al16(d.saved) && d.lds % (d.saved_f32 ? 4 : 8) == 0));
     const int cols = (int)((d.N + DZ_COLS - 1) / DZ_COLS);
-    if (!launch(linear_dz_kernel, dim3(cols, chunks), DZ_THREADS, 0, stream, p)) return kLaunchFailed;
+    void (*const kern[kActs][2])(DzParams) = {{linear_dz_kernel<kActNone, false>, nullptr}, {linear_dz_kernel<kActRelu, false>, linear_dz_kernel<kActRelu, false>},
+        {linear_dz_kernel<kActRelu2, false>, linear_dz_kernel<kActRelu2, true>}, {linear_dz_kernel<kActTanh, false>, nullptr}, {linear_dz_kernel<kActSigmoid, false>, nullptr},
+        {linear_dz_kernel<kActSilu, false>, nullptr}, {linear_dz_kernel<kActGelu, false>, nullptr}};
+    if (!kern[d.act][d.from_y]) return kBadShape;
+    if (!launch(kern[d.act][d.from_y], dim3(cols, chunks), DZ_THREADS, 0, stream, p)) return kLaunchFailed;
     if (d.dbias && !launch(linear_dbias_kernel, dim3((unsigned)((d.N + 31) / 32)), 256, 0, stream, (const float*)d.partial, d.dbias, d.N, chunks)) return kLaunchFailed;
     return kOk;
 }

@@ -12,10 +12,10 @@ struct LinearEpilogue {
     const void* bias;      // [cols] or null
     const void* residual;  // [rows, cols], of y's type, or null
     void* y;               // [rows, cols]
-    void* z;               // [rows, ldz] bf16, the argument of the activation, or null
+    void* z;               // [rows, ldz] bf16 or fp32, the argument of the activation, or null
     long long ldr, ldy, ldz, rows, cols;
     int act;
-    bool bias_f32, y_f32;
+    bool bias_f32, y_f32, z_f32;
 };
 
 // y[rows, cols] = epilogue(sum_k P[i, k] Q[j, k]); an operand is [index, k] with k contiguous, or (`_mn`) [k, index] with the index contiguous
@@ -33,7 +33,7 @@ struct LinearDz {
     float *dbias, *partial;  // partial: linear_dz_chunks(M, N) x N floats, where dbias is wanted
     long long M, N, lddy, lds, ldz;
     int act;
-    bool dy_f32, from_y;     // from_y: `saved` is the activation's value, not its argument
+    bool dy_f32, saved_f32, from_y;     // from_y: `saved` is the activation's value, not its argument
 };
 int linear_dz_chunks(long long M, long long N);
 int launch_linear_dz(const LinearDz& p, cudaStream_t stream);

@@ -477,18 +477,18 @@ bool operand_rows(const Tensor& t, int64_t* ld) {
     return pitched_rows(t, ld) && t.scalar_type() == at::kBFloat16 && *ld % 8 == 0 && !(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15);
 }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-// y, z (z undefined unless save_z)
-std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& residual, int64_t act, bool out_f32, bool save_z) {
+// y, z (undefined unless z_type is given)
+std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& residual, int64_t act, bool out_f32, std::optional<at::ScalarType> z_type) {
     const int64_t K = x.size(-1), N = w.size(0), M = x.numel() / K, n8 = (N + 7) / 8 * 8;
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = N;
     Tensor y = at::empty(shape, x.options().dtype(out_f32 ? at::kFloat : at::kBFloat16)), z;
-    if (save_z) z = at::empty({M, n8}, x.options());
+    if (z_type) z = at::empty({M, n8}, x.options().dtype(*z_type));
     int64_t ldx = K, ldw = K, ldr = N;
     operand_rows(x, &ldx);
     operand_rows(w, &ldw);
     if (residual.defined()) pitched_rows(residual, &ldr);
-    const int flags = (out_f32 ? WKV7_LINEAR_F32_OUT : 0) | (bias.defined() && bias.scalar_type() == at::kFloat ? WKV7_LINEAR_F32_BIAS : 0);
+    const int flags = (out_f32 ? WKV7_LINEAR_F32_OUT : 0) | (bias.defined() && bias.scalar_type() == at::kFloat ? WKV7_LINEAR_F32_BIAS : 0) | (z_type == at::kFloat ? WKV7_LINEAR_F32_Z : 0);
     check(wkv7_linear_fwd(x.data_ptr(), w.data_ptr(), ptr(bias), ptr(residual), y.data_ptr(), ptr(z), M, N, K, ldx, ldw, ldr, N, n8, (int)act, flags, stream()),
           "wkv7_linear_fwd");
     return {y, z};
@@ -496,9 +496,12 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const
 struct LinearFn : public Function<LinearFn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias_, const OptTensor& residual_, int64_t act, bool out_f32, bool grad) {
         const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
-        // relu and relu2 have their derivative in their value; of the others it is formed from the argument
-        const bool from_y = (act == WKV7_ACT_RELU || act == WKV7_ACT_RELU2) && !out_f32 && !residual.defined();
-        const auto [y, z] = linear_forward(x, w, bias, residual, act, out_f32, grad && act && !from_y);
+        // relu and relu2 have their derivative in their value; of the others it is formed from the argument, kept in fp32 beside a bias in fp32, whose gradient
+        // goes out in fp32
+        const bool z32 = bias.defined() && bias.scalar_type() == at::kFloat && act != WKV7_ACT_RELU;
+        const bool from_y = (act == WKV7_ACT_RELU || act == WKV7_ACT_RELU2) && !out_f32 && !residual.defined() && !z32;
+        const auto [y, z] = linear_forward(x, w, bias, residual, act, out_f32,
+                                           grad && act && !from_y ? std::optional<at::ScalarType>(z32 ? at::kFloat : at::kBFloat16) : std::nullopt);
         if (grad) ctx->save_for_backward({x, w, from_y ? y : z});
         ctx->set_materialize_grads(false);
         ctx->saved_data["act"] = act;
@@ -536,7 +539,8 @@ struct LinearFn : public Function<LinearFn> {
         if (want_db) db = at::empty({N}, x.options().dtype(at::kFloat));
         Tensor ws = at::empty({wkv7_linear_bwd_workspace_bytes(M, N)}, x.options().dtype(at::kByte));
         check(wkv7_linear_bwd(x.data_ptr(), w.data_ptr(), act ? ptr(saved) : nullptr, dy.data_ptr(), ptr(g[0]), ptr(g[1]), f32(db),
-                              M, N, K, ldx, ldw, act ? lds : N, lddy, (int)act, (out_f32 ? WKV7_LINEAR_F32_OUT : 0) | (from_y ? WKV7_LINEAR_FROM_Y : 0), ws.data_ptr(), stream()),
+                              M, N, K, ldx, ldw, act ? lds : N, lddy, (int)act, (out_f32 ? WKV7_LINEAR_F32_OUT : 0) | (from_y ? WKV7_LINEAR_FROM_Y : 0) |
+                              (act && saved.scalar_type() == at::kFloat ? WKV7_LINEAR_F32_Z : 0), ws.data_ptr(), stream()),
               "wkv7_linear_bwd");
         if (want_db) g[2] = db.to((at::ScalarType)bias);
         return g;
@@ -567,7 +571,7 @@ py::object linear(const Tensor& x, const Tensor& w, const OptTensor& bias_, cons
             y = LinearFn::apply(x, w, opt(bias), opt(residual), act, out_f32, grad_wanted({&x, &w, &bias}));
         } else {
             at::NoGradGuard ng;
-            y = linear_forward(x, w, bias, residual, act, out_f32, false).first;
+            y = linear_forward(x, w, bias, residual, act, out_f32, std::nullopt).first;
         }
     }
     return py::cast(y);

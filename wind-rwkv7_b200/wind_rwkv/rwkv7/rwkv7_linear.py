@@ -10,7 +10,7 @@ import torch as th
 from . import _lib
 
 ACTS = {None: 0, 'relu': 1, 'relu2': 2, 'tanh': 3, 'sigmoid': 4, 'silu': 5, 'gelu': 6}
-F32_OUT, F32_BIAS, FROM_Y = 1, 2, 4
+F32_OUT, F32_BIAS, FROM_Y, F32_Z = 1, 2, 4, 8
 
 
 def rows_of(t):
@@ -37,26 +37,30 @@ def operand_of(t):
     return t, ld
 
 
-def saves(act, out_f32, residual):
-    """What the backward needs of the forward: nothing, 'y' or 'z'.  relu and relu^2 have their derivative in their value (2 sqrt(y), a bf16 y's
-    rounding halved by the root); of the others it is formed from the argument, kept in bf16."""
+def saves(act, out_f32, residual, bias_f32):
+    """What the backward needs of the forward: None, 'y', 'z' or 'z32'.  relu and relu^2 have their derivative in their value (2 sqrt(y), a bf16 y's
+    rounding halved by the root); of the others it is formed from the argument, kept in bf16: no worse than the rounding of dz for the products.  With
+    a bias in fp32, whose gradient goes out in fp32, what is summed for it is formed from an argument in fp32."""
     if act == 0:
         return None
-    return 'y' if act in (1, 2) and not out_f32 and not residual else 'z'
+    if bias_f32 and act != ACTS['relu']:
+        return 'z32'
+    return 'y' if act in (ACTS['relu'], ACTS['relu2']) and not out_f32 and not residual else 'z'
 
 
-def fw_linear(x, w, bias, residual, act, out_f32, save_z):
-    """Launcher: y [..., N], z [rows, N rounded up to 8] (empty where it is not wanted)."""
+def fw_linear(x, w, bias, residual, act, out_f32, save):
+    """Launcher: y [..., N], z [rows, N rounded up to 8] (empty unless save is 'z' or 'z32')."""
+    save_z = save in ('z', 'z32')
     K, N = x.shape[-1], w.shape[0]
     M = x.numel() // K
     n8 = (N + 7) // 8 * 8
     y = th.empty(*x.shape[:-1], N, dtype=th.float32 if out_f32 else th.bfloat16, device=x.device)
-    z = th.empty(M if save_z else 0, n8, dtype=th.bfloat16, device=x.device)
+    z = th.empty(M if save_z else 0, n8, dtype=th.float32 if save == 'z32' else th.bfloat16, device=x.device)
     x, ldx = operand_of(x)
     w, ldw = operand_of(w)
     r, ldr = (None, N) if residual is None else rows_of(residual)
     b = None if bias is None else bias.contiguous()
-    flags = (F32_OUT if out_f32 else 0) | (F32_BIAS if b is not None and b.dtype == th.float32 else 0)
+    flags = (F32_OUT if out_f32 else 0) | (F32_BIAS if b is not None and b.dtype == th.float32 else 0) | (F32_Z if save == 'z32' else 0)
     with _lib.on_device(x, w, b, r):
         rc = _lib.lib().wkv7_linear_fwd(x.data_ptr(), w.data_ptr(), _lib.ptr(b), _lib.ptr(r), y.data_ptr(), z.data_ptr() if save_z else None,
                                         M, N, K, ldx, ldw, ldr, N, n8, act, flags, _lib.stream_of(x))
@@ -77,7 +81,7 @@ def bw_linear(x, w, saved, dy, act, out_f32, from_y, want_dx, want_dw, want_db):
     dy, lddy = rows_of(dy)
     saved, lds = rows_of(saved) if act else (None, N)
     ws = th.empty(_lib.lib().wkv7_linear_bwd_workspace_bytes(M, N), dtype=th.uint8, device=dev)
-    flags = (F32_OUT if out_f32 else 0) | (FROM_Y if from_y else 0)
+    flags = (F32_OUT if out_f32 else 0) | (FROM_Y if from_y else 0) | (F32_Z if act and saved.dtype == th.float32 else 0)
     with _lib.on_device(x, w, dy, saved):
         rc = _lib.lib().wkv7_linear_bwd(x.data_ptr(), w.data_ptr(), _lib.ptr(saved), dy.data_ptr(), dx.data_ptr() if want_dx else None,
                                         dw.data_ptr() if want_dw else None, db.data_ptr() if want_db else None, M, N, K, ldx, ldw, lds, lddy, act, flags,
@@ -86,11 +90,11 @@ def bw_linear(x, w, saved, dy, act, out_f32, from_y, want_dx, want_dw, want_db):
     return dx, dw, db
 
 
-def _fake_fw(x, w, bias, residual, act, out_f32, save_z):
+def _fake_fw(x, w, bias, residual, act, out_f32, save):
     N = w.shape[0]
     rows = x.numel() // x.shape[-1]
     return (x.new_empty((*x.shape[:-1], N), dtype=th.float32 if out_f32 else th.bfloat16),
-            x.new_empty((rows if save_z else 0, (N + 7) // 8 * 8), dtype=th.bfloat16))
+            x.new_empty((rows if save in ('z', 'z32') else 0, (N + 7) // 8 * 8), dtype=th.float32 if save == 'z32' else th.bfloat16))
 
 
 def _fake_bw(x, w, saved, dy, act, out_f32, from_y, want_dx, want_dw, want_db):
@@ -99,7 +103,7 @@ def _fake_bw(x, w, saved, dy, act, out_f32, from_y, want_dx, want_dw, want_db):
 
 
 _fw_op = _lib.opaque_op('linear_fwd', fw_linear, _fake_fw,
-                        '(Tensor x, Tensor w, Tensor? bias, Tensor? residual, int act, bool out_f32, bool save_z) -> (Tensor, Tensor)')
+                        '(Tensor x, Tensor w, Tensor? bias, Tensor? residual, int act, bool out_f32, str save) -> (Tensor, Tensor)')
 _bw_op = _lib.opaque_op('linear_bwd', bw_linear, _fake_bw,
                         '(Tensor x, Tensor w, Tensor saved, Tensor dy, int act, bool out_f32, bool from_y, bool want_dx, bool want_dw, bool want_db) -> '
                         '(Tensor, Tensor, Tensor)')
@@ -109,8 +113,8 @@ class Linear(th.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act, out_f32):
         grad = any(ctx.needs_input_grad[:3])
-        save = saves(act, out_f32, residual is not None) if grad else None
-        y, z = _lib.call(_fw_op, fw_linear, x, w, bias, residual, act, out_f32, save == 'z')
+        save = saves(act, out_f32, residual is not None, bias is not None and bias.dtype == th.float32) if grad else None
+        y, z = _lib.call(_fw_op, fw_linear, x, w, bias, residual, act, out_f32, save or '')
         if grad:
             ctx.save_for_backward(x, w, y if save == 'y' else z)
         ctx.how = (act, out_f32, save == 'y', None if bias is None else bias.dtype)
