@@ -32,58 +32,146 @@ template <bool F32> __device__ __forceinline__ void load_edge(const void* base, 
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = at + i < V ? (F32 ? ((const float*)base)[row + at + i] : __bfloat162float(((const bf16*)base)[row + at + i])) : NEG_INF;
 }
-// The same as whole 16-byte words, of which the logits start `skip` bytes into the first.  A row may lie on any element's boundary; every lane then still
-// has the same logits whatever the alignment, so that equal rows give equal sums.  Words that reach beyond the row are not read: false.
-template <bool F32, bool ALIGNED> struct Raw {
-    static constexpr int WORDS = (F32 ? 2 : 1) + (ALIGNED ? 0 : 1);
-    uint4 w[WORDS];
-    __device__ __forceinline__ bool load(const void* base, long long row, int at, int V) {
-        const int size = F32 ? 4 : 2;
-        const unsigned char *start = (const unsigned char*)base + row * size, *end = start + (long long)V * size, *p = start + (long long)at * size;
-        p -= reinterpret_cast<uintptr_t>(p) & 15;
-        if (p < start || p + 16 * WORDS > end) return false;
+// 16 bytes of logits (eight, or four in fp32) out of whole 16-byte words, `skip` bytes into the first.  A row may lie on any element's boundary; every lane then
+// still has the same logits whatever the alignment, so that equal rows give equal sums.
+template <bool F32, bool ALIGNED> __device__ __forceinline__ void take(const unsigned char* b, int skip, float* f) {
+    const uint4 w = *reinterpret_cast<const uint4*>(b);
+    uint32_t o[4] = {w.x, w.y, w.z, w.w};
+    if (!ALIGNED) {
+        const uint4 v = *reinterpret_cast<const uint4*>(b + 16);
+        const uint32_t x[8] = {w.x, w.y, w.z, w.w, v.x, v.y, v.z, v.w};
+        const int words = skip >> 2, bits = (skip & 3) * 8;
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
-        return true;
+        for (int c = 0; c < 4; ++c)
+            if (words == c) {  // (the same for the whole row)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = F32 ? x[i + c] : __funnelshift_r(x[i + c], x[i + c + 1 < 8 ? i + c + 1 : 7], bits);
+            }
     }
-    __device__ __forceinline__ void take(int skip, float (&f)[8]) const {
-        uint32_t x[4 * WORDS], o[F32 ? 8 : 4];
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) { x[4 * i] = w[i].x; x[4 * i + 1] = w[i].y; x[4 * i + 2] = w[i].z; x[4 * i + 3] = w[i].w; }
-        constexpr int N_ = F32 ? 8 : 4;
-        if (ALIGNED) {
-#pragma unroll
-            for (int i = 0; i < N_; ++i) o[i] = x[i];
+    for (int i = 0; i < 4; ++i) {
+        if (F32) {
+            f[i] = __uint_as_float(o[i]);
         } else {
-            const int words = skip >> 2, bits = (skip & 3) * 8;
+            f[2 * i] = __uint_as_float(o[i] << 16);
+            f[2 * i + 1] = __uint_as_float(o[i] & 0xffff0000u);
+        }
+    }
+}
+__device__ __forceinline__ float warp_max(float x) {  // (a NaN is passed over)
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max8(const float (&f)[8]) { return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7]))); }
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int AHEAD = 2, DEPTH = 4;  // segments that are worked, and requested, together (a batch); batches of the ring
+constexpr float FAR_OUT = 1e30f;  // beyond it a logit is a mask, and its multiple by LOG2E may overflow
+
+// A part of a row (segments [first, last)) by a warp, AHEAD segments at a time: their maxima, the part's (m) and the lane's share of sum exp(l - m), formed
+// as 2^(l LOG2E - c), c = m LOG2E rounded: one multiply-add a logit.  What the rounding of c makes of it is one factor for the whole sum, taken out at the end.
+// The logits come by asynchronous copies into a ring of the warp's own, DEPTH - 1 batches ahead: what a warp has requested takes no registers.
+// CAREFUL: NaN and +inf are ruled out one by one, and l - m comes first; without it such a part's s is a NaN, or m is far out.
+template <bool F32, bool ALIGNED> __host__ __device__ constexpr int stage_bytes() { return AHEAD * SEG * (F32 ? 4 : 2) + (ALIGNED ? 0 : 16); }
+template <bool F32, bool ALIGNED, bool CAREFUL> __device__ __forceinline__ void scan_part(const BeamParams& p, long long row, int first, int last, float* seg_max, unsigned char* ring, int lane, float& m, float& s) {
+    constexpr int SIZE = F32 ? 4 : 2, STAGE = stage_bytes<F32, ALIGNED>(), BATCH = AHEAD * SEG * SIZE;
+    const unsigned char* at = (const unsigned char*)p.logits + row * SIZE;
+    const int skip = (int)(reinterpret_cast<uintptr_t>(at) & 15);
+    at -= skip;
+    // whether a batch's words lie within the row (those of an unaligned one reach up to a word further on both sides)
+    auto within = [&](int g) { return !CAREFUL && g < last && (ALIGNED || g > 0) && (long long)(g + AHEAD) * SEG + (ALIGNED ? 0 : 8) <= p.V; };
+    auto request = [&](int g, int stage) {
+        if (within(g)) {
+            const unsigned char* from = at + (long long)g * SEG * SIZE;
+            unsigned char* to = ring + stage * STAGE;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (words == c) {  // (the same for the whole row)
+            for (int i = 0; i < BATCH / 512; ++i) cp_async16(to + 512 * i + 16 * lane, from + 512 * i + 16 * lane);
+            if (!ALIGNED && lane == 0) cp_async16(to + BATCH, from + BATCH);
+        }
+        cp_async_commit();
+    };
+    auto anchor = [](float x) { return fmaxf(x, -FAR_OUT) * LOG2E; };
+    m = NEG_INF;
+    F2 sum = f2(0.f, 0.f);
+    int stage = 0;
+    if (!CAREFUL)
 #pragma unroll
-                    for (int i = 0; i < N_; ++i) o[i] = F32 ? x[i + c] : __funnelshift_r(x[i + c], x[i + c + 1 < 4 * WORDS ? i + c + 1 : i + c], bits);
+        for (int i = 0; i < DEPTH - 1; ++i) request(first + i * AHEAD, i);
+#pragma unroll 1
+    for (int g0 = first; g0 < last; g0 += AHEAD) {
+        float f[AHEAD][8], top[AHEAD];
+        if (!CAREFUL) {
+            cp_async_wait<DEPTH - 2>();
+            __syncwarp();  // the batch is there for all lanes, and all have taken the one before it
+            request(g0 + (DEPTH - 1) * AHEAD, stage ? stage - 1 : DEPTH - 1);
+        }
+        if (within(g0)) {
+            const unsigned char* b = ring + stage * STAGE;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                if (F32) {  // any eight of the segment's logits will do: two groups of four, without bank conflicts
+                    take<true, ALIGNED>(b + i * 1024 + 16 * lane, skip, f[i]);
+                    take<true, ALIGNED>(b + i * 1024 + 512 + 16 * lane, skip, f[i] + 4);
+                } else {
+                    take<false, ALIGNED>(b + i * 512 + 16 * lane, skip, f[i]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) load_edge<F32>(p.logits, row, (g0 + i) * SEG + 8 * lane, p.V, f[i]);
+        }
+        if (!CAREFUL && ++stage == DEPTH) stage = 0;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (CAREFUL) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[i][e] = sane(f[i][e]);
+            }
+            top[i] = warp_max(max8(f[i]));
+        }
+        if (lane == 0) {  // (segments come in fours)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i += 2) *reinterpret_cast<float2*>(seg_max + g0 + i) = make_float2(top[i], top[i + 1]);
+        }
+        float most = m;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) most = fmaxf(most, top[i]);
+        if (CAREFUL) {
+            if (most == NEG_INF) continue;
+            const float old = ex2_approx((m - most) * LOG2E);
+            sum = mul2(sum, f2(old, old));
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum.x += ex2_approx((f[i][e] - most) * LOG2E);
+        } else {
+            const float c = anchor(most), old = ex2_approx(anchor(m) - c);
+            const F2 minus = f2(-c, -c), log2e = f2(LOG2E, LOG2E);
+            sum = mul2(sum, f2(old, old));
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const F2 x = fma2(f2(f[i][e], f[i][e + 1]), log2e, minus);
+                    sum = add2(sum, f2(ex2_approx(x.x), ex2_approx(x.y)));
                 }
         }
-        if (F32) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[i % N_]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(o[i] << 16); f[2 * i + 1] = __uint_as_float(o[i] & 0xffff0000u); }
-        }
+        m = most;
     }
-};
-__device__ __forceinline__ float warp_max(float x) { return unordered(__reduce_max_sync(0xffffffffu, ordered(x))); }
+    s = sum.x + sum.y;
+    if (!CAREFUL && m > -FAR_OUT) s = fmaf(-LN2 * fmaf(m, LOG2E, -anchor(m)), s, s);  // 2^-r = 1 - r ln 2 for the rounding r of c
+}
 
-// A warp per part of a row (per_part segments), four segments' words requested at once.
 template <bool F32, bool ALIGNED> __global__ void __launch_bounds__(32 * SCAN_WARPS) beam_scan_kernel(const __grid_constant__ BeamParams p) {
+    extern __shared__ __align__(16) unsigned char rings[];
     stream_order();
     const int lane = threadIdx.x & 31;
+    unsigned char* ring = rings + (threadIdx.x >> 5) * (DEPTH * stage_bytes<F32, ALIGNED>());
     const long long unit = (long long)blockIdx.x * SCAN_WARPS + (threadIdx.x >> 5);
     if (unit >= (long long)p.B * p.W * p.parts) return;
     const long long r = unit / p.parts;
     const int part = (int)(unit - r * p.parts), first = part * p.per_part, last = min(first + p.per_part, p.segments);
     const long long row = r / p.W * p.sb + r % p.W * p.sw;
-    const int skip = (int)((reinterpret_cast<uintptr_t>(p.logits) + row * (F32 ? 4 : 2)) & 15);
     float* seg_max = p.seg_max + r * p.segments;
     float m = NEG_INF, s = 0.f;
     if (p.finished && p.finished[r]) {  // goes on with eos alone, at no cost
@@ -93,31 +181,9 @@ template <bool F32, bool ALIGNED> __global__ void __launch_bounds__(32 * SCAN_WA
             if (lane == 0) seg_max[g] = here ? 0.f : NEG_INF;
         }
     } else {
-        constexpr int AHEAD = 4;
-        for (int g0 = first; g0 < last; g0 += AHEAD) {
-            Raw<F32, ALIGNED> raw[AHEAD];
-            bool whole[AHEAD];
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) whole[i] = g0 + i < last && raw[i].load(p.logits, row, (g0 + i) * SEG + 8 * lane, p.V);
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                if (g0 + i >= last) break;
-                float f[8];
-                if (whole[i]) raw[i].take(skip, f);
-                else load_edge<F32>(p.logits, row, (g0 + i) * SEG + 8 * lane, p.V, f);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = sane(f[e]);
-                const float top = warp_max(fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7]))));
-                if (lane == 0) seg_max[g0 + i] = top;
-                if (top > m) {  // (the warp's maximum: all lanes take the same way)
-                    s *= ex2_approx((m - top) * 1.4426950408889634f);
-                    m = top;
-                }
-                if (m == NEG_INF) continue;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s += ex2_approx((f[e] - m) * 1.4426950408889634f);
-            }
-        }
+        scan_part<F32, ALIGNED, false>(p, row, first, last, seg_max, ring, lane, m, s);
+        // (a NaN, which maxima pass over, is in some lane's sum; +inf and rows of the type's lowest value are far out)
+        if (__any_sync(0xffffffffu, s != s) || (m != NEG_INF && !(fabsf(m) < FAR_OUT))) scan_part<F32, false, true>(p, row, first, last, seg_max, ring, lane, m, s);
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
@@ -130,33 +196,35 @@ template <bool F32, bool ALIGNED> __global__ void __launch_bounds__(32 * SCAN_WA
 constexpr int PICK_THREADS = 1024, CAP = 256, LIST = PICK_THREADS + BEAM_MAX_K;
 struct Pick {
     double top[BEAM_MAX_W], logz[BEAM_MAX_W], base[BEAM_MAX_W];  // a beam's largest logit, log sum exp(l - top), score
+    float offset[BEAM_MAX_W], least[BEAM_MAX_W];                 // about base - top - logz; the least logit that may reach the threshold
     double score[LIST];
     uint32_t index[LIST];
-    uint32_t segs[CAP];
+    int2 segs[CAP];        // beam, segment
+    uint32_t group[128];   // the best of each group of threads
     unsigned char fin[BEAM_MAX_W];
     double best_score[32];
     uint32_t best_index[32];
     double out_score[BEAM_MAX_K];
     uint32_t out_index[BEAM_MAX_K];
-    int nsegs, n, kept;
+    int nsegs, n;
+    float t;
     unsigned char ruled_out[2 * BEAM_MAX_K];
 };
 __device__ __forceinline__ bool better(double a, uint32_t i, double b, uint32_t j) { return a > b || (a == b && i < j); }
 __device__ __forceinline__ double score_of(const Pick& q, int w, float l) { return l == NEG_INF ? (double)NEG_INF : q.base[w] + (((double)l - q.top[w]) - q.logz[w]); }
 
-// eight adjacent candidates of beam w: their scores
-__device__ __forceinline__ void scores8(const BeamParams& p, const Pick& q, long long seq, int w, int at, double (&s)[8]) {
-    float f[8];
+// eight adjacent candidates of beam w: their logits, as far as they count
+__device__ __forceinline__ void logits8(const BeamParams& p, const Pick& q, long long seq, int w, int at, float (&f)[8]) {
     if (q.fin[w]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = at + i == p.eos ? 0.f : NEG_INF;
-    } else {
-        const long long row = seq * p.sb + w * p.sw;
-        if (p.f32) load_edge<true>(p.logits, row, at, p.V, f);
-        else load_edge<false>(p.logits, row, at, p.V, f);
+        return;
     }
+    const long long row = seq * p.sb + w * p.sw;
+    if (p.f32) load_edge<true>(p.logits, row, at, p.V, f);
+    else load_edge<false>(p.logits, row, at, p.V, f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = score_of(q, w, sane(f[i]));
+    for (int i = 0; i < 8; ++i) f[i] = sane(f[i]);
 }
 
 // the k best of q.score[0 .. n), n <= LIST, in order, to the front; all threads.  Each round takes the best that is left.
@@ -208,57 +276,100 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
     __shared__ Pick q;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long seq = blockIdx.x, row0 = seq * p.W;
-    const int k = p.k, total = p.W * p.segments;
-    stream_order();
+    const int k = p.k;
     if (tid == 0) { q.nsegs = 0; q.n = 0; }
+    if (tid < 128) q.group[tid] = 0;
+    stream_order();
+    // warps to a beam, and of a beam's segments those 32 * wide apart to a lane; their maxima are requested here and used behind the normalisers
+    const int wide = p.W < 32 ? 32 / p.W : 1, per_round = 32 / wide;
+    constexpr int HELD = 4;
+    float held[HELD];
+    const int my_w = warp / wide, my_g = warp % wide * 32 + lane;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const int g = my_g + i * 32 * wide;
+        held[i] = my_w < p.W && my_w < per_round && g < p.segments ? p.seg_max[(row0 + my_w) * p.segments + g] : NEG_INF;
+    }
     // the beams' normalisers, a warp each: the parts' sums joined in 64 bits, in a fixed order
     for (int w = warp; w < p.W; w += 32) {
-        const float* part = p.part + 2 * (row0 + w) * p.parts;
-        float m = NEG_INF;
-        for (int i = lane; i < p.parts; i += 32) m = fmaxf(m, part[2 * i]);
+        const float2* part = reinterpret_cast<const float2*>(p.part) + (row0 + w) * p.parts;
+        const float2 mine = lane < p.parts ? part[lane] : make_float2(NEG_INF, 0.f);
+        const float base = p.scores[row0 + w];
+        const unsigned char fin = p.finished ? p.finished[row0 + w] : 0;
+        float m = mine.x;
+        for (int i = lane + 32; i < p.parts; i += 32) m = fmaxf(m, part[i].x);
         m = warp_max(m);
-        double s = 0.;
-        for (int i = lane; i < p.parts; i += 32)
-            if (part[2 * i] != NEG_INF) s += (double)part[2 * i + 1] * exp((double)part[2 * i] - (double)m);
+        double s = mine.x == NEG_INF ? 0. : (double)mine.y * (double)ex2_approx((mine.x - m) * LOG2E);
+        for (int i = lane + 32; i < p.parts; i += 32)
+            if (part[i].x != NEG_INF) s += (double)part[i].y * (double)ex2_approx((part[i].x - m) * LOG2E);
 #pragma unroll
         for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
         if (lane == 0) {
             // (kept apart: in a row of the type's lowest values their sum would lose logz.  A row without a candidate has none that would read them.)
-            q.top[w] = (double)m;
-            q.logz[w] = log(s);
-            q.base[w] = (double)sane(p.scores[row0 + w]);
-            q.fin[w] = p.finished ? p.finished[row0 + w] : 0;
+            const double logz = m == NEG_INF ? 0. : log(s);
+            q.top[w] = m == NEG_INF ? 0. : (double)m;
+            q.logz[w] = logz;
+            q.base[w] = (double)sane(base);
+            q.offset[w] = m == NEG_INF ? NEG_INF : fminf((float)(((double)sane(base) - logz) - (double)m), 3.402823466e38f);
+            q.fin[w] = fin;
         }
     }
     __syncthreads();
-    // the best segment of each thread's, rounded to 32 bits
+    // A threshold that k candidates reach at least: the k-th best of the bests of 32, 64 or 128 groups of segments, two of them or more for each of the k.  A
+    // group has segments of all beams (the best candidates are often of a few), so that some 1.4 k segments reach it as a rule.  The segments' scores in
+    // 32 bits here, less what the roundings may have added.  Candidates at -inf are left to the end.
+    auto at_least = [&](int w, float l) {
+        const float s = l + q.offset[w];
+        return s == NEG_INF ? 0u : ordered(s - 2.4e-7f * (fabsf(l) + fabsf(q.offset[w])));
+    };
+    auto more_segments = [&](auto f) {  // those that are not held
+        if (my_w >= per_round) return;
+        for (int w = my_w, from = my_g + HELD * 32 * wide; w < p.W; w += per_round, from = my_g)
+            for (int g = from; g < p.segments; g += 32 * wide) f(w, g, p.seg_max[(row0 + w) * p.segments + g]);
+    };
     uint32_t best = 0;
-    for (int g = tid; g < total; g += PICK_THREADS) best = max(best, ordered((float)score_of(q, g / p.segments, p.seg_max[row0 * p.segments + g])));
-    // the largest t that k threads reach, bit by bit; fewer steps where somewhat more than k do.  Candidates at -inf are left to the end.
-    uint32_t t = 0;
-    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-        const int c = __syncthreads_count(best >= (t | bit));
-        if (c >= k) t |= bit;
-        if (c >= k && c <= 2 * k) break;
+    if (my_w < p.W && my_w < per_round)
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) best = max(best, at_least(my_w, held[i]));
+    more_segments([&](int w, int, float l) { best = max(best, at_least(w, l)); });
+    const int groups = k <= 16 ? 32 : k <= 32 ? 64 : 128;
+    atomicMax(&q.group[tid & (groups - 1)], best);
+    __syncthreads();
+    for (int g = warp; g < groups; g += 32) {  // a group's place among them
+        const uint32_t mine = q.group[g];
+        int ahead = 0;
+        for (int i = lane; i < groups; i += 32) ahead += __popc(__ballot_sync(0xffffffffu, q.group[i] > mine || (q.group[i] == mine && i < g)));
+        if (ahead == k - 1 && lane == 0) q.t = mine ? unordered(mine) : -3.402823466e38f;
     }
-    t = max(t, ordered(NEG_INF) + 1);
-    for (int g = tid; g < total; g += PICK_THREADS)
-        if (ordered((float)score_of(q, g / p.segments, p.seg_max[row0 * p.segments + g])) >= t) {
+    __syncthreads();
+    // score >= t is l >= (t - base + logz) + top, less a little for the roundings on the way
+    if (tid < p.W) {
+        const double t = q.t, l = ((t - q.base[tid]) + q.logz[tid]) + q.top[tid];
+        q.least[tid] = __double2float_rd(l - 1e-15 * (fabs(t) + fabs(q.base[tid]) + fabs(q.top[tid]) + 64.));
+    }
+    __syncthreads();
+    auto list_segment = [&](int w, int g, float l) {
+        if (l >= q.least[w] && l > NEG_INF) {
             const int i = atomicAdd(&q.nsegs, 1);
-            if (i < CAP) q.segs[i] = g;
+            if (i < CAP) q.segs[i] = make_int2(w, g);
         }
+    };
+    if (my_w < p.W && my_w < per_round)
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) list_segment(my_w, my_g + i * 32 * wide, held[i]);
+    more_segments(list_segment);
     __syncthreads();
     const int nsegs = q.nsegs;
     if (nsegs <= CAP) {
         for (int i = warp; i < nsegs; i += 32) {
-            const int w = q.segs[i] / p.segments, at = (q.segs[i] - w * p.segments) * SEG + 8 * lane;
-            double s[8];
-            scores8(p, q, seq, w, at, s);
+            const int w = q.segs[i].x, at = q.segs[i].y * SEG + 8 * lane;
+            float l[8];
+            logits8(p, q, seq, w, at, l);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (ordered((float)s[e]) >= t) {
+                if (l[e] >= q.least[w] && (float)score_of(q, w, l[e]) > NEG_INF) {
                     const int j = atomicAdd(&q.n, 1);
-                    if (j < CAP) { q.score[j] = s[e]; q.index[j] = w * p.V + at + e; }
+                    if (j < CAP) { q.score[j] = score_of(q, w, l[e]); q.index[j] = w * p.V + at + e; }
                 }
         }
         __syncthreads();
@@ -266,12 +377,12 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
     int n = q.n;
     if (nsegs <= CAP && n <= CAP) {
         // each candidate's place is the number of better ones
-        if (tid < n) {
-            const double s = q.score[tid];
-            const uint32_t ix = q.index[tid];
+        for (int c = warp; c < n; c += 32) {
+            const double s = q.score[c];
+            const uint32_t ix = q.index[c];
             int place = 0;
-            for (int i = 0; i < n; ++i) place += better(q.score[i], q.index[i], s, ix);
-            if (place < k) { q.out_score[place] = s; q.out_index[place] = ix; }
+            for (int i = lane; i < (n + 31) / 32 * 32; i += 32) place += __popc(__ballot_sync(0xffffffffu, i < n && better(q.score[i], q.index[i], s, ix)));
+            if (place < k && lane == 0) { q.out_score[place] = s; q.out_index[place] = ix; }
         }
         n = min(n, k);
     } else {
@@ -286,17 +397,19 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
             if (tid < PICK_THREADS / 8) {
                 const long long c = c0 + tid;
                 const int g = (int)(c / (SEG / 8));
-                if (g < total) {
+                if (g < p.W * p.segments) {
                     const int w = g / p.segments, at = (g - w * p.segments) * SEG + 8 * (int)(c % (SEG / 8));
-                    if (ordered((float)score_of(q, w, p.seg_max[row0 * p.segments + g])) >= t) {
-                        double s[8];
-                        scores8(p, q, seq, w, at, s);
+                    const float l = p.seg_max[row0 * p.segments + g];
+                    if (l >= q.least[w] && l > NEG_INF) {
+                        float f[8];
+                        logits8(p, q, seq, w, at, f);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const uint32_t ix = (uint32_t)(w * p.V + at + e);
-                            if (ordered((float)s[e]) >= t && (kept < k || better(s[e], ix, q.score[k - 1], q.index[k - 1]))) {
+                            const double s = score_of(q, w, f[e]);
+                            if (f[e] >= q.least[w] && (float)s > NEG_INF && (kept < k || better(s, ix, q.score[k - 1], q.index[k - 1]))) {
                                 const int j = kept + atomicAdd(&q.n, 1);
-                                q.score[j] = s[e];
+                                q.score[j] = s;
                                 q.index[j] = ix;
                             }
                         }
@@ -415,11 +528,9 @@ template <int K> __global__ void __launch_bounds__(RE_THREADS) reorder_kernel(co
 
 // ---- host ------------------------------------------------------------------------------------------------------
 static void beam_plan(long long B, long long W, long long V, int& segments, int& per_part, int& parts) {
-    segments = (int)((V + beam::SEG - 1) / beam::SEG);
-    // a warp takes up to eight segments, fewer while the SMs (148, 32 warps each) are not full of warps
-    const long long all = B * W * segments;
-    per_part = 8;
-    while (per_part > 1 && all / per_part < 148 * 32) per_part /= 2;
+    segments = (int)((V + beam::SEG - 1) / beam::SEG + 3) / 4 * 4;  // (those behind the row's end hold -inf)
+    // a warp takes four segments, or eight, where that still gives every place on the SMs (148, 32 warps each) two
+    per_part = B * W * segments / 16 >= 2 * 148 * 32 ? 16 : B * W * segments / 8 >= 2 * 148 * 32 ? 8 : 4;
     parts = (segments + per_part - 1) / per_part;
 }
 size_t beam_workspace_bytes(long long B, long long W, long long V) {
@@ -437,7 +548,11 @@ int launch_beam_select(BeamParams p, void* workspace, cudaStream_t stream) {
     const bool aligned = (((uintptr_t)p.logits | p.sb * size | p.sw * size) & 15) == 0;
     auto scan = p.f32 ? aligned ? beam::beam_scan_kernel<true, true> : beam::beam_scan_kernel<true, false>
                       : aligned ? beam::beam_scan_kernel<false, true> : beam::beam_scan_kernel<false, false>;
-    if (!launch(scan, dim3((unsigned)ctas), 32 * beam::SCAN_WARPS, 0, stream, p)) return kLaunchFailed;
+    const int stage = p.f32 ? aligned ? beam::stage_bytes<true, true>() : beam::stage_bytes<true, false>()
+                            : aligned ? beam::stage_bytes<false, true>() : beam::stage_bytes<false, false>();
+    const int smem = beam::SCAN_WARPS * beam::DEPTH * stage;
+    if (cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return kLaunchFailed;
+    if (!launch(scan, dim3((unsigned)ctas), 32 * beam::SCAN_WARPS, smem, stream, p)) return kLaunchFailed;
     return launch(beam::beam_pick_kernel, dim3((unsigned)p.B), beam::PICK_THREADS, 0, stream, p) ? kOk : kLaunchFailed;
 }
 

@@ -35,6 +35,11 @@ __device__ __forceinline__ float tanh_f(float x) {
 }
 constexpr float GELU_C = 1.5957691216057308f;  // 2 sqrt(2 / pi): gelu(x) = x sigmoid(GELU_C (x + 0.044715 x^3))
 __device__ __forceinline__ float gelu_s(float x) { return sigmoid_f(GELU_C * x * (1.f + 0.044715f * x * x)); }
+__device__ __forceinline__ float sqrt_f(float x) {  // relative error 2^-23
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ float relu_f(float x) { return x < 0.f ? 0.f : x; }  // (a NaN stays one)
 
 __device__ __forceinline__ void act8(int act, float (&f)[8]) {
@@ -70,7 +75,7 @@ __device__ __forceinline__ void act8(int act, float (&f)[8]) {
 template <int ACT, bool FROM_Y> __device__ __forceinline__ float act_grad(float z) {
     switch (ACT) {
         case kActRelu: return z > 0.f ? 1.f : 0.f;
-        case kActRelu2: return FROM_Y ? 2.f * sqrtf(z) : 2.f * relu_f(z);
+        case kActRelu2: return FROM_Y ? 2.f * sqrt_f(z) : 2.f * relu_f(z);
         case kActTanh: { const float e = ex2_approx(-2.f * LOG2E * fabsf(z)), r = rcp_mufu(1.f + e); return 4.f * e * r * r; }
         case kActSigmoid: { const float s = sigmoid_f(z); return s * (1.f - s); }
         case kActSilu: { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }
@@ -92,6 +97,23 @@ __device__ __forceinline__ void load8g(const void* base, bool f32, long long at,
         f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
     } else {
         unpack8(*reinterpret_cast<const uint4*>((const bf16*)base + at), f);
+    }
+}
+// the same in two steps, for several rows requested at once
+struct Words8 { uint4 lo, hi; };
+__device__ __forceinline__ Words8 request8(const void* base, bool f32, long long at) {
+    const uint4* p = reinterpret_cast<const uint4*>((const unsigned char*)base + at * (f32 ? 4 : 2));
+    Words8 w;
+    w.lo = p[0];
+    w.hi = f32 ? p[1] : w.lo;
+    return w;
+}
+__device__ __forceinline__ void floats8(const Words8& w, bool f32, float (&f)[8]) {
+    if (f32) {
+        f[0] = __uint_as_float(w.lo.x); f[1] = __uint_as_float(w.lo.y); f[2] = __uint_as_float(w.lo.z); f[3] = __uint_as_float(w.lo.w);
+        f[4] = __uint_as_float(w.hi.x); f[5] = __uint_as_float(w.hi.y); f[6] = __uint_as_float(w.hi.z); f[7] = __uint_as_float(w.hi.w);
+    } else {
+        unpack8(w.lo, f);
     }
 }
 __device__ __forceinline__ float load1g(const void* base, bool f32, long long at) {
@@ -567,14 +589,19 @@ template <int ACT, bool FROM_Y> __global__ void __launch_bounds__(DZ_THREADS) li
         const bool whole = p.vec && col + 8 <= p.N;
         long long m = lo + r;
         for (; whole && m + 8 * (DZ_AHEAD - 1) < hi; m += 8 * DZ_AHEAD) {
-            float d[DZ_AHEAD][8], z[DZ_AHEAD][8];
+            Words8 dw[DZ_AHEAD], zw[DZ_AHEAD];
 #pragma unroll
             for (int a = 0; a < DZ_AHEAD; ++a) {
-                load8g(p.dy, p.dy_f32, (m + 8 * a) * p.lddy + col, d[a]);
-                if (ACT) load8g(p.saved, p.saved_f32, (m + 8 * a) * p.lds + col, z[a]);
+                dw[a] = request8(p.dy, p.dy_f32, (m + 8 * a) * p.lddy + col);
+                if (ACT) zw[a] = request8(p.saved, p.saved_f32, (m + 8 * a) * p.lds + col);
             }
 #pragma unroll
-            for (int a = 0; a < DZ_AHEAD; ++a) row(m + 8 * a, d[a], z[a]);
+            for (int a = 0; a < DZ_AHEAD; ++a) {
+                float d[8], z[8];
+                floats8(dw[a], p.dy_f32, d);
+                if (ACT) floats8(zw[a], p.saved_f32, z);
+                row(m + 8 * a, d, z);
+            }
         }
         for (; m < hi; m += 8) {
             float d[8], z[8];
