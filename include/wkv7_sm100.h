@@ -288,7 +288,9 @@ int wkv7_proj_gemm_group_ld(int count, const void* const* A, const void* const* 
  * with WKV7_LINEAR_F32_BIAS, or null; residual [M,N] of y's type, or null (may be y itself).  K, ldx and ldw multiples of 8, x and w 16-byte
  * aligned (bulk tensor copies); any M >= 0, N > 0, any ldr, ldy >= N.  z: null, or [M,N] bf16, fp32 with
  * WKV7_LINEAR_F32_Z, with rows ldz apart (a multiple of 8, 16-byte aligned), where the activation's argument goes for the backward; the columns between N and the next multiple of 8 may be written.
- * tcgen05 products, fp32 accumulation; Results are the same from call to call.  May report
+ * tcgen05 products, fp32 accumulation; Results are the same from call to call.  workspace:
+ * wkv7_linear_fwd_workspace_bytes(M, N, K) bytes of device scratch with the call's device current (0: none), 16-byte aligned, overwritten; null: the
+ * tiles of the last round are not shared out (slower by up to a quarter).  May report
  * WKV7_ERR_DEVICE_TIMEOUT through the status word (bounded waits).
  */
 #define WKV7_ACT_NONE 0
@@ -302,15 +304,17 @@ int wkv7_proj_gemm_group_ld(int count, const void* const* A, const void* const* 
 #define WKV7_LINEAR_F32_BIAS 2
 #define WKV7_LINEAR_FROM_Y 4
 #define WKV7_LINEAR_F32_Z 8
+int64_t wkv7_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int wkv7_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, int64_t M, int64_t N, int64_t K,
-                    int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int64_t ldz, int act, int flags, void* stream);
+                    int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int64_t ldz, int act, int flags, void* workspace, void* stream);
 /*
  * Its backward: dz = dy act'(z), dx = dz w [M,K] bf16, dw = dz^T x [N,K] bf16, dbias = column sums of dz [N] fp32; each of the three may be null.
  * (The residual's gradient is dy.)  dy [M,N] of y's type, rows lddy apart.  saved: z as wkv7_linear_fwd wrote it (WKV7_LINEAR_F32_Z: fp32), rows lds apart; with
  * WKV7_LINEAR_FROM_Y (WKV7_ACT_RELU and _RELU2, bf16 y, no residual) y itself; not read with WKV7_ACT_NONE.  dz is rounded to bf16 for the
- * products, not for dbias.  No atomics: results are the same from call to call.  workspace: wkv7_linear_bwd_workspace_bytes(M, N) bytes, 16-byte aligned.
+ * products, not for dbias.  No atomics: results are the same from call to call.  workspace: wkv7_linear_bwd_workspace_bytes(M, N, K) bytes, 16-byte
+ * aligned, asked for with the call's device current.
  */
-int64_t wkv7_linear_bwd_workspace_bytes(int64_t M, int64_t N);
+int64_t wkv7_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void* dy, void* dx, void* dw, float* dbias, int64_t M, int64_t N, int64_t K,
                     int64_t ldx, int64_t ldw, int64_t lds, int64_t lddy, int act, int flags, void* workspace, void* stream);
 

@@ -13,8 +13,8 @@ def lib():
     return _lib.lib()
 
 
-def fwd(lib, M=4, N=16, K=64, ldx=64, ldw=64, ldr=16, ldy=16, ldz=16, act=0, flags=0, x=0x1000, w=0x1000, bias=None, r=None, y=0x1000, z=None):
-    return lib.wkv7_linear_fwd(x, w, bias, r, y, z, M, N, K, ldx, ldw, ldr, ldy, ldz, act, flags, None)
+def fwd(lib, M=4, N=16, K=64, ldx=64, ldw=64, ldr=16, ldy=16, ldz=16, act=0, flags=0, x=0x1000, w=0x1000, bias=None, r=None, y=0x1000, z=None, ws=None):
+    return lib.wkv7_linear_fwd(x, w, bias, r, y, z, M, N, K, ldx, ldw, ldr, ldy, ldz, act, flags, ws, None)
 
 
 def bwd(lib, M=4, N=16, K=64, lds=16, lddy=16, act=2, flags=0, saved=0x1000, dy=0x1000, dx=0x1000, dw=0x1000, db=None, ws=0x1000):
@@ -27,7 +27,7 @@ def test_forward_checks(lib):
     assert fwd(lib, ldx=56) == fwd(lib, ldw=56) == fwd(lib, ldy=15) == fwd(lib, r=0x1000, ldr=15) == -1
     assert fwd(lib, N=17, ldy=17, z=0x1000, ldz=17) == -1                     # z's rows hold the next multiple of 8
     assert fwd(lib, K=60) == fwd(lib, ldx=68) == fwd(lib, ldw=68) == -4
-    assert fwd(lib, x=0x1008) == fwd(lib, w=0x1008) == fwd(lib, y=0x1001) == fwd(lib, r=0x1001) == fwd(lib, z=0x1008) == -4
+    assert fwd(lib, x=0x1008) == fwd(lib, w=0x1008) == fwd(lib, y=0x1001) == fwd(lib, r=0x1001) == fwd(lib, z=0x1008) == fwd(lib, ws=0x1008) == -4
     assert fwd(lib, flags=1, y=0x1002) == fwd(lib, flags=2, bias=0x1002) == -4
     assert fwd(lib, x=None) == fwd(lib, w=None) == fwd(lib, y=None) == -6
     assert fwd(lib, M=1 << 31) == fwd(lib, ldx=1 << 31) == -8
@@ -40,9 +40,9 @@ def test_backward_checks(lib):
     assert bwd(lib, dy=None) == bwd(lib, saved=None) == bwd(lib, ws=None) == -6
     assert bwd(lib, dx=0x1008) == bwd(lib, dw=0x1008) == bwd(lib, ws=0x1008) == bwd(lib, db=0x1002) == bwd(lib, saved=0x1001) == -4
     assert bwd(lib, M=0, dx=None, dw=None) == 0
-    assert lib.wkv7_linear_bwd_workspace_bytes(0, 5) == lib.wkv7_linear_bwd_workspace_bytes(-1, 5) == 0
+    assert lib.wkv7_linear_bwd_workspace_bytes(0, 5, 8) == lib.wkv7_linear_bwd_workspace_bytes(-1, 5, 8) == lib.wkv7_linear_fwd_workspace_bytes(0, 5, 8) == 0
     for M, N in ((1, 1), (333, 77), (70000, 5)):
-        assert lib.wkv7_linear_bwd_workspace_bytes(M, N) >= M * ((N + 7) // 8 * 8) * 2 + 4 * N
+        assert lib.wkv7_linear_bwd_workspace_bytes(M, N, 64) >= M * ((N + 7) // 8 * 8) * 2 + 4 * N
 
 
 def test_python_refusals(lib):

@@ -445,12 +445,12 @@ static int linear_check(const void* x, const void* w, int64_t M, int64_t N, int6
 }
 
 int wkv7_linear_fwd(const void* x, const void* w, const void* bias, const void* residual, void* y, void* z, int64_t M, int64_t N, int64_t K,
-                    int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int64_t ldz, int act, int flags, void* stream) {
+                    int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int64_t ldz, int act, int flags, void* workspace, void* stream) {
     int rc = linear_check(x, w, M, N, K, ldx, ldw, act, flags, WKV7_LINEAR_F32_OUT | WKV7_LINEAR_F32_BIAS | WKV7_LINEAR_F32_Z);
     if (rc) return rc;
     const int64_t n8 = (N + 7) / 8 * 8;
     if (ldy < N || (residual && ldr < N) || (z && ldz < n8)) return WKV7_ERR_SHAPE;
-    if (z && (ldz % 8 != 0 || !aligned16(z))) return WKV7_ERR_ALIGN;
+    if ((z && (ldz % 8 != 0 || !aligned16(z))) || !aligned16(workspace)) return WKV7_ERR_ALIGN;
     if (M == 0) return WKV7_OK;
     if (!y) return WKV7_ERR_NULL;
     const uintptr_t ysize = flags & WKV7_LINEAR_F32_OUT ? 4 : 2, bsize = flags & WKV7_LINEAR_F32_BIAS ? 4 : 2;
@@ -458,14 +458,19 @@ int wkv7_linear_fwd(const void* x, const void* w, const void* bias, const void* 
     int* status = status_ptr();
     if (!status) return WKV7_ERR_LAUNCH;
     const wkv7::LinearEpilogue e{bias, residual, y, z, ldr, ldy, ldz, M, N, act, bsize == 4, ysize == 4, (flags & WKV7_LINEAR_F32_Z) != 0};
-    return wkv7::launch_linear({x, ldx, false}, {w, ldw, false}, K, e, status, (cudaStream_t)stream);
+    return wkv7::launch_linear({x, ldx, false}, {w, ldw, false}, K, e, workspace, status, (cudaStream_t)stream);
 }
+
+int64_t wkv7_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K) { return M <= 0 || N <= 0 || K <= 0 ? 0 : (int64_t)wkv7::linear_workspace_bytes(M, N, K, false); }
 
 static int64_t linear_dz_bytes(int64_t M, int64_t N) { return (M * ((N + 7) / 8 * 8) * 2 + 15) / 16 * 16; }
 
-int64_t wkv7_linear_bwd_workspace_bytes(int64_t M, int64_t N) {
-    if (M <= 0 || N <= 0) return 0;
-    return linear_dz_bytes(M, N) + (int64_t)wkv7::linear_dz_chunks(M, N) * N * 4;
+// dz, the chunks' sums for dbias, and the scratch of the two products, which follow one another
+static int64_t linear_sums_bytes(int64_t M, int64_t N) { return ((int64_t)wkv7::linear_dz_chunks(M, N) * N * 4 + 15) / 16 * 16; }
+int64_t wkv7_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    const size_t a = wkv7::linear_workspace_bytes(M, K, N, false), b = wkv7::linear_workspace_bytes(N, K, M, true);
+    return linear_dz_bytes(M, N) + linear_sums_bytes(M, N) + (int64_t)(a > b ? a : b);
 }
 
 int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void* dy, void* dx, void* dw, float* dbias, int64_t M, int64_t N, int64_t K,
@@ -497,14 +502,15 @@ int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void*
             if (rc) return rc;
         }
     }
+    void* const scratch = (char*)workspace + linear_dz_bytes(M, N) + linear_sums_bytes(M, N);
     if (dx) {
         const wkv7::LinearEpilogue e{nullptr, nullptr, dx, nullptr, 0, K, 0, M, K, 0, false, false, false};
-        rc = wkv7::launch_linear(dz, {w, ldw, true}, N, e, status, s);
+        rc = wkv7::launch_linear(dz, {w, ldw, true}, N, e, scratch, status, s);
         if (rc) return rc;
     }
     if (dw) {
         const wkv7::LinearEpilogue e{nullptr, nullptr, dw, nullptr, 0, K, 0, N, K, 0, false, false, false};
-        rc = wkv7::launch_linear({dz.p, dz.ld, true}, {x, ldx, true}, M, e, status, s);
+        rc = wkv7::launch_linear({dz.p, dz.ld, true}, {x, ldx, true}, M, e, scratch, status, s);
     }
     return rc;
 }

@@ -42,33 +42,15 @@ __device__ __forceinline__ float sqrt_f(float x) {  // relative error 2^-23
 }
 __device__ __forceinline__ float relu_f(float x) { return x < 0.f ? 0.f : x; }  // (a NaN stays one)
 
-__device__ __forceinline__ void act8(int act, float (&f)[8]) {
-    switch (act) {
-        case kActRelu:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = relu_f(f[i]);
-            break;
-        case kActRelu2:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { f[i] = relu_f(f[i]); f[i] *= f[i]; }
-            break;
-        case kActTanh:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = tanh_f(f[i]);
-            break;
-        case kActSigmoid:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = sigmoid_f(f[i]);
-            break;
-        case kActSilu:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] *= sigmoid_f(f[i]);
-            break;
-        case kActGelu:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] *= gelu_s(f[i]);
-            break;
-        default: break;
+template <int ACT> __device__ __forceinline__ float act(float x) {
+    switch (ACT) {
+        case kActRelu: return relu_f(x);
+        case kActRelu2: { const float r = relu_f(x); return r * r; }
+        case kActTanh: return tanh_f(x);
+        case kActSigmoid: return sigmoid_f(x);
+        case kActSilu: return x * sigmoid_f(x);
+        case kActGelu: return x * gelu_s(x);
+        default: return x;
     }
 }
 // act'(z); FROM_Y: of relu and relu2 from their values, 2 sqrt(y) for 2 relu(z)
@@ -89,7 +71,8 @@ template <int ACT, bool FROM_Y> __device__ __forceinline__ float act_grad(float 
 
 // ---- epilogue --------------------------------------------------------------------------------------------
 struct Epi : LinearEpilogue {
-    bool vec;  // rows of y and of the residual start on 16-byte boundaries
+    bool vec;       // rows of y and of the residual start on 16-byte boundaries
+    bool bias_vec;  // so does the bias
 };
 __device__ __forceinline__ void load8g(const void* base, bool f32, long long at, float (&f)[8]) {
     if (f32) {
@@ -131,11 +114,21 @@ __device__ __forceinline__ void store8g(void* base, bool f32, long long at, cons
         *reinterpret_cast<uint4*>((bf16*)base + at) = pack8(f);
     }
 }
+// the bias of eight adjacent columns
+__device__ __forceinline__ void bias8(const Epi& e, long long col, float (&f)[8]) {
+    if (e.bias_vec && col + 8 <= e.cols) {
+        load8g(e.bias, e.bias_f32, col, f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = col + i < e.cols ? load1g(e.bias, e.bias_f32, col + i) : 0.f;
+    }
+}
 // eight adjacent columns of a row, from the accumulator to memory; bias already added
-__device__ __forceinline__ void finish8(const Epi& e, long long row, long long col, float (&f)[8]) {
+template <int ACT> __device__ __forceinline__ void finish8(const Epi& e, long long row, long long col, float (&f)[8]) {
     const int live = (int)(e.cols - col < 8 ? e.cols - col : 8);
     if (e.z) store8g(e.z, e.z_f32, row * e.ldz + col, f);  // (ldz is a multiple of 8: room for all eight)
-    act8(e.act, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = act<ACT>(f[i]);
     if (e.vec && live == 8) {
         if (e.residual) {
             float r[8];
@@ -146,14 +139,110 @@ __device__ __forceinline__ void finish8(const Epi& e, long long row, long long c
         store8g(e.y, e.y_f32, row * e.ldy + col, f);
         return;
     }
+    if (e.residual) {  // (all of it is read before anything is stored: y may be the residual, so the compiler keeps them in order)
+        float r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = i < live ? load1g(e.residual, e.y_f32, row * e.ldr + col + i) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] += r[i];
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (i < live) {
-            float v = f[i];
-            if (e.residual) v += load1g(e.residual, e.y_f32, row * e.ldr + col + i);
-            if (e.y_f32) ((float*)e.y)[row * e.ldy + col + i] = v;
-            else ((bf16*)e.y)[row * e.ldy + col + i] = __float2bfloat16_rn(v);
+            if (e.y_f32) ((float*)e.y)[row * e.ldy + col + i] = f[i];
+            else ((bf16*)e.y)[row * e.ldy + col + i] = __float2bfloat16_rn(f[i]);
         }
+}
+// A warp's block of 32 rows x 32 columns of y whose rows are not aligned: lane has rows row + 8 it, columns [col, col + 8), taken by read(it, f) behind ready().
+template <int ACT, typename Ready, typename Read> __device__ __forceinline__ void finish_block(const Epi& e, long long row, long long col, Ready ready, Read read) {
+    float bias[8];
+    ready();
+    if (e.bias) bias8(e, col, bias);
+#pragma unroll 1
+    for (int it = 0; it < 4; ++it) {
+        float f[8];
+        read(it, f);
+        if (e.bias)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] += bias[i];
+        if (row + 8 * it < e.rows && col < e.cols) finish8<ACT>(e, row + 8 * it, col, f);
+    }
+}
+// A block of 32 x 32 results to memory by a bulk tensor store, which clips it: a lane has a row of it, or (TURNED) a column.  `turn`: which half of the
+// staging area is next (bf16; fp32 takes all of it); it is written again when the store that reads it has.  `all`: wait for all stores, where halves do not alternate.
+template <bool TURNED> __device__ __forceinline__ void bulk_store_block(float* staging, const CUtensorMap* map, bool f32, bool all, const float (&v)[32], int lane, int& turn, long long col0, long long row0) {
+    unsigned char* to = reinterpret_cast<unsigned char*>(staging) + (f32 ? 0 : 2048 * turn);
+    if (lane == 0) {
+        if (f32 || all) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    }
+    __syncwarp();
+    if (f32) {  // rows of 128 bytes, piece u of row r at u ^ (r % 8)
+        if (TURNED) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) *reinterpret_cast<float*>(to + c * 128 + (((lane >> 2) ^ (c & 7)) << 4) + (lane & 3) * 4) = v[c];
+        } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) *reinterpret_cast<float4*>(to + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+        }
+    } else {    // rows of 64 bytes, piece u of row r at u ^ (r / 2 % 4)
+        if (TURNED) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) *reinterpret_cast<bf16*>(to + c * 64 + (((lane >> 3) ^ (c >> 1 & 3)) << 4) + (lane & 7) * 2) = __float2bfloat16_rn(v[c]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                *reinterpret_cast<uint4*>(to + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4)) = make_uint4(pack_bf16x2(v[8 * u], v[8 * u + 1]), pack_bf16x2(v[8 * u + 2], v[8 * u + 3]),
+                                                                                                   pack_bf16x2(v[8 * u + 4], v[8 * u + 5]), pack_bf16x2(v[8 * u + 6], v[8 * u + 7]));
+        }
+        turn ^= 1;
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"((int)col0), "r"((int)row0), "r"(smem_u32(to)) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+}
+
+// A warp's block of 32 x 32, a lane a row of y: the sums come by sums(v), residual and bias are applied as they lie.
+template <int ACT, typename Sums> __device__ __forceinline__ void finish_rows(const Epi& e, const CUtensorMap* Y, const CUtensorMap* Z, float* mine, bool mixed, int lane, int& turn,
+                                                                             long long row0, long long col0, Sums sums) {
+    const bool whole = row0 + lane < e.rows && col0 + 32 <= e.cols;
+    const long long at = (row0 + lane) * e.ldr + col0;
+    Words8 res[4];
+    if (e.residual && whole)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) res[c] = request8(e.residual, e.y_f32, at + 8 * c);
+    float v[32];
+    sums(v);
+    if (e.bias)
+#pragma unroll
+        for (int c = 0; c < 32; c += 8) {
+            float f[8];
+            bias8(e, col0 + c, f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c + i] += f[i];
+        }
+    if (e.z) bulk_store_block<false>(mine, Z, e.z_f32, mixed, v, lane, turn, col0, row0);
+#pragma unroll
+    for (int c = 0; c < 32; ++c) v[c] = act<ACT>(v[c]);
+    if (e.residual) {
+        if (whole) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float f[8];
+                floats8(res[c], e.y_f32, f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[8 * c + i] += f[i];
+            }
+        } else if (row0 + lane < e.rows) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+                if (col0 + c < e.cols) v[c] += load1g(e.residual, e.y_f32, at + c);
+        }
+    }
+    bulk_store_block<false>(mine, Y, e.y_f32, mixed, v, lane, turn, col0, row0);
 }
 
 // ---- tensor core and copy helpers --------------------------------------------------------------------------
@@ -200,9 +289,9 @@ __device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
 
 // ---- tiles of 128 x NT, k split over a cluster ---------------------------------------------------------------
 struct TileParams {
-    CUtensorMap P, Q;
+    CUtensorMap P, Q, Y, Z;  // Y, Z: as the pairs'
     Epi e;
-    int p_mn, q_mn, nt, kblocks, splits, stages, accs, swap, p_tiles;  // swap: P runs over the columns of y, Q over its rows
+    int p_mn, q_mn, nt, kblocks, splits, stages, accs, swap, direct, p_tiles;  // swap: P runs over the columns of y, Q over its rows
     uint32_t tmem_cols;
 };
 struct TileCtrl {
@@ -221,7 +310,7 @@ __host__ __device__ constexpr int part_bytes(int nt) { return BM * part_pitch(nt
 
 __device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
-__global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_constant__ TileParams p, int* status) {
+template <int ACT> __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_constant__ TileParams p, int* status) {
     extern __shared__ unsigned char smem_dyn[];
     TileCtrl* ctrl = reinterpret_cast<TileCtrl*>(smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u));
     unsigned char* sm = reinterpret_cast<unsigned char*>(ctrl) + 1024;
@@ -240,6 +329,10 @@ __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_
         mbar_init(&ctrl->accum, 1); mbar_init(&ctrl->drain, 1);
         ctrl->abort = 0; ctrl->zero = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 4 && elect_one()) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&p.P) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&p.Q) : "memory");
     }
     if (warp == 0) {
         __syncwarp();
@@ -307,6 +400,35 @@ __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_
     if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     else __syncthreads();  // the ring, where the result goes, is read no more, and its last copies have landed
     const int pitch = part_pitch(p.nt), rows = BM / p.splits;
+    if (p.direct) {
+        // nothing to join: from the accumulator to the result
+        if (warp < 4 && !ctrl->abort) {
+            const Epi& e = p.e;
+            const bool mixed = e.z && e.z_f32 != e.y_f32;
+            float* mine = parts + warp * 1024;
+            const uint32_t acc = tmem + ((uint32_t)(32 * warp) << 16);
+            int turn = 0;
+#pragma unroll 1
+            for (int c = 0; c < p.nt; c += 32) {
+                auto sums = [&](float (&v)[32]) {
+                    tmem_ld32(acc + c, reinterpret_cast<uint32_t(&)[32]>(v));
+                    for (int a = 1; a < min(p.accs, hi - lo); ++a) {
+                        float u[32];
+                        tmem_ld32(acc + a * p.nt + c, reinterpret_cast<uint32_t(&)[32]>(u));
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] += u[i];
+                    }
+                };
+                if (p0 + 32 * warp < e.rows && q0 + c < e.cols) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, p0 + 32 * warp, q0 + c, sums);
+            }
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncthreads();
+        if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+        return;
+    }
     if (warp < 4) {
         // a lane has a row of the accumulators and sends it to the CTA that finishes it
         const int row = 32 * warp + lane;
@@ -346,16 +468,18 @@ __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_
                 x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
             }
             const float bias = e.bias ? load1g(e.bias, e.bias_f32, col) : 0.f;
-            float f[8] = {x.x + bias, x.y + bias, x.z + bias, x.w + bias};
-            for (int q = 0; q < 4; ++q)
-                if (e.z && q0 + j + q < e.rows) store_z1(e, q0 + j + q, col, f[q]);
-            act8(e.act, f);
+            const float f[4] = {x.x + bias, x.y + bias, x.z + bias, x.w + bias};
+            float res[4] = {};
+            if (e.residual)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (q0 + j + q < e.rows) res[q] = load1g(e.residual, e.y_f32, (long long)(q0 + j + q) * e.ldr + col);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const long long row = q0 + j + q;
                 if (row >= e.rows) break;
-                float v = f[q];
-                if (e.residual) v += load1g(e.residual, e.y_f32, row * e.ldr + col);
+                if (e.z) store_z1(e, row, col, f[q]);
+                const float v = act<ACT>(f[q]) + res[q];
                 if (e.y_f32) ((float*)e.y)[row * e.ldy + col] = v;
                 else ((bf16*)e.y)[row * e.ldy + col] = __float2bfloat16_rn(v);
             }
@@ -373,26 +497,34 @@ __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_
                 f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
             }
             if (e.bias) {
+                float bias[8];
+                bias8(e, col, bias);
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (col + q < e.cols) f[q] += load1g(e.bias, e.bias_f32, col + q);
+                for (int q = 0; q < 8; ++q) f[q] += bias[q];
             }
-            finish8(e, row, col, f);
+            finish8<ACT>(e, row, col, f);
         }
     }
 }
 
 // ---- pairs of CTAs, persistent ------------------------------------------------------------------------------------
+// A pair takes every pairs-th tile.  What is left when the tiles no longer fill all pairs (`whole` is a multiple of their number) is cut along k, `splits` units
+// to a tile, so that the last round takes a part of a tile's time: each unit writes its sums to the workspace, and of the warps that do so for one block of a tile the
+// last to arrive adds all parts, in their order, and finishes the block.  Nobody waits for another.
 struct PairParams {
-    CUtensorMap P, Q;
+    CUtensorMap P, Q, Y, Z;  // Y, Z: boxes of 32 x 32 for the results' bulk stores, where rows of y are aligned
     Epi e;
-    int p_mn, q_mn, bn, kblocks, p_tiles, q_tiles;
-    long long tiles;
+    int p_mn, q_mn, bn, kblocks, p_tiles, q_tiles, swap, splits;  // swap: P runs over the columns of y, Q over its rows
+    long long tiles, whole;
+    float4* parts;         // [units of the cut tiles][CTA of the pair][warp][block][8][lane]
+    unsigned* arrived;     // [cut tiles][CTA][warp], zero
 };
 constexpr int PAIR_STAGES = 6, PAIR_THREADS = 384;  // warp 0: copies, 1: products, 4-11: epilogue
 constexpr int PAIR_P = BM * 128, PAIR_Q = 128 * 128, PAIR_STAGE = PAIR_P + PAIR_Q;
-constexpr int PAIR_STAGING = 32 * 32 * 4;  // a block of 32 x 32 per epilogue warp
+constexpr int PAIR_STAGING = 32 * 32 * 4;  // a block of 32 x 32 in fp32, or two in bf16, per epilogue warp
 constexpr int BAND = 8;                    // tile rows of 256 that are walked together, column by column, so that concurrent tiles share operands in L2
+constexpr int PART_BLOCKS = 4;             // blocks of 32 columns a warp has of a tile at most
+constexpr int PART_F4 = 2 * 8 * PART_BLOCKS * 8 * 32;  // float4 of a unit
 struct PairCtrl {
     uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], accum_full[2], accum_empty[2], drain;
     uint32_t tmem_base;
@@ -401,15 +533,42 @@ struct PairCtrl {
 constexpr int PAIR_SMEM = 1024 + PAIR_STAGES * PAIR_STAGE + 8 * PAIR_STAGING + (int)sizeof(PairCtrl);
 static_assert(PAIR_SMEM <= 232448, "shared memory of a CTA");
 
-__device__ __forceinline__ void pair_tile(const PairParams& p, long long t, int& pi, int& qi) {
+// the n-th piece of work of a pair
+struct PairWork {
+    int pi, qi, lo, hi;  // tile, k blocks
+    int unit, cut;       // of a cut tile: unit among all, and which of the cut tiles; -1: a whole one
+};
+__device__ __forceinline__ bool pair_work(const PairParams& p, int n, PairWork& w) {
+    const long long pairs = gridDim.x >> 1, pair = blockIdx.x >> 1;
+    long long t = n * pairs + pair;
+    w.lo = 0; w.hi = p.kblocks; w.unit = w.cut = -1;
+    if (t >= p.whole) {
+        const long long u = t - p.whole;  // (whole is a multiple of the number of pairs)
+        if (u >= (p.tiles - p.whole) * p.splits) return false;
+        const int part = (int)(u % p.splits);
+        t = p.whole + u / p.splits;
+        if (p.splits > 1) {
+            w.unit = (int)u;
+            w.cut = (int)(t - p.whole);
+            w.lo = (int)((long long)p.kblocks * part / p.splits);
+            w.hi = (int)((long long)p.kblocks * (part + 1) / p.splits);
+        }
+    }
     const long long per_band = (long long)BAND * p.q_tiles;
     const int band = (int)(t / per_band), rows = min(BAND, p.p_tiles - band * BAND);
     const int r = (int)(t - band * per_band);
-    pi = band * BAND + r % rows;
-    qi = r / rows;
+    w.pi = band * BAND + r % rows;
+    w.qi = r / rows;
+    return true;
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) linear_pair_kernel(const __grid_constant__ PairParams p, int* status) {
+__global__ void __launch_bounds__(256) linear_zero_kernel(unsigned* p, int n) {
+    stream_order();
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = 0;
+}
+
+template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) linear_pair_kernel(const __grid_constant__ PairParams p, int* status) {
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* sm = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
     unsigned char* staging = sm + PAIR_STAGES * PAIR_STAGE;
@@ -417,7 +576,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) lin
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const uint32_t rank = cluster_rank();
-    const long long first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
     if (tid == 0) {
         for (int s = 0; s < PAIR_STAGES; ++s) { mbar_init(&ctrl->full[s], 1); mbar_init(&ctrl->empty[s], 1); }
@@ -425,6 +583,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) lin
         mbar_init(&ctrl->drain, 1);
         ctrl->abort = 0; ctrl->zero = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 3 && elect_one()) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&p.P) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&p.Q) : "memory");
     }
     if (warp == 2) {
         __syncwarp();
@@ -438,6 +600,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) lin
     const uint32_t tmem = ctrl->tmem_base;
     stream_wait();
 
+    PairWork w;
     if (warp == 0) {
         if (elect_one()) {
             const int half = p.bn / 2;
@@ -445,11 +608,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) lin
             int s = 0, round = 0;
             long long issued = 0;
             bool going = true;
-            for (long long t = first; t < p.tiles && going; t += step) {
-                int pi, qi;
-                pair_tile(p, t, pi, qi);
-                const int p0 = pi * 2 * BM + (int)rank * BM, q0 = qi * p.bn + (int)rank * half;
-                for (int kb = 0; kb < p.kblocks; ++kb) {
+            for (int n = 0; going && pair_work(p, n, w); ++n) {
+                const int p0 = w.pi * 2 * BM + (int)rank * BM, q0 = w.qi * p.bn + (int)rank * half;
+                for (int kb = w.lo; kb < w.hi; ++kb) {
                     if (round > 0 && !mbar_wait_bounded<true>(&ctrl->empty[s], (round - 1) & 1, &ctrl->abort, status)) { going = false; break; }
                     // both CTAs' copies count at the first CTA's barrier, whose thread issues the products
                     if (rank == 0) expect_tx(&ctrl->full[s], 2 * (PAIR_P + q_tx));
@@ -481,20 +642,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) lin
             auto commit = [](uint64_t* bar) {
                 asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
             };
-            int s = 0, round = 0, n = 0;
-            for (long long t = first; t < p.tiles; t += step, ++n) {
+            int s = 0, round = 0;
+            for (int n = 0; pair_work(p, n, w); ++n) {
                 const int buf = n & 1;
                 if (n >= 2) mbar_wait_bounded<false>(&ctrl->accum_empty[buf], ((n >> 1) - 1) & 1, &ctrl->abort, status);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t acc = tmem + buf * 256;
-                for (int kb = 0; kb < p.kblocks; ++kb) {
+                for (int kb = w.lo; kb < w.hi; ++kb) {
                     mbar_wait_bounded<false>(&ctrl->full[s], round & 1, &ctrl->abort, status);
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t da = desc_of(smem_u32(sm + s * PAIR_STAGE), p.p_mn), db = desc_of(smem_u32(sm + s * PAIR_STAGE + PAIR_P), p.q_mn);
 #pragma unroll
                     for (int ks = 0; ks < BK / 16; ++ks)
                         asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                                     ::"r"(acc), "l"(da + ks * step_p), "l"(db + ks * step_q), "r"(idesc), "r"((kb > 0 || ks > 0) ? 1u : 0u) : "memory");
+                                     ::"r"(acc), "l"(da + ks * step_p), "l"(db + ks * step_q), "r"(idesc), "r"((kb > w.lo || ks > 0) ? 1u : 0u) : "memory");
                     commit(&ctrl->empty[s]);
                     if (++s == PAIR_STAGES) { s = 0; ++round; }
                 }
@@ -507,54 +668,132 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) lin
         }
         __syncwarp();
     } else if (warp >= 4) {
-        // warps 4-7 take the first half of the tile's columns, 8-11 the second; a warp reads the 32 accumulator rows that it may, 32 columns at a time, and
-        // turns the block in shared memory (16-byte units, unit u of row r at u ^ (r % 8): no conflicts either way), so that four lanes have
-        // 32 adjacent columns of a row: 64 bytes of bf16, two whole sectors a row and instruction
+        // Warps 4-7 take the first half of the tile's Q indices, 8-11 the second; a warp reads the 32 accumulator rows that it may, 32 columns at a time: a lane has
+        // a row of y (swap: a column).  Bias, activation and residual are applied as it lies; the block leaves through shared memory by a bulk tensor store,
+        // whose swizzle (16-byte pieces, xor of the row) spares bank conflicts.  That is 16 wavefronts of shared memory a block of bf16: the operands'
+        // copies and products need all but an eighth of its bandwidth.  (Through shared memory in fp32 and out by 16-byte stores: 64 and the stores'.)
+        // Where rows of y are not aligned the block is turned there in fp32, so that four lanes have 32 adjacent columns of a row.
         const int quarter = warp & 3, side = (warp - 4) >> 2;
-        unsigned char* mine = staging + (warp - 4) * PAIR_STAGING;
+        float* mine = reinterpret_cast<float*>(staging + (warp - 4) * PAIR_STAGING);
+        int turn = 0;
         const Epi& e = p.e;
-        int n = 0;
-        for (long long t = first; t < p.tiles; t += step, ++n) {
-            int pi, qi;
-            pair_tile(p, t, pi, qi);
+        const bool mixed = e.z && e.z_f32 != e.y_f32;
+        const int blocks = p.bn / 32, b0 = side ? (blocks + 1) / 2 : 0, b1 = side ? blocks : (blocks + 1) / 2;
+        for (int n = 0; pair_work(p, n, w); ++n) {
             const int buf = n & 1;
             mbar_wait_bounded<true>(&ctrl->accum_full[buf], (n >> 1) & 1, &ctrl->abort, status);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const bool ok = !ctrl->abort;
-            const long long row0 = (long long)pi * 2 * BM + rank * BM + 32 * quarter;
-            const int blocks = p.bn / 32, b0 = side ? (blocks + 1) / 2 : 0, b1 = side ? blocks : (blocks + 1) / 2;
+            if (ctrl->abort) break;
+            const long long p0 = (long long)w.pi * 2 * BM + rank * BM + 32 * quarter;
+            const uint32_t acc = tmem + buf * 256 + ((uint32_t)(32 * quarter) << 16);
+            auto emptied = [&] {  // the accumulator may be filled again (no memory is handed over: a release would wait for all of this warp's stores, 1600 cycles)
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_rank(smem_u32(&ctrl->accum_empty[buf]), 0)) : "memory");
+            };
+            float4* parts = nullptr;
+            if (w.cut >= 0) {  // this unit's sums to memory; the last of the tile's units goes on
+                parts = p.parts + ((rank * 8 + warp - 4) * PART_BLOCKS) * 256 + lane;
+                float4* to = parts + (long long)w.unit * PART_F4;
+#pragma unroll 1
+                for (int b = b0; b < b1; ++b) {
+                    uint32_t v[32];
+                    tmem_ld32(acc + 32 * b, v);
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        __stcg(to + (b - b0) * 256 + u * 32, make_float4(__uint_as_float(v[4 * u]), __uint_as_float(v[4 * u + 1]), __uint_as_float(v[4 * u + 2]), __uint_as_float(v[4 * u + 3])));
+                }
+                emptied();
+                __threadfence();
+                __syncwarp();
+                unsigned before = 0;
+                if (lane == 0) before = atomicAdd(p.arrived + (w.cut * 2 + rank) * 8 + warp - 4, 1u);
+                if (__shfl_sync(0xffffffffu, before, 0) != (unsigned)p.splits - 1) continue;
+                __threadfence();
+                parts += (long long)w.cut * p.splits * PART_F4;
+            }
 #pragma unroll 1
             for (int b = b0; b < b1; ++b) {
-                uint32_t v[32];
-                tmem_ld32(tmem + buf * 256 + ((uint32_t)(32 * quarter) << 16) + 32 * b, v);
-                if (b == b1 - 1) {  // the accumulator may be filled again
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                const long long q0 = (long long)w.qi * p.bn + 32 * b;
+                const long long row0 = p.swap ? q0 : p0, col0 = p.swap ? p0 : q0;
+                auto sums = [&](float (&v)[32]) {
+                    if (parts) {
+                        const float4* from = parts + (b - b0) * 256;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+#pragma unroll 2
+                        for (int c = 0; c < p.splits; ++c, from += PART_F4) {
+                            float4 x[8];
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) x[u] = __ldcg(from + u * 32);
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) { v[4 * u] += x[u].x; v[4 * u + 1] += x[u].y; v[4 * u + 2] += x[u].z; v[4 * u + 3] += x[u].w; }
+                        }
+                    } else {
+                        tmem_ld32(acc + 32 * b, reinterpret_cast<uint32_t(&)[32]>(v));
+                        if (b == b1 - 1) emptied();
+                    }
+                };
+                if (e.vec) {
+                    if (row0 >= e.rows || col0 >= e.cols) {
+                        if (b == b1 - 1 && !parts) emptied();
+                        continue;
+                    }
+                    if (p.swap) {
+                        float v[32];
+                        const long long col = col0 + lane;
+                        const bool in = col < e.cols;
+                        float res[32];
+                        if (e.residual)
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) res[c] = in && row0 + c < e.rows ? load1g(e.residual, e.y_f32, (row0 + c) * e.ldr + col) : 0.f;
+                        const float bias = e.bias && in ? load1g(e.bias, e.bias_f32, col) : 0.f;
+                        sums(v);
+                        if (e.bias)
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) v[c] += bias;
+                        if (e.z) bulk_store_block<true>(mine, &p.Z, e.z_f32, mixed, v, lane, turn, col0, row0);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) v[c] = act<ACT>(v[c]);
+                        if (e.residual)
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) v[c] += res[c];
+                        bulk_store_block<true>(mine, &p.Y, e.y_f32, mixed, v, lane, turn, col0, row0);
+                    } else {
+                        finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, sums);
+                    }
+                    continue;
+                }
+                const int g = lane & 3, r = lane >> 2;
+                auto ready = [&] {
+                    float v[32];
+                    sums(v);
+                    if (p.swap) {  // element c of row `lane` at c ^ lane, else 16-byte unit u at u ^ (lane % 8): no conflicts either way
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) mine[lane * 32 + (c ^ lane)] = v[c];
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            *reinterpret_cast<float4*>(mine + lane * 32 + ((u ^ (lane & 7)) << 2)) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+                    }
                     __syncwarp();
-                    if (lane == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_rank(smem_u32(&ctrl->accum_empty[buf]), 0)) : "memory");
-                }
+                };
+                auto read = [&](int it, float (&f)[8]) {
+                    if (p.swap) {
 #pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    *reinterpret_cast<uint4*>(mine + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-                __syncwarp();
-                const int g = lane & 3;
-                const long long col = (long long)qi * p.bn + 32 * b + 8 * g;
-                float bias[8] = {};
-                if (e.bias && col < e.cols) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (col + i < e.cols) bias[i] = load1g(e.bias, e.bias_f32, col + i);
-                }
-#pragma unroll
-                for (int it = 0; it < 4; ++it) {
-                    const int r = 8 * it + (lane >> 2);
-                    const float4 x = *reinterpret_cast<const float4*>(mine + r * 128 + (((2 * g) ^ (r & 7)) << 4));
-                    const float4 y = *reinterpret_cast<const float4*>(mine + r * 128 + (((2 * g + 1) ^ (r & 7)) << 4));
-                    float f[8] = {x.x + bias[0], x.y + bias[1], x.z + bias[2], x.w + bias[3], y.x + bias[4], y.y + bias[5], y.z + bias[6], y.w + bias[7]};
-                    if (ok && row0 + r < e.rows && col < e.cols) finish8(e, row0 + r, col, f);
-                }
+                        for (int i = 0; i < 8; ++i) f[i] = mine[(8 * g + i) * 32 + ((8 * it + r) ^ (8 * g + i))];
+                    } else {  // (row 8 it + r)
+                        const float* at = mine + (8 * it + r) * 32;
+                        const float4 x = ld4(at + (((2 * g) ^ r) << 2)), y = ld4(at + (((2 * g + 1) ^ r) << 2));
+                        f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w; f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
+                    }
+                };
+                finish_block<ACT>(e, row0 + r, col0 + 8 * g, ready, read);
                 __syncwarp();
             }
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory must outlive the stores' reads
+        __syncwarp();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -587,31 +826,42 @@ template <int ACT, bool FROM_Y> __global__ void __launch_bounds__(DZ_THREADS) li
             if (p.dz) *reinterpret_cast<uint4*>((bf16*)p.dz + m * p.ldz + col) = pack8(d);  // (ldz is a multiple of 8)
         };
         const bool whole = p.vec && col + 8 <= p.N;
-        long long m = lo + r;
-        for (; whole && m + 8 * (DZ_AHEAD - 1) < hi; m += 8 * DZ_AHEAD) {
-            Words8 dw[DZ_AHEAD], zw[DZ_AHEAD];
+        for (long long m = lo + r; m < hi; m += 8 * DZ_AHEAD) {
+            // (rows behind the chunk: the last one again, not stored and not summed)
+            float d[DZ_AHEAD][8], z[DZ_AHEAD][8];
+            if (whole) {
+                Words8 dw[DZ_AHEAD], zw[DZ_AHEAD];
 #pragma unroll
-            for (int a = 0; a < DZ_AHEAD; ++a) {
-                dw[a] = request8(p.dy, p.dy_f32, (m + 8 * a) * p.lddy + col);
-                if (ACT) zw[a] = request8(p.saved, p.saved_f32, (m + 8 * a) * p.lds + col);
+                for (int a = 0; a < DZ_AHEAD; ++a) {
+                    const long long n = m + 8 * a < hi ? m + 8 * a : m;
+                    dw[a] = request8(p.dy, p.dy_f32, n * p.lddy + col);
+                    if (ACT) zw[a] = request8(p.saved, p.saved_f32, n * p.lds + col);
+                }
+#pragma unroll
+                for (int a = 0; a < DZ_AHEAD; ++a) {
+                    floats8(dw[a], p.dy_f32, d[a]);
+                    if (ACT) floats8(zw[a], p.saved_f32, z[a]);
+                }
+            } else {
+#pragma unroll
+                for (int a = 0; a < DZ_AHEAD; ++a) {
+                    const long long n = m + 8 * a < hi ? m + 8 * a : m;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const long long c = col + i < p.N ? col + i : p.N - 1;  // (columns behind the last: that one again, and zero)
+                        d[a][i] = load1g(p.dy, p.dy_f32, n * p.lddy + c);
+                        if (ACT) z[a][i] = load1g(p.saved, p.saved_f32, n * p.lds + c);
+                    }
+                }
+#pragma unroll
+                for (int a = 0; a < DZ_AHEAD; ++a)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (col + i >= p.N) d[a][i] = 0.f;
             }
 #pragma unroll
-            for (int a = 0; a < DZ_AHEAD; ++a) {
-                float d[8], z[8];
-                floats8(dw[a], p.dy_f32, d);
-                if (ACT) floats8(zw[a], p.saved_f32, z);
-                row(m + 8 * a, d, z);
-            }
-        }
-        for (; m < hi; m += 8) {
-            float d[8], z[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool in = col + i < p.N;
-                d[i] = in ? load1g(p.dy, p.dy_f32, m * p.lddy + col + i) : 0.f;
-                z[i] = in && ACT ? load1g(p.saved, p.saved_f32, m * p.lds + col + i) : 0.f;
-            }
-            row(m, d, z);
+            for (int a = 0; a < DZ_AHEAD; ++a)
+                if (m + 8 * a < hi) row(m + 8 * a, d[a], z[a]);
         }
     }
     if (!p.dbias) return;
@@ -666,7 +916,40 @@ static bool encode(CUtensorMap* m, const LinearOperand& o, long long n, long lon
     return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(o.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// results: boxes of 32 columns x 32 rows
+static bool encode_out(CUtensorMap* m, const void* p, bool f32, long long rows, long long cols, long long ld) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * (f32 ? 4 : 2)};
+    const cuuint32_t box[2] = {32, 32}, es[2] = {1, 1};
+    return fn(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 static bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static bool encode_results(const Epi& e, CUtensorMap* Y, CUtensorMap* Z) {
+    return encode_out(Y, e.y, e.y_f32, e.rows, e.cols, e.ldy) && (!e.z || encode_out(Z, e.z, e.z_f32, e.rows, e.cols, e.ldz));
+}
+
+// Shared memory beyond 48 KB has to be allowed once per kernel and device.  A thread's first call on a device (one of autograd's may have made no other) does so again:
+// that gives it the context which encoding a tensor map needs.
+template <typename K> static bool allow_smem(K kern, int which, int bytes) {
+    static thread_local uint32_t done[64];
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return false;
+    if (dev < 64 && (done[dev] >> which & 1)) return true;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    if (dev < 64) done[dev] |= 1u << which;
+    return true;
+}
+template <typename P> struct Kernels { void (*k[kActs])(P, int*); };
+#define WKV7_PER_ACT(kernel) {{kernel<kActNone>, kernel<kActRelu>, kernel<kActRelu2>, kernel<kActTanh>, kernel<kActSigmoid>, kernel<kActSilu>, kernel<kActGelu>}}
+static const Kernels<TileParams> tile_kernels = WKV7_PER_ACT(linear_tile_kernel);
+static const Kernels<PairParams> pair_kernels = WKV7_PER_ACT(linear_pair_kernel);
 
 template <typename P> static bool launch_cluster(void (*kern)(P, int*), unsigned grid, unsigned threads, int smem, int cluster, cudaStream_t stream, const P& p, int* status) {
     cudaLaunchConfig_t c{};
@@ -686,13 +969,15 @@ template <typename P> static bool launch_cluster(void (*kern)(P, int*), unsigned
 }
 
 static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb, long long k, const Epi& e, bool swap, int nt, int splits, int* status, cudaStream_t stream) {
-    // (first of all: it gives a thread that has made no other call yet, one of autograd's, the context that encoding a tensor map needs)
-    if (cudaFuncSetAttribute(linear_tile_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess) return kLaunchFailed;
+    const auto kern = tile_kernels.k[e.act];
+    if (!allow_smem(kern, e.act, 227 * 1024)) return kLaunchFailed;
     TileParams p;
     memset(&p, 0, sizeof(p));
     if (!encode(&p.P, a, na, k, BM) || !encode(&p.Q, b, nb, k, nt)) return kLaunchFailed;
     p.e = e;
     p.p_mn = a.mn; p.q_mn = b.mn; p.nt = nt; p.swap = swap;
+    p.direct = e.vec && !swap && splits == 1;
+    if (p.direct && !encode_results(e, &p.Y, &p.Z)) return kLaunchFailed;
     p.kblocks = (int)((k + BK - 1) / BK);
     p.splits = splits;
     p.p_tiles = (int)((na + BM - 1) / BM);
@@ -701,7 +986,7 @@ static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb
     const int stage = P_BYTES + q_bytes(nt), part = part_bytes(nt), most = (p.kblocks + splits - 1) / splits;
     // CTAs that share an SM: as many as let the whole grid run at once, up to four; clusters of four and eight, two (they do not find whole free SMs everywhere)
     int per_sm = (int)((grid + sm_count() - 1) / sm_count());
-    if (per_sm < 2 && splits > 2) per_sm = 2;
+    if (per_sm < 2 && splits > 2 && nt <= 64) per_sm = 2;
     const int cap = nt > 64 ? 2 : 4;
     if (per_sm > cap) per_sm = cap;
     const int room = 227 * 1024 / per_sm - 1024 - 2048 - (splits > 1 ? part : 0);  // (the system has a KB of each CTA's)
@@ -716,47 +1001,123 @@ static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb
     p.tmem_cols = 32;
     while ((int)p.tmem_cols < nt * p.accs) p.tmem_cols *= 2;
     const int ring = splits > 1 ? p.stages * stage + part : p.stages * stage > part ? p.stages * stage : part;
-    return launch_cluster(linear_tile_kernel, (unsigned)grid, TILE_THREADS, 2048 + ring, splits, stream, p, status) ? kOk : kLaunchFailed;
+    return launch_cluster(kern, (unsigned)grid, TILE_THREADS, 2048 + ring, splits, stream, p, status) ? kOk : kLaunchFailed;
 }
 
-static int run_pair(LinearOperand a, LinearOperand b, long long na, long long nb, long long k, const Epi& e, int bn, int* status, cudaStream_t stream) {
-    if (cudaFuncSetAttribute(linear_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM) != cudaSuccess) return kLaunchFailed;
+static long long pairs_of_sms() { const int n = sm_count() / 2; return n > 0 ? n : 1; }  // (asked for sizes without a device, too)
+// How a product is cut into tiles of 256 x bn for the pairs.
+struct PairPlan {
+    int bn, splits;
+    bool swap;
+    long long tiles, whole;
+    double time;  // in k blocks of a tile of 256 x 256
+};
+static PairPlan plan_pair(long long rows, long long cols, int kblocks, bool can_swap, bool can_split) {
+    const long long pairs = pairs_of_sms();
+    PairPlan best{};
+    for (int swap = 0; swap <= (can_swap ? 1 : 0); ++swap)
+        for (int bn = 256; bn >= 128; bn -= 32) {
+            const long long np = swap ? cols : rows, nq = swap ? rows : cols;
+            PairPlan x{bn, 1, swap != 0, ((np + 255) / 256) * ((nq + bn - 1) / bn), 0, 0.};
+            x.whole = x.tiles / pairs * pairs;
+            const long long left = x.tiles - x.whole;
+            // a k block of a tile of 256 x bn, relative to bn = 256 and its width: narrow tiles wait for operands (8192 x 8192 x 2048, us: 256 175, 224 180 to 187,
+            // 192 196 to 211, 128 233 to 282; columns of y along P, where the tiles are not square, is a little better: 64-byte pieces that fill whole lines)
+            static constexpr double factor[5] = {1.45, 1.22, 1.12, 1.05, 1.};
+            const double each = factor[bn / 32 - 4] * (bn / 256.) * (swap ? 1.01 : bn < 256 ? 1.04 : 1.);
+            // the last round: as it is, or cut, which costs 8 k blocks' time and 8 for each part that is written and read (8192 x 2048, K = 8192: 202 -> 184 us)
+            double last = left ? kblocks : 0;
+            if (left && can_split)
+                for (int c = 2; c <= 8 && left * c <= pairs; ++c) {
+                    const double cut = (kblocks + c - 1) / c + 8 + 8 * c;
+                    if (cut < last) { last = cut; x.splits = c; }
+                }
+            x.time = ((double)(x.whole / pairs) * kblocks + last) * each;
+            if (!best.bn || x.time < best.time) best = x;
+        }
+    return best;
+}
+static size_t pair_ws(const PairPlan& x) { return x.splits > 1 ? (size_t)(x.tiles - x.whole) * ((size_t)x.splits * PART_F4 * 16 + 64) : 0; }
+
+static int run_pair(LinearOperand rows, LinearOperand cols, long long k, const Epi& e, const PairPlan& x, void* workspace, int* status, cudaStream_t stream) {
+    const auto kern = pair_kernels.k[e.act];
+    if (!allow_smem(kern, 16 + e.act, PAIR_SMEM)) return kLaunchFailed;
     PairParams p;
     memset(&p, 0, sizeof(p));
-    if (!encode(&p.P, a, na, k, BM) || !encode(&p.Q, b, nb, k, bn / 2)) return kLaunchFailed;
+    const LinearOperand &a = x.swap ? cols : rows, &b = x.swap ? rows : cols;
+    const long long na = x.swap ? e.cols : e.rows, nb = x.swap ? e.rows : e.cols;
+    if (!encode(&p.P, a, na, k, BM) || !encode(&p.Q, b, nb, k, x.bn / 2)) return kLaunchFailed;
+    if (e.vec && !encode_results(e, &p.Y, &p.Z)) return kLaunchFailed;
     p.e = e;
-    p.p_mn = a.mn; p.q_mn = b.mn; p.bn = bn;
+    p.p_mn = a.mn; p.q_mn = b.mn; p.bn = x.bn; p.swap = x.swap; p.splits = x.splits;
     p.kblocks = (int)((k + BK - 1) / BK);
     p.p_tiles = (int)((na + 2 * BM - 1) / (2 * BM));
-    p.q_tiles = (int)((nb + bn - 1) / bn);
-    p.tiles = (long long)p.p_tiles * p.q_tiles;
-    const long long pairs = sm_count() / 2;
-    const unsigned grid = 2 * (unsigned)(p.tiles < pairs ? p.tiles : pairs);
-    return launch_cluster(linear_pair_kernel, grid, PAIR_THREADS, PAIR_SMEM, 1, stream, p, status) ? kOk : kLaunchFailed;
+    p.q_tiles = (int)((nb + x.bn - 1) / x.bn);
+    p.tiles = x.tiles; p.whole = x.whole;
+    if (x.splits > 1) {
+        const int cut = (int)(x.tiles - x.whole);
+        p.parts = (float4*)workspace;
+        p.arrived = (unsigned*)((char*)workspace + (size_t)cut * x.splits * PART_F4 * 16);
+        if (!launch(linear_zero_kernel, dim3((cut * 16 + 255) / 256), 256, 0, stream, p.arrived, cut * 16)) return kLaunchFailed;
+    }
+    const long long pairs = pairs_of_sms(), units = x.whole + (x.tiles - x.whole) * x.splits;
+    const unsigned grid = 2 * (unsigned)(units < pairs ? units : pairs);
+    return launch_cluster(kern, grid, PAIR_THREADS, PAIR_SMEM, 1, stream, p, status) ? kOk : kLaunchFailed;
+}
+
+// Which kernel, and its shape
+struct Plan {
+    bool pair, swap;
+    int nt, splits;  // of tiles of 128 x nt
+    PairPlan x;
+};
+static Plan make_plan(long long rows, long long cols, long long k, bool rows_mn, bool can_split) {
+    const int kblocks = (int)((k + BK - 1) / BK), sms = sm_count();
+    Plan p{};
+    auto split = [&](long long tiles, int most) {  // CTAs of one tile: as many as fill the SMs
+        int s = 1;
+        while (s < most && 2 * s <= kblocks && tiles * s * 2 <= sms) s *= 2;
+        return s;
+    };
+    if (rows <= 64 && !rows_mn) {
+        p.swap = true;
+        p.nt = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+        p.splits = split((cols + BM - 1) / BM, 8);
+        return p;
+    }
+    // In us: pairs 6.5 and 0.3 for a k block of 256 x 256; tiles of 128 x 128 and 128 x 64, one after the other on an SM, 6 (1.5 more to join parts) and 0.27 or 0.2 for
+    // a k block, which is what their operands take from L2.
+    p.x = plan_pair(rows, cols, kblocks, true, can_split);
+    double best = 6.5 + 0.3 * p.x.time;
+    p.pair = true;
+    for (int nt = 128; nt >= 64; nt /= 2) {
+        const long long tiles = ((rows + BM - 1) / BM) * ((cols + nt - 1) / nt);
+        const int s = split(tiles, nt == 128 ? 4 : 8);
+        const double rounds = (double)((tiles * s + sms - 1) / (sms > 0 ? sms : 1));
+        const double t = 6. + (s > 1 ? 1.5 : 0.) + rounds * ((kblocks + s - 1) / s) * (nt == 128 ? 0.27 : 0.2);
+        if (t < best) { best = t; p.pair = false; p.nt = nt; p.splits = s; }
+    }
+    return p;
 }
 
 }  // namespace lin
 
-int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const LinearEpilogue& ep, int* status, cudaStream_t stream) {
+size_t linear_workspace_bytes(long long rows, long long cols, long long k, bool rows_mn) {
+    const lin::Plan p = lin::make_plan(rows, cols, k, rows_mn, true);
+    return p.pair ? lin::pair_ws(p.x) : 0;
+}
+
+int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const LinearEpilogue& ep, void* workspace, int* status, cudaStream_t stream) {
     using namespace lin;
     Epi e;
     static_cast<LinearEpilogue&>(e) = ep;
     const int per16 = ep.y_f32 ? 4 : 8;
     e.vec = al16(ep.y) && ep.ldy % per16 == 0 && (!ep.residual || (al16(ep.residual) && ep.ldr % per16 == 0));
-    const int kblocks = (int)((k + BK - 1) / BK), sms = sm_count();
-    auto split = [&](long long tiles) {  // CTAs of one tile: as many as fill the SMs
-        int s = 1;
-        while (s < 8 && 2 * s <= kblocks && tiles * s * 2 <= sms) s *= 2;
-        return s;
-    };
-    if (ep.rows <= 64 && !rows.mn) {
-        const int nt = ep.rows <= 16 ? 16 : ep.rows <= 32 ? 32 : 64;
-        return run_tile(cols, rows, ep.cols, ep.rows, k, e, true, nt, split((ep.cols + BM - 1) / BM), status, stream);
-    }
-    const long long pair_tiles = ((ep.rows + 255) / 256) * ((ep.cols + 255) / 256);
-    if (2 * pair_tiles >= sms) return run_pair(rows, cols, ep.rows, ep.cols, k, e, 256, status, stream);
-    const long long tiles = ((ep.rows + BM - 1) / BM) * ((ep.cols + 127) / 128);
-    return run_tile(rows, cols, ep.rows, ep.cols, k, e, false, 128, split(tiles), status, stream);
+    e.bias_vec = al16(ep.bias);
+    const Plan p = make_plan(ep.rows, ep.cols, k, rows.mn, workspace != nullptr);
+    if (p.pair) return run_pair(rows, cols, k, e, p.x, workspace, status, stream);
+    if (p.swap) return run_tile(cols, rows, ep.cols, ep.rows, k, e, true, p.nt, p.splits, status, stream);
+    return run_tile(rows, cols, ep.rows, ep.cols, k, e, false, p.nt, p.splits, status, stream);
 }
 
 int linear_dz_chunks(long long M, long long N) {

@@ -24,7 +24,9 @@ struct LinearOperand {
     long long ld;
     bool mn;
 };
-int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const LinearEpilogue& e, int* status, cudaStream_t stream);
+// workspace: linear_workspace_bytes() bytes (rows_mn: the rows' operand is [k, index]), or null: no tile is cut along k
+size_t linear_workspace_bytes(long long rows, long long cols, long long k, bool rows_mn);
+int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const LinearEpilogue& e, void* workspace, int* status, cudaStream_t stream);
 
 // dz = dy act'(saved) as bf16 [M, ldz] (not written where dz is null) and dbias = column sums of dz (or null; then of dz before its rounding)
 struct LinearDz {

@@ -489,7 +489,9 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const
     operand_rows(w, &ldw);
     if (residual.defined()) pitched_rows(residual, &ldr);
     const int flags = (out_f32 ? WKV7_LINEAR_F32_OUT : 0) | (bias.defined() && bias.scalar_type() == at::kFloat ? WKV7_LINEAR_F32_BIAS : 0) | (z_type == at::kFloat ? WKV7_LINEAR_F32_Z : 0);
-    check(wkv7_linear_fwd(x.data_ptr(), w.data_ptr(), ptr(bias), ptr(residual), y.data_ptr(), ptr(z), M, N, K, ldx, ldw, ldr, N, n8, (int)act, flags, stream()),
+    Tensor ws;
+    if (const int64_t bytes = wkv7_linear_fwd_workspace_bytes(M, N, K)) ws = at::empty({bytes}, x.options().dtype(at::kByte));
+    check(wkv7_linear_fwd(x.data_ptr(), w.data_ptr(), ptr(bias), ptr(residual), y.data_ptr(), ptr(z), M, N, K, ldx, ldw, ldr, N, n8, (int)act, flags, ptr(ws), stream()),
           "wkv7_linear_fwd");
     return {y, z};
 }
@@ -537,7 +539,7 @@ struct LinearFn : public Function<LinearFn> {
         if (want_dx) g[0] = at::empty(x.sizes(), x.options());
         if (want_dw) g[1] = at::empty(w.sizes(), w.options());
         if (want_db) db = at::empty({N}, x.options().dtype(at::kFloat));
-        Tensor ws = at::empty({wkv7_linear_bwd_workspace_bytes(M, N)}, x.options().dtype(at::kByte));
+        Tensor ws = at::empty({wkv7_linear_bwd_workspace_bytes(M, N, K)}, x.options().dtype(at::kByte));
         check(wkv7_linear_bwd(x.data_ptr(), w.data_ptr(), act ? ptr(saved) : nullptr, dy.data_ptr(), ptr(g[0]), ptr(g[1]), f32(db),
                               M, N, K, ldx, ldw, act ? lds : N, lddy, (int)act, (out_f32 ? WKV7_LINEAR_F32_OUT : 0) | (from_y ? WKV7_LINEAR_FROM_Y : 0) |
                               (act && saved.scalar_type() == at::kFloat ? WKV7_LINEAR_F32_Z : 0), ws.data_ptr(), stream()),

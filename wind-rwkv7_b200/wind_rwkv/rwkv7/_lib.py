@@ -62,8 +62,9 @@ _SIGNATURES = {
     'wkv7_ddlerp_bwd': (_int, [_vp] * 16 + [_i64] * 4 + [_vp]),
     'wkv7_ddlerp_bwd_tc': (_int, [_vp] * 17 + [_i64] * 4 + [_vp]),
     'wkv7_ddlerp_bwd_tc_workspace_bytes': (ctypes.c_size_t, [_i64] * 2),
-    'wkv7_linear_fwd': (_int, [_vp] * 6 + [_i64] * 8 + [_int] * 2 + [_vp]),
-    'wkv7_linear_bwd_workspace_bytes': (_i64, [_i64] * 2),
+    'wkv7_linear_fwd_workspace_bytes': (_i64, [_i64] * 3),
+    'wkv7_linear_fwd': (_int, [_vp] * 6 + [_i64] * 8 + [_int] * 2 + [_vp] * 2),
+    'wkv7_linear_bwd_workspace_bytes': (_i64, [_i64] * 3),
     'wkv7_linear_bwd': (_int, [_vp] * 7 + [_i64] * 7 + [_int] * 2 + [_vp] * 2),
     'wkv7_beam_select_workspace_bytes': (_i64, [_i64] * 3),
     'wkv7_beam_select': (_int, [_vp] * 7 + [_i64] * 7 + [_int] + [_vp] * 2),

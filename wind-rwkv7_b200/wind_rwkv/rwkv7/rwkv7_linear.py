@@ -62,8 +62,9 @@ def fw_linear(x, w, bias, residual, act, out_f32, save):
     b = None if bias is None else bias.contiguous()
     flags = (F32_OUT if out_f32 else 0) | (F32_BIAS if b is not None and b.dtype == th.float32 else 0) | (F32_Z if save == 'z32' else 0)
     with _lib.on_device(x, w, b, r):
+        ws = th.empty(_lib.lib().wkv7_linear_fwd_workspace_bytes(M, N, K), dtype=th.uint8, device=x.device)
         rc = _lib.lib().wkv7_linear_fwd(x.data_ptr(), w.data_ptr(), _lib.ptr(b), _lib.ptr(r), y.data_ptr(), z.data_ptr() if save_z else None,
-                                        M, N, K, ldx, ldw, ldr, N, n8, act, flags, _lib.stream_of(x))
+                                        M, N, K, ldx, ldw, ldr, N, n8, act, flags, ws.data_ptr() or None, _lib.stream_of(x))
     _lib.check(rc, 'wkv7_linear_fwd')
     return y, z
 
@@ -80,9 +81,9 @@ def bw_linear(x, w, saved, dy, act, out_f32, from_y, want_dx, want_dw, want_db):
     w, ldw = operand_of(w)
     dy, lddy = rows_of(dy)
     saved, lds = rows_of(saved) if act else (None, N)
-    ws = th.empty(_lib.lib().wkv7_linear_bwd_workspace_bytes(M, N), dtype=th.uint8, device=dev)
     flags = (F32_OUT if out_f32 else 0) | (FROM_Y if from_y else 0) | (F32_Z if act and saved.dtype == th.float32 else 0)
     with _lib.on_device(x, w, dy, saved):
+        ws = th.empty(_lib.lib().wkv7_linear_bwd_workspace_bytes(M, N, K), dtype=th.uint8, device=dev)
         rc = _lib.lib().wkv7_linear_bwd(x.data_ptr(), w.data_ptr(), _lib.ptr(saved), dy.data_ptr(), dx.data_ptr() if want_dx else None,
                                         dw.data_ptr() if want_dw else None, db.data_ptr() if want_db else None, M, N, K, ldx, ldw, lds, lddy, act, flags,
                                         ws.data_ptr(), _lib.stream_of(x))
