@@ -92,7 +92,7 @@ def compare(x, w, b, r, dy, act, out=th.bfloat16, call=None):
 SHAPES = [  # rows, columns, k
     (1, 1, 8), (1, 8192, 2048), (3, 77, 200), (16, 129, 1024), (17, 2048, 8192), (33, 1000, 64), (64, 257, 4104),   # few rows
     (65, 64, 64), (100, 130, 72), (333, 77, 200), (513, 200, 768), (700, 1000, 136),                                # tiles
-    (1300, 4096, 72), (1283, 4001, 200), (2500, 2053, 1032), (5000, 96, 2048), (20000, 40, 24)]                     # pairs, and mixtures in the backward
+    (1300, 4096, 72), (1283, 4001, 200), (2500, 2053, 1032), (5000, 96, 2048), (20000, 40, 24), (9000, 40, 200)]                     # pairs, and mixtures in the backward
 
 
 @pytest.mark.parametrize('M,N,K', SHAPES)
@@ -112,6 +112,90 @@ def test_activations(act, M, N, K, residual):
 @pytest.mark.parametrize('M,N,K', [(7, 50001, 64), (300, 203, 256), (1400, 3333, 64), (1536, 4096, 64)])
 def test_fp32_output(act, M, N, K):
     compare(*inputs(M, N, K, th.float32, True, th.float32, 9), act, out=th.float32)
+
+
+@pytest.mark.parametrize('M,N,K', [(3328, 1536, 8192), (1536, 8192, 3336), (60000, 80, 200), (30000, 33, 264), (40, 1000, 8192)])
+def test_long_sums(M, N, K):
+    """Sums that are shared out: over the clusters of a tile, over the units of the tiles of the last round, and both in the backward."""
+    compare(*inputs(M, N, K, th.float32, True, th.bfloat16, 21), 'silu')
+    compare(*inputs(M, N, K, None, False, th.bfloat16, 22), None)
+
+
+@pytest.mark.parametrize('act', ['relu2', 'tanh'])
+@pytest.mark.parametrize('bias,residual,out', [(None, False, th.bfloat16), (th.float32, True, th.bfloat16), (th.bfloat16, True, th.float32), (th.float32, True, th.float32)])
+@pytest.mark.parametrize('M,N,K', [(1283, 10240, 256), (1283, 10236, 256), (1283, 10235, 256)])
+def test_columns_of_y_along_the_accumulators_rows(M, N, K, act, bias, residual, out):
+    """Shapes that the pairs take turned over, with every kind of result: aligned rows (bulk stores), rows that only fp32 ones are, odd ones."""
+    compare(*inputs(M, N, K, bias, residual, out, 31), act, out=out)
+
+
+def test_results_go_where_they_belong():
+    """Nothing is written beside y, z, dx or dw: C entry points with outputs inside larger buffers."""
+    from wind_rwkv.rwkv7 import _lib
+    L = _lib.lib()
+    for M, N, K in ((5, 77, 64), (40, 264, 64), (130, 77, 72), (200, 264, 512), (1283, 4100, 64), (1283, 4101, 64), (3000, 3333, 64)):
+        x, w, _, _, dy = inputs(M, N, K, None, False, th.bfloat16, 2)
+        n8 = (N + 7) // 8 * 8
+        for f32 in (0, 1):
+            ldy = n8 + 16
+            y = th.full((M + 2, ldy), 7., dtype=th.float32 if f32 else th.bfloat16, device='cuda')
+            z = th.full((M + 2, n8 + 8), 7., dtype=th.bfloat16, device='cuda')
+            ws = th.empty(max(16, L.wkv7_linear_fwd_workspace_bytes(M, N, K)), dtype=th.uint8, device='cuda')
+            rc = L.wkv7_linear_fwd(x.data_ptr(), w.data_ptr(), None, None, y[1:].data_ptr(), z[1:].data_ptr(), M, N, K, K, K, 0, ldy, n8 + 8, 5, f32, ws.data_ptr(),
+                                   _lib.stream_of(x))
+            assert rc == 0
+            ref = x.double() @ w.double().T
+            assert bool((y[0] == 7).all()) and bool((y[-1] == 7).all()) and bool((y[:, N:] == 7).all())
+            assert bool((z[0] == 7).all()) and bool((z[-1] == 7).all()) and bool((z[:, n8:] == 7).all())
+            tol = U * ref.abs() + acc(K) * (x.double().abs() @ w.double().abs().T)
+            assert bool(((z[1:-1, :N].double() - ref).abs() <= tol).all())
+            check('y', y[1:-1, :N], F64['silu'](ref), U * F64['silu'](ref).abs() + 1.1 * acc(K) * (x.double().abs() @ w.double().abs().T) + 2. ** -17 * (1 + ref.abs()))
+        d = th.full((M + N + 3, K), 7., dtype=th.bfloat16, device='cuda')
+        dx, dw = d[1:M + 1], d[M + 2:M + N + 2]
+        ws = th.empty(L.wkv7_linear_bwd_workspace_bytes(M, N, K), dtype=th.uint8, device='cuda')
+        rc = L.wkv7_linear_bwd(x.data_ptr(), w.data_ptr(), None, dy.data_ptr(), dx.data_ptr(), dw.data_ptr(), None, M, N, K, K, K, N, N, 0, 0, ws.data_ptr(), _lib.stream_of(x))
+        assert rc == 0
+        assert bool((d[0] == 7).all()) and bool((d[M + 1] == 7).all()) and bool((d[-1] == 7).all())
+        D, X, W = dy.double(), x.double(), w.double()
+        check('dx', dx, D @ W, U * (D @ W).abs() + (U + acc(N)) * (D.abs() @ W.abs()) * (1 if N % 8 else 0.5))
+        check('dw', dw, D.T @ X, U * (D.T @ X).abs() + acc(M) * (D.abs().T @ X.abs()))
+
+
+def test_without_workspace():
+    """wkv7_linear_fwd with a null workspace: the same sums in another order."""
+    from wind_rwkv.rwkv7 import _lib
+    L = _lib.lib()
+    M, N, K = 3328, 1536, 8192
+    x, w, _, _, _ = inputs(M, N, K, None, False, th.bfloat16, 2)
+    y = th.empty(M, N, dtype=th.bfloat16, device='cuda')
+    assert L.wkv7_linear_fwd(x.data_ptr(), w.data_ptr(), None, None, y.data_ptr(), None, M, N, K, K, K, N, N, 0, 0, 0, None, _lib.stream_of(x)) == 0
+    ref = x.double() @ w.double().T
+    check('y', y, ref, U * ref.abs() + acc(K) * (x.double().abs() @ w.double().abs().T))
+
+
+def test_training_step_in_a_graph():
+    """Forward and backward captured together and replayed on other inputs."""
+    from wind_rwkv.rwkv7 import linear
+    for M, N, K in ((37, 77, 200), (1300, 4096, 512)):
+        x, w, b, r, dy = inputs(M, N, K, th.float32, True, th.bfloat16, 5)
+
+        def step(x, w, b, r):
+            leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+            y = linear(leaves[0], leaves[1], leaves[2], act='gelu', residual=leaves[3])
+            return [y.detach(), *th.autograd.grad(y, leaves, dy)]
+
+        side = th.cuda.Stream()
+        side.wait_stream(th.cuda.current_stream())
+        with th.cuda.stream(side):
+            step(x, w, b, r)
+        th.cuda.current_stream().wait_stream(side)
+        graph = th.cuda.CUDAGraph()
+        with th.cuda.graph(graph):
+            out = step(x, w, b, r)
+        for _ in range(2):
+            x.copy_(x.flip(0))
+            graph.replay()
+            assert all(th.equal(a, c) for a, c in zip(out, step(x, w, b, r)))
 
 
 def test_large_arguments():

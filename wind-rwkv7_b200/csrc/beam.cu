@@ -551,7 +551,8 @@ int launch_beam_select(BeamParams p, void* workspace, cudaStream_t stream) {
     const int stage = p.f32 ? aligned ? beam::stage_bytes<true, true>() : beam::stage_bytes<true, false>()
                             : aligned ? beam::stage_bytes<false, true>() : beam::stage_bytes<false, false>();
     const int smem = beam::SCAN_WARPS * beam::DEPTH * stage;
-    if (cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return kLaunchFailed;
+    static thread_local uint32_t smem_allowed[64];
+    if (!allow_smem(scan, smem_allowed, 2 * p.f32 + aligned, smem)) return kLaunchFailed;
     if (!launch(scan, dim3((unsigned)ctas), 32 * beam::SCAN_WARPS, smem, stream, p)) return kLaunchFailed;
     return launch(beam::beam_pick_kernel, dim3((unsigned)p.B), beam::PICK_THREADS, 0, stream, p) ? kOk : kLaunchFailed;
 }

@@ -71,7 +71,7 @@ template <int ACT, bool FROM_Y> __device__ __forceinline__ float act_grad(float 
 
 // ---- epilogue --------------------------------------------------------------------------------------------
 struct Epi : LinearEpilogue {
-    bool vec;       // rows of y and of the residual start on 16-byte boundaries
+    bool vec;       // rows of y start and end on 16-byte boundaries (bulk stores clip in steps of 16 bytes), those of the residual start there
     bool bias_vec;  // so does the bias
 };
 __device__ __forceinline__ void load8g(const void* base, bool f32, long long at, float (&f)[8]) {
@@ -153,21 +153,6 @@ template <int ACT> __device__ __forceinline__ void finish8(const Epi& e, long lo
             else ((bf16*)e.y)[row * e.ldy + col + i] = __float2bfloat16_rn(f[i]);
         }
 }
-// A warp's block of 32 rows x 32 columns of y whose rows are not aligned: lane has rows row + 8 it, columns [col, col + 8), taken by read(it, f) behind ready().
-template <int ACT, typename Ready, typename Read> __device__ __forceinline__ void finish_block(const Epi& e, long long row, long long col, Ready ready, Read read) {
-    float bias[8];
-    ready();
-    if (e.bias) bias8(e, col, bias);
-#pragma unroll 1
-    for (int it = 0; it < 4; ++it) {
-        float f[8];
-        read(it, f);
-        if (e.bias)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] += bias[i];
-        if (row + 8 * it < e.rows && col < e.cols) finish8<ACT>(e, row + 8 * it, col, f);
-    }
-}
 // A block of 32 x 32 results to memory by a bulk tensor store, which clips it: a lane has a row of it, or (TURNED) a column.  `turn`: which half of the
 // staging area is next (bf16; fp32 takes all of it); it is written again when the store that reads it has.  `all`: wait for all stores, where halves do not alternate.
 template <bool TURNED> __device__ __forceinline__ void bulk_store_block(float* staging, const CUtensorMap* map, bool f32, bool all, const float (&v)[32], int lane, int& turn, long long col0, long long row0) {
@@ -205,6 +190,58 @@ template <bool TURNED> __device__ __forceinline__ void bulk_store_block(float* s
     }
 }
 
+// A warp's block of 32 x 32, a lane a column of y; the sums come by sums(v).  Rows that are not aligned are stored, 32 adjacent elements an instruction, as they lie.
+template <int ACT, typename Sums> __device__ __forceinline__ void finish_cols(const Epi& e, const CUtensorMap* Y, const CUtensorMap* Z, float* mine, bool mixed, int lane, int& turn,
+                                                                             long long row0, long long col0, Sums sums) {
+    const long long col = col0 + lane;
+    const bool in = col < e.cols;
+    const int rows = (int)(e.rows - row0 < 32 ? e.rows - row0 : 32);
+    float v[32];
+    const float bias = e.bias && in ? load1g(e.bias, e.bias_f32, col) : 0.f;
+    sums(v);
+    if (e.bias)
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] += bias;
+    if (e.z) {
+        if (e.vec) {
+            bulk_store_block<true>(mine, Z, e.z_f32, mixed, v, lane, turn, col0, row0);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+                if (in && c < rows) store_z1(e, row0 + c, col, v[c]);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < 32; ++c) v[c] = act<ACT>(v[c]);
+#pragma unroll
+    for (int half = 0; half < 32; half += 16) {
+        if (e.residual) {  // (sixteen rows of it before they are stored: y may be the residual, so the compiler keeps them in order)
+            float res[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) res[c] = in && half + c < rows ? load1g(e.residual, e.y_f32, (row0 + half + c) * e.ldr + col) : 0.f;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) v[half + c] += res[c];
+        }
+        if (e.vec) continue;
+#pragma unroll
+        for (int c = half; c < half + 16; ++c)
+            if (in && c < rows) {
+                if (e.y_f32) ((float*)e.y)[(row0 + c) * e.ldy + col] = v[c];
+                else ((bf16*)e.y)[(row0 + c) * e.ldy + col] = __float2bfloat16_rn(v[c]);
+            }
+    }
+    if (e.vec) bulk_store_block<true>(mine, Y, e.y_f32, mixed, v, lane, turn, col0, row0);
+}
+// a block of which each lane has a row, turned so that each has a column
+__device__ __forceinline__ void turn_block(float* mine, int lane, float (&v)[32]) {
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < 8; ++u)  // 16-byte unit u of row r at u ^ (r % 8)
+        *reinterpret_cast<float4*>(mine + lane * 32 + ((u ^ (lane & 7)) << 2)) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 32; ++c) v[c] = mine[c * 32 + (((lane >> 2) ^ (c & 7)) << 2) + (lane & 3)];
+}
 // A warp's block of 32 x 32, a lane a row of y: the sums come by sums(v), residual and bias are applied as they lie.
 template <int ACT, typename Sums> __device__ __forceinline__ void finish_rows(const Epi& e, const CUtensorMap* Y, const CUtensorMap* Z, float* mine, bool mixed, int lane, int& turn,
                                                                              long long row0, long long col0, Sums sums) {
@@ -291,13 +328,18 @@ __device__ __forceinline__ void expect_tx(uint64_t* bar, uint32_t bytes) {
 struct TileParams {
     CUtensorMap P, Q, Y, Z;  // Y, Z: as the pairs'
     Epi e;
-    int p_mn, q_mn, nt, kblocks, splits, stages, accs, swap, direct, p_tiles;  // swap: P runs over the columns of y, Q over its rows
+    int p_mn, q_mn, nt, kblocks, splits, stages, accs, swap, direct, outer, p_tiles;  // swap: P runs over the columns of y, Q over its rows
     uint32_t tmem_cols;
+    // outer > 1: each tile has that many clusters, which leave their sums in memory; of the CTAs that have the same rows of a tile the last to arrive adds them, in
+    // their order, and finishes
+    float* sums;        // [outer][tile][128][nt]
+    unsigned* arrived;  // [tile][rank], zero
 };
 struct TileCtrl {
     uint64_t full[MAXSTAGES], empty[MAXSTAGES], accum, drain;
     uint32_t tmem_base;
     volatile int abort, zero;
+    int last;
 };
 static_assert(sizeof(TileCtrl) <= 1024, "the KB ahead of the ring");
 constexpr int TILE_THREADS = 192;  // warps 0-3: accumulator rows, warp 4: copies, warp 5: products; all six: the result
@@ -320,9 +362,11 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS) linear_tile_k
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int rank = blockIdx.x % p.splits;
-    const long long tile = blockIdx.x / p.splits;
+    const long long tile = blockIdx.x / p.splits / p.outer;
+    const int cluster = blockIdx.x / p.splits % p.outer;
     const int p0 = (int)(tile % p.p_tiles) * BM, q0 = (int)(tile / p.p_tiles) * p.nt;
-    const int lo = (int)((long long)p.kblocks * rank / p.splits), hi = (int)((long long)p.kblocks * (rank + 1) / p.splits);
+    const int share = cluster * p.splits + rank, shares = p.splits * p.outer;
+    const int lo = (int)((long long)p.kblocks * share / shares), hi = (int)((long long)p.kblocks * (share + 1) / shares);
 
     if (tid == 0) {
         for (int s = 0; s < p.stages; ++s) { mbar_init(&ctrl->full[s], 1); mbar_init(&ctrl->empty[s], 1); }
@@ -419,7 +463,9 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS) linear_tile_k
                         for (int i = 0; i < 32; ++i) v[i] += u[i];
                     }
                 };
-                if (p0 + 32 * warp < e.rows && q0 + c < e.cols) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, p0 + 32 * warp, q0 + c, sums);
+                if (p0 + 32 * warp >= e.rows || q0 + c >= e.cols) continue;
+                if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, p0 + 32 * warp, q0 + c, sums);
+                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, p0 + 32 * warp, q0 + c, [&](float (&v)[32]) { sums(v); turn_block(mine, lane, v); });
             }
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
@@ -485,16 +531,50 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS) linear_tile_k
             }
         }
     } else {
-        const int per_row = p.nt / 8;
-        for (int u = tid; u < rows * per_row; u += TILE_THREADS) {
+        const int per_row = p.nt / 8, units = rows * per_row;
+        const long long plane = (long long)gridDim.x / shares * BM * p.nt;
+        float* const mine = p.sums + (tile * BM + r0) * p.nt;
+        auto joined = [&](int u, float (&f)[8]) {  // the cluster's parts
             const int i = u / per_row, j = 8 * (u % per_row);
-            const long long row = p0 + r0 + i, col = q0 + j;
-            if (row >= e.rows || col >= e.cols) continue;
-            float f[8] = {};
+#pragma unroll
+            for (int q = 0; q < 8; ++q) f[q] = 0.f;
             for (int r = 0; r < p.splits; ++r) {
                 const float* x = parts + (r * rows + i) * pitch + j;
                 const float4 a = ld4(x), b = ld4(x + 4);
                 f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+            }
+        };
+        if (p.outer > 1) {
+            for (int u = tid; u < units; u += TILE_THREADS) {
+                float f[8];
+                joined(u, f);
+                float4* to = reinterpret_cast<float4*>(mine + cluster * plane + 8 * u);
+                __stcg(to, make_float4(f[0], f[1], f[2], f[3]));
+                __stcg(to + 1, make_float4(f[4], f[5], f[6], f[7]));
+            }
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) ctrl->last = atomicAdd(p.arrived + tile * p.splits + rank, 1u) == (unsigned)p.outer - 1;
+            __syncthreads();
+            if (!ctrl->last) return;
+            __threadfence();
+        }
+        for (int u = tid; u < units; u += TILE_THREADS) {
+            const int i = u / per_row, j = 8 * (u % per_row);
+            const long long row = p0 + r0 + i, col = q0 + j;
+            if (row >= e.rows || col >= e.cols) continue;
+            float f[8];
+            if (p.outer > 1) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) f[q] = 0.f;
+#pragma unroll 4
+                for (int c = 0; c < p.outer; ++c) {
+                    const float4* x = reinterpret_cast<const float4*>(mine + c * plane + 8 * u);
+                    const float4 a = __ldcg(x), b = __ldcg(x + 1);
+                    f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+                }
+            } else {
+                joined(u, f);
             }
             if (e.bias) {
                 float bias[8];
@@ -672,7 +752,7 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
         // a row of y (swap: a column).  Bias, activation and residual are applied as it lies; the block leaves through shared memory by a bulk tensor store,
         // whose swizzle (16-byte pieces, xor of the row) spares bank conflicts.  That is 16 wavefronts of shared memory a block of bf16: the operands'
         // copies and products need all but an eighth of its bandwidth.  (Through shared memory in fp32 and out by 16-byte stores: 64 and the stores'.)
-        // Where rows of y are not aligned the block is turned there in fp32, so that four lanes have 32 adjacent columns of a row.
+        // Where rows of y are not aligned the block is turned there in fp32, so that a lane has a column.
         const int quarter = warp & 3, side = (warp - 4) >> 2;
         float* mine = reinterpret_cast<float*>(staging + (warp - 4) * PAIR_STAGING);
         int turn = 0;
@@ -681,6 +761,13 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
         const int blocks = p.bn / 32, b0 = side ? (blocks + 1) / 2 : 0, b1 = side ? blocks : (blocks + 1) / 2;
         for (int n = 0; pair_work(p, n, w); ++n) {
             const int buf = n & 1;
+            if (e.residual) {  // on its way to L2 while the products go on: a lane's row of a block, 64 or 128 bytes
+                for (int b = b0; b < b1; ++b) {
+                    const long long q0 = (long long)w.qi * p.bn + 32 * b, first = (long long)w.pi * 2 * BM + rank * BM + 32 * quarter;
+                    const long long row = (p.swap ? q0 : first) + lane, col = p.swap ? first : q0;
+                    if (row < e.rows && col < e.cols) asm volatile("prefetch.global.L2 [%0];" ::"l"((const unsigned char*)e.residual + (row * e.ldr + col) * (e.y_f32 ? 4 : 2)));
+                }
+            }
             mbar_wait_bounded<true>(&ctrl->accum_full[buf], (n >> 1) & 1, &ctrl->abort, status);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (ctrl->abort) break;
@@ -734,62 +821,13 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
                         if (b == b1 - 1) emptied();
                     }
                 };
-                if (e.vec) {
-                    if (row0 >= e.rows || col0 >= e.cols) {
-                        if (b == b1 - 1 && !parts) emptied();
-                        continue;
-                    }
-                    if (p.swap) {
-                        float v[32];
-                        const long long col = col0 + lane;
-                        const bool in = col < e.cols;
-                        float res[32];
-                        if (e.residual)
-#pragma unroll
-                            for (int c = 0; c < 32; ++c) res[c] = in && row0 + c < e.rows ? load1g(e.residual, e.y_f32, (row0 + c) * e.ldr + col) : 0.f;
-                        const float bias = e.bias && in ? load1g(e.bias, e.bias_f32, col) : 0.f;
-                        sums(v);
-                        if (e.bias)
-#pragma unroll
-                            for (int c = 0; c < 32; ++c) v[c] += bias;
-                        if (e.z) bulk_store_block<true>(mine, &p.Z, e.z_f32, mixed, v, lane, turn, col0, row0);
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) v[c] = act<ACT>(v[c]);
-                        if (e.residual)
-#pragma unroll
-                            for (int c = 0; c < 32; ++c) v[c] += res[c];
-                        bulk_store_block<true>(mine, &p.Y, e.y_f32, mixed, v, lane, turn, col0, row0);
-                    } else {
-                        finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, sums);
-                    }
+                if (row0 >= e.rows || col0 >= e.cols) {
+                    if (b == b1 - 1 && !parts) emptied();
                     continue;
                 }
-                const int g = lane & 3, r = lane >> 2;
-                auto ready = [&] {
-                    float v[32];
-                    sums(v);
-                    if (p.swap) {  // element c of row `lane` at c ^ lane, else 16-byte unit u at u ^ (lane % 8): no conflicts either way
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) mine[lane * 32 + (c ^ lane)] = v[c];
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            *reinterpret_cast<float4*>(mine + lane * 32 + ((u ^ (lane & 7)) << 2)) = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-                    }
-                    __syncwarp();
-                };
-                auto read = [&](int it, float (&f)[8]) {
-                    if (p.swap) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) f[i] = mine[(8 * g + i) * 32 + ((8 * it + r) ^ (8 * g + i))];
-                    } else {  // (row 8 it + r)
-                        const float* at = mine + (8 * it + r) * 32;
-                        const float4 x = ld4(at + (((2 * g) ^ r) << 2)), y = ld4(at + (((2 * g + 1) ^ r) << 2));
-                        f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w; f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
-                    }
-                };
-                finish_block<ACT>(e, row0 + r, col0 + 8 * g, ready, read);
-                __syncwarp();
+                if (p.swap) finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, sums);
+                else if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, sums);
+                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); turn_block(mine, lane, v); });
             }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory must outlive the stores' reads
@@ -808,8 +846,8 @@ struct DzParams : LinearDz {
     long long rows_per;
     bool vec;  // rows of dy and saved start on 16-byte boundaries
 };
-constexpr int DZ_AHEAD = 4;  // rows a thread has requested at a time
-template <int ACT, bool FROM_Y> __global__ void __launch_bounds__(DZ_THREADS) linear_dz_kernel(const __grid_constant__ DzParams p) {
+// WIDE: dy or saved is in fp32 (which of them, is looked up)
+template <int ACT, bool FROM_Y, bool WIDE> __global__ void __launch_bounds__(DZ_THREADS, WIDE ? 2 : 3) linear_dz_kernel(const __grid_constant__ DzParams p) {
     stream_order();
     __shared__ float sums[8][DZ_COLS + 4];
     const int g = threadIdx.x & 31, r = threadIdx.x >> 5;
@@ -825,43 +863,47 @@ template <int ACT, bool FROM_Y> __global__ void __launch_bounds__(DZ_THREADS) li
             }
             if (p.dz) *reinterpret_cast<uint4*>((bf16*)p.dz + m * p.ldz + col) = pack8(d);  // (ldz is a multiple of 8)
         };
-        const bool whole = p.vec && col + 8 <= p.N;
-        for (long long m = lo + r; m < hi; m += 8 * DZ_AHEAD) {
-            // (rows behind the chunk: the last one again, not stored and not summed)
-            float d[DZ_AHEAD][8], z[DZ_AHEAD][8];
-            if (whole) {
-                Words8 dw[DZ_AHEAD], zw[DZ_AHEAD];
+        const bool dy_f32 = WIDE && p.dy_f32, z_f32 = WIDE && p.saved_f32;
+        // rows a thread has requested at a time; behind the chunk's end the last one again, not stored and not summed
+        constexpr int AHEAD = 4, EDGE = 2;
+        if (p.vec && col + 8 <= p.N) {
+            for (long long m = lo + r; m < hi; m += 8 * AHEAD) {
+                Words8 dw[AHEAD], zw[AHEAD];
 #pragma unroll
-                for (int a = 0; a < DZ_AHEAD; ++a) {
+                for (int a = 0; a < AHEAD; ++a) {
                     const long long n = m + 8 * a < hi ? m + 8 * a : m;
-                    dw[a] = request8(p.dy, p.dy_f32, n * p.lddy + col);
-                    if (ACT) zw[a] = request8(p.saved, p.saved_f32, n * p.lds + col);
+                    dw[a] = request8(p.dy, dy_f32, n * p.lddy + col);
+                    if (ACT) zw[a] = request8(p.saved, z_f32, n * p.lds + col);
                 }
 #pragma unroll
-                for (int a = 0; a < DZ_AHEAD; ++a) {
-                    floats8(dw[a], p.dy_f32, d[a]);
-                    if (ACT) floats8(zw[a], p.saved_f32, z[a]);
+                for (int a = 0; a < AHEAD; ++a) {
+                    float d[8], z[8];
+                    floats8(dw[a], dy_f32, d);
+                    if (ACT) floats8(zw[a], z_f32, z);
+                    if (m + 8 * a < hi) row(m + 8 * a, d, z);
                 }
-            } else {
+            }
+        } else {
+            for (long long m = lo + r; m < hi; m += 8 * EDGE) {
+                float d[EDGE][8], z[EDGE][8];
 #pragma unroll
-                for (int a = 0; a < DZ_AHEAD; ++a) {
+                for (int a = 0; a < EDGE; ++a) {
                     const long long n = m + 8 * a < hi ? m + 8 * a : m;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const long long c = col + i < p.N ? col + i : p.N - 1;  // (columns behind the last: that one again, and zero)
-                        d[a][i] = load1g(p.dy, p.dy_f32, n * p.lddy + c);
-                        if (ACT) z[a][i] = load1g(p.saved, p.saved_f32, n * p.lds + c);
+                        d[a][i] = load1g(p.dy, dy_f32, n * p.lddy + c);
+                        if (ACT) z[a][i] = load1g(p.saved, z_f32, n * p.lds + c);
                     }
                 }
 #pragma unroll
-                for (int a = 0; a < DZ_AHEAD; ++a)
+                for (int a = 0; a < EDGE; ++a) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         if (col + i >= p.N) d[a][i] = 0.f;
+                    if (m + 8 * a < hi) row(m + 8 * a, d[a], z[a]);
+                }
             }
-#pragma unroll
-            for (int a = 0; a < DZ_AHEAD; ++a)
-                if (m + 8 * a < hi) row(m + 8 * a, d[a], z[a]);
         }
     }
     if (!p.dbias) return;
@@ -932,20 +974,7 @@ static bool encode_results(const Epi& e, CUtensorMap* Y, CUtensorMap* Z) {
     return encode_out(Y, e.y, e.y_f32, e.rows, e.cols, e.ldy) && (!e.z || encode_out(Z, e.z, e.z_f32, e.rows, e.cols, e.ldz));
 }
 
-// Shared memory beyond 48 KB has to be allowed once per kernel and device.  A thread's first call on a device (one of autograd's may have made no other) does so again:
-// that gives it the context which encoding a tensor map needs.
-template <typename K> static bool allow_smem(K kern, int which, int bytes) {
-    static thread_local uint32_t done[64];
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return false;
-    if (dev < 64 && (done[dev] >> which & 1)) return true;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
-        cudaGetLastError();
-        return false;
-    }
-    if (dev < 64) done[dev] |= 1u << which;
-    return true;
-}
+static thread_local uint32_t smem_allowed[64];
 template <typename P> struct Kernels { void (*k[kActs])(P, int*); };
 #define WKV7_PER_ACT(kernel) {{kernel<kActNone>, kernel<kActRelu>, kernel<kActRelu2>, kernel<kActTanh>, kernel<kActSigmoid>, kernel<kActSilu>, kernel<kActGelu>}}
 static const Kernels<TileParams> tile_kernels = WKV7_PER_ACT(linear_tile_kernel);
@@ -968,27 +997,32 @@ template <typename P> static bool launch_cluster(void (*kern)(P, int*), unsigned
     return false;
 }
 
-static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb, long long k, const Epi& e, bool swap, int nt, int splits, int* status, cudaStream_t stream) {
+static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb, long long k, const Epi& e, bool swap, int nt, int splits, int outer, void* workspace, int* status,
+                    cudaStream_t stream) {
     const auto kern = tile_kernels.k[e.act];
-    if (!allow_smem(kern, e.act, 227 * 1024)) return kLaunchFailed;
+    if (!allow_smem(kern, smem_allowed, e.act, 227 * 1024)) return kLaunchFailed;
     TileParams p;
     memset(&p, 0, sizeof(p));
     if (!encode(&p.P, a, na, k, BM) || !encode(&p.Q, b, nb, k, nt)) return kLaunchFailed;
     p.e = e;
     p.p_mn = a.mn; p.q_mn = b.mn; p.nt = nt; p.swap = swap;
-    p.direct = e.vec && !swap && splits == 1;
-    if (p.direct && !encode_results(e, &p.Y, &p.Z)) return kLaunchFailed;
+    p.outer = outer;
+    p.direct = !swap && splits == 1 && outer == 1;
+    if (p.direct && e.vec && !encode_results(e, &p.Y, &p.Z)) return kLaunchFailed;
     p.kblocks = (int)((k + BK - 1) / BK);
     p.splits = splits;
     p.p_tiles = (int)((na + BM - 1) / BM);
-    const long long tiles = p.p_tiles * ((nb + nt - 1) / nt), grid = tiles * splits;
+    const long long tiles = p.p_tiles * ((nb + nt - 1) / nt), grid = tiles * splits * outer;
     if (grid > 0x7fffffffLL) return kTooLarge;
-    const int stage = P_BYTES + q_bytes(nt), part = part_bytes(nt), most = (p.kblocks + splits - 1) / splits;
-    // CTAs that share an SM: as many as let the whole grid run at once, up to four; clusters of four and eight, two (they do not find whole free SMs everywhere)
-    int per_sm = (int)((grid + sm_count() - 1) / sm_count());
-    if (per_sm < 2 && splits > 2 && nt <= 64) per_sm = 2;
-    const int cap = nt > 64 ? 2 : 4;
-    if (per_sm > cap) per_sm = cap;
+    if (outer > 1) {
+        p.sums = (float*)workspace;
+        p.arrived = (unsigned*)((char*)workspace + tiles * outer * BM * nt * 4);
+        if (!launch(linear_zero_kernel, dim3((unsigned)((tiles * splits + 255) / 256)), 256, 0, stream, p.arrived, (int)(tiles * splits))) return kLaunchFailed;
+    }
+    const int stage = P_BYTES + q_bytes(nt), part = part_bytes(nt), most = (p.kblocks + splits * outer - 1) / (splits * outer);
+    // Two CTAs share an SM where there are more than SMs, and in clusters of four and eight of narrow tiles (they do not find whole free SMs everywhere)
+    // and three where the tiles of a wide weight then all run at once (16 x 2048 x 50001: 41 -> 37 us)
+    const int per_sm = splits == 1 && nt <= 32 && grid > 2 * sm_count() ? 3 : grid > sm_count() || (splits > 2 && nt <= 64) ? 2 : 1;
     const int room = 227 * 1024 / per_sm - 1024 - 2048 - (splits > 1 ? part : 0);  // (the system has a KB of each CTA's)
     p.stages = room / stage;
     if (p.stages < 2) p.stages = 2;
@@ -1041,7 +1075,7 @@ static size_t pair_ws(const PairPlan& x) { return x.splits > 1 ? (size_t)(x.tile
 
 static int run_pair(LinearOperand rows, LinearOperand cols, long long k, const Epi& e, const PairPlan& x, void* workspace, int* status, cudaStream_t stream) {
     const auto kern = pair_kernels.k[e.act];
-    if (!allow_smem(kern, 16 + e.act, PAIR_SMEM)) return kLaunchFailed;
+    if (!allow_smem(kern, smem_allowed, 16 + e.act, PAIR_SMEM)) return kLaunchFailed;
     PairParams p;
     memset(&p, 0, sizeof(p));
     const LinearOperand &a = x.swap ? cols : rows, &b = x.swap ? rows : cols;
@@ -1068,34 +1102,44 @@ static int run_pair(LinearOperand rows, LinearOperand cols, long long k, const E
 // Which kernel, and its shape
 struct Plan {
     bool pair, swap;
-    int nt, splits;  // of tiles of 128 x nt
+    int nt, splits, outer;  // of tiles of 128 x nt
     PairPlan x;
 };
 static Plan make_plan(long long rows, long long cols, long long k, bool rows_mn, bool can_split) {
     const int kblocks = (int)((k + BK - 1) / BK), sms = sm_count();
     Plan p{};
-    auto split = [&](long long tiles, int most) {  // CTAs of one tile: as many as fill the SMs
+    p.outer = 1;
+    auto split = [&](long long tiles, int most, int places) {  // CTAs of one tile: as many as there are places for
         int s = 1;
-        while (s < most && 2 * s <= kblocks && tiles * s * 2 <= sms) s *= 2;
+        while (s < most && 2 * s <= kblocks && tiles * s * 2 <= places) s *= 2;
         return s;
     };
     if (rows <= 64 && !rows_mn) {
         p.swap = true;
         p.nt = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-        p.splits = split((cols + BM - 1) / BM, 8);
+        // us, shared out over 1, 2, 4 and 8 CTAs a tile, two an SM: 1 x 2048 x 8192 12, 9.8, 9.7, 15; 1 x 8192 x 2048 37, 19, 12.7, 10; 1 x 2560 x 10240 14, 12.4, 17, -;
+        // 16 x 2048 x 50001 42, 46, -, -; 64 x 2048 x 2048 (parts of 34 KB) -, 11, 8.7, 9.1
+        p.splits = split((cols + BM - 1) / BM, p.nt == 64 ? 4 : 8, 2 * sms);
         return p;
     }
-    // In us: pairs 6.5 and 0.3 for a k block of 256 x 256; tiles of 128 x 128 and 128 x 64, one after the other on an SM, 6 (1.5 more to join parts) and 0.27 or 0.2 for
+    // In us: pairs 7 and 0.3 for a k block of 256 x 256; tiles of 128 x 128 and 128 x 64, one after the other on an SM, 6 (1.5 more to join parts) and 0.27 or 0.2 for
     // a k block, which is what their operands take from L2.
     p.x = plan_pair(rows, cols, kblocks, true, can_split);
-    double best = 6.5 + 0.3 * p.x.time;
+    double best = 7. + 0.3 * p.x.time;
     p.pair = true;
     for (int nt = 128; nt >= 64; nt /= 2) {
         const long long tiles = ((rows + BM - 1) / BM) * ((cols + nt - 1) / nt);
-        const int s = split(tiles, nt == 128 ? 4 : 8);
-        const double rounds = (double)((tiles * s + sms - 1) / (sms > 0 ? sms : 1));
-        const double t = 6. + (s > 1 ? 1.5 : 0.) + rounds * ((kblocks + s - 1) / s) * (nt == 128 ? 0.27 : 0.2);
-        if (t < best) { best = t; p.pair = false; p.nt = nt; p.splits = s; }
+        // (clusters of four with an SM to each CTA do not use all SMs: 36 of them ran in two rounds)
+        int s = split(tiles, nt == 128 ? 4 : 8, sms);
+        if (nt == 128 && s == 4 && tiles * s > sms - sms / 8) s = 2;
+        // few tiles and a long sum (the gradient of a narrow weight): several clusters to a tile, 16 k blocks or more to each CTA
+        long long outer = can_split ? sms / (tiles * s) : 1;
+        if (outer > kblocks / (16 * s)) outer = kblocks / (16 * s);
+        if (outer > 32) outer = 32;
+        if (outer < 2) outer = 1;
+        const double rounds = (double)((tiles * s * outer + sms - 1) / (sms > 0 ? sms : 1));
+        const double t = 6. + (s > 1 ? 1.5 : 0.) + (outer > 1 ? 4. + 0.15 * outer : 0.) + rounds * ((kblocks + s * outer - 1) / (s * outer)) * (nt == 128 ? 0.27 : 0.2);
+        if (t < best) { best = t; p.pair = false; p.nt = nt; p.splits = s; p.outer = (int)outer; }
     }
     return p;
 }
@@ -1104,7 +1148,9 @@ static Plan make_plan(long long rows, long long cols, long long k, bool rows_mn,
 
 size_t linear_workspace_bytes(long long rows, long long cols, long long k, bool rows_mn) {
     const lin::Plan p = lin::make_plan(rows, cols, k, rows_mn, true);
-    return p.pair ? lin::pair_ws(p.x) : 0;
+    if (p.pair) return lin::pair_ws(p.x);
+    const long long tiles = ((rows + lin::BM - 1) / lin::BM) * ((cols + p.nt - 1) / p.nt);
+    return p.outer > 1 ? (size_t)tiles * ((size_t)p.outer * lin::BM * p.nt * 4 + (size_t)p.splits * 4) : 0;
 }
 
 int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const LinearEpilogue& ep, void* workspace, int* status, cudaStream_t stream) {
@@ -1112,12 +1158,12 @@ int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const Lin
     Epi e;
     static_cast<LinearEpilogue&>(e) = ep;
     const int per16 = ep.y_f32 ? 4 : 8;
-    e.vec = al16(ep.y) && ep.ldy % per16 == 0 && (!ep.residual || (al16(ep.residual) && ep.ldr % per16 == 0));
+    e.vec = al16(ep.y) && ep.ldy % per16 == 0 && ep.cols % per16 == 0 && (!ep.residual || (al16(ep.residual) && ep.ldr % per16 == 0));
     e.bias_vec = al16(ep.bias);
     const Plan p = make_plan(ep.rows, ep.cols, k, rows.mn, workspace != nullptr);
     if (p.pair) return run_pair(rows, cols, k, e, p.x, workspace, status, stream);
-    if (p.swap) return run_tile(cols, rows, ep.cols, ep.rows, k, e, true, p.nt, p.splits, status, stream);
-    return run_tile(rows, cols, ep.rows, ep.cols, k, e, false, p.nt, p.splits, status, stream);
+    if (p.swap) return run_tile(cols, rows, ep.cols, ep.rows, k, e, true, p.nt, p.splits, 1, nullptr, status, stream);
+    return run_tile(rows, cols, ep.rows, ep.cols, k, e, false, p.nt, p.splits, p.outer, workspace, status, stream);
 }
 
 int linear_dz_chunks(long long M, long long N) {
@@ -1137,11 +1183,13 @@ int launch_linear_dz(const LinearDz& d, cudaStream_t stream) {
     p.rows_per = (d.M + chunks - 1) / chunks;
     p.vec = al16(d.dy) && d.lddy % (d.dy_f32 ? 4 : 8) == 0 && (!d.act || (al16(d.saved) && d.lds % (d.saved_f32 ? 4 : 8) == 0));
     const int cols = (int)((d.N + DZ_COLS - 1) / DZ_COLS);
-    void (*const kern[kActs][2])(DzParams) = {{linear_dz_kernel<kActNone, false>, nullptr}, {linear_dz_kernel<kActRelu, false>, linear_dz_kernel<kActRelu, false>},
-        {linear_dz_kernel<kActRelu2, false>, linear_dz_kernel<kActRelu2, true>}, {linear_dz_kernel<kActTanh, false>, nullptr}, {linear_dz_kernel<kActSigmoid, false>, nullptr},
-        {linear_dz_kernel<kActSilu, false>, nullptr}, {linear_dz_kernel<kActGelu, false>, nullptr}};
-    if (!kern[d.act][d.from_y]) return kBadShape;
-    if (!launch(kern[d.act][d.from_y], dim3(cols, chunks), DZ_THREADS, 0, stream, p)) return kLaunchFailed;
+#define WKV7_DZ(act, from_y) {linear_dz_kernel<act, from_y, false>, linear_dz_kernel<act, from_y, true>}
+    static void (*const kern[kActs][2])(DzParams) = {WKV7_DZ(kActNone, false), WKV7_DZ(kActRelu, false), WKV7_DZ(kActRelu2, false), WKV7_DZ(kActTanh, false),
+                                                     WKV7_DZ(kActSigmoid, false), WKV7_DZ(kActSilu, false), WKV7_DZ(kActGelu, false)};
+    const bool wide = d.dy_f32 || (d.act && d.saved_f32);
+    // (relu's derivative is the same function of its value as of its argument)
+    const auto k = d.from_y && d.act == kActRelu2 ? linear_dz_kernel<kActRelu2, true, false> : kern[d.act][wide];
+    if (!launch(k, dim3(cols, chunks), DZ_THREADS, 0, stream, p)) return kLaunchFailed;
     if (d.dbias && !launch(linear_dbias_kernel, dim3((unsigned)((d.N + 31) / 32)), 256, 0, stream, (const float*)d.partial, d.dbias, d.N, chunks)) return kLaunchFailed;
     return kOk;
 }

@@ -22,6 +22,20 @@ template <typename... P, typename... A> inline bool launch(void (*kern)(P...), d
     return false;
 }
 
+// Shared memory beyond 48 KB has to be allowed once per kernel and device; `done` is the caller's memory of it, a thread_local array, `which` a kernel's bit.
+// A thread's first call on a device (one of autograd's threads may have made no other) does so again: that gives it the context which encoding a tensor map needs.
+template <typename K> inline bool allow_smem(K kern, uint32_t (&done)[64], int which, int bytes) {
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0) return false;
+    if (dev < 64 && (done[dev] >> which & 1)) return true;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    if (dev < 64) done[dev] |= 1u << which;
+    return true;
+}
+
 struct FwdParams {
     const void *r, *w, *k, *v, *a, *b;  // [B,T,H,N], io dtype
     const void* g;                      // attn_ln only
