@@ -233,6 +233,22 @@ def test_layouts():
     assert th.equal(compare(x, w, bb[::2], r, dy, 'silu'), first)
 
 
+@pytest.mark.parametrize('M,N,K', [(20, 77, 64), (200, 77, 72), (1300, 4099, 72)])
+def test_what_lies_beside_rows_is_not_read(M, N, K):
+    """NaN behind the rows of x, w, the residual and dy, whose pitches the copies can take as they are."""
+    x, w, b, r, dy = inputs(M, N, K, th.float32, True, th.bfloat16, 5)
+
+    def wide(t):
+        n = (t.shape[1] + 7) // 8 * 8 + 8
+        o = th.full((t.shape[0] + 1, n), float('nan'), dtype=t.dtype, device='cuda')
+        o[:-1, :t.shape[1]] = t
+        return o[:-1, :t.shape[1]]
+
+    for act in (None, 'relu2'):
+        first = compare(x, w, b, r, dy, act)
+        assert th.equal(compare(wide(x), wide(w), b, wide(r), wide(dy), act), first)
+
+
 def test_empty():
     from wind_rwkv.rwkv7 import linear
     x = th.zeros(0, 64, dtype=th.bfloat16, device='cuda', requires_grad=True)

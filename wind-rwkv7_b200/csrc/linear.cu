@@ -22,6 +22,9 @@ namespace lin {
 
 constexpr int BM = 128, BK = 64;
 constexpr int MAXSTAGES = 12;
+// A wait for an accumulator lasts for a whole sum.  2^21 k blocks (k = 2^27) at 0.35 us are 0.7 s; the limit is 1.1 s.
+constexpr long long SUM_LIMIT = ACROSS_HANDOFF_LIMIT;
+constexpr int MAX_KBLOCKS = 1 << 21;
 
 // ---- activations -----------------------------------------------------------------------------------------
 constexpr float LOG2E = 1.4426950408889634f;
@@ -438,7 +441,7 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS) linear_tile_k
     }
     __syncwarp();
     if (warp < 4) {
-        mbar_wait_bounded<true>(&ctrl->accum, 0, &ctrl->abort, status);
+        mbar_wait_bounded<true>(&ctrl->accum, 0, &ctrl->abort, status, SUM_LIMIT);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
     if (p.splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -768,7 +771,7 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
                     if (row < e.rows && col < e.cols) asm volatile("prefetch.global.L2 [%0];" ::"l"((const unsigned char*)e.residual + (row * e.ldr + col) * (e.y_f32 ? 4 : 2)));
                 }
             }
-            mbar_wait_bounded<true>(&ctrl->accum_full[buf], (n >> 1) & 1, &ctrl->abort, status);
+            mbar_wait_bounded<true>(&ctrl->accum_full[buf], (n >> 1) & 1, &ctrl->abort, status, SUM_LIMIT);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (ctrl->abort) break;
             const long long p0 = (long long)w.pi * 2 * BM + rank * BM + 32 * quarter;
@@ -1160,6 +1163,7 @@ int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const Lin
     const int per16 = ep.y_f32 ? 4 : 8;
     e.vec = al16(ep.y) && ep.ldy % per16 == 0 && ep.cols % per16 == 0 && (!ep.residual || (al16(ep.residual) && ep.ldr % per16 == 0));
     e.bias_vec = al16(ep.bias);
+    if ((k + BK - 1) / BK > MAX_KBLOCKS) return kTooLarge;
     const Plan p = make_plan(ep.rows, ep.cols, k, rows.mn, workspace != nullptr);
     if (p.pair) return run_pair(rows, cols, k, e, p.x, workspace, status, stream);
     if (p.swap) return run_tile(cols, rows, ep.cols, ep.rows, k, e, true, p.nt, p.splits, 1, nullptr, status, stream);

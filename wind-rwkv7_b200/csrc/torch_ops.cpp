@@ -534,6 +534,7 @@ struct LinearFn : public Function<LinearFn> {
         if (!operand_rows(w, &ldw)) { w = dense(w); ldw = w.size(-1); }
         const int64_t K = x.size(-1), N = w.size(0), M = x.numel() / K;
         if (act && !pitched_rows(saved, &lds)) { saved = dense(saved); lds = saved.size(-1); }
+        dy = dy.to(out_f32 ? at::kFloat : at::kBFloat16);
         if (!pitched_rows(dy, &lddy)) { dy = dy.contiguous(); lddy = N; }
         Tensor db;
         if (want_dx) g[0] = at::empty(x.sizes(), x.options());
@@ -638,11 +639,11 @@ py::object reorder_states(const variable_list& states, const Tensor& parents, bo
         if (inplace && grad_mode && t.requires_grad()) return py::none();
         src[i] = t.data_ptr();
     }
-    if (inplace && count > 1) {  // rows that share memory are refused by the Python path; so, to be looked at there, are tensors within one another's extent
-        std::vector<std::pair<uintptr_t, uintptr_t>> at(count);
+    if (inplace) {  // rows that share memory are refused by the Python path; so, to be looked at there, are tensors within one another's extent
+        std::vector<std::pair<uintptr_t, uintptr_t>> at(count + 1, {(uintptr_t)parents.data_ptr(), (uintptr_t)parents.data_ptr() + parents.nbytes()});
         for (int64_t i = 0; i < count; ++i) at[i] = {(uintptr_t)src[i], (uintptr_t)src[i] + (rows - 1) * sp[i] + bytes[i]};
         std::sort(at.begin(), at.end());
-        for (int64_t i = 1; i < count; ++i)
+        for (int64_t i = 1; i <= count; ++i)
             if (at[i].first < at[i - 1].second) return py::none();
     }
     variable_list out;

@@ -150,13 +150,14 @@ def _check_reorder(states, parents, inplace):
         lays = [_row_layout(t) for t in states]
         if None in lays:
             raise ValueError('reorder_states in place takes states whose rows are contiguous and apart')
-        at = sorted((t.data_ptr(), t.shape[0], *p) for t, p in zip(states, lays))
+        at = [(t.data_ptr(), t.shape[0], *p) for t, p in zip(states, lays)]
+        at = sorted(at + [(parents.data_ptr(), 1, parents.numel() * parents.element_size(), 1)])
         for i, a in enumerate(at):
             for b in at[i + 1:]:
-                if b[0] >= a[0] + a[1] * a[3]:
+                if b[0] >= a[0] + max(a[1] * a[3], a[2]):
                     break
                 if _overlap(a, b):
-                    raise ValueError('reorder_states in place: two of the states share memory')
+                    raise ValueError('reorder_states in place: two of the states, or one and parents, share memory')
 
 
 def reorder_states(states, parents, *, inplace=False):

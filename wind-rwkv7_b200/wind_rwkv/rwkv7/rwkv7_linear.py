@@ -128,7 +128,7 @@ class Linear(th.autograd.Function):
         dx = dw = db = None
         if any(want[:3]):
             x, w, saved = ctx.saved_tensors
-            dx, dw, db = _lib.call(_bw_op, bw_linear, x, w, saved, dy, act, out_f32, from_y, want[0], want[1], want[2])
+            dx, dw, db = _lib.call(_bw_op, bw_linear, x, w, saved, dy.to(th.float32 if out_f32 else th.bfloat16), act, out_f32, from_y, want[0], want[1], want[2])
             dx, dw, db = dx if want[0] else None, dw if want[1] else None, db.to(bias_dtype) if want[2] else None
         return dx, dw, db, dy if want[3] else None, None, None
 
