@@ -15,7 +15,7 @@ namespace wkv7 {
 namespace beam {
 
 constexpr int SEG = 256;  // logits of a segment: eight a lane
-constexpr int SCAN_WARPS = 8;
+constexpr int SCAN_WARPS = 4;
 constexpr float NEG_INF = -__builtin_huge_valf(), POS_INF = __builtin_huge_valf();
 
 // floats in the order of their values, as unsigned numbers

@@ -1127,9 +1127,13 @@ static Plan make_plan(long long rows, long long cols, long long k, bool rows_mn,
     }
     // In us: pairs 7 and 0.3 for a k block of 256 x 256; tiles of 128 x 128 and 128 x 64, one after the other on an SM, 6 (1.5 more to join parts) and 0.27 or 0.2 for
     // a k block, which is what their operands take from L2.
-    p.x = plan_pair(rows, cols, kblocks, true, can_split);
-    double best = 7. + 0.3 * p.x.time;
-    p.pair = true;
+    // (Not looked at where they would be fewer than eight: planning takes the host a us.)
+    double best = 1e30;
+    if (((rows + 255) / 256) * ((cols + 127) / 128) >= 8) {
+        p.x = plan_pair(rows, cols, kblocks, true, can_split);
+        best = 7. + 0.3 * p.x.time;
+        p.pair = true;
+    }
     for (int nt = 128; nt >= 64; nt /= 2) {
         const long long tiles = ((rows + BM - 1) / BM) * ((cols + nt - 1) / nt);
         // (clusters of four with an SM to each CTA do not use all SMs: 36 of them ran in two rounds)

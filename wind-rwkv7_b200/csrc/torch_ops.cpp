@@ -496,6 +496,13 @@ std::pair<Tensor, Tensor> linear_forward(const Tensor& x, const Tensor& w, const
     return {y, z};
 }
 struct LinearFn : public Function<LinearFn> {
+    struct How {  // of the call, as one number: looking a value up by name costs half a us
+        int64_t act;
+        bool out_f32, from_y, grad, bias, bias_f32, residual;
+        int64_t pack() const { return act | out_f32 << 8 | from_y << 9 | grad << 10 | bias << 11 | bias_f32 << 12 | residual << 13; }
+        How(int64_t a, bool f, bool y, bool g, bool b, bool b32, bool r) : act(a), out_f32(f), from_y(y), grad(g), bias(b), bias_f32(b32), residual(r) {}
+        explicit How(int64_t p) : How(p & 255, p >> 8 & 1, p >> 9 & 1, p >> 10 & 1, p >> 11 & 1, p >> 12 & 1, p >> 13 & 1) {}
+    };
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias_, const OptTensor& residual_, int64_t act, bool out_f32, bool grad) {
         const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
         // relu and relu2 have their derivative in their value; of the others it is formed from the argument, kept in fp32 beside a bias in fp32, whose gradient
@@ -506,24 +513,21 @@ struct LinearFn : public Function<LinearFn> {
                                            grad && act && !from_y ? std::optional<at::ScalarType>(z32 ? at::kFloat : at::kBFloat16) : std::nullopt);
         if (grad) ctx->save_for_backward({x, w, from_y ? y : z});
         ctx->set_materialize_grads(false);
-        ctx->saved_data["act"] = act;
-        ctx->saved_data["f32"] = out_f32;
-        ctx->saved_data["from_y"] = from_y;
-        ctx->saved_data["grad"] = grad;
-        ctx->saved_data["bias"] = bias.defined() ? (int64_t)bias.scalar_type() : (int64_t)-1;
-        ctx->saved_data["residual"] = residual.defined();
+        How how{act, out_f32, from_y, grad, bias.defined(), bias.defined() && bias.scalar_type() == at::kFloat, residual.defined()};
+        ctx->saved_data["how"] = how.pack();
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list go) {
         variable_list g(7);
         Tensor dy = go[0];
         if (!dy.defined()) return g;
-        const int64_t bias = ctx->saved_data["bias"].toInt(), act = ctx->saved_data["act"].toInt();
-        const bool out_f32 = ctx->saved_data["f32"].toBool(), from_y = ctx->saved_data["from_y"].toBool();
+        const How how(ctx->saved_data["how"].toInt());
+        const int64_t act = how.act;
+        const bool out_f32 = how.out_f32, from_y = how.from_y;
         // (edges are counted over the arguments that are tensors)
-        const bool want_db = bias >= 0 && ctx->needs_input_grad(2), want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1);
-        if (ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(bias >= 0 ? 3 : 2)) g[3] = dy;
-        if (!ctx->saved_data["grad"].toBool() || !(want_dx || want_dw || want_db)) return g;
+        const bool want_db = how.bias && ctx->needs_input_grad(2), want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1);
+        if (how.residual && ctx->needs_input_grad(how.bias ? 3 : 2)) g[3] = dy;
+        if (!how.grad || !(want_dx || want_dw || want_db)) return g;
         const variable_list s = ctx->get_saved_variables();
         const c10::cuda::CUDAGuard guard(s[0].device());
         at::NoGradGuard ng;
@@ -545,7 +549,7 @@ struct LinearFn : public Function<LinearFn> {
                               M, N, K, ldx, ldw, act ? lds : N, lddy, (int)act, (out_f32 ? WKV7_LINEAR_F32_OUT : 0) | (from_y ? WKV7_LINEAR_FROM_Y : 0) |
                               (act && saved.scalar_type() == at::kFloat ? WKV7_LINEAR_F32_Z : 0), ws.data_ptr(), stream()),
               "wkv7_linear_bwd");
-        if (want_db) g[2] = db.to((at::ScalarType)bias);
+        if (want_db) g[2] = how.bias_f32 ? db : db.to(at::kBFloat16);
         return g;
     }
 };
