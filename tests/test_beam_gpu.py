@@ -146,6 +146,23 @@ def test_finished():
                     compare(logits, scores, k, finished, eos)
 
 
+def test_refusals_with_device_tensors():
+    from wind_rwkv.rwkv7 import beam_select, reorder_states
+    logits, scores = make(2, 4, 100)
+    fin = th.zeros(2, 4, dtype=th.bool, device='cuda')
+    for bad in (dict(eos=-1), dict(eos=3), dict(finished=fin), dict(finished=fin, eos=-1), dict(finished=fin, eos=100), dict(k=0), dict(k=-1), dict(k=65)):
+        with pytest.raises(ValueError, match='beam_select'):
+            beam_select(logits, scores, **bad)
+    with pytest.raises(RuntimeError):
+        beam_select(logits, scores.cpu())
+    t, p = th.zeros(8, 6, device='cuda'), th.zeros(2, 4, dtype=th.int64, device='cuda')
+    for states, parents in (([t, t], p), ([t[:, :4], t[:, 3:]], p), ([p.view(8, 1)], p), ([t], p[:, :3]), ([t[:7]], p)):
+        with pytest.raises(ValueError, match='reorder_states'):
+            reorder_states(states, parents, inplace=True)
+    with pytest.raises(RuntimeError):
+        reorder_states([t, t.cpu()], p)
+
+
 def test_layouts():
     base, scores = make(3, 5, 4100)
     for view in (base[:, :, 1:], base[:, :, 3:4000], base.transpose(0, 1)[:3, :3], base[:, ::2], base[..., ::3], base[:, :, 8:4096]):

@@ -161,6 +161,25 @@ def test_results_go_where_they_belong():
         check('dw', dw, D.T @ X, U * (D.T @ X).abs() + acc(M) * (D.abs().T @ X.abs()))
 
 
+def test_large_offsets():
+    """Results and gradients beyond 2^31 elements."""
+    from wind_rwkv.rwkv7 import linear
+    M, N, K = 66000, 33000, 16
+    x, w = [inputs(n, 1, K, None, False, th.bfloat16, n)[0] for n in (M, N)]
+    x.requires_grad_()
+    y = linear(x, w, act='relu2')
+    for rows in (slice(0, 3), slice(M - 3, M)):
+        ref = th.relu(x.detach()[rows].double() @ w.double().T).square()
+        check('y', y[rows], ref, U * ref + 2.0 ** -18 * (1 + ref) * K)
+    dy = th.zeros_like(y)
+    dy[M - 2, N - 5:] = 1.
+    dx, = th.autograd.grad(y, x, dy)
+    z = th.relu(x.detach()[M - 2].double() @ w[N - 5:].double().T)
+    ref = (2 * z) @ w[N - 5:].double()
+    check('dx', dx[M - 2], ref, 3 * U * ((2 * z) @ w[N - 5:].double().abs()) + 1e-6)
+    assert not dx[:M - 2].any() and not dx[M - 1].any()
+
+
 def test_without_workspace():
     """wkv7_linear_fwd with a null workspace: the same sums in another order."""
     from wind_rwkv.rwkv7 import _lib

@@ -593,7 +593,7 @@ py::object beam_select(const Tensor& logits, const Tensor& scores, int64_t k, co
     if ((!f32 && logits.scalar_type() != at::kBFloat16) || (V > 1 && logits.stride(2) != 1) || scores.scalar_type() != at::kFloat || !scores.is_contiguous() ||
         scores.device() != logits.device() || scores.size(0) != B || scores.size(1) != W || W > 64 || k < 1 || k > 64 || k > W * V)
         return py::none();
-    if (finished.defined() != (eos >= 0) || eos >= V) return py::none();
+    if (finished.defined() != (eos != -1) || eos < -1 || eos >= V) return py::none();  // (-1: none given)
     if (finished.defined() && (!plain(finished) || finished.scalar_type() != at::kBool || !finished.is_contiguous() || finished.device() != logits.device() ||
                                finished.dim() != 2 || finished.size(0) != B || finished.size(1) != W))
         return py::none();

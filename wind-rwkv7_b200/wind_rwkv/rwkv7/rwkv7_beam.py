@@ -74,7 +74,7 @@ def beam_select(logits, scores, k=None, *, finished=None, eos=None):
     ended.  Up to 64 beams and 64 results.  No autograd."""
     k = logits.shape[1] if k is None and logits.dim() == 3 else k
     if not th.compiler.is_compiling():
-        out = _lib.ext().beam_select(logits, scores, -1 if k is None else k, finished, -1 if eos is None else eos)
+        out = _lib.ext().beam_select(logits, scores, -1 if k is None else k, finished, -1 if eos is None else eos if eos >= 0 else -2)
         if out is not None:
             return out
         _check_select(logits, scores, k, finished, eos)
