@@ -70,7 +70,7 @@ def make(B, W, V, dtype=th.bfloat16, seed=0, std=3.0):
 
 @pytest.mark.parametrize('dtype', [th.bfloat16, th.float32])
 @pytest.mark.parametrize('B,W,V,k', [(1, 1, 1, 1), (1, 1, 7, 7), (2, 3, 1, 3), (1, 4, 256, 4), (3, 5, 257, 10), (2, 1, 1000, 32), (4, 6, 5003, 6), (1, 4, 65536, 4),
-                                     (2, 8, 50001, 16), (1, 64, 3001, 64), (3, 16, 8192, 64), (2, 32, 131072, 32), (70, 4, 300, 8)])
+                                     (2, 8, 50001, 16), (1, 64, 3001, 64), (3, 16, 8192, 64), (2, 32, 131072, 32), (70, 4, 300, 8), (8, 23, 3577, 46)])
 def test_sizes(B, W, V, k, dtype):
     logits, scores = make(B, W, V, dtype)
     compare(logits, scores, k)
@@ -118,6 +118,20 @@ def test_equal_scores(V):
     logits, scores = make(2, 6, V)
     compare((logits / 4).round(), scores, 64)
     compare(logits.expand(2, 6, V)[:, :1].expand(2, 6, V), scores.fill_(0.), 7)          # one row for all beams
+
+
+@pytest.mark.parametrize('W,V', [(8, 65536), (5, 20001)])
+def test_few_allowed(W, V):
+    """A mask of the type's lowest value, or of -inf, that leaves the same few tokens to all beams: more and fewer than are asked for."""
+    for dtype in (th.bfloat16, th.float32):
+        for fill in (th.finfo(dtype).min, -INF):
+            for left in (slice(0, 3), slice(V // 2, V // 2 + 40), slice(V - 1, V)):
+                logits, scores = make(2, W, V, dtype)
+                keep = logits[..., left].clone()
+                logits.fill_(fill)
+                logits[..., left] = keep
+                for k in (W, 64):
+                    compare(logits, scores, k)
 
 
 def test_orders():

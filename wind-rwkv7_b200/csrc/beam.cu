@@ -16,7 +16,7 @@ namespace beam {
 
 constexpr int SEG = 256;  // logits of a segment: eight a lane
 constexpr int SCAN_WARPS = 4;
-constexpr float NEG_INF = -__builtin_huge_valf(), POS_INF = __builtin_huge_valf();
+constexpr float LOWEST = -3.402823466e38f, NEG_INF = -__builtin_huge_valf(), POS_INF = __builtin_huge_valf();
 
 // floats in the order of their values, as unsigned numbers
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -193,20 +193,22 @@ template <bool F32, bool ALIGNED> __global__ void __launch_bounds__(32 * SCAN_WA
     }
 }
 
-constexpr int PICK_THREADS = 1024, CAP = 256, LIST = PICK_THREADS + BEAM_MAX_K;
+// SEGS segments and LIST candidates above the threshold fit; up to RANKED candidates each finds its own place (n / 32 squared steps of a warp), beyond that the best
+// are taken out one by one (k rounds of the CTA).
+constexpr int PICK_THREADS = 1024, SEGS = 512, LIST = 2 * PICK_THREADS, RANKED = 320;
 struct Pick {
     double top[BEAM_MAX_W], logz[BEAM_MAX_W], base[BEAM_MAX_W];  // a beam's largest logit, log sum exp(l - top), score
     float offset[BEAM_MAX_W], least[BEAM_MAX_W];                 // about base - top - logz; the least logit that may reach the threshold
     double score[LIST];
     uint32_t index[LIST];
-    int2 segs[CAP];        // beam, segment
+    int2 segs[SEGS];       // beam, segment
     uint32_t group[128];   // the best of each group of threads
     unsigned char fin[BEAM_MAX_W];
     double best_score[32];
     uint32_t best_index[32];
     double out_score[BEAM_MAX_K];
     uint32_t out_index[BEAM_MAX_K];
-    int nsegs, n;
+    int nsegs, n, count[32];
     float t;
     unsigned char ruled_out[2 * BEAM_MAX_K];
 };
@@ -228,6 +230,7 @@ __device__ __forceinline__ void logits8(const BeamParams& p, const Pick& q, long
 }
 
 // the k best of q.score[0 .. n), n <= LIST, in order, to the front; all threads.  Each round takes the best that is left.
+// (All have read their part of the list before the first barrier.)
 __device__ __forceinline__ void keep_best(Pick& q, int n, int k) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     double s[2];
@@ -280,16 +283,13 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
     if (tid == 0) { q.nsegs = 0; q.n = 0; }
     if (tid < 128) q.group[tid] = 0;
     stream_order();
-    // warps to a beam, and of a beam's segments those 32 * wide apart to a lane; their maxima are requested here and used behind the normalisers
-    const int wide = p.W < 32 ? 32 / p.W : 1, per_round = 32 / wide;
+    // a thread has every 1024th of the sequence's segments; their maxima are requested here and used behind the normalisers
+    const int total = p.W * p.segments;
+    const float* const seg_max = p.seg_max + row0 * p.segments;
     constexpr int HELD = 4;
     float held[HELD];
-    const int my_w = warp / wide, my_g = warp % wide * 32 + lane;
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        const int g = my_g + i * 32 * wide;
-        held[i] = my_w < p.W && my_w < per_round && g < p.segments ? p.seg_max[(row0 + my_w) * p.segments + g] : NEG_INF;
-    }
+    for (int i = 0; i < HELD; ++i) held[i] = tid + i * PICK_THREADS < total ? seg_max[tid + i * PICK_THREADS] : NEG_INF;
     // the beams' normalisers, a warp each: the parts' sums joined in 64 bits, in a fixed order
     for (int w = warp; w < p.W; w += 32) {
         const float2* part = reinterpret_cast<const float2*>(p.part) + (row0 + w) * p.parts;
@@ -322,16 +322,16 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
         const float s = l + q.offset[w];
         return s == NEG_INF ? 0u : ordered(s - 2.4e-7f * (fabsf(l) + fabsf(q.offset[w])));
     };
-    auto more_segments = [&](auto f) {  // those that are not held
-        if (my_w >= per_round) return;
-        for (int w = my_w, from = my_g + HELD * 32 * wide; w < p.W; w += per_round, from = my_g)
-            for (int g = from; g < p.segments; g += 32 * wide) f(w, g, p.seg_max[(row0 + w) * p.segments + g]);
+    auto each_segment = [&](auto f) {  // f(beam, segment, maximum)
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const int c = tid + i * PICK_THREADS, w = c / p.segments;
+            if (c < total) f(w, c - w * p.segments, held[i]);
+        }
+        for (int c = tid + HELD * PICK_THREADS; c < total; c += PICK_THREADS) f(c / p.segments, c % p.segments, seg_max[c]);
     };
     uint32_t best = 0;
-    if (my_w < p.W && my_w < per_round)
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) best = max(best, at_least(my_w, held[i]));
-    more_segments([&](int w, int, float l) { best = max(best, at_least(w, l)); });
+    each_segment([&](int w, int, float l) { best = max(best, at_least(w, l)); });
     const int groups = k <= 16 ? 32 : k <= 32 ? 64 : 128;
     atomicMax(&q.group[tid & (groups - 1)], best);
     __syncthreads();
@@ -339,28 +339,26 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
         const uint32_t mine = q.group[g];
         int ahead = 0;
         for (int i = lane; i < groups; i += 32) ahead += __popc(__ballot_sync(0xffffffffu, q.group[i] > mine || (q.group[i] == mine && i < g)));
-        if (ahead == k - 1 && lane == 0) q.t = mine ? unordered(mine) : -3.402823466e38f;
+        if (ahead == k - 1 && lane == 0) q.t = mine ? unordered(mine) : LOWEST;
     }
     __syncthreads();
-    // score >= t is l >= (t - base + logz) + top, less a little for the roundings on the way
-    if (tid < p.W) {
-        const double t = q.t, l = ((t - q.base[tid]) + q.logz[tid]) + q.top[tid];
-        q.least[tid] = __double2float_rd(l - 1e-15 * (fabs(t) + fabs(q.base[tid]) + fabs(q.top[tid]) + 64.));
-    }
-    __syncthreads();
-    auto list_segment = [&](int w, int g, float l) {
-        if (l >= q.least[w] && l > NEG_INF) {
-            const int i = atomicAdd(&q.nsegs, 1);
-            if (i < CAP) q.segs[i] = make_int2(w, g);
+    // the segments that reach t, and their candidates that do
+    auto list = [&] {
+        // score >= t is l >= (t - base + logz) + top, less a little for the roundings on the way
+        if (tid < p.W) {
+            const double t = q.t, l = ((t - q.base[tid]) + q.logz[tid]) + q.top[tid];
+            q.least[tid] = __double2float_rd(l - 1e-15 * (fabs(t) + fabs(q.base[tid]) + fabs(q.top[tid]) + 64.));
         }
-    };
-    if (my_w < p.W && my_w < per_round)
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) list_segment(my_w, my_g + i * 32 * wide, held[i]);
-    more_segments(list_segment);
-    __syncthreads();
-    const int nsegs = q.nsegs;
-    if (nsegs <= CAP) {
+        __syncthreads();
+        each_segment([&](int w, int g, float l) {
+            if (l >= q.least[w] && l > NEG_INF) {
+                const int i = atomicAdd(&q.nsegs, 1);
+                if (i < SEGS) q.segs[i] = make_int2(w, g);
+            }
+        });
+        __syncthreads();
+        const int nsegs = q.nsegs;
+        if (nsegs > SEGS) return false;
         for (int i = warp; i < nsegs; i += 32) {
             const int w = q.segs[i].x, at = q.segs[i].y * SEG + 8 * lane;
             float l[8];
@@ -369,13 +367,35 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
             for (int e = 0; e < 8; ++e)
                 if (l[e] >= q.least[w] && (float)score_of(q, w, l[e]) > NEG_INF) {
                     const int j = atomicAdd(&q.n, 1);
-                    if (j < CAP) { q.score[j] = score_of(q, w, l[e]); q.index[j] = w * p.V + at + e; }
+                    if (j < LIST) { q.score[j] = score_of(q, w, l[e]); q.index[j] = w * p.V + at + e; }
                 }
         }
         __syncthreads();
+        return q.n <= LIST;
+    };
+    bool listed = list();
+    if (!listed) {
+        // Too many: the groups' threshold is the exact one only as far as the best segments lie in different groups.  (A mask of the type's lowest value that leaves a few
+        // tokens puts them in a few segments.)  The exact one, bit by bit, and once more.
+        uint32_t t = 0;
+        if (tid < 32) q.count[tid] = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            __syncthreads();
+            const uint32_t trial = t | 1u << bit;
+            int c = 0;
+            each_segment([&](int w, int, float l) { c += at_least(w, l) >= trial; });
+            c = __reduce_add_sync(0xffffffffu, c);
+            if (lane == 0 && c) atomicAdd(&q.count[bit], c);
+            __syncthreads();
+            if (q.count[bit] >= k) t = trial;
+        }
+        __syncthreads();
+        if (tid == 0) { q.t = t ? unordered(t) : LOWEST; q.nsegs = 0; q.n = 0; }
+        __syncthreads();
+        listed = list();
     }
-    int n = q.n;
-    if (nsegs <= CAP && n <= CAP) {
+    int n = listed ? q.n : 0;
+    if (listed && n <= RANKED) {
         // each candidate's place is the number of better ones
         for (int c = warp; c < n; c += 32) {
             const double s = q.score[c];
@@ -385,48 +405,55 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
             if (place < k && lane == 0) { q.out_score[place] = s; q.out_index[place] = ix; }
         }
         n = min(n, k);
+    } else if (listed) {
+        keep_best(q, n, k);
+        n = min(n, k);
     } else {
-        // many equal or nearly equal ones: all segments that reach t in order, with the k best so far at the front of the list; a candidate joins it only if it
-        // is better than the last of those, which one of equal score behind it is not
+        // Many equal or nearly equal ones: all that reach t in order, into a list whose first `kept` are the k best so far.  A candidate joins it only if it
+        // is better than the last of those, which one of equal score behind it is not.  The list is thinned out when it might not take another step's.
         __syncthreads();
         if (tid == 0) q.n = 0;
         __syncthreads();
-        int kept = 0;
-        for (long long c0 = 0; c0 < (long long)p.W * p.segments * (SEG / 8); c0 += PICK_THREADS / 8) {
-            // 128 threads' worth of eight candidates: 1024 at most join at once
-            if (tid < PICK_THREADS / 8) {
-                const long long c = c0 + tid;
-                const int g = (int)(c / (SEG / 8));
-                if (g < p.W * p.segments) {
-                    const int w = g / p.segments, at = (g - w * p.segments) * SEG + 8 * (int)(c % (SEG / 8));
-                    const float l = p.seg_max[row0 * p.segments + g];
-                    if (l >= q.least[w] && l > NEG_INF) {
-                        float f[8];
-                        logits8(p, q, seq, w, at, f);
+        int kept = 0, filled = 0;
+        constexpr int STEP = PICK_THREADS / 8;  // threads whose eight candidates each join in one step: 1024 at most
+        for (long long c0 = 0; c0 < (long long)total * (SEG / 8); c0 += PICK_THREADS) {
+            const long long c = c0 + tid;
+            const int g = (int)(c / (SEG / 8)), w = g < total ? g / p.segments : 0, at = (g - w * p.segments) * SEG + 8 * (int)(c % (SEG / 8));
+            const float l = g < total ? seg_max[g] : NEG_INF;
+            float f[8];
+            uint32_t mask = 0;
+            auto joins = [&](int e) {
+                const double s = score_of(q, w, f[e]);
+                return f[e] >= q.least[w] && (float)s > NEG_INF && (kept < k || better(s, (uint32_t)(w * p.V + at + e), q.score[k - 1], q.index[k - 1]));
+            };
+            if (l >= q.least[w] && l > NEG_INF) {
+                logits8(p, q, seq, w, at, f);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const uint32_t ix = (uint32_t)(w * p.V + at + e);
-                            const double s = score_of(q, w, f[e]);
-                            if (f[e] >= q.least[w] && (float)s > NEG_INF && (kept < k || better(s, ix, q.score[k - 1], q.index[k - 1]))) {
-                                const int j = kept + atomicAdd(&q.n, 1);
-                                q.score[j] = s;
-                                q.index[j] = ix;
-                            }
-                        }
-                    }
-                }
+                for (int e = 0; e < 8; ++e) mask |= joins(e) ? 1u << e : 0u;
             }
-            __syncthreads();
-            const int fresh = q.n;
-            __syncthreads();
-            if (fresh) {
-                if (tid == 0) q.n = 0;
-                keep_best(q, kept + fresh, k);
-                kept = min(kept + fresh, k);
+            if (!__syncthreads_or(mask != 0)) continue;
+            for (int step = 0; step < PICK_THREADS; step += STEP) {
+                if (mask && tid >= step && tid < step + STEP) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if ((mask >> e & 1) && joins(e)) {
+                            const int j = atomicAdd(&q.n, 1);
+                            q.score[j] = score_of(q, w, f[e]);
+                            q.index[j] = (uint32_t)(w * p.V + at + e);
+                        }
+                }
+                __syncthreads();
+                filled = q.n;
+                if (filled > LIST - PICK_THREADS) {
+                    keep_best(q, filled, k);
+                    filled = kept = min(filled, k);
+                    if (tid == 0) q.n = kept;
+                }
+                __syncthreads();
             }
         }
-        if (tid < kept) { q.out_score[tid] = q.score[tid]; q.out_index[tid] = q.index[tid]; }
-        n = kept;
+        keep_best(q, filled, k);
+        n = min(filled, k);
     }
     __syncthreads();
     if (n < k) {

@@ -983,23 +983,6 @@ template <typename P> struct Kernels { void (*k[kActs])(P, int*); };
 static const Kernels<TileParams> tile_kernels = WKV7_PER_ACT(linear_tile_kernel);
 static const Kernels<PairParams> pair_kernels = WKV7_PER_ACT(linear_pair_kernel);
 
-template <typename P> static bool launch_cluster(void (*kern)(P, int*), unsigned grid, unsigned threads, int smem, int cluster, cudaStream_t stream, const P& p, int* status) {
-    cudaLaunchConfig_t c{};
-    c.gridDim = dim3(grid); c.blockDim = dim3(threads); c.dynamicSmemBytes = smem; c.stream = stream;
-    cudaLaunchAttribute attr[2]{};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    c.attrs = attr; c.numAttrs = 1;
-    if (cluster > 1) {
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
-        c.numAttrs = 2;
-    }
-    if (cudaLaunchKernelEx(&c, kern, p, status) == cudaSuccess) return true;
-    cudaGetLastError();
-    return false;
-}
-
 static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb, long long k, const Epi& e, bool swap, int nt, int splits, int outer, void* workspace, int* status,
                     cudaStream_t stream) {
     const auto kern = tile_kernels.k[e.act];
@@ -1038,7 +1021,7 @@ static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb
     p.tmem_cols = 32;
     while ((int)p.tmem_cols < nt * p.accs) p.tmem_cols *= 2;
     const int ring = splits > 1 ? p.stages * stage + part : p.stages * stage > part ? p.stages * stage : part;
-    return launch_cluster(kern, (unsigned)grid, TILE_THREADS, 2048 + ring, splits, stream, p, status) ? kOk : kLaunchFailed;
+    return launch_clusters(kern, dim3((unsigned)grid), TILE_THREADS, 2048 + ring, splits, stream, p, status) ? kOk : kLaunchFailed;
 }
 
 static long long pairs_of_sms() { const int n = sm_count() / 2; return n > 0 ? n : 1; }  // (asked for sizes without a device, too)
@@ -1099,7 +1082,7 @@ static int run_pair(LinearOperand rows, LinearOperand cols, long long k, const E
     }
     const long long pairs = pairs_of_sms(), units = x.whole + (x.tiles - x.whole) * x.splits;
     const unsigned grid = 2 * (unsigned)(units < pairs ? units : pairs);
-    return launch_cluster(kern, grid, PAIR_THREADS, PAIR_SMEM, 1, stream, p, status) ? kOk : kLaunchFailed;
+    return launch_clusters(kern, dim3(grid), PAIR_THREADS, PAIR_SMEM, 1, stream, p, status) ? kOk : kLaunchFailed;
 }
 
 // Which kernel, and its shape

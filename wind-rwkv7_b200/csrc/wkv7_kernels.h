@@ -10,16 +10,22 @@ namespace wkv7 {
 // closely.  Without / with this alone, us: B32 T1024 C768, ddlerp forward and backward 307 / 288, expand_loras 277 / 269, time mixer 2104 /
 // 2073; layer of 515 rows, C = 2048, forward 149 / 134; attn forward and backward, B3 T1003 H16 170 / 163, fp32 B8 T512 H12 289 / 285.  (Not so
 // launched, since it did not pay: the fp32 forward, B8 T512 H12 287 -> 293 us, and the sums between the two walks of time_split, 497 -> 521.)
-template <typename... P, typename... A> inline bool launch(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, A&&... args) {
+// launch_clusters: in clusters of `cluster` CTAs (1: as the kernel says).
+template <typename... P, typename... A> inline bool launch_clusters(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem, int cluster, cudaStream_t stream, A&&... args) {
     cudaLaunchConfig_t c{};
     c.gridDim = grid; c.blockDim = dim3(threads); c.dynamicSmemBytes = smem; c.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    c.attrs = &attr; c.numAttrs = 1;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+    c.attrs = attr; c.numAttrs = cluster > 1 ? 2 : 1;
     if (cudaLaunchKernelEx(&c, kern, std::forward<A>(args)...) == cudaSuccess) return true;
     cudaGetLastError();  // (reported by the status; not left for the caller's next check)
     return false;
+}
+template <typename... P, typename... A> inline bool launch(void (*kern)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, A&&... args) {
+    return launch_clusters(kern, grid, threads, smem, 1, stream, std::forward<A>(args)...);
 }
 
 // Shared memory beyond 48 KB has to be allowed once per kernel and device; `done` is the caller's memory of it, a thread_local array, `which` a kernel's bit.
