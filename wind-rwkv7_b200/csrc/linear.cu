@@ -667,6 +667,8 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
         ctrl->abort = 0; ctrl->zero = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (waited for behind the rest of the preparation)
     if (warp == 3 && elect_one()) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&p.P) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&p.Q) : "memory");
@@ -678,7 +680,7 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    cluster_sync();  // the other CTA's barriers are set up
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the other CTA's barriers are set up
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = ctrl->tmem_base;
     stream_wait();
