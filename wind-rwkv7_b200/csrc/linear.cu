@@ -193,6 +193,60 @@ template <bool TURNED> __device__ __forceinline__ void bulk_store_block(float* s
     }
 }
 
+// The same for two bf16 blocks side by side, a lane a row: one wait and one fence for both.
+__device__ __forceinline__ void bulk_store_two(float* staging, const CUtensorMap* map, const float (&v)[2][32], int lane, long long col0, long long row0) {
+    unsigned char* to = reinterpret_cast<unsigned char*>(staging);
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<uint4*>(to + 2048 * h + lane * 64 + ((u ^ (lane >> 1 & 3)) << 4)) =
+                make_uint4(pack_bf16x2(v[h][8 * u], v[h][8 * u + 1]), pack_bf16x2(v[h][8 * u + 2], v[h][8 * u + 3]),
+                           pack_bf16x2(v[h][8 * u + 4], v[h][8 * u + 5]), pack_bf16x2(v[h][8 * u + 6], v[h][8 * u + 7]));
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                         ::"l"(map), "r"((int)col0 + 32 * h), "r"((int)row0), "r"(smem_u32(to + 2048 * h)) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+}
+// Two blocks side by side, wholly among the columns and all bf16: one block's latencies are spent on the other.
+template <int ACT, typename Sums> __device__ __forceinline__ void finish_rows_two(const Epi& e, const CUtensorMap* Y, const CUtensorMap* Z, float* mine, int lane, long long row0, long long col0,
+                                                                                 Sums sums) {
+    const bool in = row0 + lane < e.rows;
+    const long long at = (row0 + lane) * e.ldr + col0;
+    uint4 res[8];
+    if (e.residual && in)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) res[c] = *reinterpret_cast<const uint4*>((const bf16*)e.residual + at + 8 * c);
+    float v[2][32];
+    sums(v);
+    if (e.bias)
+#pragma unroll
+        for (int c = 0; c < 64; c += 8) {
+            float f[8];
+            bias8(e, col0 + c, f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c / 32][c % 32 + i] += f[i];
+        }
+    if (e.z) bulk_store_two(mine, Z, v, lane, col0, row0);
+#pragma unroll
+    for (int c = 0; c < 64; ++c) v[c / 32][c % 32] = act<ACT>(v[c / 32][c % 32]);
+    if (e.residual && in)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            float f[8];
+            unpack8(res[c], f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c / 4][8 * (c % 4) + i] += f[i];
+        }
+    bulk_store_two(mine, Y, v, lane, col0, row0);
+}
 // A warp's block of 32 x 32, a lane a column of y; the sums come by sums(v).  Rows that are not aligned are stored, 32 adjacent elements an instruction, as they lie.
 template <int ACT, typename Sums> __device__ __forceinline__ void finish_cols(const Epi& e, const CUtensorMap* Y, const CUtensorMap* Z, float* mine, bool mixed, int lane, int& turn,
                                                                              long long row0, long long col0, Sums sums) {
@@ -355,7 +409,7 @@ __host__ __device__ constexpr int part_bytes(int nt) { return BM * part_pitch(nt
 
 __device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
-template <int ACT> __global__ void __launch_bounds__(TILE_THREADS) linear_tile_kernel(const __grid_constant__ TileParams p, int* status) {
+template <int ACT> __global__ void __launch_bounds__(TILE_THREADS, 3) linear_tile_kernel(const __grid_constant__ TileParams p, int* status) {
     extern __shared__ unsigned char smem_dyn[];
     TileCtrl* ctrl = reinterpret_cast<TileCtrl*>(smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u));
     unsigned char* sm = reinterpret_cast<unsigned char*>(ctrl) + 1024;
@@ -466,9 +520,11 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS) linear_tile_k
                         for (int i = 0; i < 32; ++i) v[i] += u[i];
                     }
                 };
-                if (p0 + 32 * warp >= e.rows || q0 + c >= e.cols) continue;
-                if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, p0 + 32 * warp, q0 + c, sums);
-                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, p0 + 32 * warp, q0 + c, [&](float (&v)[32]) { sums(v); turn_block(mine, lane, v); });
+                // (blocks two by two, as the pairs have them, would take 190 registers and more: one CTA an SM)
+                const int row0 = p0 + 32 * warp, col0 = q0 + c;
+                if (row0 >= e.rows || col0 >= e.cols) continue;
+                if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, sums);
+                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); turn_block(mine, lane, v); });
             }
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
@@ -762,7 +818,8 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
         float* mine = reinterpret_cast<float*>(staging + (warp - 4) * PAIR_STAGING);
         int turn = 0;
         const Epi& e = p.e;
-        const bool mixed = e.z && e.z_f32 != e.y_f32;
+        const bool two = e.vec && !p.swap && !e.y_f32 && !(e.z && e.z_f32);  // blocks go two by two
+        const bool mixed = two || (e.z && e.z_f32 != e.y_f32);               // stores do not take the staging area's halves in turn
         const int blocks = p.bn / 32, b0 = side ? (blocks + 1) / 2 : 0, b1 = side ? blocks : (blocks + 1) / 2;
         for (int n = 0; pair_work(p, n, w); ++n) {
             const int buf = n & 1;
@@ -808,6 +865,15 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
             for (int b = b0; b < b1; ++b) {
                 const long long q0 = (long long)w.qi * p.bn + 32 * b;
                 const long long row0 = p.swap ? q0 : p0, col0 = p.swap ? p0 : q0;
+                if (two && !parts && b + 1 < b1 && row0 < e.rows && col0 + 64 <= e.cols) {
+                    finish_rows_two<ACT>(e, &p.Y, &p.Z, mine, lane, row0, col0, [&](float (&v)[2][32]) {
+                        tmem_ld32(acc + 32 * b, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+                        tmem_ld32(acc + 32 * b + 32, reinterpret_cast<uint32_t(&)[32]>(v[1]));
+                        if (b + 1 == b1 - 1) emptied();
+                    });
+                    ++b;
+                    continue;
+                }
                 auto sums = [&](float (&v)[32]) {
                     if (parts) {
                         const float4* from = parts + (b - b0) * 256;
