@@ -222,6 +222,8 @@ def test_large_arguments():
     x, w, _, _, dy = inputs(70, 96, 64, None, False, th.bfloat16, 3)
     for act in F64:
         compare(x * 64, w, None, None, dy, act)
+        if act != 'relu2':  # (whose values leave the range)
+            compare(x * 1e19, w, None, None, dy, act)
 
 
 def test_layouts():

@@ -59,12 +59,13 @@ template <int ACT> __device__ __forceinline__ float act(float x) {
 // act'(z); FROM_Y: of relu and relu2 from their values, 2 sqrt(y) for 2 relu(z)
 template <int ACT, bool FROM_Y> __device__ __forceinline__ float act_grad(float z) {
     switch (ACT) {
-        case kActRelu: return z > 0.f ? 1.f : 0.f;
+        case kActRelu: return z <= 0.f ? 0.f : 1.f;
         case kActRelu2: return FROM_Y ? 2.f * sqrt_f(z) : 2.f * relu_f(z);
         case kActTanh: { const float e = ex2_approx(-2.f * LOG2E * fabsf(z)), r = rcp_mufu(1.f + e); return 4.f * e * r * r; }
         case kActSigmoid: { const float s = sigmoid_f(z); return s * (1.f - s); }
         case kActSilu: { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }
         case kActGelu: {
+            z = z > 64.f ? 64.f : z < -64.f ? -64.f : z;  // (1 and 0 long before; z^3 would leave fp32's range)
             const float s = gelu_s(z);
             return s + z * s * (1.f - s) * GELU_C * (1.f + 3.f * 0.044715f * z * z);
         }
