@@ -318,6 +318,28 @@ def test_gradient_against_differences():
         assert abs(float(got - num)) <= 4 * U * float(scale)
 
 
+@pytest.mark.parametrize('B,T,C,F', [(1, 1, 128, 512), (3, 77, 192, 640), (2, 700, 512, 2048)])
+def test_channel_mixer_training(B, T, C, F):
+    """Both halves of a channel mixer, as a model trains them: x + relu2(x wk^T) wv^T.  Between the inputs and each gradient lie at most six roundings to bf16
+    (h, y; dh and its dz; the gradient's two terms and their sum), of u each relative to what is rounded: 6 u in the L2 norm, relative to the norm of the
+    larger of the result and its terms."""
+    from wind_rwkv.rwkv7 import linear
+    g = th.Generator(device='cuda').manual_seed(B + T)
+
+    def rn(*s, std=1.0):
+        return (th.randn(*s, generator=g, device='cuda') * std).bfloat16()
+
+    x, wk, wv, dy = rn(B, T, C), rn(F, C, std=C ** -0.5), rn(C, F, std=F ** -0.5), rn(B, T, C)
+    leaves = [t.clone().requires_grad_() for t in (x, wk, wv)]
+    y = linear(linear(leaves[0], leaves[1], act='relu2'), leaves[2], residual=leaves[0])
+    grads = th.autograd.grad(y, leaves, dy)
+    ref = [t.double().requires_grad_() for t in (x, wk, wv)]
+    Y = ref[0] + th.relu(ref[0] @ ref[1].T).square() @ ref[2].T
+    want = th.autograd.grad(Y, ref, dy.double())
+    for a, b in ((y.detach(), Y.detach()), *zip(grads, want)):
+        assert float((a.double() - b).norm()) <= 6 * U * float(b.norm())
+
+
 def test_same_results_every_time_and_in_a_graph():
     from wind_rwkv.rwkv7 import linear
     for M, N, K in ((1, 2048, 2048), (300, 96, 2048), (1400, 3328, 512)):
