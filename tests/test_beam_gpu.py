@@ -134,6 +134,71 @@ def test_few_allowed(W, V):
                     compare(logits, scores, k)
 
 
+FILLS = (-1e4, -65504., -1e6, -1e8, -1e9, -2e9, -1e10, -1e12, 1e6, 1e9)
+
+
+@pytest.mark.parametrize('dtype', [th.bfloat16, th.float32])
+@pytest.mark.parametrize('W,V', [(4, 4096), (5, 3001), (2, 263000)])
+def test_masks_of_any_size(W, V, dtype):
+    """Masks of the constants that programs write: whole beams, beams that are not there, rows with a few tokens left, everything; a beam that has ended among them."""
+    for fill in FILLS:
+        for whole in ([1], [0, 1], list(range(W))):
+            logits, scores = make(2, W, V, dtype)
+            logits[:, whole] = fill
+            finished = th.arange(2 * W, device='cuda').view(2, W) % 4 == 2
+            for k in (1, W, 64):
+                compare(logits, scores, k)
+            compare(logits, scores, W, finished, V - 1)
+            scores[:, whole] = -INF
+            compare(logits, scores, W)
+            compare(logits, scores, 2 * W, finished, 0)
+        for left in (1, 3, 40):
+            logits, scores = make(2, W, V, dtype, seed=left)
+            keep = logits[..., 5:5 + left].clone()
+            logits.fill_(fill)
+            logits[..., 5:5 + left] = keep
+            for k in (1, W, 64):
+                compare(logits, scores, k)
+
+
+@pytest.mark.parametrize('dtype', [th.bfloat16, th.float32])
+def test_large_logits(dtype):
+    """Rows that lie far from zero, on either side."""
+    for by in (1e2, 1e3, 1e4, 1e5, 1e6, 1e7, 1e8, 1e30):
+        for sign in (1, -1):
+            logits, scores = make(2, 6, 5003, th.float32)
+            for k in (6, 64):
+                compare((logits + sign * by).to(dtype), scores, k)
+                compare((logits * (sign * by)).to(dtype), scores, k)
+
+
+@pytest.mark.parametrize('dtype', [th.bfloat16, th.float32])
+def test_normalisers_of_long_parts(dtype):
+    """The best scores themselves, brought next to zero by the beams' own so that no rounding of theirs hides the normaliser's error.  B W V is large enough for parts of sixteen
+    segments."""
+    from wind_rwkv.rwkv7 import beam_select
+    B, W, V = 74, 8, 65536
+    g = th.Generator(device='cuda').manual_seed(3)
+    x = th.randn(B * W, V, generator=g, device='cuda') * 3
+    for shift in (0., 20., 100., -1000., 10000.):
+        logits = (x + shift).to(dtype)
+        want, tol = [], 0.
+        for rows in logits.split(74):
+            d = rows.double()
+            m = d.amax(-1, keepdim=True)
+            p = th.exp(d - m)
+            z = p.transpose(0, 1).contiguous().sum(0)
+            want.append(-z.log())
+            tol = max(tol, float(((p * (m - d)).sum(-1) / z).max()))
+        want = th.cat(want).view(B * W, 1)          # the best candidate's log-probability
+        tol = 2 ** -22 + 2 ** -23 * tol + 70 * 2 ** -24
+        scores = -want.float()
+        got, _, tokens = beam_select(logits.view(B * W, 1, V), scores)
+        err = (got.double() - (want + scores.double())).abs() - 2.0 ** -24 * 1e-5
+        assert bool((err <= tol).all()), (shift, float(err.max()))
+        assert th.equal(logits.gather(1, tokens), logits.amax(-1, keepdim=True))
+
+
 def test_orders():
     """Sorted vocabularies, and candidates that crowd into one segment or one thread's segments."""
     V = 20000

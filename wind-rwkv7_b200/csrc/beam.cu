@@ -67,14 +67,14 @@ __device__ __forceinline__ float warp_max(float x) {  // (a NaN is passed over)
     return y;
 }
 __device__ __forceinline__ float max8(const float (&f)[8]) { return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7]))); }
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr int AHEAD = 2, DEPTH = 4;  // segments that are worked, and requested, together (a batch); batches of the ring
-constexpr float FAR_OUT = 1e30f;  // beyond it a logit is a mask, and its multiple by LOG2E may overflow
 
 // A part of a row (segments [first, last)) by a warp, AHEAD segments at a time: their maxima, the part's (m) and the lane's share of sum exp(l - m), formed
-// as 2^(l LOG2E - c), c = m LOG2E rounded: one multiply-add a logit.  What the rounding of c makes of it is one factor for the whole sum, taken out at the end.
+// as 2^((l - m) LOG2E).  The difference comes first: it is right for logits of any magnitude (rows masked with -1e9 or the type's lowest value among them), where
+// l LOG2E and m LOG2E would each be rounded to their own magnitude.
 // The logits come by asynchronous copies into a ring of the warp's own, DEPTH - 1 batches ahead: what a warp has requested takes no registers.
-// CAREFUL: NaN and +inf are ruled out one by one, and l - m comes first; without it such a part's s is a NaN, or m is far out.
+// CAREFUL: NaN and +inf are ruled out one by one; without it such a part's s is a NaN.
 template <bool F32, bool ALIGNED> __host__ __device__ constexpr int stage_bytes() { return AHEAD * SEG * (F32 ? 4 : 2) + (ALIGNED ? 0 : 16); }
 template <bool F32, bool ALIGNED, bool CAREFUL> __device__ __forceinline__ void scan_part(const BeamParams& p, long long row, int first, int last, float* seg_max, unsigned char* ring, int lane, float& m, float& s) {
     constexpr int SIZE = F32 ? 4 : 2, STAGE = stage_bytes<F32, ALIGNED>(), BATCH = AHEAD * SEG * SIZE;
@@ -93,7 +93,6 @@ template <bool F32, bool ALIGNED, bool CAREFUL> __device__ __forceinline__ void 
         }
         cp_async_commit();
     };
-    auto anchor = [](float x) { return fmaxf(x, -FAR_OUT) * LOG2E; };
     m = NEG_INF;
     F2 sum = f2(0.f, 0.f);
     int stage = 0;
@@ -139,30 +138,20 @@ template <bool F32, bool ALIGNED, bool CAREFUL> __device__ __forceinline__ void 
         float most = m;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) most = fmaxf(most, top[i]);
-        if (CAREFUL) {
-            if (most == NEG_INF) continue;
-            const float old = ex2_approx((m - most) * LOG2E);
-            sum = mul2(sum, f2(old, old));
+        // (from -inf itself a difference would be a NaN)
+        const float c = fmaxf(most, LOWEST), old = ex2_approx((fmaxf(m, LOWEST) - c) * LOG2E);
+        const F2 minus = f2(-c, -c), log2e = f2(LOG2E, LOG2E);
+        sum = mul2(sum, f2(old, old));
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
+        for (int i = 0; i < AHEAD; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sum.x += ex2_approx((f[i][e] - most) * LOG2E);
-        } else {
-            const float c = anchor(most), old = ex2_approx(anchor(m) - c);
-            const F2 minus = f2(-c, -c), log2e = f2(LOG2E, LOG2E);
-            sum = mul2(sum, f2(old, old));
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const F2 x = fma2(f2(f[i][e], f[i][e + 1]), log2e, minus);
-                    sum = add2(sum, f2(ex2_approx(x.x), ex2_approx(x.y)));
-                }
-        }
+            for (int e = 0; e < 8; e += 2) {
+                const F2 x = mul2(add2(f2(f[i][e], f[i][e + 1]), minus), log2e);
+                sum = add2(sum, f2(ex2_approx(x.x), ex2_approx(x.y)));
+            }
         m = most;
     }
     s = sum.x + sum.y;
-    if (!CAREFUL && m > -FAR_OUT) s = fmaf(-LN2 * fmaf(m, LOG2E, -anchor(m)), s, s);  // 2^-r = 1 - r ln 2 for the rounding r of c
 }
 
 template <bool F32, bool ALIGNED> __global__ void __launch_bounds__(32 * SCAN_WARPS) beam_scan_kernel(const __grid_constant__ BeamParams p) {
@@ -185,8 +174,8 @@ template <bool F32, bool ALIGNED> __global__ void __launch_bounds__(32 * SCAN_WA
         }
     } else {
         scan_part<F32, ALIGNED, false>(p, row, first, last, seg_max, ring, lane, m, s);
-        // (a NaN, which maxima pass over, is in some lane's sum; +inf and rows of the type's lowest value are far out)
-        if (__any_sync(0xffffffffu, s != s) || (m != NEG_INF && !(fabsf(m) < FAR_OUT))) scan_part<F32, false, true>(p, row, first, last, seg_max, ring, lane, m, s);
+        // (a NaN, which maxima pass over, is in some lane's sum; +inf makes one there, as inf - inf)
+        if (__any_sync(0xffffffffu, s != s)) scan_part<F32, false, true>(p, row, first, last, seg_max, ring, lane, m, s);
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
