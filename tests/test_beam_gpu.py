@@ -199,6 +199,29 @@ def test_normalisers_of_long_parts(dtype):
         assert th.equal(logits.gather(1, tokens), logits.amax(-1, keepdim=True))
 
 
+@pytest.mark.parametrize('dtype', [th.bfloat16, th.float32])
+@pytest.mark.parametrize('W,V', [(1, 300), (2, 300), (6, 5000)])
+def test_scores_at_the_end_of_the_range(W, V, dtype):
+    """Beams whose score is fp32's lowest value: a candidate below it that rounds to it counts, one that rounds to -inf does not."""
+    from wind_rwkv.rwkv7 import beam_select
+    low = th.finfo(th.float32).min
+    for score in (low, low / 2):
+        for fill in (-1e30, -3e30, -2e31, low / 2, low):
+            for left in (0, 1, 2, 40):
+                logits, scores = make(2, W, V, dtype, seed=left)
+                keep = logits[..., 5:5 + left].clone()
+                logits.fill_(max(fill, th.finfo(dtype).min))
+                logits[..., 5:5 + left] = keep
+                scores.fill_(score)
+                scores[1, :-1] = -INF
+                every = reference(logits, scores, 1)[2]
+                every = th.where(every.float() > -INF, every, -INF)
+                best, index = every.sort(dim=1, descending=True, stable=True)
+                for k in (1, 4, 64):
+                    got, parents, tokens = beam_select(logits, scores, k)
+                    assert th.equal(got, best[:, :k].float()) and th.equal(parents * V + tokens, index[:, :k])
+
+
 def test_orders():
     """Sorted vocabularies, and candidates that crowd into one segment or one thread's segments."""
     V = 20000

@@ -273,6 +273,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
     const long long seq = blockIdx.x, row0 = seq * p.W;
     const int k = p.k;
     if (tid == 0) { q.nsegs = 0; q.n = 0; }
+    if (tid < BEAM_MAX_K) { q.out_score[tid] = (double)NEG_INF; q.out_index[tid] = tid; }  // (a candidate that there is: k is W V at most)
     if (tid < 128) q.group[tid] = 0;
     stream_order();
     // a thread has every 1024th of the sequence's segments; their maxima are requested here and used behind the normalisers
@@ -309,7 +310,8 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
     __syncthreads();
     // A threshold that k candidates reach at least: the k-th best of the bests of 32, 64 or 128 groups of segments, two of them or more for each of the k.  A
     // group has segments of all beams (the best candidates are often of a few), so that some 1.4 k segments reach it as a rule.  The segments' scores in
-    // 32 bits here, less what the roundings may have added.  Candidates at -inf are left to the end.
+    // 32 bits here, less what the roundings may have added.  Candidates at -inf are left to the end; where fewer than k groups have others t is -inf, since a score may lie
+    // a little below fp32's lowest value and still be rounded to it.
     auto at_least = [&](int w, float l) {
         const float s = l + q.offset[w];
         return s == NEG_INF ? 0u : ordered(s - 2.4e-7f * (fabsf(l) + fabsf(q.offset[w])));
@@ -331,12 +333,12 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
         const uint32_t mine = q.group[g];
         int ahead = 0;
         for (int i = lane; i < groups; i += 32) ahead += __popc(__ballot_sync(0xffffffffu, q.group[i] > mine || (q.group[i] == mine && i < g)));
-        if (ahead == k - 1 && lane == 0) q.t = mine ? unordered(mine) : LOWEST;
+        if (ahead == k - 1 && lane == 0) q.t = mine ? unordered(mine) : NEG_INF;
     }
     __syncthreads();
     // the segments that reach t, and their candidates that do
     auto list = [&] {
-        // score >= t is l >= (t - base + logz) + top, less a little for the roundings on the way
+        // score >= t is l >= (t - base + logz) + top, less a little for the roundings on the way (a NaN, which nothing reaches, for a beam at -inf where t is)
         if (tid < p.W) {
             const double t = q.t, l = ((t - q.base[tid]) + q.logz[tid]) + q.top[tid];
             q.least[tid] = __double2float_rd(l - 1e-15 * (fabs(t) + fabs(q.base[tid]) + fabs(q.top[tid]) + 64.));
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
             if (q.count[bit] >= k) t = trial;
         }
         __syncthreads();
-        if (tid == 0) { q.t = t ? unordered(t) : LOWEST; q.nsegs = 0; q.n = 0; }
+        if (tid == 0) { q.t = t ? unordered(t) : NEG_INF; q.nsegs = 0; q.n = 0; }
         __syncthreads();
         listed = list();
     }
