@@ -62,6 +62,29 @@ def test_python_refusals(lib):
         linear(x, w)
 
 
+@pytest.mark.parametrize('dynamic', [False, True])
+def test_refusals_while_torch_compile_traces(lib, dynamic):
+    from wind_rwkv.rwkv7 import linear
+    x, w, b, r = th.zeros(4, 64, dtype=BF), th.zeros(16, 64, dtype=BF), th.zeros(16), th.zeros(4, 16, dtype=BF)
+
+    def call(x, w, bias=None, residual=None, **how):
+        th.compiler.reset()
+        return th.compile(lambda *t: linear(t[0], t[1], t[2], residual=t[3], **how) * 1, backend='eager', dynamic=dynamic)(x, w, bias, residual)
+
+    for bad in (dict(act='swish'), dict(bias=b[:15]), dict(bias=b[:1]), dict(bias=b.double()), dict(residual=r[:, :15]), dict(residual=r[:3]), dict(residual=r.float()),
+                dict(residual=r, out_dtype=th.float32), dict(bias=b[None])):
+        with pytest.raises(ValueError, match='linear'):
+            call(x, w, **bad)
+    for bx, bw in ((x, w[:, :56]), (x[:, :56], w), (x, w[None]), (x[:, :60], w[:, :60]), (x, w[:0])):
+        with pytest.raises(ValueError, match='linear'):
+            call(bx, bw)
+    for bx, bw, out in ((x.float(), w, None), (x, w.half(), None), (x.half(), w, None), (x, w, th.float16)):
+        with pytest.raises(TypeError, match='linear'):
+            call(bx, bw, out_dtype=out)
+    with pytest.raises(RuntimeError, match='CUDA'):
+        call(x, w, b, r, act='relu2')
+
+
 def test_rows_are_taken_as_they_lie():
     from wind_rwkv.rwkv7.rwkv7_linear import operand_of, rows_of
     t = th.zeros(4, 6, 32, dtype=BF)

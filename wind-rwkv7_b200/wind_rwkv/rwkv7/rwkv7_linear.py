@@ -163,6 +163,6 @@ def linear(x, w, bias=None, *, act=None, residual=None, out_dtype=None):
             out = _lib.ext().linear(x, w, bias, residual, ACTS[act], out_dtype == th.float32)
             if out is not None:
                 return out
-        _check(x, w, bias, residual, act, out_dtype)
-        _lib.require_cuda(x, w, bias, residual)
+    _check(x, w, bias, residual, act, out_dtype)  # (while torch.compile traces, too: the launchers take what they are given)
+    _lib.require_cuda(x, w, bias, residual)
     return Linear.apply(x, w, bias, residual, ACTS[act], out_dtype == th.float32)
