@@ -64,6 +64,28 @@ def test_select_refusals(lib):
         beam_select(logits, scores)
 
 
+@pytest.mark.parametrize('dynamic', [False, True])
+def test_select_refusals_while_torch_compile_traces(lib, dynamic):
+    from wind_rwkv.rwkv7 import beam_select
+    logits, scores = th.zeros(2, 4, 50), th.zeros(2, 4)
+    fin = th.zeros(2, 4, dtype=th.bool)
+
+    def call(logits, scores, k=None, finished=None, eos=None):
+        th.compiler.reset()
+        return th.compile(lambda l, s, f: beam_select(l, s, k, finished=f, eos=eos)[0] * 1, backend='eager', dynamic=dynamic)(logits, scores, finished)
+
+    for bad in (dict(k=0), dict(k=65), dict(finished=fin), dict(eos=3), dict(finished=fin, eos=50), dict(finished=fin, eos=-2), dict(finished=fin[:1], eos=3),
+                dict(finished=fin.int(), eos=3)):
+        with pytest.raises(ValueError, match='beam_select'):
+            call(logits, scores, **bad)
+    for bl, bs in ((logits[0], scores), (logits.half(), scores), (logits.double(), scores), (logits, scores[:1]), (logits, scores[:, :3]), (logits, scores.double()),
+                   (th.zeros(1, 65, 5), th.zeros(1, 65))):
+        with pytest.raises(ValueError, match='beam_select'):
+            call(bl, bs)
+    with pytest.raises(RuntimeError, match='CUDA'):
+        call(logits, scores, None, fin, 3)
+
+
 def test_reorder_refusals(lib):
     from wind_rwkv.rwkv7 import reorder_states
     t, p = th.zeros(8, 6), th.zeros(2, 4, dtype=th.int64)

@@ -77,8 +77,8 @@ def beam_select(logits, scores, k=None, *, finished=None, eos=None):
         out = _lib.ext().beam_select(logits, scores, -1 if k is None else k, finished, -1 if eos is None else eos if eos >= 0 else -2)
         if out is not None:
             return out
-        _check_select(logits, scores, k, finished, eos)
-        _lib.require_cuda(logits, scores, finished)
+    _check_select(logits, scores, k, finished, eos)  # (while torch.compile traces, too: the launcher takes what it is given)
+    _lib.require_cuda(logits, scores, finished)
     out, parents, tokens, fin = _lib.call(_select_op, select, logits.detach(), scores.detach(), finished, k, -1 if eos is None else eos)
     return (out, parents, tokens) if finished is None else (out, parents, tokens, fin)
 
