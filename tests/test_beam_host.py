@@ -104,6 +104,27 @@ def test_reorder_refusals(lib):
         reorder_states([t[:, :3], t[:, 3:]], p, inplace=True)
 
 
+@pytest.mark.parametrize('dynamic', [False, True])
+def test_reorder_refusals_while_torch_compile_traces(lib, dynamic):
+    from wind_rwkv.rwkv7 import reorder_states
+    t, p = th.zeros(8, 6), th.zeros(2, 4, dtype=th.int64)
+
+    def call(states, parents, inplace=False):
+        th.compiler.reset()
+        return th.compile(lambda ts, p: [o * 1 for o in reorder_states(ts, p, inplace=inplace)], backend='eager', dynamic=dynamic)(states, parents)
+
+    for states, parents, inplace in (([t], p.float(), False), ([t], p[0], False), ([t], p[:, :0], False), ([t, t[:4]], p, False), ([t[:4], t], p, False), ([t[:7]], p, False),
+                                     ([th.zeros(())], p, False), ([t], p[:, :3], True), ([th.zeros(130, 2)], p, False), ([t.t().contiguous().t()], p, True),
+                                     ([t[:1].expand(8, 6)], p, True), ([t], th.zeros(2, 65, dtype=th.int64), False)):
+        with pytest.raises(ValueError, match='reorder_states'):
+            call(states, parents, inplace)
+    with pytest.raises(RuntimeError, match='autograd'):
+        call([th.zeros(8, 6, requires_grad=True)], p, True)
+    for inplace in (False, True):
+        with pytest.raises(RuntimeError, match='CUDA'):
+            call([t[:, :3], t[:, 3:]], p, inplace)
+
+
 def test_rows_that_share_memory():
     from wind_rwkv.rwkv7.rwkv7_beam import _overlap, _row_layout
     t = th.zeros(8, 6, 4)

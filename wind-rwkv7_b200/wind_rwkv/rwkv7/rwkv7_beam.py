@@ -136,10 +136,10 @@ def _check_reorder(states, parents, inplace):
     B, k = parents.shape
     if k < 1 or k > MAX_BEAMS:
         raise ValueError(f'reorder_states takes 1 to {MAX_BEAMS} parents a sequence, got {k}')
-    rows = {t.shape[0] if t.dim() else None for t in states}
-    if len(rows) > 1 or None in rows:
+    if any(t.dim() == 0 or t.shape[0] != states[0].shape[0] for t in states):
         raise ValueError(f'reorder_states: all states have a row per beam, got {[list(t.shape) for t in states]}')
-    for n in rows:
+    if states:
+        n = states[0].shape[0]
         if (n % B or not 1 <= n // B <= MAX_BEAMS) if B else n:
             raise ValueError(f'reorder_states: {n} rows are not 1 to {MAX_BEAMS} beams for each of {B} sequences')
         if inplace and n != B * k:
@@ -147,17 +147,19 @@ def _check_reorder(states, parents, inplace):
     if inplace:
         if th.is_grad_enabled() and any(t.requires_grad for t in states):
             raise RuntimeError('reorder_states has no autograd: in place it takes states that require no gradient')
-        lays = [_row_layout(t) for t in states]
-        if None in lays:
+        if any(_row_layout(t) is None for t in states):
             raise ValueError('reorder_states in place takes states whose rows are contiguous and apart')
-        at = [(t.data_ptr(), t.shape[0], *p) for t, p in zip(states, lays)]
-        at = sorted(at + [(parents.data_ptr(), 1, parents.numel() * parents.element_size(), 1)])
-        for i, a in enumerate(at):
-            for b in at[i + 1:]:
-                if b[0] >= a[0] + max(a[1] * a[3], a[2]):
-                    break
-                if _overlap(a, b):
-                    raise ValueError('reorder_states in place: two of the states, or one and parents, share memory')
+
+
+def _check_apart(states, parents):
+    at = [(t.data_ptr(), t.shape[0], *_row_layout(t)) for t in states]
+    at = sorted(at + [(parents.data_ptr(), 1, parents.numel() * parents.element_size(), 1)])
+    for i, a in enumerate(at):
+        for b in at[i + 1:]:
+            if b[0] >= a[0] + max(a[1] * a[3], a[2]):
+                break
+            if _overlap(a, b):
+                raise ValueError('reorder_states in place: two of the states, or one and parents, share memory')
 
 
 def reorder_states(states, parents, *, inplace=False):
@@ -172,6 +174,8 @@ def reorder_states(states, parents, *, inplace=False):
         out = _lib.ext().reorder_states(ts, parents, inplace)
         if out is None:
             _check_reorder(ts, parents, inplace)
+            if inplace:
+                _check_apart(ts, parents)
             _lib.require_cuda(parents, *ts)
             if inplace:
                 _launch(ts, ts, parents)
@@ -180,6 +184,8 @@ def reorder_states(states, parents, *, inplace=False):
             else:
                 out = reorder([t.detach() for t in ts], parents)
         return out[0] if one else out
+    _check_reorder(ts, parents, inplace)  # (the launcher takes what it is given)
+    _lib.require_cuda(parents, *ts)
     out = _reorder_op([t.detach() for t in ts], parents)
     if inplace:
         for t, o in zip(ts, out):
