@@ -335,11 +335,14 @@ int wkv7_beam_select(const void* logits, const float* scores, const void* finish
 /*
  * The beams' states follow their parents: row b k + j of dst[i] := row b W + parents[b][j] of src[i], for `count` tensors whose rows are row_bytes[i] adjacent
  * bytes, src_pitch[i] and dst_pitch[i] bytes apart (the arrays are host memory; any count).  dst[i] == src[i] with equal pitches and k == W: in place, rows that
- * stay are not touched; otherwise dst must not overlap any src, and no dst another.  parents [B,k] int64, or int32 with parents_i32, device
- * memory.  A parent outside 0 .. W-1 leaves its row as it is (in place) or zero, and WKV7_ERR_INDEX in the status word.  W, k <= 64.
+ * stay are not touched; otherwise dst must not overlap any src, and no dst another.  parents [B,k] int64, or int32 with WKV7_REORDER_I32, device
+ * memory.  A parent outside 0 .. W-1 leaves its row as it is (in place), as it is in src (WKV7_REORDER_KEEP, k == W: results that are to replace src) or zero, and
+ * WKV7_ERR_INDEX in the status word.  W, k <= 64.
  */
+#define WKV7_REORDER_I32 1
+#define WKV7_REORDER_KEEP 2
 int wkv7_reorder(int count, const void* const* src, void* const* dst, const int64_t* row_bytes, const int64_t* src_pitch, const int64_t* dst_pitch,
-                 const void* parents, int parents_i32, int64_t B, int64_t W, int64_t k, void* stream);
+                 const void* parents, int flags, int64_t B, int64_t W, int64_t k, void* stream);
 
 /*
  * expand_loras: second-stage LoRA expansion producing (w, k, kk, b) for the mixer.  Replaces

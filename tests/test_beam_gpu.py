@@ -425,6 +425,49 @@ def test_parent_that_does_not_exist():
         assert th.equal(t[i], before[i if r is None else r])
 
 
+@pytest.mark.parametrize('dynamic', [False, True])
+def test_compiled_in_place(dynamic):
+    """Traced in place: a parent that does not exist leaves its row as it is, states that share memory are refused, rows that lie in wider tensors, layers of one tensor, and
+    states made inside the traced function."""
+    from wind_rwkv.rwkv7 import _lib, reorder_states
+    th.compiler.reset()
+
+    def f(ts, p):
+        made = ts[0] * 2
+        reorder_states([made, *ts], p, inplace=True)
+        return [made + 1] + [t * 1 for t in ts]
+
+    g = th.compile(f, fullgraph=True, dynamic=dynamic)
+    for B, W in ((2, 4), (3, 5), (1, 64)):
+        p = parents_of(B, W, W, 1)
+        for bad in (False, True):
+            if bad:
+                p[0, 1], p[-1, -1] = W, -1
+            wide = th.randn(B * W, 40, device='cuda')
+            both = [[t.clone() for t in tensors(B * W)[:4]] + list((w := wide.clone())[:, :36].unflatten(1, (4, 9)).unbind(1)) + [w] for _ in range(2)]
+            outs = []
+            for call, (*ts, w) in zip((f, g), both):
+                outs.append(call(ts, p))
+                th.cuda.synchronize()
+                assert _lib.device_status() == (-11 if bad else 0)
+                assert all(th.equal(o, t) for o, t in zip(outs[-1][1:], ts))
+            assert all(th.equal(a, b) for a, b in zip(*both)) and all(th.equal(a, b) for a, b in zip(*outs))
+            assert th.equal(both[1][-1][:, 36:], wide[:, 36:])
+    t, p = th.randn(8, 6, device='cuda'), parents_of(2, 4, 4, 0)
+    before = t.clone()
+    for ts in ([t, t], [t[:, :4], t[:, 3:]], [t[:, :3], t[:, 1:4], t[:, 4:]]):
+        th.compiler.reset()
+        with pytest.raises(ValueError, match='share memory'):
+            th.compile(f, dynamic=dynamic)(ts, p)
+        assert th.equal(t, before)
+    th.compiler.reset()
+    with pytest.raises(ValueError, match='share memory'):
+        th.compile(lambda s, p: reorder_states([s], p, inplace=True)[0] * 1, dynamic=dynamic)(p.view(8, 1), p)
+    q = th.zeros(8, 2, device='cuda', requires_grad=True)
+    with th.no_grad():
+        th.compile(lambda s, p: reorder_states(s, p, inplace=True) * 1, dynamic=dynamic)(q, p)
+
+
 def test_large_offsets():
     """States whose rows lie beyond 2^32 bytes."""
     from wind_rwkv.rwkv7 import reorder_states

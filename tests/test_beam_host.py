@@ -43,6 +43,7 @@ def test_reorder_checks(lib):
     assert reorder(lib, B=-1) == reorder(lib, W=0) == reorder(lib, k=0) == reorder(lib, W=65) == reorder(lib, k=65) == reorder(lib, count=-1) == -1
     assert reorder(lib, row=-1) == reorder(lib, sp=63) == reorder(lib, dp=63) == -1
     assert reorder(lib, dst=P, k=3) == reorder(lib, dst=P, dp=128) == -1                  # in place: as many rows, one pitch
+    assert reorder(lib, i32=4) == reorder(lib, i32=-1) == reorder(lib, i32=2, k=3) == reorder(lib, i32=3, W=3) == -1
     assert reorder(lib, src=None) == reorder(lib, dst=None) == reorder(lib, parents=None) == -6
     assert reorder(lib, parents=P + 4) == reorder(lib, parents=P + 2, i32=1) == -4
     assert reorder(lib, B=0, src=None) == reorder(lib, count=0) == 0

@@ -519,7 +519,7 @@ template <int K> __global__ void __launch_bounds__(RE_THREADS) reorder_kernel(co
         const long long f = p.idx64 ? ((const int64_t*)p.parents)[at] : ((const int32_t*)p.parents)[at];
         int use = (int)f;  // -1: nothing to do, -2: zeros
         if (f < 0 || f >= p.W) {
-            use = inplace ? -1 : -2;
+            use = inplace ? -1 : p.keep ? (int)threadIdx.x : -2;
             *reinterpret_cast<volatile int*>(p.status) = (int)kBadIndex;
             __threadfence_system();
         } else if (inplace && f == (long long)threadIdx.x) {

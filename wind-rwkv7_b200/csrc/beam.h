@@ -29,7 +29,7 @@ struct ReorderParams {
     long long row_bytes[REORDER_MAX], src_pitch[REORDER_MAX], dst_pitch[REORDER_MAX];
     const void* parents;  // [B, k]
     int B, W, k, count;
-    bool idx64;
+    bool idx64, keep;     // keep: a row whose parent does not exist is src's own, not zero
     int* status;
 };
 int launch_reorder(const ReorderParams& p, cudaStream_t stream);

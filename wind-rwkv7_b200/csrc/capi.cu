@@ -546,7 +546,9 @@ int wkv7_beam_select(const void* logits, const float* scores, const void* finish
 }
 
 int wkv7_reorder(int count, const void* const* src, void* const* dst, const int64_t* row_bytes, const int64_t* src_pitch, const int64_t* dst_pitch,
-                 const void* parents, int parents_i32, int64_t B, int64_t W, int64_t k, void* stream) {
+                 const void* parents, int flags, int64_t B, int64_t W, int64_t k, void* stream) {
+    const bool parents_i32 = flags & WKV7_REORDER_I32, keep = flags & WKV7_REORDER_KEEP;
+    if ((flags & ~(WKV7_REORDER_I32 | WKV7_REORDER_KEEP)) || (keep && k != W)) return WKV7_ERR_SHAPE;
     if (count < 0 || B < 0 || W < 1 || k < 1 || W > wkv7::BEAM_MAX_W || k > wkv7::BEAM_MAX_K) return WKV7_ERR_SHAPE;
     if (B > 0x7fffffffLL / wkv7::BEAM_MAX_W) return WKV7_ERR_TOO_LARGE;
     for (int i = 0; i < count; ++i) {
@@ -562,7 +564,7 @@ int wkv7_reorder(int count, const void* const* src, void* const* dst, const int6
     if (!status) return WKV7_ERR_LAUNCH;
     for (int from = 0; from < count; from += wkv7::REORDER_MAX) {
         wkv7::ReorderParams p{};
-        p.parents = parents; p.idx64 = !parents_i32;
+        p.parents = parents; p.idx64 = !parents_i32; p.keep = keep;
         p.B = (int)B; p.W = (int)W; p.k = (int)k; p.status = status;
         for (int i = from; i < count && i < from + wkv7::REORDER_MAX; ++i) {
             if (row_bytes[i] == 0) continue;

@@ -15,6 +15,7 @@ import torch as th
 from . import _lib
 
 MAX_BEAMS = 64
+I32, KEEP = 1, 2
 
 
 def select(logits, scores, finished, k, eos):
@@ -103,16 +104,19 @@ def _overlap(a, b):
     return not (ld == le and d >= n and d + o <= ld)
 
 
-def reorder(states, parents):
-    """Launcher: the reordered states, as new tensors."""
+def reorder(states, parents, replaces=False):
+    """Launcher: the reordered states, as new tensors.  `replaces`: the states will be overwritten with them, so that what holds in place holds here: a row
+    whose parent does not exist stays, and no two states share memory (which only addresses show; they cannot be looked at while a call is traced)."""
     B, k = parents.shape
+    if replaces:
+        _check_apart(states, parents)
     outs = [th.empty((B * k, *t.shape[1:]), dtype=t.dtype, device=t.device) for t in states]
     states = [t.resolve_conj().resolve_neg() for t in states]
-    _launch([t if _row_layout(t) else t.contiguous() for t in states], outs, parents)
+    _launch([t if _row_layout(t) else t.contiguous() for t in states], outs, parents, KEEP if replaces else 0)
     return outs
 
 
-def _launch(src, dst, parents):
+def _launch(src, dst, parents, flags=0):
     B, k = parents.shape
     if B == 0 or not src:
         return
@@ -122,12 +126,12 @@ def _launch(src, dst, parents):
     parents = parents.contiguous()
     with _lib.on_device(parents, *src, *dst):
         rc = _lib.lib().wkv7_reorder(n, ptrs(*[t.data_ptr() for t in src]), ptrs(*[t.data_ptr() for t in dst]), i64s(*[p[0] for p in ps]), i64s(*[p[1] for p in ps]),
-                                     i64s(*[p[1] for p in pd]), parents.data_ptr(), int(parents.dtype == th.int32), B, src[0].shape[0] // B, k, _lib.stream_of(parents))
+                                     i64s(*[p[1] for p in pd]), parents.data_ptr(), flags | (I32 if parents.dtype == th.int32 else 0), B, src[0].shape[0] // B, k, _lib.stream_of(parents))
     _lib.check(rc, 'wkv7_reorder')
 
 
-_reorder_op = _lib.opaque_op('reorder_states', reorder, lambda states, parents: [t.new_empty((parents.numel(), *t.shape[1:])) for t in states],
-                             '(Tensor[] states, Tensor parents) -> Tensor[]')
+_reorder_op = _lib.opaque_op('reorder_states', reorder, lambda states, parents, replaces: [t.new_empty((parents.numel(), *t.shape[1:])) for t in states],
+                             '(Tensor[] states, Tensor parents, bool replaces) -> Tensor[]')
 
 
 def _check_reorder(states, parents, inplace):
@@ -152,7 +156,7 @@ def _check_reorder(states, parents, inplace):
 
 
 def _check_apart(states, parents):
-    at = [(t.data_ptr(), t.shape[0], *_row_layout(t)) for t in states]
+    at = [(t.data_ptr(), t.shape[0], *lay) for t in states if (lay := _row_layout(t))]
     at = sorted(at + [(parents.data_ptr(), 1, parents.numel() * parents.element_size(), 1)])
     for i, a in enumerate(at):
         for b in at[i + 1:]:
@@ -186,7 +190,7 @@ def reorder_states(states, parents, *, inplace=False):
         return out[0] if one else out
     _check_reorder(ts, parents, inplace)  # (the launcher takes what it is given)
     _lib.require_cuda(parents, *ts)
-    out = _reorder_op([t.detach() for t in ts], parents)
+    out = _reorder_op([t.detach() for t in ts], parents, inplace)
     if inplace:
         for t, o in zip(ts, out):
             t.copy_(o)
