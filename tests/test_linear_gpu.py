@@ -226,6 +226,31 @@ def test_large_arguments():
             compare(x * 1e19, w, None, None, dy, act)
 
 
+@pytest.mark.parametrize('act', ['sigmoid', 'silu', 'gelu', 'tanh'])
+def test_derivatives_to_their_own_size(act):
+    """act' where it is small, relative to it: z is an fp32 bias alone, and its gradient, of one row, is act'(z) in fp32.  With s = sigmoid(u), q = 1 - s, in units of 2^-24: the exponential 4,
+    its argument a |u| (product and constant 1.25; gelu's u 7 more, tanh's the same), reciprocal 2 and its argument 1, products; each of s and q is off by E = 13 + a |u| at most."""
+    from wind_rwkv.rwkv7 import linear
+    z = th.linspace(-6, 6, 4001) if act == 'gelu' else th.linspace(-24, 24, 4001)
+    b = z.cuda().requires_grad_()
+    x, w = th.zeros(1, 8, dtype=th.bfloat16, device='cuda'), th.zeros(4001, 8, dtype=th.bfloat16, device='cuda')
+    y = linear(x, w, b, act=act, out_dtype=th.float32)
+    got, = th.autograd.grad(y, b, th.ones_like(y))
+    z = b.detach().double()
+    C = 2 * (2 / th.pi) ** 0.5
+    u = {'gelu': C * (z + 0.044715 * z ** 3), 'tanh': 2 * z}.get(act, z)
+    E = (13 + (8.25 if act == 'gelu' else 1.25) * u.abs()) * 2.0 ** -24
+    s, q = th.sigmoid(u), th.sigmoid(-u)
+    if act in ('sigmoid', 'tanh'):
+        want = s * q * (4 if act == 'tanh' else 1)
+        bound = 2 * E * want
+    else:
+        du = C * (1 + 3 * 0.044715 * z ** 2) if act == 'gelu' else 1
+        want = s + z * s * q * du
+        bound = (2 * E + 8 * 2.0 ** -24) * (s + z.abs() * s * q * du)
+    check(act, got, want, bound)
+
+
 def test_layouts():
     """Rows that lie in wider tensors, batch dimensions, orders and alignments that are copied."""
     x, w, b, r, dy = inputs(60, 72, 64, th.float32, True, th.bfloat16, 5)

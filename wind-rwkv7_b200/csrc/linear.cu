@@ -62,8 +62,8 @@ template <int ACT, bool FROM_Y> __device__ __forceinline__ float act_grad(float 
         case kActRelu: return z <= 0.f ? 0.f : 1.f;
         case kActRelu2: return FROM_Y ? 2.f * sqrt_f(z) : 2.f * relu_f(z);
         case kActTanh: { const float e = ex2_approx(-2.f * LOG2E * fabsf(z)), r = rcp_mufu(1.f + e); return 4.f * e * r * r; }
-        case kActSigmoid: { const float s = sigmoid_f(z); return s * (1.f - s); }
-        case kActSilu: { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }
+        case kActSigmoid: { const float e = ex2_approx(-LOG2E * fabsf(z)), r = rcp_mufu(1.f + e); return e * r * r; }  // (s (1 - s) would be 0 from z = 17 on)
+        case kActSilu: { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }  // (beside a 1 what 1 - s loses does not count; nor in gelu')
         case kActGelu: {
             z = z > 64.f ? 64.f : z < -64.f ? -64.f : z;  // (1 and 0 long before; z^3 would leave fp32's range)
             const float s = gelu_s(z);
