@@ -162,6 +162,20 @@ def test_masks_of_any_size(W, V, dtype):
 
 
 @pytest.mark.parametrize('dtype', [th.bfloat16, th.float32])
+@pytest.mark.parametrize('V', [4096, 3001])
+def test_masks_of_any_size_beside_nan(V, dtype):
+    """Parts of rows that are worked twice, since a NaN or +inf is among them."""
+    for fill in FILLS:
+        for odd in (float('nan'), INF):
+            logits, scores = make(2, 4, V, dtype)
+            logits[:, 1] = fill
+            logits[:, 2, ::2] = fill
+            logits[:, :, 1::7] = odd
+            for k in (4, 64):
+                compare(logits, scores, k)
+
+
+@pytest.mark.parametrize('dtype', [th.bfloat16, th.float32])
 def test_large_logits(dtype):
     """Rows that lie far from zero, on either side."""
     for by in (1e2, 1e3, 1e4, 1e5, 1e6, 1e7, 1e8, 1e30):
