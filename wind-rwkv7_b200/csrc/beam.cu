@@ -344,8 +344,10 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
             q.least[tid] = __double2float_rd(l - 1e-15 * (fabs(t) + fabs(q.base[tid]) + fabs(q.top[tid]) + 64.));
         }
         __syncthreads();
+        // (that is in the logits' steps, in which all of a beam that is masked with -1e9 are near t: what passes is looked at once more in 64 bits)
+        const double t = q.t;
         each_segment([&](int w, int g, float l) {
-            if (l >= q.least[w] && l > NEG_INF) {
+            if (l >= q.least[w] && l > NEG_INF && score_of(q, w, l) >= t) {
                 const int i = atomicAdd(&q.nsegs, 1);
                 if (i < SEGS) q.segs[i] = make_int2(w, g);
             }
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
             logits8(p, q, seq, w, at, l);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (l[e] >= q.least[w] && (float)score_of(q, w, l[e]) > NEG_INF) {
+                if (l[e] >= q.least[w] && score_of(q, w, l[e]) >= t && (float)score_of(q, w, l[e]) > NEG_INF) {
                     const int j = atomicAdd(&q.n, 1);
                     if (j < LIST) { q.score[j] = score_of(q, w, l[e]); q.index[j] = w * p.V + at + e; }
                 }
