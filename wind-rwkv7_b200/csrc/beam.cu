@@ -190,6 +190,7 @@ template <bool F32, bool ALIGNED> __global__ void __launch_bounds__(32 * SCAN_WA
 constexpr int PICK_THREADS = 1024, SEGS = 512, LIST = 2 * PICK_THREADS, RANKED = 320;
 struct Pick {
     double top[BEAM_MAX_W], logz[BEAM_MAX_W], base[BEAM_MAX_W];  // a beam's largest logit, log sum exp(l - top), score
+    double bar[BEAM_MAX_W];                                      // the threshold, less what a score in 64 bits may be off by
     float offset[BEAM_MAX_W], least[BEAM_MAX_W];                 // about base - top - logz; the least logit that may reach the threshold
     double score[LIST];
     uint32_t index[LIST];
@@ -341,13 +342,14 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
         // score >= t is l >= (t - base + logz) + top, less a little for the roundings on the way (a NaN, which nothing reaches, for a beam at -inf where t is)
         if (tid < p.W) {
             const double t = q.t, l = ((t - q.base[tid]) + q.logz[tid]) + q.top[tid];
-            q.least[tid] = __double2float_rd(l - 1e-15 * (fabs(t) + fabs(q.base[tid]) + fabs(q.top[tid]) + 64.));
+            const double off = 1e-15 * (fabs(t) + fabs(q.base[tid]) + 64.);
+            q.least[tid] = __double2float_rd(l - (off + 1e-15 * fabs(q.top[tid])));
+            q.bar[tid] = t - off;  // (score_of takes l - top first, which is exact where it matters)
         }
         __syncthreads();
-        // (that is in the logits' steps, in which all of a beam that is masked with -1e9 are near t: what passes is looked at once more in 64 bits)
-        const double t = q.t;
+        // (that is in the logits' steps, in which all of a beam that is masked with -1e9 are near t: segments that pass are looked at once more in 64 bits)
         each_segment([&](int w, int g, float l) {
-            if (l >= q.least[w] && l > NEG_INF && score_of(q, w, l) >= t) {
+            if (l >= q.least[w] && l > NEG_INF && score_of(q, w, l) >= q.bar[w]) {
                 const int i = atomicAdd(&q.nsegs, 1);
                 if (i < SEGS) q.segs[i] = make_int2(w, g);
             }
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(PICK_THREADS, 1) beam_pick_kernel(const __grid
             logits8(p, q, seq, w, at, l);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (l[e] >= q.least[w] && score_of(q, w, l[e]) >= t && (float)score_of(q, w, l[e]) > NEG_INF) {
+                if (l[e] >= q.least[w] && (float)score_of(q, w, l[e]) > NEG_INF) {
                     const int j = atomicAdd(&q.n, 1);
                     if (j < LIST) { q.score[j] = score_of(q, w, l[e]); q.index[j] = w * p.V + at + e; }
                 }
