@@ -288,7 +288,7 @@ int wkv7_proj_gemm_group_ld(int count, const void* const* A, const void* const* 
  * with WKV7_LINEAR_F32_BIAS, or null; residual [M,N] of y's type, or null (may be y itself).  K, ldx and ldw multiples of 8, x and w 16-byte
  * aligned (bulk tensor copies); any M >= 0, N > 0, any ldr, ldy >= N; no sum longer than 2^27 (K, in the backward M and N).  z: null, or [M,N] bf16, fp32 with
  * WKV7_LINEAR_F32_Z, with rows ldz apart (a multiple of 8, 16-byte aligned), where the activation's argument goes for the backward; the columns between N and the next multiple of 8 may be written.
- * tcgen05 products, fp32 accumulation; Results are the same from call to call.  workspace:
+ * tcgen05 products, fp32 accumulation in tensor memory, whose additions cut (fp32 results: relative error some 1e-9 K).  Results are the same from call to call.  workspace:
  * wkv7_linear_fwd_workspace_bytes(M, N, K) bytes of device scratch with the call's device current (0: none), 16-byte aligned, overwritten; null: the
  * tiles of the last round are not shared out (slower by up to a quarter).  May report
  * WKV7_ERR_DEVICE_TIMEOUT through the status word (bounded waits).

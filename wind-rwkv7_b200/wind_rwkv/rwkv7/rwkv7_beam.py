@@ -171,7 +171,7 @@ def reorder_states(states, parents, *, inplace=False):
 
     Returns a tensor, or a list of them, of B * k rows; with inplace=True (k == W) the states themselves, of which only rows that change are
     touched.  All tensors in one launch (64 at a time).  A parent outside 0 .. W - 1 leaves its row zero (in place: as it is), and the next call that looks
-    at the device status raises.  No autograd."""
+    at the device status raises.  No autograd.  (While torch.compile traces, in place is a reordering out of place and a copy back.)"""
     one = isinstance(states, th.Tensor)
     ts = [states] if one else list(states)
     if not th.compiler.is_compiling():

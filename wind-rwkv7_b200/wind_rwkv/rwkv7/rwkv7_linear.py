@@ -156,8 +156,12 @@ def linear(x, w, bias=None, *, act=None, residual=None, out_dtype=None):
     """y = act(x @ w^T + bias) + residual: x [..., K], w [N, K] bf16, K a multiple of 8, any N; bias [N] bf16 or fp32; residual [..., N] of y's type.
 
     act: None, 'relu', 'relu2' (relu(z)^2, the channel mixer's), 'tanh', 'sigmoid', 'silu', 'gelu' (its tanh form).  y is bf16, or fp32 with
-    out_dtype=torch.float32 (logits).  Sums are formed in fp32 and rounded once.  Backward for x, w, bias and residual; the gradient that enters the
-    products, dy act'(z), is rounded to bf16.  Rows may lie in a wider tensor; other layouts are copied."""
+    out_dtype=torch.float32 (logits).  Sums are formed in the tensor cores' fp32 accumulators, whose additions cut, and rounded once: results in fp32 are off by some 1e-9 K
+    (as the library's are; less for few rows).  Backward for x, w, bias and residual; the gradient that enters the products, dy act'(z), is rounded to bf16, and
+    z is kept in bf16 (in fp32 beside an fp32 bias; of relu and relu2 y is kept instead).  Rows may lie in a wider tensor; other layouts are copied.
+
+    What it saves is the passes over y that an activation, bias or residual would take, and in few rows the weight's time.  A product alone of a few hundred to a few
+    thousand rows is quicker by x @ w.mT: 512 x 2048 x 2048 11 against 6 us, 2048^3 15 against 13.5, 1283 x 2560 x 10240 52 against 48; from 8192 rows on they are equal."""
     if not th.compiler.is_compiling():
         if act in ACTS and out_dtype in (None, th.bfloat16, th.float32):
             out = _lib.ext().linear(x, w, bias, residual, ACTS[act], out_dtype == th.float32)
