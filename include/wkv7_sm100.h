@@ -319,6 +319,57 @@ int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void*
                     int64_t ldx, int64_t ldw, int64_t lds, int64_t lddy, int act, int flags, void* workspace, void* stream);
 
 /*
+ * The same product with both operands in 8 bits (no reference counterpart; forward only, for serving):
+ *   y = act((sum_k x[m][k] w[n][k]) xs[m] ws[n] + bias[n]) + residual
+ * x [M,K], w [N,K] signed 8-bit integers, rows ldx, ldw elements apart (multiples of 16, both 16-byte aligned: bulk tensor copies); xs fp32 [M], ws fp32 [N] (a scale
+ * a row and a channel); 0 < K < 2^17, whose sums fit 32 bits whatever the operands hold.  The sum is exact; then come one rounding to fp32, one for each scale
+ * and the epilogue's, as wkv7_linear_fwd's.  y, bias, residual, act, flags (WKV7_LINEAR_F32_OUT, _F32_BIAS) and workspace as there; workspace:
+ * wkv7_linear_int8_workspace_bytes(M, N, K) bytes.
+ */
+int64_t wkv7_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int wkv7_linear_int8(const void* x, const float* xs, const void* w, const float* ws, const void* bias, const void* residual, void* y, int64_t M, int64_t N, int64_t K,
+                     int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int act, int flags, void* workspace, void* stream);
+/*
+ * Rows to 8 bits: a = max |x[m][k]|, q = rint(127 x / a) (ties to even, decided exactly for bf16 x), scale[m] = a / 127.  x [M,K] bf16, or fp32 with WKV7_X_F32, rows
+ * ldx apart; q signed 8-bit [M,K], rows ldq apart; any K > 0.  A row without a magnitude above 2^-100 becomes zeros with scale 0; one that holds a NaN or an
+ * infinity zeros with a NaN for its scale, and so are its products.
+ */
+#define WKV7_X_F32 1
+#define WKV7_R_F32 2
+#define WKV7_W_F32 4
+#define WKV7_Y_F32 8
+#define WKV7_Y_INT8 16
+int wkv7_quantize(const void* x, void* q, float* scale, int64_t M, int64_t K, int64_t ldx, int64_t ldq, int flags, void* stream);
+/*
+ * The residual stream between the mixers (no reference counterpart; upstream leaves it to the model):
+ *   h = residual + dropout(x), rounded to the residual's type;   y = h weight / sqrt(mean h^2 + eps)
+ * x [M,D] bf16, or fp32 with WKV7_X_F32; residual and h [M,D] bf16, or fp32 with WKV7_R_F32, both null: h is x (then p is 0); weight [D] bf16, or fp32 with WKV7_W_F32, or
+ * null; y [M,D] bf16, fp32 with WKV7_Y_F32, or with WKV7_Y_INT8 signed 8 bits beside scale fp32 [M], as wkv7_quantize has them (a row counts as zeros where no h weight is
+ * above 2^-100).  Rows are ldx, ldr, ldy, ldh elements apart; h may be residual itself.  rstd fp32 [M] receives 1 / sqrt(mean h^2 + eps) for the backward, or is null.
+ * 0 < D <= WKV7_NORM_MAX_D, any M.  Squares are summed in fp32.  p, seed, seed_ptr: as wkv7_dropout's, elements counted in row-major order of [M,D].
+ */
+#define WKV7_NORM_MAX_D 16384
+int wkv7_rms_norm_fwd(const void* x, const void* residual, const void* weight, void* y, void* h, float* rstd, float* scale, int64_t M, int64_t D,
+                      int64_t ldx, int64_t ldr, int64_t ldy, int64_t ldh, float eps, double p, uint64_t seed, const void* seed_ptr, int flags, void* stream);
+/*
+ * Its backward, from h as it is kept (without a residual x itself) and rstd:  g = dy weight,  dr = dh + rstd (g - h rstd^2 mean(g h)),  dx = dr where x was
+ * kept, over 1 - p, else 0;  dw = sum over the rows of dy h rstd, fp32 [D].  dy has y's type, dh (null: zero) and dr h's, dx x's; h's type is given by WKV7_R_F32, also
+ * without a residual; dx, dr and dw may be null.  No atomics: results are the same from call to call.  workspace: wkv7_rms_norm_bwd_workspace_bytes(M, D) bytes of
+ * device scratch, 16-byte aligned, where dw is wanted.
+ */
+int64_t wkv7_rms_norm_bwd_workspace_bytes(int64_t M, int64_t D);
+int wkv7_rms_norm_bwd(const void* h, const float* rstd, const void* weight, const void* dy, const void* dh, void* dx, void* dr, float* dw, int64_t M, int64_t D,
+                      int64_t ldh, int64_t lddy, int64_t lddh, int64_t lddx, int64_t lddr, double p, uint64_t seed, const void* seed_ptr, int flags, void* workspace,
+                      void* stream);
+/*
+ * y = residual + x / (1 - p) where an element is kept, else residual; n adjacent elements each, 16-byte aligned.  x bf16, or fp32 with WKV7_X_F32; residual
+ * (WKV7_R_F32) or null; y (WKV7_Y_F32).  Element i is kept where word i % 4 of Philox4x32-10 with counter (i / 4, 64 bits; 0; 0) and key seed (64 bits) is at least
+ * round(p 2^32).  seed_ptr: null, or device memory (8-byte aligned) that holds the seed when the kernel runs, so that a captured graph draws other elements
+ * when it is replayed; seed is not used then.  0 <= p <= 1.  No mask is stored: the backward is the same call on the gradient without residual.
+ */
+int wkv7_dropout(const void* x, const void* residual, void* y, int64_t n, double p, uint64_t seed, const void* seed_ptr, int flags, void* stream);
+
+/*
  * Beam search's selection (no reference counterpart).  For each of B sequences with W beams over a vocabulary of V: the k best of the W V
  * candidates by scores[b][w] + logits[b][w][v] - log sum_v' exp(logits[b][w][v']), best first, equal ones by the lowest w V + v.
  * logits [B,W,V] bf16, or fp32 with logits_f32, strides (stride_b, stride_w, 1) in elements; scores fp32 [B,W], the beams' sums of log-probabilities.

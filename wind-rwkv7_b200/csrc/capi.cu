@@ -1,6 +1,7 @@
 // extern "C" entry points of libwkv7_sm100.so (declared in include/wkv7_sm100.h): host-side
 // validation, the per-device status word, and dispatch to the kernel launchers.
 #include <atomic>
+#include <cmath>
 #include <cstdlib>
 #include "../../include/wkv7_sm100.h"
 #include "wkv7_kernels.h"
@@ -8,6 +9,7 @@
 #include "expand_loras.h"
 #include "linear.h"
 #include "beam.h"
+#include "norm.h"
 
 #include <mutex>
 
@@ -513,6 +515,102 @@ int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void*
         rc = wkv7::launch_linear({dz.p, dz.ld, true}, {x, ldx, true}, M, e, scratch, status, s);
     }
     return rc;
+}
+
+int64_t wkv7_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    return M <= 0 || N <= 0 || K <= 0 ? 0 : (int64_t)wkv7::linear_workspace_bytes(M, N, K, false, true);
+}
+
+int wkv7_linear_int8(const void* x, const float* xs, const void* w, const float* ws, const void* bias, const void* residual, void* y, int64_t M, int64_t N, int64_t K,
+                     int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int act, int flags, void* workspace, void* stream) {
+    if (M < 0 || N <= 0 || K <= 0 || ldx < K || ldw < K || act < 0 || act >= wkv7::kActs || (flags & ~(WKV7_LINEAR_F32_OUT | WKV7_LINEAR_F32_BIAS))) return WKV7_ERR_SHAPE;
+    if (ldy < N || (residual && ldr < N)) return WKV7_ERR_SHAPE;
+    if (ldx % 16 != 0 || ldw % 16 != 0) return WKV7_ERR_ALIGN;
+    constexpr int64_t most = 0x7fffffffLL - 256;  // as wkv7_linear_fwd
+    if (M > most || N > most || K >= 1 << 17 || ldx > most || ldw > most) return WKV7_ERR_TOO_LARGE;
+    if (M == 0) return WKV7_OK;
+    if (!x || !w || !xs || !ws || !y) return WKV7_ERR_NULL;
+    const uintptr_t ysize = flags & WKV7_LINEAR_F32_OUT ? 4 : 2, bsize = flags & WKV7_LINEAR_F32_BIAS ? 4 : 2;
+    if (!aligned16(x) || !aligned16(w) || !aligned16(workspace) || (uintptr_t)xs % 4 || (uintptr_t)ws % 4 || (uintptr_t)y % ysize || (uintptr_t)residual % ysize ||
+        (uintptr_t)bias % bsize)
+        return WKV7_ERR_ALIGN;
+    int* status = status_ptr();
+    if (!status) return WKV7_ERR_LAUNCH;
+    const wkv7::LinearEpilogue e{bias, residual, y, nullptr, ldr, ldy, 0, M, N, act, bsize == 4, ysize == 4, false, xs, ws};
+    return wkv7::launch_linear({x, ldx, false}, {w, ldw, false}, K, e, workspace, status, (cudaStream_t)stream);
+}
+
+int wkv7_quantize(const void* x, void* q, float* scale, int64_t M, int64_t K, int64_t ldx, int64_t ldq, int flags, void* stream) {
+    if (M < 0 || K <= 0 || ldx < K || ldq < K || (flags & ~WKV7_X_F32)) return WKV7_ERR_SHAPE;
+    if (M == 0) return WKV7_OK;
+    if (!x || !q || !scale) return WKV7_ERR_NULL;
+    if ((uintptr_t)x % (flags & WKV7_X_F32 ? 4 : 2) || (uintptr_t)scale % 4) return WKV7_ERR_ALIGN;
+    return wkv7::launch_quantize({x, (signed char*)q, scale, M, K, ldx, ldq, (flags & WKV7_X_F32) != 0}, (cudaStream_t)stream);
+}
+
+static_assert(WKV7_NORM_MAX_D == wkv7::NORM_MAX_D, "mirrored constants");
+
+// false: no probability
+static bool dropout_of(double p, uint64_t seed, const void* seed_ptr, wkv7::Dropout* d) {
+    if (!(p >= 0. && p <= 1.)) return false;
+    *d = wkv7::Dropout{(unsigned long long)std::nearbyint(p * 4294967296.), p < 1. ? (float)(1. / (1. - p)) : 0.f, seed, (const unsigned long long*)seed_ptr};
+    return true;
+}
+
+int wkv7_rms_norm_fwd(const void* x, const void* residual, const void* weight, void* y, void* h, float* rstd, float* scale, int64_t M, int64_t D,
+                      int64_t ldx, int64_t ldr, int64_t ldy, int64_t ldh, float eps, double p, uint64_t seed, const void* seed_ptr, int flags, void* stream) {
+    wkv7::NormFwdParams n{};
+    const bool int8 = flags & WKV7_Y_INT8;
+    if (M < 0 || D <= 0 || ldx < D || ldy < D || (residual && (ldr < D || ldh < D)) || !(eps >= 0.f) || (flags & ~(WKV7_X_F32 | WKV7_R_F32 | WKV7_W_F32 | WKV7_Y_F32 | WKV7_Y_INT8)) ||
+        (int8 && (flags & WKV7_Y_F32)) || !dropout_of(p, seed, seed_ptr, &n.d))
+        return WKV7_ERR_SHAPE;
+    if (D > WKV7_NORM_MAX_D) return WKV7_ERR_TOO_LARGE;
+    if (M == 0) return WKV7_OK;
+    if (p > 0. && !residual) return WKV7_ERR_SHAPE;
+    if (!x || !y || !residual != !h || int8 != (scale != nullptr)) return WKV7_ERR_NULL;
+    const auto size = [&](int f) -> uintptr_t { return flags & f ? 4 : 2; };
+    if ((uintptr_t)x % size(WKV7_X_F32) || (uintptr_t)residual % size(WKV7_R_F32) || (uintptr_t)h % size(WKV7_R_F32) || (uintptr_t)weight % size(WKV7_W_F32) ||
+        (!int8 && (uintptr_t)y % size(WKV7_Y_F32)) || (uintptr_t)rstd % 4 || (uintptr_t)scale % 4 || (uintptr_t)seed_ptr % 8)
+        return WKV7_ERR_ALIGN;
+    n.x = x; n.residual = residual; n.weight = weight; n.y = y; n.h = h; n.rstd = rstd; n.scale = scale;
+    n.M = M; n.ldx = ldx; n.ldr = ldr; n.ldy = ldy; n.ldh = ldh; n.D = (int)D; n.eps = eps;
+    n.x_f32 = flags & WKV7_X_F32; n.r_f32 = flags & WKV7_R_F32; n.w_f32 = flags & WKV7_W_F32; n.y_f32 = flags & WKV7_Y_F32;
+    return wkv7::launch_norm_fwd(n, (cudaStream_t)stream);
+}
+
+int64_t wkv7_rms_norm_bwd_workspace_bytes(int64_t M, int64_t D) {
+    return M <= 0 || D <= 0 || D > WKV7_NORM_MAX_D ? 0 : (int64_t)wkv7::norm_bwd_partials(M, D) * D * 4;
+}
+
+int wkv7_rms_norm_bwd(const void* h, const float* rstd, const void* weight, const void* dy, const void* dh, void* dx, void* dr, float* dw, int64_t M, int64_t D,
+                      int64_t ldh, int64_t lddy, int64_t lddh, int64_t lddx, int64_t lddr, double p, uint64_t seed, const void* seed_ptr, int flags, void* workspace,
+                      void* stream) {
+    wkv7::NormBwdParams n{};
+    if (M < 0 || D <= 0 || ldh < D || lddy < D || (dh && lddh < D) || (dx && lddx < D) || (dr && lddr < D) || (flags & ~(WKV7_X_F32 | WKV7_R_F32 | WKV7_W_F32 | WKV7_Y_F32)) ||
+        !dropout_of(p, seed, seed_ptr, &n.d))
+        return WKV7_ERR_SHAPE;
+    if (D > WKV7_NORM_MAX_D) return WKV7_ERR_TOO_LARGE;
+    if (M == 0) return dw && cudaMemsetAsync(dw, 0, (size_t)D * 4, (cudaStream_t)stream) != cudaSuccess ? WKV7_ERR_LAUNCH : WKV7_OK;  // a sum over nothing
+    if (!h || !rstd || !dy || (dw && !workspace)) return WKV7_ERR_NULL;
+    const auto size = [&](int f) -> uintptr_t { return flags & f ? 4 : 2; };
+    if ((uintptr_t)h % size(WKV7_R_F32) || (uintptr_t)dh % size(WKV7_R_F32) || (uintptr_t)dr % size(WKV7_R_F32) || (uintptr_t)dx % size(WKV7_X_F32) ||
+        (uintptr_t)weight % size(WKV7_W_F32) || (uintptr_t)dy % size(WKV7_Y_F32) || (uintptr_t)rstd % 4 || (uintptr_t)dw % 4 || !aligned16(workspace) || (uintptr_t)seed_ptr % 8)
+        return WKV7_ERR_ALIGN;
+    n.h = h; n.weight = weight; n.dy = dy; n.dh = dh; n.rstd = rstd; n.dx = dx; n.dr = dr; n.dw = dw; n.partial = (float*)workspace;
+    n.M = M; n.ldh = ldh; n.lddy = lddy; n.lddh = lddh; n.lddx = lddx; n.lddr = lddr; n.D = (int)D;
+    n.h_f32 = flags & WKV7_R_F32; n.w_f32 = flags & WKV7_W_F32; n.y_f32 = flags & WKV7_Y_F32; n.x_f32 = flags & WKV7_X_F32;
+    return wkv7::launch_norm_bwd(n, (cudaStream_t)stream);
+}
+
+int wkv7_dropout(const void* x, const void* residual, void* y, int64_t n, double p, uint64_t seed, const void* seed_ptr, int flags, void* stream) {
+    wkv7::DropoutParams d{};
+    if (n < 0 || (flags & ~(WKV7_X_F32 | WKV7_R_F32 | WKV7_Y_F32)) || !dropout_of(p, seed, seed_ptr, &d.d)) return WKV7_ERR_SHAPE;
+    if (n == 0) return WKV7_OK;
+    if (!x || !y) return WKV7_ERR_NULL;
+    if (!aligned16(x) || !aligned16(residual) || !aligned16(y) || (uintptr_t)seed_ptr % 8) return WKV7_ERR_ALIGN;
+    d.x = x; d.residual = residual; d.y = y; d.n = n;
+    d.x_f32 = flags & WKV7_X_F32; d.r_f32 = flags & WKV7_R_F32; d.y_f32 = flags & WKV7_Y_F32;
+    return wkv7::launch_dropout(d, (cudaStream_t)stream);
 }
 
 static_assert(WKV7_ERR_INDEX == wkv7::kBadIndex, "mirrored constants");

@@ -21,6 +21,7 @@ namespace wkv7 {
 namespace lin {
 
 constexpr int BM = 128, BK = 64;
+__host__ __device__ constexpr int kb_of(bool i8) { return i8 ? 2 * BK : BK; }  // k of a block: rows of 128 bytes of an operand
 constexpr int MAXSTAGES = 12;
 // A wait for an accumulator lasts for a whole sum.  2^21 k blocks (k = 2^27) at 0.35 us are 0.7 s; the limit is 1.1 s.
 constexpr long long SUM_LIMIT = ACROSS_HANDOFF_LIMIT;
@@ -77,6 +78,7 @@ template <int ACT, bool FROM_Y> __device__ __forceinline__ float act_grad(float 
 struct Epi : LinearEpilogue {
     bool vec;       // rows of y start and end on 16-byte boundaries (bulk stores clip in steps of 16 bytes), those of the residual start there
     bool bias_vec;  // so does the bias
+    bool ws_vec;    // so do the columns' scales
 };
 __device__ __forceinline__ void load8g(const void* base, bool f32, long long at, float (&f)[8]) {
     if (f32) {
@@ -126,6 +128,45 @@ __device__ __forceinline__ void bias8(const Epi& e, long long col, float (&f)[8]
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = col + i < e.cols ? load1g(e.bias, e.bias_f32, col + i) : 0.f;
     }
+}
+// Sums of products in 8 bits are 32-bit integers, exact, and go through registers and memory as floats of the same bits.  They become numbers, times their row's
+// and their column's scale, where an epilogue takes them: one rounding in the conversion (from 2^24 on) and one for each scale.
+template <bool I8> __device__ __forceinline__ float add_sums(float a, float b) { return I8 ? __int_as_float(__float_as_int(a) + __float_as_int(b)) : a + b; }
+template <bool I8> __device__ __forceinline__ void add_sums(float4& a, const float4& b) {
+    a.x = add_sums<I8>(a.x, b.x); a.y = add_sums<I8>(a.y, b.y); a.z = add_sums<I8>(a.z, b.z); a.w = add_sums<I8>(a.w, b.w);
+}
+template <bool I8> __device__ __forceinline__ void add_sums8(float (&f)[8], const float4& a, const float4& b) {
+    f[0] = add_sums<I8>(f[0], a.x); f[1] = add_sums<I8>(f[1], a.y); f[2] = add_sums<I8>(f[2], a.z); f[3] = add_sums<I8>(f[3], a.w);
+    f[4] = add_sums<I8>(f[4], b.x); f[5] = add_sums<I8>(f[5], b.y); f[6] = add_sums<I8>(f[6], b.z); f[7] = add_sums<I8>(f[7], b.w);
+}
+__device__ __forceinline__ float scaled(float sum, float xs, float ws) { return __fmul_rn(__fmul_rn((float)__float_as_int(sum), xs), ws); }
+// eight adjacent columns' scales
+__device__ __forceinline__ void ws8(const Epi& e, long long col, float (&f)[8]) {
+    if (e.ws_vec && col + 8 <= e.cols) {
+        load8g(e.ws, true, col, f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = col + i < e.cols ? e.ws[col + i] : 0.f;
+    }
+}
+// n adjacent columns of a row
+template <bool I8, int N> __device__ __forceinline__ void scale_row(const Epi& e, long long row, long long col, float (&v)[N]) {
+    if (!I8) return;
+    const float xs = row < e.rows ? e.xs[row] : 0.f;
+#pragma unroll
+    for (int c = 0; c < N; c += 8) {
+        float f[8];
+        ws8(e, col + c, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[c + i] = scaled(v[c + i], xs, f[i]);
+    }
+}
+// a column of 32 rows
+template <bool I8> __device__ __forceinline__ void scale_col(const Epi& e, long long row, long long col, float (&v)[32]) {
+    if (!I8) return;
+    const float ws = col < e.cols ? e.ws[col] : 0.f;
+#pragma unroll
+    for (int c = 0; c < 32; ++c) v[c] = scaled(v[c], row + c < e.rows ? e.xs[row + c] : 0.f, ws);
 }
 // eight adjacent columns of a row, from the accumulator to memory; bias already added
 template <int ACT> __device__ __forceinline__ void finish8(const Epi& e, long long row, long long col, float (&f)[8]) {
@@ -351,6 +392,18 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t saddr, bool mn) {
 __host__ __device__ constexpr uint32_t idesc_of(int m, int n, bool p_mn, bool q_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((p_mn ? 1u : 0u) << 15) | ((q_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+// 32-bit integer sums, signed 8-bit operands, K-major
+__host__ __device__ constexpr uint32_t idesc_i8_of(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+// one product of 32 bytes of k, by this CTA or by the pair
+template <bool I8, int CTAS> __device__ __forceinline__ void product(uint32_t acc, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+#define WKV7_MMA(group, kind) \
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::" #group ".kind::" #kind " [%0], %1, %2, %3, p;\n}\n" ::"r"(acc), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u) : "memory")
+    if (I8 && CTAS == 1) WKV7_MMA(1, i8);
+    else if (I8) WKV7_MMA(2, i8);
+    else if (CTAS == 1) WKV7_MMA(1, f16);
+    else WKV7_MMA(2, f16);
+#undef WKV7_MMA
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -410,7 +463,8 @@ __host__ __device__ constexpr int part_bytes(int nt) { return BM * part_pitch(nt
 
 __device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
-template <int ACT> __global__ void __launch_bounds__(TILE_THREADS, 3) linear_tile_kernel(const __grid_constant__ TileParams p, int* status) {
+template <int ACT, bool I8> __global__ void __launch_bounds__(TILE_THREADS, 3) linear_tile_kernel(const __grid_constant__ TileParams p, int* status) {
+    constexpr int KB = kb_of(I8);
     extern __shared__ unsigned char smem_dyn[];
     TileCtrl* ctrl = reinterpret_cast<TileCtrl*>(smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u));
     unsigned char* sm = reinterpret_cast<unsigned char*>(ctrl) + 1024;
@@ -459,10 +513,10 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS, 3) linear_til
                     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                                  ::"r"(to), "l"(m), "r"(bar), "r"(x), "r"(y) : "memory");
                 };
-                if (p.p_mn) { load(&p.P, dst, p0, kb * BK); load(&p.P, dst + 8192, p0 + 64, kb * BK); }
-                else load(&p.P, dst, kb * BK, p0);
-                if (p.q_mn) for (int b = 0; b < p.nt; b += 64) load(&p.Q, dst + P_BYTES + b * 128, q0 + b, kb * BK);
-                else load(&p.Q, dst + P_BYTES, kb * BK, q0);
+                if (p.p_mn) { load(&p.P, dst, p0, kb * KB); load(&p.P, dst + 8192, p0 + 64, kb * KB); }
+                else load(&p.P, dst, kb * KB, p0);
+                if (p.q_mn) for (int b = 0; b < p.nt; b += 64) load(&p.Q, dst + P_BYTES + b * 128, q0 + b, kb * KB);
+                else load(&p.Q, dst + P_BYTES, kb * KB, q0);
                 ++issued;
                 if (++s == p.stages) { s = 0; ++round; }
             }
@@ -471,7 +525,7 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS, 3) linear_til
         __syncwarp();
     } else if (warp == 5) {
         if (elect_one()) {
-            const uint32_t idesc = idesc_of(BM, p.nt, p.p_mn, p.q_mn);
+            const uint32_t idesc = I8 ? idesc_i8_of(BM, p.nt) : idesc_of(BM, p.nt, p.p_mn, p.q_mn);
             const uint64_t step_p = p.p_mn ? 2048 >> 4 : 2, step_q = p.q_mn ? 2048 >> 4 : 2;  // 16 k
             int s = 0, round = 0, a = 0;
             for (int kb = lo; kb < hi; ++kb) {
@@ -480,8 +534,7 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS, 3) linear_til
                 const uint64_t da = desc_of(smem_u32(sm + s * stage_bytes), p.p_mn), db = desc_of(smem_u32(sm + s * stage_bytes + P_BYTES), p.q_mn);
 #pragma unroll
                 for (int ks = 0; ks < BK / 16; ++ks)
-                    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                                 ::"r"(tmem + a * p.nt), "l"(da + ks * step_p), "l"(db + ks * step_q), "r"(idesc), "r"((kb >= lo + p.accs || ks > 0) ? 1u : 0u) : "memory");
+                    product<I8, 1>(tmem + a * p.nt, da + ks * step_p, db + ks * step_q, idesc, kb >= lo + p.accs || ks > 0);
                 asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&ctrl->empty[s])) : "memory");
                 if (++s == p.stages) { s = 0; ++round; }
                 if (++a == p.accs) a = 0;
@@ -518,14 +571,14 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS, 3) linear_til
                         float u[32];
                         tmem_ld32(acc + a * p.nt + c, reinterpret_cast<uint32_t(&)[32]>(u));
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] += u[i];
+                        for (int i = 0; i < 32; ++i) v[i] = add_sums<I8>(v[i], u[i]);
                     }
                 };
                 // (blocks two by two, as the pairs have them, would take 190 registers and more: one CTA an SM)
                 const int row0 = p0 + 32 * warp, col0 = q0 + c;
                 if (row0 >= e.rows || col0 >= e.cols) continue;
-                if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, sums);
-                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); turn_block(mine, lane, v); });
+                if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); scale_row<I8>(e, row0 + lane, col0, v); });
+                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); turn_block(mine, lane, v); scale_col<I8>(e, row0, col0 + lane, v); });
             }
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
@@ -547,7 +600,7 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS, 3) linear_til
                 uint32_t u[16];
                 tmem_ld16(tmem + ((uint32_t)(32 * warp) << 16) + a * p.nt + c, u);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(u[i]));
+                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(add_sums<I8>(__uint_as_float(v[i]), __uint_as_float(u[i])));
             }
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
@@ -570,8 +623,13 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS, 3) linear_til
             if (col >= e.cols || q0 + j >= e.rows) continue;
             float4 x = ld4(parts + i * pitch + j);
             for (int r = 1; r < p.splits; ++r) {
-                const float4 y = ld4(parts + (r * rows + i) * pitch + j);
-                x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+                add_sums<I8>(x, ld4(parts + (r * rows + i) * pitch + j));
+            }
+            if (I8) {
+                const float ws = e.ws[col];
+                float* const sum[4] = {&x.x, &x.y, &x.z, &x.w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) *sum[q] = scaled(*sum[q], q0 + j + q < e.rows ? e.xs[q0 + j + q] : 0.f, ws);
             }
             const float bias = e.bias ? load1g(e.bias, e.bias_f32, col) : 0.f;
             const float f[4] = {x.x + bias, x.y + bias, x.z + bias, x.w + bias};
@@ -601,7 +659,7 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS, 3) linear_til
             for (int r = 0; r < p.splits; ++r) {
                 const float* x = parts + (r * rows + i) * pitch + j;
                 const float4 a = ld4(x), b = ld4(x + 4);
-                f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+                add_sums8<I8>(f, a, b);
             }
         };
         if (p.outer > 1) {
@@ -631,11 +689,12 @@ template <int ACT> __global__ void __launch_bounds__(TILE_THREADS, 3) linear_til
                 for (int c = 0; c < p.outer; ++c) {
                     const float4* x = reinterpret_cast<const float4*>(mine + c * plane + 8 * u);
                     const float4 a = __ldcg(x), b = __ldcg(x + 1);
-                    f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w; f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+                    add_sums8<I8>(f, a, b);
                 }
             } else {
                 joined(u, f);
             }
+            scale_row<I8>(e, row, col, f);
             if (e.bias) {
                 float bias[8];
                 bias8(e, col, bias);
@@ -708,7 +767,8 @@ __global__ void __launch_bounds__(256) linear_zero_kernel(unsigned* p, int n) {
     if (i < n) p[i] = 0;
 }
 
-template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) linear_pair_kernel(const __grid_constant__ PairParams p, int* status) {
+template <int ACT, bool I8> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1) linear_pair_kernel(const __grid_constant__ PairParams p, int* status) {
+    constexpr int KB = kb_of(I8);
     extern __shared__ unsigned char smem_dyn[];
     unsigned char* sm = smem_dyn + ((1024u - (smem_u32(smem_dyn) & 1023u)) & 1023u);
     unsigned char* staging = sm + PAIR_STAGES * PAIR_STAGE;
@@ -761,10 +821,10 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
                         asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];"
                                      ::"r"(to), "l"(m), "r"(bar), "r"(x), "r"(y) : "memory");
                     };
-                    if (p.p_mn) { load(&p.P, dst, p0, kb * BK); load(&p.P, dst + 8192, p0 + 64, kb * BK); }
-                    else load(&p.P, dst, kb * BK, p0);
-                    if (p.q_mn) for (int b = 0; b < half; b += 64) load(&p.Q, dst + PAIR_P + b * 128, q0 + b, kb * BK);
-                    else load(&p.Q, dst + PAIR_P, kb * BK, q0);
+                    if (p.p_mn) { load(&p.P, dst, p0, kb * KB); load(&p.P, dst + 8192, p0 + 64, kb * KB); }
+                    else load(&p.P, dst, kb * KB, p0);
+                    if (p.q_mn) for (int b = 0; b < half; b += 64) load(&p.Q, dst + PAIR_P + b * 128, q0 + b, kb * KB);
+                    else load(&p.Q, dst + PAIR_P, kb * KB, q0);
                     ++issued;
                     if (++s == PAIR_STAGES) { s = 0; ++round; }
                 }
@@ -779,7 +839,7 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
         __syncwarp();
     } else if (warp == 1 && rank == 0) {
         if (elect_one()) {
-            const uint32_t idesc = idesc_of(2 * BM, p.bn, p.p_mn, p.q_mn);
+            const uint32_t idesc = I8 ? idesc_i8_of(2 * BM, p.bn) : idesc_of(2 * BM, p.bn, p.p_mn, p.q_mn);
             const uint64_t step_p = p.p_mn ? 2048 >> 4 : 2, step_q = p.q_mn ? 2048 >> 4 : 2;
             auto commit = [](uint64_t* bar) {
                 asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
@@ -796,8 +856,7 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
                     const uint64_t da = desc_of(smem_u32(sm + s * PAIR_STAGE), p.p_mn), db = desc_of(smem_u32(sm + s * PAIR_STAGE + PAIR_P), p.q_mn);
 #pragma unroll
                     for (int ks = 0; ks < BK / 16; ++ks)
-                        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-                                     ::"r"(acc), "l"(da + ks * step_p), "l"(db + ks * step_q), "r"(idesc), "r"((kb > w.lo || ks > 0) ? 1u : 0u) : "memory");
+                        product<I8, 2>(acc, da + ks * step_p, db + ks * step_q, idesc, kb > w.lo || ks > 0);
                     commit(&ctrl->empty[s]);
                     if (++s == PAIR_STAGES) { s = 0; ++round; }
                 }
@@ -871,6 +930,8 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
                         tmem_ld32(acc + 32 * b, reinterpret_cast<uint32_t(&)[32]>(v[0]));
                         tmem_ld32(acc + 32 * b + 32, reinterpret_cast<uint32_t(&)[32]>(v[1]));
                         if (b + 1 == b1 - 1) emptied();
+                        scale_row<I8>(e, row0 + lane, col0, v[0]);
+                        scale_row<I8>(e, row0 + lane, col0 + 32, v[1]);
                     });
                     ++b;
                     continue;
@@ -886,7 +947,10 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
 #pragma unroll
                             for (int u = 0; u < 8; ++u) x[u] = __ldcg(from + u * 32);
 #pragma unroll
-                            for (int u = 0; u < 8; ++u) { v[4 * u] += x[u].x; v[4 * u + 1] += x[u].y; v[4 * u + 2] += x[u].z; v[4 * u + 3] += x[u].w; }
+                            for (int u = 0; u < 8; ++u) {
+                                v[4 * u] = add_sums<I8>(v[4 * u], x[u].x); v[4 * u + 1] = add_sums<I8>(v[4 * u + 1], x[u].y);
+                                v[4 * u + 2] = add_sums<I8>(v[4 * u + 2], x[u].z); v[4 * u + 3] = add_sums<I8>(v[4 * u + 3], x[u].w);
+                            }
                         }
                     } else {
                         tmem_ld32(acc + 32 * b, reinterpret_cast<uint32_t(&)[32]>(v));
@@ -897,9 +961,10 @@ template <int ACT> __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P
                     if (b == b1 - 1 && !parts) emptied();
                     continue;
                 }
-                if (p.swap) finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, sums);
-                else if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, sums);
-                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); turn_block(mine, lane, v); });
+                const auto column = [&](float (&v)[32]) { sums(v); scale_col<I8>(e, row0, col0 + lane, v); };
+                if (p.swap) finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, column);
+                else if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); scale_row<I8>(e, row0 + lane, col0, v); });
+                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); turn_block(mine, lane, v); scale_col<I8>(e, row0, col0 + lane, v); });
             }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory must outlive the stores' reads
@@ -1020,15 +1085,15 @@ static EncodeTiledFn encode_fn() {
     }();
     return fn;
 }
-// box_rows: indices of a K-major box; an MN-major one is 64 indices x 64 k
-static bool encode(CUtensorMap* m, const LinearOperand& o, long long n, long long k, int box_rows) {
+// box_rows: indices of a K-major box; an MN-major one is 64 indices x 64 k (8 bits: K-major alone)
+static bool encode(CUtensorMap* m, const LinearOperand& o, long long n, long long k, int box_rows, bool i8) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)(o.mn ? n : k), (cuuint64_t)(o.mn ? k : n)};
-    const cuuint64_t strides[1] = {(cuuint64_t)o.ld * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)(o.mn ? BK : box_rows)};
+    const cuuint64_t strides[1] = {(cuuint64_t)o.ld * (i8 ? 1 : 2)};
+    const cuuint32_t box[2] = {(cuuint32_t)kb_of(i8), (cuuint32_t)(o.mn ? BK : box_rows)};
     const cuuint32_t es[2] = {1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(o.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    return fn(m, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(o.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 // results: boxes of 32 columns x 32 rows
@@ -1047,25 +1112,27 @@ static bool encode_results(const Epi& e, CUtensorMap* Y, CUtensorMap* Z) {
     return encode_out(Y, e.y, e.y_f32, e.rows, e.cols, e.ldy) && (!e.z || encode_out(Z, e.z, e.z_f32, e.rows, e.cols, e.ldz));
 }
 
-static thread_local uint32_t smem_allowed[64];
-template <typename P> struct Kernels { void (*k[kActs])(P, int*); };
-#define WKV7_PER_ACT(kernel) {{kernel<kActNone>, kernel<kActRelu>, kernel<kActRelu2>, kernel<kActTanh>, kernel<kActSigmoid>, kernel<kActSilu>, kernel<kActGelu>}}
-static const Kernels<TileParams> tile_kernels = WKV7_PER_ACT(linear_tile_kernel);
-static const Kernels<PairParams> pair_kernels = WKV7_PER_ACT(linear_pair_kernel);
+static int kblocks_of(long long k, bool i8) { return (int)((k + kb_of(i8) - 1) / kb_of(i8)); }
+static thread_local uint32_t smem_allowed[2][64];  // [8 bits][device]
+template <typename P> struct Kernels { void (*k[2][kActs])(P, int*); };
+#define WKV7_PER_ACT(kernel, i8) {kernel<kActNone, i8>, kernel<kActRelu, i8>, kernel<kActRelu2, i8>, kernel<kActTanh, i8>, kernel<kActSigmoid, i8>, kernel<kActSilu, i8>, kernel<kActGelu, i8>}
+static const Kernels<TileParams> tile_kernels = {{WKV7_PER_ACT(linear_tile_kernel, false), WKV7_PER_ACT(linear_tile_kernel, true)}};
+static const Kernels<PairParams> pair_kernels = {{WKV7_PER_ACT(linear_pair_kernel, false), WKV7_PER_ACT(linear_pair_kernel, true)}};
 
 static int run_tile(LinearOperand a, LinearOperand b, long long na, long long nb, long long k, const Epi& e, bool swap, int nt, int splits, int outer, void* workspace, int* status,
                     cudaStream_t stream) {
-    const auto kern = tile_kernels.k[e.act];
-    if (!allow_smem(kern, smem_allowed, e.act, 227 * 1024)) return kLaunchFailed;
+    const bool i8 = e.xs != nullptr;
+    const auto kern = tile_kernels.k[i8][e.act];
+    if (!allow_smem(kern, smem_allowed[i8], e.act, 227 * 1024)) return kLaunchFailed;
     TileParams p;
     memset(&p, 0, sizeof(p));
-    if (!encode(&p.P, a, na, k, BM) || !encode(&p.Q, b, nb, k, nt)) return kLaunchFailed;
+    if (!encode(&p.P, a, na, k, BM, i8) || !encode(&p.Q, b, nb, k, nt, i8)) return kLaunchFailed;
     p.e = e;
     p.p_mn = a.mn; p.q_mn = b.mn; p.nt = nt; p.swap = swap;
     p.outer = outer;
     p.direct = !swap && splits == 1 && outer == 1;
     if (p.direct && e.vec && !encode_results(e, &p.Y, &p.Z)) return kLaunchFailed;
-    p.kblocks = (int)((k + BK - 1) / BK);
+    p.kblocks = kblocks_of(k, i8);
     p.splits = splits;
     p.p_tiles = (int)((na + BM - 1) / BM);
     const long long tiles = p.p_tiles * ((nb + nt - 1) / nt), grid = tiles * splits * outer;
@@ -1131,17 +1198,18 @@ static PairPlan plan_pair(long long rows, long long cols, int kblocks, bool can_
 static size_t pair_ws(const PairPlan& x) { return x.splits > 1 ? (size_t)(x.tiles - x.whole) * ((size_t)x.splits * PART_F4 * 16 + 64) : 0; }
 
 static int run_pair(LinearOperand rows, LinearOperand cols, long long k, const Epi& e, const PairPlan& x, void* workspace, int* status, cudaStream_t stream) {
-    const auto kern = pair_kernels.k[e.act];
-    if (!allow_smem(kern, smem_allowed, 16 + e.act, PAIR_SMEM)) return kLaunchFailed;
+    const bool i8 = e.xs != nullptr;
+    const auto kern = pair_kernels.k[i8][e.act];
+    if (!allow_smem(kern, smem_allowed[i8], 16 + e.act, PAIR_SMEM)) return kLaunchFailed;
     PairParams p;
     memset(&p, 0, sizeof(p));
     const LinearOperand &a = x.swap ? cols : rows, &b = x.swap ? rows : cols;
     const long long na = x.swap ? e.cols : e.rows, nb = x.swap ? e.rows : e.cols;
-    if (!encode(&p.P, a, na, k, BM) || !encode(&p.Q, b, nb, k, x.bn / 2)) return kLaunchFailed;
+    if (!encode(&p.P, a, na, k, BM, i8) || !encode(&p.Q, b, nb, k, x.bn / 2, i8)) return kLaunchFailed;
     if (e.vec && !encode_results(e, &p.Y, &p.Z)) return kLaunchFailed;
     p.e = e;
     p.p_mn = a.mn; p.q_mn = b.mn; p.bn = x.bn; p.swap = x.swap; p.splits = x.splits;
-    p.kblocks = (int)((k + BK - 1) / BK);
+    p.kblocks = kblocks_of(k, i8);
     p.p_tiles = (int)((na + 2 * BM - 1) / (2 * BM));
     p.q_tiles = (int)((nb + x.bn - 1) / x.bn);
     p.tiles = x.tiles; p.whole = x.whole;
@@ -1162,8 +1230,8 @@ struct Plan {
     int nt, splits, outer;  // of tiles of 128 x nt
     PairPlan x;
 };
-static Plan make_plan(long long rows, long long cols, long long k, bool rows_mn, bool can_split) {
-    const int kblocks = (int)((k + BK - 1) / BK), sms = sm_count();
+static Plan make_plan(long long rows, long long cols, long long k, bool rows_mn, bool can_split, bool i8) {
+    const int kblocks = kblocks_of(k, i8), sms = sm_count();
     Plan p{};
     p.outer = 1;
     auto split = [&](long long tiles, int most, int places) {  // CTAs of one tile: as many as there are places for
@@ -1207,8 +1275,8 @@ static Plan make_plan(long long rows, long long cols, long long k, bool rows_mn,
 
 }  // namespace lin
 
-size_t linear_workspace_bytes(long long rows, long long cols, long long k, bool rows_mn) {
-    const lin::Plan p = lin::make_plan(rows, cols, k, rows_mn, true);
+size_t linear_workspace_bytes(long long rows, long long cols, long long k, bool rows_mn, bool i8) {
+    const lin::Plan p = lin::make_plan(rows, cols, k, rows_mn, true, i8);
     if (p.pair) return lin::pair_ws(p.x);
     const long long tiles = ((rows + lin::BM - 1) / lin::BM) * ((cols + p.nt - 1) / p.nt);
     return p.outer > 1 ? (size_t)tiles * ((size_t)p.outer * lin::BM * p.nt * 4 + (size_t)p.splits * 4) : 0;
@@ -1221,8 +1289,10 @@ int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const Lin
     const int per16 = ep.y_f32 ? 4 : 8;
     e.vec = al16(ep.y) && ep.ldy % per16 == 0 && ep.cols % per16 == 0 && (!ep.residual || (al16(ep.residual) && ep.ldr % per16 == 0));
     e.bias_vec = al16(ep.bias);
+    e.ws_vec = al16(ep.ws);
+    const bool i8 = ep.xs != nullptr;
     if ((k + BK - 1) / BK > MAX_KBLOCKS) return kTooLarge;
-    const Plan p = make_plan(ep.rows, ep.cols, k, rows.mn, workspace != nullptr);
+    const Plan p = make_plan(ep.rows, ep.cols, k, rows.mn, workspace != nullptr, i8);
     if (p.pair) return run_pair(rows, cols, k, e, p.x, workspace, status, stream);
     if (p.swap) return run_tile(cols, rows, ep.cols, ep.rows, k, e, true, p.nt, p.splits, 1, nullptr, status, stream);
     return run_tile(rows, cols, ep.rows, ep.cols, k, e, false, p.nt, p.splits, p.outer, workspace, status, stream);

@@ -16,6 +16,7 @@ struct LinearEpilogue {
     long long ldr, ldy, ldz, rows, cols;
     int act;
     bool bias_f32, y_f32, z_f32;
+    const float *xs = nullptr, *ws = nullptr;  // operands in 8 bits: the rows' and the columns' scales, [rows] and [cols]; null: bf16 operands
 };
 
 // y[rows, cols] = epilogue(sum_k P[i, k] Q[j, k]); an operand is [index, k] with k contiguous, or (`_mn`) [k, index] with the index contiguous
@@ -24,8 +25,9 @@ struct LinearOperand {
     long long ld;
     bool mn;
 };
+// 8-bit operands: K-major, rows a multiple of 16 bytes apart, k < 2^17 (the sum of 2^17 products of -128 leaves 32 bits); neither bias nor z differ.
 // workspace: linear_workspace_bytes() bytes (rows_mn: the rows' operand is [k, index]), or null: no tile is cut along k
-size_t linear_workspace_bytes(long long rows, long long cols, long long k, bool rows_mn);
+size_t linear_workspace_bytes(long long rows, long long cols, long long k, bool rows_mn, bool i8 = false);
 int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const LinearEpilogue& e, void* workspace, int* status, cudaStream_t stream);
 
 // dz = dy act'(saved) as bf16 [M, ldz] (not written where dz is null) and dbias = column sums of dz (or null; then of dz before its rounding)

@@ -584,6 +584,230 @@ py::object linear(const Tensor& x, const Tensor& w, const OptTensor& bias_, cons
     return py::cast(y);
 }
 
+// ---- the residual stream, rows in 8 bits --------------------------------------------------------------------
+bool float_type(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
+bool is_f32(const Tensor& t) { return t.defined() && t.scalar_type() == at::kFloat; }
+int64_t pitch8(int64_t n) { return (n + 15) / 16 * 16; }  // bytes from row to row of a tensor in 8 bits
+// [..., n] in 8 bits, its rows pitch8(n) apart
+Tensor empty8(const Tensor& like) {
+    std::vector<int64_t> shape = like.sizes().vec();
+    shape.back() = pitch8(like.size(-1));
+    return at::empty(shape, like.options().dtype(at::kChar));
+}
+Tensor as_rows(const Tensor& t, int64_t* ld) {  // (hooks on saved tensors, and gradients, may come in other layouts)
+    if (!t.defined()) return t;
+    if (pitched_rows(t, ld)) return t;
+    Tensor c = t.contiguous();
+    *ld = t.size(-1);
+    return c;
+}
+struct NormHow {  // of a call, for its backward
+    double eps, p;
+    int64_t seed;
+    int64_t out;  // of y: 0 bf16, 1 fp32, 2 8 bits
+};
+// y, h (undefined without residual), rstd (undefined without save), scale (undefined unless 8 bits)
+std::array<Tensor, 4> norm_forward(const Tensor& x, const Tensor& w, const Tensor& r, const Tensor& seed, const NormHow& n, bool save) {
+    const int64_t D = x.size(-1), M = x.numel() / D;
+    Tensor y, h, rstd, scale;
+    if (n.out == 2) {
+        y = empty8(x);
+        scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    } else {
+        y = at::empty(x.sizes(), x.options().dtype(n.out ? at::kFloat : at::kBFloat16));
+    }
+    if (r.defined()) h = at::empty(x.sizes(), r.options());
+    if (save) rstd = at::empty({M}, x.options().dtype(at::kFloat));
+    int64_t ldx = D, ldr = D;
+    pitched_rows(x, &ldx);
+    if (r.defined()) pitched_rows(r, &ldr);
+    check(wkv7_rms_norm_fwd(x.data_ptr(), ptr(r), ptr(w), y.data_ptr(), ptr(h), f32(rstd), f32(scale), M, D, ldx, ldr, y.size(-1), D, (float)n.eps, n.p, (uint64_t)n.seed, ptr(seed),
+                            (is_f32(x) ? WKV7_X_F32 : 0) | (is_f32(r) ? WKV7_R_F32 : 0) | (is_f32(w) ? WKV7_W_F32 : 0) | (n.out == 2 ? WKV7_Y_INT8 : n.out ? WKV7_Y_F32 : 0), stream()),
+          "wkv7_rms_norm_fwd");
+    return {y, h, rstd, scale};
+}
+int64_t bits_of(double d) { int64_t b; memcpy(&b, &d, 8); return b; }
+double double_of(int64_t b) { double d; memcpy(&d, &b, 8); return d; }
+struct RmsNormFn : public Function<RmsNormFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w_, const OptTensor& r_, const OptTensor& seed_, double eps, double p, int64_t seed, int64_t out) {
+        const Tensor w = w_.value_or(Tensor()), r = r_.value_or(Tensor()), s = seed_.value_or(Tensor());
+        const auto [y, h, rstd, scale] = norm_forward(x, w, r, s, NormHow{eps, p, seed, out}, true);
+        ctx->save_for_backward({r.defined() ? h : x, rstd, w, s});
+        ctx->set_materialize_grads(false);
+        // (one value: each looked up by name costs half a us)
+        ctx->saved_data["how"] = std::vector<int64_t>{out | is_f32(x) << 8 | w.defined() << 9 | r.defined() << 10, bits_of(p), seed};
+        return r.defined() ? variable_list{y, h} : variable_list{y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list go) {
+        variable_list g(8);
+        const auto how = ctx->saved_data["how"].toIntVector();
+        const bool out_f32 = how[0] & 255, x_f32 = how[0] >> 8 & 1, weight = how[0] >> 9 & 1, residual = how[0] >> 10 & 1;
+        const double p = double_of(how[1]);
+        Tensor dy = go[0], dh = residual ? go[1] : Tensor();
+        // (edges are counted over the arguments that are tensors)
+        const bool want_x = ctx->needs_input_grad(0), want_w = weight && ctx->needs_input_grad(1), want_r = residual && ctx->needs_input_grad(weight ? 2 : 1);
+        if ((!dy.defined() && !dh.defined()) || !(want_x || want_w || want_r)) return g;
+        const variable_list s = ctx->get_saved_variables();
+        const c10::cuda::CUDAGuard guard(s[0].device());
+        at::NoGradGuard ng;
+        const int64_t D = s[0].size(-1), M = s[0].numel() / D;
+        int64_t ldh = D, lddy = D, lddh = D;
+        const Tensor h = as_rows(s[0], &ldh), rstd = s[1].contiguous(), w = weight ? s[2].contiguous() : Tensor(), seed = s[3].defined() ? s[3].contiguous() : Tensor();
+        const auto y_type = out_f32 ? at::kFloat : at::kBFloat16;
+        dy = as_rows(dy.defined() ? dy.to(y_type) : at::zeros(h.sizes(), h.options().dtype(y_type)), &lddy);
+        if (dh.defined()) dh = as_rows(dh.to(h.scalar_type()), &lddh);
+        const bool one = p == 0. && x_f32 == is_f32(h);  // x and the stream have the same gradient
+        Tensor dx, dr, dw, ws;
+        if (want_x && !one) dx = at::empty(h.sizes(), h.options().dtype(x_f32 ? at::kFloat : at::kBFloat16));
+        if (want_r || (want_x && one)) dr = at::empty(h.sizes(), h.options());
+        if (want_w) {
+            dw = at::empty({D}, h.options().dtype(at::kFloat));
+            ws = at::empty({wkv7_rms_norm_bwd_workspace_bytes(M, D)}, h.options().dtype(at::kByte));
+        }
+        check(wkv7_rms_norm_bwd(h.data_ptr(), f32_of(rstd), ptr(w), dy.data_ptr(), ptr(dh), ptr(dx), ptr(dr), f32(dw), M, D, ldh, lddy, lddh, D, D, p, (uint64_t)how[2], ptr(seed),
+                                (x_f32 ? WKV7_X_F32 : 0) | (is_f32(h) ? WKV7_R_F32 : 0) | (is_f32(w) ? WKV7_W_F32 : 0) | (out_f32 ? WKV7_Y_F32 : 0), ptr(ws), stream()),
+              "wkv7_rms_norm_bwd");
+        if (want_x) g[0] = one ? dr : dx;
+        if (want_w) g[1] = dw.to(w.scalar_type());
+        if (want_r) g[2] = dr;
+        return g;
+    }
+};
+// p and where the seed is; seed < 0: no number
+bool dropout_ok(double p, int64_t seed, const Tensor& seed_t, const Tensor& x) {
+    if (!(p >= 0. && p <= 1.)) return false;
+    if (seed_t.defined()) return plain(seed_t) && seed_t.scalar_type() == at::kLong && seed_t.numel() == 1 && seed_t.device() == x.device();
+    return seed >= 0;
+}
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+py::object rms_norm(const Tensor& x, const OptTensor& w_, const OptTensor& r_, double eps, double p, int64_t seed, const OptTensor& seed_, int64_t out) {
+    const Tensor w = w_.value_or(Tensor()), r = r_.value_or(Tensor()), s = seed_.value_or(Tensor());
+    int64_t ld;
+    if (!eager({&x, &w, &r, &s}) || x.dim() < 1 || x.numel() == 0 || !float_type(x) || !pitched_rows(x, &ld) || x.size(-1) > WKV7_NORM_MAX_D || !(eps >= 0.) || out < -1) return py::none();
+    if (w.defined() && (!plain(w) || !float_type(w) || w.dim() != 1 || w.size(0) != x.size(-1) || !w.is_contiguous() || w.device() != x.device())) return py::none();
+    if (r.defined() && (!plain(r) || !float_type(r) || r.sizes() != x.sizes() || r.device() != x.device() || !pitched_rows(r, &ld))) return py::none();
+    if (p != 0. && !r.defined()) return py::none();
+    if (p == 0. ? s.defined() && !dropout_ok(p, seed, s, x) : !dropout_ok(p, seed, s, x)) return py::none();
+    if (out < 0) out = is_f32(x);
+    const bool grad = grad_wanted({&x, &w, &r});
+    if (grad && out == 2) return py::none();
+    variable_list o;
+    {
+        py::gil_scoped_release nogil;
+        const c10::cuda::CUDAGuard guard(x.device());
+        if (grad) {
+            o = RmsNormFn::apply(x, opt(w), opt(r), opt(s), eps, p, seed < 0 ? 0 : seed, out);
+        } else {
+            at::NoGradGuard ng;
+            const auto [y, h, rstd, scale] = norm_forward(x, w, r, s, NormHow{eps, p, seed < 0 ? 0 : seed, out}, false);
+            if (out == 2) o = {y.narrow(-1, 0, x.size(-1)), scale};
+            else o = {y};
+            if (r.defined()) o.push_back(h);
+        }
+    }
+    if (o.size() == 1) return py::cast(o[0]);
+    return o.size() == 2 ? py::make_tuple(o[0], o[1]) : py::make_tuple(o[0], o[1], o[2]);
+}
+
+// adjacent elements from a 16-byte boundary on
+Tensor dropped(const Tensor& x, const Tensor& r, const Tensor& seed_t, double p, int64_t seed, at::ScalarType type) {
+    Tensor y = at::empty(x.sizes(), x.options().dtype(type));
+    check(wkv7_dropout(x.data_ptr(), ptr(r), y.data_ptr(), x.numel(), p, (uint64_t)seed, ptr(seed_t), (is_f32(x) ? WKV7_X_F32 : 0) | (is_f32(r) ? WKV7_R_F32 : 0) | (is_f32(y) ? WKV7_Y_F32 : 0),
+                       stream()), "wkv7_dropout");
+    return y;
+}
+struct DropoutFn : public Function<DropoutFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& r_, const OptTensor& seed_, double p, int64_t seed) {
+        const Tensor r = r_.value_or(Tensor()), s = seed_.value_or(Tensor());
+        ctx->save_for_backward({s});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["how"] = std::vector<int64_t>{is_f32(x) | r.defined() << 1, bits_of(p), seed};
+        return dropped(x, r, s, p, seed, r.defined() ? r.scalar_type() : x.scalar_type());
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list go) {
+        variable_list g(5);
+        const Tensor dy = go[0];
+        if (!dy.defined()) return g;
+        const auto how = ctx->saved_data["how"].toIntVector();
+        if (how[0] >> 1 && ctx->needs_input_grad(1)) g[1] = dy;
+        if (!ctx->needs_input_grad(0)) return g;
+        const c10::cuda::CUDAGuard guard(dy.device());
+        at::NoGradGuard ng;
+        const Tensor s = ctx->get_saved_variables()[0];
+        g[0] = dropped(dense(dy), Tensor(), s, double_of(how[1]), how[2], how[0] & 1 ? at::kFloat : at::kBFloat16);
+        return g;
+    }
+};
+py::object dropout(const Tensor& x, double p, int64_t seed, const OptTensor& seed_, const OptTensor& r_) {
+    const Tensor r = r_.value_or(Tensor()), s = seed_.value_or(Tensor());
+    if (!eager({&x, &r, &s}) || !plain(x) || x.numel() == 0 || !float_type(x) || !dropout_ok(p, seed, s, x)) return py::none();
+    if (r.defined() && (!plain(r) || !float_type(r) || r.sizes() != x.sizes() || r.device() != x.device())) return py::none();
+    Tensor y;
+    {
+        py::gil_scoped_release nogil;
+        const c10::cuda::CUDAGuard guard(x.device());
+        if (seed < 0) seed = 0;
+        const Tensor xd = dense(x), rd = dense(r);  // (with autograd: copies are part of the graph)
+        if (grad_wanted({&x, &r})) {
+            y = DropoutFn::apply(xd, opt(rd), opt(s), p, seed);
+        } else {
+            at::NoGradGuard ng;
+            y = dropped(xd, rd, s, p, seed, r.defined() ? r.scalar_type() : x.scalar_type());
+        }
+    }
+    return py::cast(y);
+}
+
+py::object quantize(const Tensor& x) {
+    int64_t ld;
+    if (!eager({&x}, false) || x.dim() < 1 || x.numel() == 0 || !float_type(x) || !pitched_rows(x, &ld)) return py::none();
+    Tensor q, scale;
+    {
+        py::gil_scoped_release nogil;
+        const c10::cuda::CUDAGuard guard(x.device());
+        at::NoGradGuard ng;
+        const int64_t K = x.size(-1);
+        q = empty8(x);
+        scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+        check(wkv7_quantize(x.data_ptr(), q.data_ptr(), f32_of(scale), x.numel() / K, K, ld, q.size(-1), is_f32(x) ? WKV7_X_F32 : 0, stream()), "wkv7_quantize");
+        if (q.size(-1) != K) q = q.narrow(-1, 0, K);
+    }
+    return py::make_tuple(q, scale);
+}
+
+bool operand8(const Tensor& t, int64_t* ld) {
+    return pitched_rows(t, ld) && t.scalar_type() == at::kChar && *ld % 16 == 0 && !(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15);
+}
+py::object linear_int8(const Tensor& xq, const Tensor& xs, const Tensor& wq, const Tensor& ws, const OptTensor& bias_, const OptTensor& residual_, int64_t act, bool out_f32) {
+    const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
+    int64_t ldx, ldw, ldr = 0;
+    if (!eager({&xq, &xs, &wq, &ws, &bias, &residual}, false) || xq.dim() < 1 || wq.dim() != 2 || !operand8(xq, &ldx) || !operand8(wq, &ldw)) return py::none();
+    const int64_t K = xq.size(-1), N = wq.size(0), M = xq.numel() / K;
+    const auto scales = [&](const Tensor& s, const Tensor& q) {
+        return plain(s) && s.scalar_type() == at::kFloat && s.sizes() == q.sizes().slice(0, q.dim() - 1) && s.is_contiguous() && s.device() == xq.device();
+    };
+    if (wq.size(1) != K || K >= 1 << 17 || wq.device() != xq.device() || !scales(xs, xq) || !scales(ws, wq)) return py::none();
+    if (bias.defined() && (!plain(bias) || !float_type(bias) || bias.dim() != 1 || bias.size(0) != N || !bias.is_contiguous() || bias.device() != xq.device())) return py::none();
+    std::vector<int64_t> shape = xq.sizes().vec();
+    shape.back() = N;
+    if (residual.defined() && (residual.sizes() != at::IntArrayRef(shape) || residual.scalar_type() != (out_f32 ? at::kFloat : at::kBFloat16) || residual.device() != xq.device() ||
+                               !pitched_rows(residual, &ldr)))
+        return py::none();
+    if (grad_wanted({&xs, &ws, &bias, &residual})) return py::none();
+    Tensor y;
+    {
+        py::gil_scoped_release nogil;
+        const c10::cuda::CUDAGuard guard(xq.device());
+        at::NoGradGuard ng;
+        y = at::empty(shape, xs.options().dtype(out_f32 ? at::kFloat : at::kBFloat16));
+        Tensor work;
+        if (const int64_t bytes = wkv7_linear_int8_workspace_bytes(M, N, K)) work = at::empty({bytes}, xs.options().dtype(at::kByte));
+        check(wkv7_linear_int8(xq.data_ptr(), f32_of(xs), wq.data_ptr(), f32_of(ws), ptr(bias), ptr(residual), y.data_ptr(), M, N, K, ldx, ldw, ldr, N, (int)act,
+                               (out_f32 ? WKV7_LINEAR_F32_OUT : 0) | (is_f32(bias) ? WKV7_LINEAR_F32_BIAS : 0), ptr(work), stream()), "wkv7_linear_int8");
+    }
+    return py::cast(y);
+}
+
 // ---- beam search --------------------------------------------------------------------------------------------
 py::object beam_select(const Tensor& logits, const Tensor& scores, int64_t k, const OptTensor& finished_, int64_t eos) {
     const Tensor finished = finished_.value_or(Tensor());
@@ -912,6 +1136,10 @@ PYBIND11_MODULE(_wkv7_torch, mod) {
     mod.def("expand_loras", expand_loras);
     mod.def("mixer", mixer);
     mod.def("linear", linear);
+    mod.def("linear_int8", linear_int8);
+    mod.def("quantize", quantize);
+    mod.def("rms_norm", rms_norm);
+    mod.def("dropout", dropout);
     mod.def("beam_select", beam_select);
     mod.def("reorder_states", reorder_states);
 }

@@ -6,6 +6,8 @@ from .rwkv7_attn_ln import attn_ln, load_attn_ln
 from .rwkv7_proj import proj
 from .rwkv7_linear import linear
 from .rwkv7_beam import beam_select, reorder_states
+from .rwkv7_norm import dropout, rms_norm
+from .rwkv7_int8 import Int8, linear_int8, quantize
 
 from .time_mixer import TimeMixer
 

@@ -31,6 +31,7 @@ def chunks(T):
 _lib = None
 
 _vp, _i64, _int, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+_u64, _f64 = ctypes.c_uint64, ctypes.c_double
 
 _SIGNATURES = {
     'wkv7_status_string': (ctypes.c_char_p, [_int]),
@@ -66,6 +67,13 @@ _SIGNATURES = {
     'wkv7_linear_fwd': (_int, [_vp] * 6 + [_i64] * 8 + [_int] * 2 + [_vp] * 2),
     'wkv7_linear_bwd_workspace_bytes': (_i64, [_i64] * 3),
     'wkv7_linear_bwd': (_int, [_vp] * 7 + [_i64] * 7 + [_int] * 2 + [_vp] * 2),
+    'wkv7_linear_int8_workspace_bytes': (_i64, [_i64] * 3),
+    'wkv7_linear_int8': (_int, [_vp] * 7 + [_i64] * 7 + [_int] * 2 + [_vp] * 2),
+    'wkv7_quantize': (_int, [_vp] * 3 + [_i64] * 4 + [_int, _vp]),
+    'wkv7_rms_norm_fwd': (_int, [_vp] * 7 + [_i64] * 6 + [_f32, _f64, _u64, _vp, _int, _vp]),
+    'wkv7_rms_norm_bwd_workspace_bytes': (_i64, [_i64] * 2),
+    'wkv7_rms_norm_bwd': (_int, [_vp] * 8 + [_i64] * 7 + [_f64, _u64, _vp, _int] + [_vp] * 2),
+    'wkv7_dropout': (_int, [_vp] * 3 + [_i64, _f64, _u64, _vp, _int, _vp]),
     'wkv7_beam_select_workspace_bytes': (_i64, [_i64] * 3),
     'wkv7_beam_select': (_int, [_vp] * 7 + [_i64] * 7 + [_int] + [_vp] * 2),
     'wkv7_reorder': (_int, [_int] + [_vp] * 6 + [_int] + [_i64] * 3 + [_vp]),
