@@ -7,98 +7,131 @@ namespace norm {
 // ---- rows to 8 bits --------------------------------------------------------------------------------------------------------
 struct QuantizeKernelParams : QuantizeParams {
     Teams t;
-    Lie lx, lq;
+    Lie at_x, at_q;
 };
 // NV 0: rows of any length, read twice
 template <int NV, bool XF, bool EVEN> __global__ void __launch_bounds__(NV ? threads_most(NV) : 1024) quantize_kernel(const __grid_constant__ QuantizeKernelParams p) {
     __shared__ Room room;
     stream_order();
-    constexpr int HELD = NV ? NV : 1;
+    constexpr int HELD = NV ? NV : 1, XS = XF ? 4 : 2;
     const int team = p.t.threads, lane = threadIdx.x % team, K = (int)p.K;
     const long long step = (long long)gridDim.x * p.t.rows;
     long long row = (long long)blockIdx.x * p.t.rows + threadIdx.x / team;
     const int col0 = first_col(row, K) + 8 * lane;
-    const int vectors = NV ? NV : (int)((K + 7 + 8LL * team - 1) / (8LL * team));
+    const Byte* x_at = p.at_x.base + (row * p.at_x.ld + col0) * XS;
+    Byte* q_at = (Byte*)p.q + row * p.at_q.ld + col0;
+    const long long x_step = step * p.at_x.ld * XS, q_step = step * p.at_q.ld;
+    const long long vectors = (K + 7 + 8LL * team - 1) / (8LL * team);
     Raw<XF> x[HELD];
-    auto ask = [&](long long m) {
-        if (m >= p.M) return;
+    auto ask = [&](bool in) {
+        if (!in) return;
 #pragma unroll
-        for (int v = 0; v < HELD; ++v) request<XF, EVEN>(x[v], p.x, p.lx, m, col0 + 8 * team * v, K);
+        for (int v = 0; v < HELD; ++v) request<XF, EVEN>(x[v], x_at + 8 * team * v * XS, p.at_x.end, col0 + 8 * team * v, K);
     };
-    if (NV) ask(row);
+    if (NV) ask(row < p.M);
     int turn = 0;
-    for (long long first = (long long)blockIdx.x * p.t.rows; first < p.M; first += step, row += step) {
+    for (long long first = (long long)blockIdx.x * p.t.rows; first < p.M; first += step) {
         const bool in = row < p.M;
         float f[HELD][8], none = 0.f, top = 0.f;
-        auto tops = [&](const Raw<XF>& r, int col, float (&to)[8]) {
-            floats<XF>(r, to);
+        auto tops = [&](int col, float (&to)[8]) {
             clear_outside<EVEN>(col, K, to);
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = max_abs(top, to[i]);
         };
+        // a piece of a long row
+        auto get = [&](long long v, float (&to)[8]) {
+            const int col = (int)(col0 + 8 * team * v);
+            Raw<XF> r{};
+            request<XF, EVEN>(r, x_at + 8 * team * v * XS, p.at_x.end, col, K);
+            complete<XF, EVEN>(r, x_at + 8 * team * v * XS, p.at_x.end, col, K);
+            floats<XF>(r, to);
+        };
         if (NV) {
 #pragma unroll
             for (int v = 0; v < HELD; ++v) {
-                if (in) complete<XF, EVEN>(x[v], p.x, p.lx, row, col0 + 8 * team * v, K);
-                tops(x[v], col0 + 8 * team * v, f[v]);
+                const int col = col0 + 8 * team * v;
+                if (in) complete<XF, EVEN>(x[v], x_at + 8 * team * v * XS, p.at_x.end, col, K);
+                floats<XF>(x[v], f[v]);
+                tops(col, f[v]);
             }
-            ask(row + step);
         } else {
 #pragma unroll 4
-            for (int v = 0; v < vectors; ++v) {
-                const long long col = col0 + 8LL * team * v;
-                Raw<XF> r{};
-                if (in && col < K) {
-                    request<XF, EVEN>(r, p.x, p.lx, row, (int)col, K);
-                    complete<XF, EVEN>(r, p.x, p.lx, row, (int)col, K);
-                }
-                tops(r, (int)(col < K ? col : K), f[0]);
+            for (long long v = 0; v < vectors; ++v) {
+                if (col0 + 8 * team * v >= K) break;
+                get(v, f[0]);
+                tops((int)(col0 + 8 * team * v), f[0]);
             }
         }
+        const Byte* const again = x_at;
+        x_at += x_step;
+        if (NV) ask(row + step < p.M);
         reduce<false, true>(team, room, turn, none, top);
         turn ^= 1;
-        if (!in) continue;
-        if (lane == 0) p.scale[row] = Rounder::scale(top, 1.f);
-        const Rounder round(top);
+        if (in) {
+            if (lane == 0) p.scale[row] = Rounder::scale(top, 1.f);
+            const Rounder round(top);
+            if (NV) {
 #pragma unroll
-        for (int v = 0; v < vectors; ++v) {
-            const long long col = col0 + 8LL * team * v;
-            if (col >= K) break;
-            if (!NV) {
-                request<XF, EVEN>(x[0], p.x, p.lx, row, (int)col, K);
-                complete<XF, EVEN>(x[0], p.x, p.lx, row, (int)col, K);
-                floats<XF>(x[0], f[0]);
+                for (int v = 0; v < HELD; ++v) store_int8<EVEN>(q_at + 8 * team * v, p.at_q.end, col0 + 8 * team * v, K, f[v], round);
+            } else {
+                x_at = again;
+#pragma unroll 4
+                for (long long v = 0; v < vectors; ++v) {
+                    const long long col = col0 + 8 * team * v;
+                    if (col >= K) break;
+                    get(v, f[0]);
+                    store_int8<EVEN>(q_at + 8 * team * v, p.at_q.end, (int)col, K, f[0], round);
+                }
+                x_at += x_step;
             }
-            store_int8<EVEN>(p.q, p.lq, row, (int)col, K, f[NV ? v : 0], round);
         }
+        row += step;
+        q_at += q_step;
     }
 }
 
 // ---- dropout alone ---------------------------------------------------------------------------------------------------------
-template <bool XF, int RES> __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
+// Two pieces a thread at a time; the last elements, less than a piece, are the first thread's.
+template <bool XF, int RES, bool LOW> __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
     constexpr bool RF = RES == 2;
+    constexpr int XS = XF ? 4 : 2, RS = RF ? 4 : 2;
     stream_order();
     const Dropper drop(p.d);
-    const Lie lie{8, p.n};  // rows of eight
-    const long long step = (long long)gridDim.x * 256 * 8;
-    for (long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; at < p.n; at += step) {
-        const int live = (int)(p.n - at < 8 ? p.n - at : 8);
-        Raw<XF> x;
-        Raw<RF> r;
-        request<XF, false>(x, p.x, lie, at >> 3, 0, live);
-        if (RES) request<RF, false>(r, p.residual, lie, at >> 3, 0, live);
+    const int ys = p.y_f32 ? 4 : 2;
+    const long long pieces = p.n >> 3, step = (long long)gridDim.x * 512;
+    auto finish = [&](const Raw<XF>& x, const Raw<RF>& r, long long n, int live) {
         float f[8];
-        complete<XF, false>(x, p.x, lie, at >> 3, 0, live);
         floats<XF>(x, f);
-        if (p.d.threshold) drop.apply(at >> 3, f);
+        if (p.d.threshold) drop.template apply<LOW>(n, f);
         if (RES) {
             float g[8];
-            complete<RF, false>(r, p.residual, lie, at >> 3, 0, live);
             floats<RF>(r, g);
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(g[i], f[i]);
         }
-        store<false>(p.y, p.y_f32, lie, at >> 3, 0, live, f);
+        if (live == 8) store<true>((Byte*)p.y + 8 * n * ys, nullptr, p.y_f32, 0, 8, f);
+        else store<false>((Byte*)p.y + 8 * n * ys, nullptr, p.y_f32, 0, live, f);
+    };
+    for (long long n = (long long)blockIdx.x * 512 + threadIdx.x; n < pieces; n += step) {
+        Raw<XF> x[2];
+        Raw<RF> r[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int there = n + 256 * b < pieces ? 0 : 8;  // (behind the end: not read)
+            request<XF, true>(x[b], (const Byte*)p.x + 8 * (n + 256 * b) * XS, nullptr, there, 8);
+            if (RES) request<RF, true>(r[b], (const Byte*)p.residual + 8 * (n + 256 * b) * RS, nullptr, there, 8);
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+            if (n + 256 * b < pieces) finish(x[b], r[b], n + 256 * b, 8);
+    }
+    const int rest = (int)(p.n & 7);
+    if (rest && blockIdx.x == 0 && threadIdx.x == 0) {
+        Raw<XF> x;
+        Raw<RF> r;
+        complete<XF, false>(x, (const Byte*)p.x + 8 * pieces * XS, nullptr, 0, rest);
+        if (RES) complete<RF, false>(r, (const Byte*)p.residual + 8 * pieces * RS, nullptr, 0, rest);
+        finish(x, r, pieces, rest);
     }
 }
 
@@ -111,23 +144,24 @@ int launch_quantize(const QuantizeParams& a, cudaStream_t stream) {
     const long long pieces = pieces_of(p.K);
     const int nv = pieces > 4 * threads_most(4) ? 0 : vectors_of(p.M, pieces);
     p.t = nv ? teams_of(pieces, nv) : Teams{1024, 1};
-    p.lx = lie_of(p.x, p.M, p.K, p.ldx, 16);
-    p.lq = lie_of(p.q, p.M, p.K, p.ldq, 8);
+    p.at_x = lie_of(p.x, p.M, p.K, p.ldx, p.x_f32 ? 4 : 2);
+    p.at_q = lie_of(p.q, p.M, p.K, p.ldq, 1);
 #define WKV7_TYPES(nv, even) {quantize_kernel<nv, false, even>, quantize_kernel<nv, true, even>}
     static void (*const kernels[4][2][2])(QuantizeKernelParams) = {{WKV7_TYPES(0, false), WKV7_TYPES(0, true)}, {WKV7_TYPES(1, false), WKV7_TYPES(1, true)},
                                                                    {WKV7_TYPES(2, false), WKV7_TYPES(2, true)}, {WKV7_TYPES(4, false), WKV7_TYPES(4, true)}};
 #undef WKV7_TYPES
-    const bool even = p.K % 8 == 0 && p.lx.end && p.lq.end;
+    const bool even = p.K % 8 == 0 && p.at_x.end && p.at_q.end;
     const unsigned grid = (unsigned)ctas_of(p.M, p.t, sm_count(), nv == 4 ? 544 : 1024);
     return launch(kernels[nv == 4 ? 3 : nv][even][p.x_f32], dim3(grid), p.t.threads * p.t.rows, 0, stream, p) ? kOk : kLaunchFailed;
 }
 
 int launch_dropout(const DropoutParams& p, cudaStream_t stream) {
     using namespace norm;
-    static void (*const kernels[2][3])(DropoutParams) = {{dropout_kernel<false, 0>, dropout_kernel<false, 1>, dropout_kernel<false, 2>},
-                                                         {dropout_kernel<true, 0>, dropout_kernel<true, 1>, dropout_kernel<true, 2>}};
-    const long long want = (p.n + 2047) / 2048, most = (long long)sm_count() * 8;
-    return launch(kernels[p.x_f32][p.residual ? 1 + p.r_f32 : 0], dim3((unsigned)(want < most ? want : most)), 256, 0, stream, p) ? kOk : kLaunchFailed;
+#define WKV7_LOW(xf, res) {dropout_kernel<xf, res, false>, dropout_kernel<xf, res, true>}
+    static void (*const kernels[2][3][2])(DropoutParams) = {{WKV7_LOW(false, 0), WKV7_LOW(false, 1), WKV7_LOW(false, 2)}, {WKV7_LOW(true, 0), WKV7_LOW(true, 1), WKV7_LOW(true, 2)}};
+#undef WKV7_LOW
+    const long long want = (p.n + 4095) / 4096, most = (long long)sm_count() * 8;
+    return launch(kernels[p.x_f32][p.residual ? 1 + p.r_f32 : 0][low_counters(p.n)], dim3((unsigned)(want < most ? want : most)), 256, 0, stream, p) ? kOk : kLaunchFailed;
 }
 
 }  // namespace wkv7

@@ -8,22 +8,22 @@ namespace wkv7 {
 namespace norm {
 
 // ---- Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3; 2011) -----------------------
-// Ten rounds of two 32 x 32 -> 64 products for four words.  No mask is stored: the backward forms the words again.
+// Ten rounds of two 32 x 32 -> 64 products for four words.  No mask is stored: the backward forms the words again.  Its products bound dropout of bf16 elements: 36 of
+// them for a piece of eight, at four cycles each in a quarter of an SM, are 43 us for 2^26 elements, as much as their traffic.
 struct Dropper {
     uint32_t k0, k1, below;  // kept: word > below (the threshold less one; 2^32 less one drops all)
     float scale;
     __device__ __forceinline__ explicit Dropper(const Dropout& d) : below((uint32_t)(d.threshold - 1)), scale(d.scale) {
         const unsigned long long s = d.where ? *d.where : d.seed;
-        k0 = __shfl_sync(0xffffffffu, (uint32_t)s, 0);  // (the same for all lanes, which the compiler cannot see: the rounds' keys then cost the lanes nothing)
+        k0 = __shfl_sync(0xffffffffu, (uint32_t)s, 0);  // (the same for all lanes, which the compiler cannot see)
         k1 = __shfl_sync(0xffffffffu, (uint32_t)(s >> 32), 0);
     }
-    // eight adjacent elements, of which the first is element 8 n
-    __device__ __forceinline__ void apply(unsigned long long n, float (&f)[8]) const {
-        uint32_t c[2][4];
+    // the eight words of counters 2 n and 2 n + 1.  LOW: both are below 2^32, so that the second round's first product is the same for all
+    template <bool LOW> __device__ __forceinline__ void words(unsigned long long n, uint32_t (&c)[2][4]) const {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             c[b][0] = (uint32_t)(2 * n) + b;
-            c[b][1] = (uint32_t)(n >> 31);
+            c[b][1] = LOW ? 0u : (uint32_t)(n >> 31);
             c[b][2] = c[b][3] = 0;
         }
 #pragma unroll
@@ -38,10 +38,60 @@ struct Dropper {
                 c[b][3] = (uint32_t)x;
             }
         }
+    }
+    // eight adjacent elements, of which the first is element 8 n
+    template <bool LOW> __device__ __forceinline__ void apply(unsigned long long n, float (&f)[8]) const {
+        uint32_t c[2][4];
+        words<LOW>(n, c);
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = c[i / 4][i % 4] > below ? __fmul_rn(f[i], scale) : 0.f;
     }
+    __device__ __forceinline__ void apply(bool low, unsigned long long n, float (&f)[8]) const {
+        if (low) apply<true>(n, f);
+        else apply<false>(n, f);
+    }
 };
+inline bool low_counters(long long elements) { return elements <= 1LL << 34; }
+
+// ---- two fp32 operations an instruction ------------------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(uint64_t r, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// a piece as four pairs
+struct Piece {
+    uint64_t p[4];
+    __device__ __forceinline__ void set(const float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = two(f[2 * i], f[2 * i + 1]);
+    }
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split(p[i], f[2 * i], f[2 * i + 1]);
+    }
+};
+__device__ __forceinline__ float sum_of(uint64_t s) {
+    float a, b;
+    split(s, a, b);
+    return a + b;
+}
 
 // ---- eight adjacent elements of a row ------------------------------------------------------------------------------------
 // A thread's elements are 8 n .. 8 n + 7 of the whole tensor, counted row-major: where rows lie back to back they are 16-byte pieces whatever the row's length, and
@@ -49,36 +99,37 @@ struct Dropper {
 // the tensor has it whole, and the rest is put to zero.  What is not read so, a tensor's last part of a piece and layouts without such pieces, is read element by
 // element where it is used, not where it is requested: a request is a load and nothing else, which nothing waits for.
 // EVEN: all tensors lie in pieces and rows are a multiple of 8 long, so that there are no parts.
+using Byte = unsigned char;
 template <bool F32> struct Raw { uint4 w[F32 ? 2 : 1]; };
-struct Lie {   // how a tensor's pieces lie
-    long long ld, end;  // elements from row to row; behind the last one; 0: by single elements
+struct Lie {          // how a tensor lies
+    const Byte* base;
+    const Byte* end;  // behind its last element; null: not in 16-byte pieces
+    long long ld;     // elements from row to row
 };
 __device__ __forceinline__ bool whole(int col, int D) { return col >= 0 && col + 8 <= D; }
 __device__ __forceinline__ bool any(int col, int D) { return col > -8 && col < D; }
-template <bool F32, bool EVEN> __device__ __forceinline__ void request(Raw<F32>& r, const void* base, const Lie& t, long long row, int col, int D) {
-    const long long at = row * t.ld + col;
-    if (EVEN ? col < D : any(col, D) && at + 8 <= t.end) {
-        const uint4* p = reinterpret_cast<const uint4*>((const unsigned char*)base + at * (F32 ? 4 : 2));
-        r.w[0] = p[0];
-        if (F32) r.w[F32] = p[1];
+// at: of the piece's first element
+template <bool F32, bool EVEN> __device__ __forceinline__ void request(Raw<F32>& r, const Byte* at, const Byte* end, int col, int D) {
+    if (EVEN ? col < D : any(col, D) && at + (F32 ? 32 : 16) <= end) {
+        r.w[0] = reinterpret_cast<const uint4*>(at)[0];
+        if (F32) r.w[F32] = reinterpret_cast<const uint4*>(at)[1];
     }
 }
 __device__ __forceinline__ void put(uint4& u, int i, uint32_t v) {
     u.x |= i == 0 ? v : 0u; u.y |= i == 1 ? v : 0u; u.z |= i == 2 ? v : 0u; u.w |= i == 3 ? v : 0u;
 }
 // what was requested, complete
-template <bool F32, bool EVEN> __device__ __forceinline__ void complete(Raw<F32>& r, const void* base, const Lie& t, long long row, int col, int D) {
-    const long long at = row * t.ld + col;
-    if (EVEN || !any(col, D) || at + 8 <= t.end) return;
+template <bool F32, bool EVEN> __device__ __forceinline__ void complete(Raw<F32>& r, const Byte* at, const Byte* end, int col, int D) {
+    if (EVEN || !any(col, D) || at + (F32 ? 32 : 16) <= end) return;
     r = Raw<F32>{};
 #pragma unroll 1
     for (int i = col < 0 ? -col : 0; i < 8 && col + i < D; ++i) {
         if (F32) {
-            const uint32_t v = ((const uint32_t*)base)[at + i];
+            const uint32_t v = reinterpret_cast<const uint32_t*>(at)[i];
             put(r.w[0], i, v);
             put(r.w[F32], i - 4, v);
         } else {
-            put(r.w[0], i >> 1, (uint32_t)((const uint16_t*)base)[at + i] << (16 * (i & 1)));
+            put(r.w[0], i >> 1, (uint32_t)reinterpret_cast<const uint16_t*>(at)[i] << (16 * (i & 1)));
         }
     }
 }
@@ -101,21 +152,19 @@ __device__ __forceinline__ float element(const float (&f)[8], int i) {
     const float a = i & 1 ? f[1] : f[0], b = i & 1 ? f[3] : f[2], c = i & 1 ? f[5] : f[4], d = i & 1 ? f[7] : f[6];
     return i & 4 ? i & 2 ? d : c : i & 2 ? b : a;
 }
-template <bool EVEN> __device__ __forceinline__ void store(void* base, bool f32, const Lie& t, long long row, int col, int D, const float (&f)[8]) {
-    const long long at = row * t.ld + col;
-    if (EVEN ? col < D : whole(col, D) && t.end) {
+template <bool EVEN> __device__ __forceinline__ void store(Byte* at, const Byte* end, bool f32, int col, int D, const float (&f)[8]) {
+    if (EVEN ? col < D : whole(col, D) && end) {
         if (f32) {
-            float4* p = reinterpret_cast<float4*>((float*)base + at);
-            p[0] = make_float4(f[0], f[1], f[2], f[3]);
-            p[1] = make_float4(f[4], f[5], f[6], f[7]);
+            reinterpret_cast<float4*>(at)[0] = make_float4(f[0], f[1], f[2], f[3]);
+            reinterpret_cast<float4*>(at)[1] = make_float4(f[4], f[5], f[6], f[7]);
         } else {
-            *reinterpret_cast<uint4*>((bf16*)base + at) = pack8(f);
+            *reinterpret_cast<uint4*>(at) = pack8(f);
         }
     } else if (!EVEN) {
 #pragma unroll 1
         for (int i = col < 0 ? -col : 0; i < 8 && col + i < D; ++i) {
-            if (f32) ((float*)base)[at + i] = element(f, i);
-            else ((bf16*)base)[at + i] = __float2bfloat16_rn(element(f, i));
+            if (f32) reinterpret_cast<float*>(at)[i] = element(f, i);
+            else reinterpret_cast<bf16*>(at)[i] = __float2bfloat16_rn(element(f, i));
         }
     }
 }
@@ -126,7 +175,7 @@ __device__ __forceinline__ void weights(const void* w, bool f32, int col, int D,
 }
 
 // ---- a row in 8 bits -------------------------------------------------------------------------------------------------------
-// top: the bits of max |y|, a NaN if there is one.  Rows without a magnitude above 2^-100 are zeros with scale 0, a row that holds a NaN or an infinity is
+// top: max |y|, a NaN if there is one.  Rows without a magnitude above 2^-100 are zeros with scale 0, a row that holds a NaN or an infinity is
 // zeros with a NaN for its scale: so are its products.
 constexpr uint32_t TINY_BITS = (127 - 100) << 23, INF_BITS = 0x7f800000u;
 __device__ __forceinline__ float max_abs(float top, float f) {  // (a NaN stays)
@@ -134,35 +183,38 @@ __device__ __forceinline__ float max_abs(float top, float f) {  // (a NaN stays)
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(f)));
     return r;
 }
-// q = rint(v c), c = 127 / a rounded up.  Of bf16 rows that is rint(127 v / a), ties to even: with 8-bit mantissas 127 v / a is n + 1/2 either because v = +-a / 2, where c
-// gives 63.5 or a little more and 64 is right; or because 127 divides a's mantissa, where c and v c are exact.  Quotients that are no ties are 2^-17 of their size
-// away from one (the numerators differ by a whole step), v c is off by 2^-22.
+// q = rint(v c), c the least number that is not below 127 / a.  Of bf16 rows that is rint(127 v / a), ties to even: with 8-bit mantissas 127 v / a is n + 1/2 either because
+// v = +-a / 2, where v c is 63.5 or a little more and 64 is right; or because 127 divides a's mantissa, where c and v c are exact.  Quotients that are no ties are 2^-17 of
+// their size away from one (the numerators differ by a whole step), v c is off by 2^-22.
 struct Rounder {
     float c;
     uint32_t mask;
     __device__ __forceinline__ explicit Rounder(float top) {
         const bool live = top > __uint_as_float(TINY_BITS) && top < __uint_as_float(INF_BITS);
-        c = live ? __fdiv_ru(127.f, top) : 0.f;
+        const float q = 127.f / top;
+        c = live ? fmaf(-q, top, 127.f) > 0.f ? __uint_as_float(__float_as_uint(q) + 1) : q : 0.f;  // (the remainder is exact)
         mask = live ? ~0u : 0u;
     }
     __device__ __forceinline__ uint32_t four(float a, float b, float d, float e) const {
-        const float M = 12582912.f;  // 1.5 * 2^23: the sum's low byte is the integer nearest to v c
-        const uint32_t x = __float_as_uint(__fadd_rn(__fmul_rn(a, c), M)), y = __float_as_uint(__fadd_rn(__fmul_rn(b, c), M));
-        const uint32_t z = __float_as_uint(__fadd_rn(__fmul_rn(d, c), M)), w = __float_as_uint(__fadd_rn(__fmul_rn(e, c), M));
-        return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410) & mask;
+        // 1.5 * 2^23: the sum's low byte is the integer nearest to v c.  (The product is rounded by itself: merged into the sum it would be, too, in effect.)
+        const uint64_t M = two(12582912.f, 12582912.f), cc = two(c, c);
+        float x, y, z, w;
+        split(add2(mul2(two(a, b), cc), M), x, y);
+        split(add2(mul2(two(d, e), cc), M), z, w);
+        return __byte_perm(__byte_perm(__float_as_uint(x), __float_as_uint(y), 0x0040), __byte_perm(__float_as_uint(z), __float_as_uint(w), 0x0040), 0x5410) & mask;
     }
     __device__ __forceinline__ static float scale(float top, float times) {
         return !(top < __uint_as_float(INF_BITS)) ? __uint_as_float(0x7fc00000u) : top > __uint_as_float(TINY_BITS) ? __fdiv_rn(top * times, 127.f) : 0.f;
     }
 };
-template <bool EVEN> __device__ __forceinline__ void store_int8(signed char* q, const Lie& t, long long row, int col, int D, const float (&f)[8], const Rounder& round) {
+// (pieces of 8 bytes)
+template <bool EVEN> __device__ __forceinline__ void store_int8(Byte* at, const Byte* end, int col, int D, const float (&f)[8], const Rounder& round) {
     const uint32_t lo = round.four(f[0], f[1], f[2], f[3]), hi = round.four(f[4], f[5], f[6], f[7]);
-    const long long at = row * t.ld + col;
-    if (EVEN ? col < D : whole(col, D) && t.end) {
-        *reinterpret_cast<uint2*>(q + at) = make_uint2(lo, hi);
+    if (EVEN ? col < D : whole(col, D) && end) {
+        *reinterpret_cast<uint2*>(at) = make_uint2(lo, hi);
     } else if (!EVEN) {
 #pragma unroll 1
-        for (int i = col < 0 ? -col : 0; i < 8 && col + i < D; ++i) q[at + i] = (signed char)((i & 4 ? hi : lo) >> (8 * (i & 3)));
+        for (int i = col < 0 ? -col : 0; i < 8 && col + i < D; ++i) at[i] = (Byte)((i & 4 ? hi : lo) >> (8 * (i & 3)));
     }
 }
 
@@ -178,23 +230,26 @@ constexpr int MAX_WARPS = 32;
 // Sum and maximum over a team, in everyone's registers.  room: two of them in turn, so that one barrier a row is enough: before a thread comes to
 // write one again all have passed the other's barrier, and so have read this one.
 struct Room { float sum[2][MAX_WARPS], top[2][MAX_WARPS]; };
+template <bool SUM, bool TOP> __device__ __forceinline__ void butterfly(int n, float& sum, float& top) {
+#pragma unroll
+    for (int o = 16; o; o /= 2)
+        if (o < n) {
+            if (SUM) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (TOP) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));
+        }
+}
 template <bool SUM, bool TOP> __device__ __forceinline__ void reduce(int team, Room& room, int turn, float& sum, float& top) {
-    for (int o = (team < 32 ? team : 32) / 2; o; o /= 2) {
-        if (SUM) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (TOP) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));
-    }
+    butterfly<SUM, TOP>(team, sum, top);
     if (team <= 32) return;
-    const int warps = team / 32, warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) {
+    const int warps = team / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) {
         if (SUM) room.sum[turn][warp] = sum;
         if (TOP) room.top[turn][warp] = top;
     }
     __syncthreads();
-    sum = 0.f;
-    for (int i = 0; i < warps; ++i) {
-        if (SUM) sum += room.sum[turn][i];
-        if (TOP) top = max_abs(top, room.top[turn][i]);
-    }
+    if (SUM) sum = lane < warps ? room.sum[turn][lane] : 0.f;
+    if (TOP) top = lane < warps ? room.top[turn][lane] : 0.f;
+    butterfly<SUM, TOP>(32, sum, top);
 }
 // The rows of a team are `step` apart, a multiple of 8 wherever a team has several and rows are no multiple of 8 long: their first pieces then all begin with the same
 // column, 0 to -7, and a thread has the same columns of each.
@@ -207,10 +262,10 @@ inline int vectors_of(long long M, long long pieces) {
     return pieces <= threads_most(1) && M <= 2 * 148 ? 1 : 2;
 }
 inline bool al(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
-// bytes: of a piece of eight elements that is read or written at once, at most 16
-inline Lie lie_of(const void* p, long long M, long long D, long long ld, int bytes) {
-    const bool pieces = al(p, bytes) && (M == 1 || ld == D || (D % 8 == 0 && ld % 8 == 0));
-    return Lie{ld, pieces ? (M - 1) * ld + D : 0};
+// size: of an element; pieces of eight lie on boundaries of 16 bytes, of 8 in 8 bits
+inline Lie lie_of(const void* p, long long M, long long D, long long ld, int size) {
+    const bool pieces = p && al(p, size == 1 ? 8 : 16) && (M == 1 || ld == D || (D % 8 == 0 && ld % 8 == 0));
+    return Lie{(const Byte*)p, pieces ? (const Byte*)p + ((M - 1) * ld + D) * size : nullptr, ld};
 }
 // teams for rows of `pieces` pieces, nv to a thread, CTAs of some 256 threads
 inline Teams teams_of(long long pieces, int nv) {

@@ -40,7 +40,7 @@ struct NormBwdParams {
     const void *h, *weight, *dy, *dh;  // weight, dh: or null
     const float* rstd;
     void *dx, *dr;                     // either or null
-    float *dw, *partial;               // or null; partial: norm_bwd_partials(M, D) x D floats
+    float *dw, *partial;               // or null; partial: norm_bwd_partials(M, D) x D floats at most
     long long M, ldh, lddy, lddh, lddx, lddr;
     int D;
     Dropout d;

@@ -16,88 +16,119 @@ constexpr int fwd_ctas(int nv) { return nv == 1 ? 4 : 1; }
 constexpr int fwd_threads(int nv) { return nv == 1 ? 1024 : nv == 2 ? 512 : 544; }
 struct FwdKernelParams : NormFwdParams {
     Teams t;
-    Lie lx, lr, ly, lh;
+    Lie at_x, at_r, at_y, at_h;
     float inv_d;  // 1 / D
+    bool low;     // dropout's counters are below 2^32
 };
 // RES: no residual, bf16, fp32.  Of rows that take four pieces a thread nothing is requested ahead and the weight is not held: registers.
-template <int NV, bool XF, int RES, bool DROP, bool INT8, bool EVEN> __global__ void __launch_bounds__(threads_most(NV), fwd_ctas(NV)) norm_fwd_kernel(const __grid_constant__ FwdKernelParams p) {
+template <int NV, bool XF, int RES, bool DROP, bool INT8, bool EVEN>
+__global__ void __launch_bounds__(threads_most(NV), fwd_ctas(NV)) norm_fwd_kernel(const __grid_constant__ FwdKernelParams p) {
     constexpr bool HELD = NV < 4, RF = RES == 2;
+    constexpr int XS = XF ? 4 : 2, RS = RF ? 4 : 2;
     __shared__ Room room;
     stream_order();
     const int team = p.t.threads, lane = threadIdx.x % team, D = p.D;
     const long long step = (long long)gridDim.x * p.t.rows;
     long long row = (long long)blockIdx.x * p.t.rows + threadIdx.x / team;
-    const int col0 = first_col(row, D) + 8 * lane;
-    float w[HELD ? NV : 1][8];
+    const int col0 = first_col(row, D) + 8 * lane, ys = INT8 ? 1 : p.y_f32 ? 4 : 2;
+    const Byte* x_at = p.at_x.base + (row * p.at_x.ld + col0) * XS;
+    const Byte* r_at = p.at_r.base + (row * p.at_r.ld + col0) * RS;
+    Byte* h_at = (Byte*)p.h + (row * p.at_h.ld + col0) * RS;
+    Byte* y_at = (Byte*)p.y + (row * p.at_y.ld + col0) * ys;
+    const long long x_step = step * p.at_x.ld * XS, r_step = step * p.at_r.ld * RS, h_step = step * p.at_h.ld * RS, y_step = step * p.at_y.ld * ys;
+    Piece w[HELD ? NV : 1];
     Raw<XF> x[NV];
     Raw<RF> r[NV];
-    auto ask = [&](long long m) {
-        if (m >= p.M) return;
+    auto ask = [&](bool in) {
+        if (!in) return;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            request<XF, EVEN>(x[v], p.x, p.lx, m, col0 + 8 * team * v, D);
-            if (RES) request<RF, EVEN>(r[v], p.residual, p.lr, m, col0 + 8 * team * v, D);
+            request<XF, EVEN>(x[v], x_at + 8 * team * v * XS, p.at_x.end, col0 + 8 * team * v, D);
+            if (RES) request<RF, EVEN>(r[v], r_at + 8 * team * v * RS, p.at_r.end, col0 + 8 * team * v, D);
         }
     };
+    auto weight = [&](Piece& to, int v) {
+        float f[8];
+        weights(p.weight, p.w_f32, col0 + 8 * team * v, D, f);
+        to.set(f);
+    };
     if (HELD) {
-        ask(row);
+        ask(row < p.M);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) weights(p.weight, p.w_f32, col0 + 8 * team * v, D, w[v]);
+        for (int v = 0; v < NV; ++v) weight(w[HELD ? v : 0], v);
     }
     const Dropper drop(p.d);
     int turn = 0;
-    for (long long first = (long long)blockIdx.x * p.t.rows; first < p.M; first += step, row += step) {  // (the same for all threads: there are barriers within)
+    for (long long first = (long long)blockIdx.x * p.t.rows; first < p.M; first += step) {  // (the same for all threads: there are barriers within)
         const bool in = row < p.M;
-        if (!HELD) ask(row);
-        float f[NV][8], sum = 0.f, top = 0.f;
+        if (!HELD) ask(in);
+        Piece y[NV];
+        uint64_t sums = 0;  // (two zeros)
+        float top = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int col = col0 + 8 * team * v;
-            if (in) complete<XF, EVEN>(x[v], p.x, p.lx, row, col, D);
-            floats<XF>(x[v], f[v]);
-            if (DROP) drop.apply((unsigned long long)(row * D + col) >> 3, f[v]);
+            float f[8];
+            if (in) complete<XF, EVEN>(x[v], x_at + 8 * team * v * XS, p.at_x.end, col, D);
+            floats<XF>(x[v], f);
+            if (DROP) drop.apply(p.low, (unsigned long long)(row * D + col) >> 3, f);
+            y[v].set(f);
             if (RES) {
                 float g[8];
-                if (in) complete<RF, EVEN>(r[v], p.residual, p.lr, row, col, D);
+                if (in) complete<RF, EVEN>(r[v], r_at + 8 * team * v * RS, p.at_r.end, col, D);
                 floats<RF>(r[v], g);
+                Piece res;
+                res.set(g);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[v][i] = __fadd_rn(g[i], f[v][i]);  // (not merged with dropout's product: what is kept is the same however it is called)
-                if (!RF) unpack8(pack8(f[v]), f[v]);
-                if (in) store<EVEN>(p.h, RF, p.lh, row, col, D, f[v]);
+                for (int i = 0; i < 4; ++i) y[v].p[i] = add2(res.p[i], y[v].p[i]);  // (not merged with dropout's product: what is kept is the same however it is called)
+                y[v].get(f);
+                if (!RF) unpack8(pack8(f), f);
+                if (in) store<EVEN>(h_at + 8 * team * v * RS, p.at_h.end, RF, col, D, f);
             }
-            clear_outside<EVEN>(col, D, f[v]);
+            clear_outside<EVEN>(col, D, f);
+            y[v].set(f);
+            if (!HELD && INT8) weight(w[0], v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(f[v][i], f[v][i], sum);
-            if (!HELD && INT8) weights(p.weight, p.w_f32, col, D, w[0]);
-            if (HELD || INT8)
+            for (int i = 0; i < 4; ++i) {
+                sums = fma2(y[v].p[i], y[v].p[i], sums);
+                if (HELD || INT8) y[v].p[i] = mul2(y[v].p[i], w[HELD ? v : 0].p[i]);
+            }
+            if (INT8) {
+                y[v].get(f);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[v][i] *= w[HELD ? v : 0][i];
-            if (INT8)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) top = max_abs(top, f[v][i]);
+                for (int i = 0; i < 8; ++i) top = max_abs(top, f[i]);
+            }
         }
-        if (HELD) ask(row + step);
+        x_at += x_step;
+        r_at += r_step;
+        if (HELD) ask(row + step < p.M);
+        float sum = sum_of(sums);
         reduce<true, INT8>(team, room, turn, sum, top);
         turn ^= 1;
         const float rstd = rsqrtf(fmaf(sum, p.inv_d, p.eps));
-        if (!in) continue;
-        if (lane == 0) {
-            if (p.rstd) p.rstd[row] = rstd;
-            if (INT8) p.scale[row] = Rounder::scale(top, rstd);
-        }
-        const Rounder round(top);
+        if (in) {
+            if (lane == 0) {
+                if (p.rstd) p.rstd[row] = rstd;
+                if (INT8) p.scale[row] = Rounder::scale(top, rstd);
+            }
+            const Rounder round(top);
+            const uint64_t rr = two(rstd, rstd);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int col = col0 + 8 * team * v;
-            if (INT8) {
-                store_int8<EVEN>((signed char*)p.y, p.ly, row, col, D, f[v], round);
-            } else {
-                if (!HELD) weights(p.weight, p.w_f32, col, D, w[0]);
+            for (int v = 0; v < NV; ++v) {
+                float f[8];
+                if (!INT8) {
+                    if (!HELD) weight(w[0], v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[v][i] *= HELD ? rstd : rstd * w[0][i];
-                store<EVEN>(p.y, p.y_f32, p.ly, row, col, D, f[v]);
+                    for (int i = 0; i < 4; ++i) y[v].p[i] = mul2(y[v].p[i], HELD ? rr : mul2(rr, w[0].p[i]));
+                }
+                y[v].get(f);
+                if (INT8) store_int8<EVEN>(y_at + 8 * team * v, p.at_y.end, col0 + 8 * team * v, D, f, round);
+                else store<EVEN>(y_at + 8 * team * v * ys, p.at_y.end, p.y_f32, col0 + 8 * team * v, D, f);
             }
         }
+        row += step;
+        h_at += h_step;
+        y_at += y_step;
     }
 }
 
@@ -111,11 +142,12 @@ int launch_norm_fwd(const NormFwdParams& a, cudaStream_t stream) {
     const int nv = vectors_of(p.M, pieces);
     p.t = teams_of(pieces, nv);
     p.inv_d = (float)(1. / p.D);
+    p.low = low_counters(p.M * p.D);
     const bool int8 = p.scale != nullptr, drop = p.d.threshold != 0;
-    p.lx = lie_of(p.x, p.M, p.D, p.ldx, 16);
-    p.lr = lie_of(p.residual, p.M, p.D, p.ldr, 16);
-    p.lh = lie_of(p.h, p.M, p.D, p.ldh, 16);
-    p.ly = lie_of(p.y, p.M, p.D, p.ldy, int8 ? 8 : 16);
+    p.at_x = lie_of(p.x, p.M, p.D, p.ldx, p.x_f32 ? 4 : 2);
+    p.at_r = lie_of(p.residual, p.M, p.D, p.ldr, p.r_f32 ? 4 : 2);
+    p.at_h = lie_of(p.h, p.M, p.D, p.ldh, p.r_f32 ? 4 : 2);
+    p.at_y = lie_of(p.y, p.M, p.D, p.ldy, int8 ? 1 : p.y_f32 ? 4 : 2);
     // (rows of four pieces a thread have no EVEN form, only a residual has dropout)
 #define WKV7_OUT(nv, xf, res, drop, even) {norm_fwd_kernel<nv, xf, res, drop, false, even>, norm_fwd_kernel<nv, xf, res, drop, true, even>}
 #define WKV7_RES(nv, xf, e) \
@@ -125,7 +157,7 @@ int launch_norm_fwd(const NormFwdParams& a, cudaStream_t stream) {
 #undef WKV7_EVEN
 #undef WKV7_RES
 #undef WKV7_OUT
-    const bool even = p.D % 8 == 0 && p.lx.end && (!p.residual || (p.lr.end && p.lh.end)) && p.ly.end;
+    const bool even = p.D % 8 == 0 && p.at_x.end && (!p.residual || (p.at_r.end && p.at_h.end)) && p.at_y.end;
     const auto kern = kernels[nv / 2][even][p.x_f32][p.residual ? 1 + p.r_f32 : 0][drop][int8];
     return launch(kern, dim3((unsigned)ctas_of(p.M, p.t, sm_count(), fwd_threads(nv))), p.t.threads * p.t.rows, 0, stream, p) ? kOk : kLaunchFailed;
 }
