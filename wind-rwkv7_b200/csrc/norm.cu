@@ -65,7 +65,7 @@ template <int NV, bool XF, bool EVEN> __global__ void __launch_bounds__(NV ? thr
         const Byte* const again = x_at;
         x_at += x_step;
         if (NV) ask(row + step < p.M);
-        reduce<false, true>(team, room, turn, none, top);
+        reduce<false, true, false>(team, room, turn, none, top);
         turn ^= 1;
         if (in) {
             if (lane == 0) p.scale[row] = Rounder::scale(top, 1.f);
@@ -143,7 +143,7 @@ int launch_quantize(const QuantizeParams& a, cudaStream_t stream) {
     static_cast<QuantizeParams&>(p) = a;
     const long long pieces = pieces_of(p.K);
     const int nv = pieces > 4 * threads_most(4) ? 0 : vectors_of(p.M, pieces);
-    p.t = nv ? teams_of(pieces, nv) : Teams{1024, 1};
+    p.t = nv ? teams_of(pieces, nv, pieces <= 32 * nv ? 256 : 1) : Teams{1024, 1};
     p.at_x = lie_of(p.x, p.M, p.K, p.ldx, p.x_f32 ? 4 : 2);
     p.at_q = lie_of(p.q, p.M, p.K, p.ldq, 1);
 #define WKV7_TYPES(nv, even) {quantize_kernel<nv, false, even>, quantize_kernel<nv, true, even>}

@@ -148,6 +148,20 @@ template <bool EVEN> __device__ __forceinline__ void clear_outside(int col, int 
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = !EVEN && col + i >= 0 && col + i < D ? f[i] : 0.f;
 }
+// Elements lo .. hi - 1 of a piece, of which one end is the piece's own: three stores at most, of one, two and four elements.  W: words of four elements.
+template <typename T1, typename T2, typename T4> __device__ __forceinline__ void store_part(Byte* at, int lo, int hi, const T1 (&e)[8], const T2 (&two)[4], const T4 (&four)[2]) {
+    T1* const p1 = reinterpret_cast<T1*>(at);
+    if (hi == 8) {
+        if (lo & 1) p1[lo] = lo & 4 ? lo & 2 ? e[7] : e[5] : lo & 2 ? e[3] : e[1];
+        const int l2 = (lo + 1) & 6;
+        if (l2 & 2) *reinterpret_cast<T2*>(p1 + l2) = l2 & 4 ? two[3] : two[1];
+        if (lo <= 4) *reinterpret_cast<T4*>(p1 + 4) = four[1];
+    } else {
+        if (hi & 4) *reinterpret_cast<T4*>(p1) = four[0];
+        if (hi & 2) *reinterpret_cast<T2*>(p1 + (hi & 4)) = hi & 4 ? two[2] : two[0];
+        if (hi & 1) p1[hi & 6] = hi & 4 ? hi & 2 ? e[6] : e[4] : hi & 2 ? e[2] : e[0];
+    }
+}
 __device__ __forceinline__ float element(const float (&f)[8], int i) {
     const float a = i & 1 ? f[1] : f[0], b = i & 1 ? f[3] : f[2], c = i & 1 ? f[5] : f[4], d = i & 1 ? f[7] : f[6];
     return i & 4 ? i & 2 ? d : c : i & 2 ? b : a;
@@ -160,11 +174,24 @@ template <bool EVEN> __device__ __forceinline__ void store(Byte* at, const Byte*
         } else {
             *reinterpret_cast<uint4*>(at) = pack8(f);
         }
-    } else if (!EVEN) {
+    } else if (!EVEN && any(col, D)) {
+        const int lo = col < 0 ? -col : 0, hi = D - col < 8 ? D - col : 8;
+        if (!end || (lo && hi < 8)) {
 #pragma unroll 1
-        for (int i = col < 0 ? -col : 0; i < 8 && col + i < D; ++i) {
-            if (f32) reinterpret_cast<float*>(at)[i] = element(f, i);
-            else reinterpret_cast<bf16*>(at)[i] = __float2bfloat16_rn(element(f, i));
+            for (int i = lo; i < hi; ++i) {
+                if (f32) reinterpret_cast<float*>(at)[i] = element(f, i);
+                else reinterpret_cast<bf16*>(at)[i] = __float2bfloat16_rn(element(f, i));
+            }
+        } else if (f32) {
+            const float2 two[4] = {{f[0], f[1]}, {f[2], f[3]}, {f[4], f[5]}, {f[6], f[7]}};
+            const float4 four[2] = {make_float4(f[0], f[1], f[2], f[3]), make_float4(f[4], f[5], f[6], f[7])};
+            store_part<float, float2, float4>(at, lo, hi, f, two, four);
+        } else {
+            const uint4 u = pack8(f);
+            const uint16_t e[8] = {(uint16_t)u.x, (uint16_t)(u.x >> 16), (uint16_t)u.y, (uint16_t)(u.y >> 16), (uint16_t)u.z, (uint16_t)(u.z >> 16), (uint16_t)u.w, (uint16_t)(u.w >> 16)};
+            const uint32_t two[4] = {u.x, u.y, u.z, u.w};
+            const uint2 four[2] = {make_uint2(u.x, u.y), make_uint2(u.z, u.w)};
+            store_part<uint16_t, uint32_t, uint2>(at, lo, hi, e, two, four);
         }
     }
 }
@@ -212,6 +239,9 @@ template <bool EVEN> __device__ __forceinline__ void store_int8(Byte* at, const 
     const uint32_t lo = round.four(f[0], f[1], f[2], f[3]), hi = round.four(f[4], f[5], f[6], f[7]);
     if (EVEN ? col < D : whole(col, D) && end) {
         *reinterpret_cast<uint2*>(at) = make_uint2(lo, hi);
+    } else if (!EVEN && whole(col, D)) {  // (rows of x lie back to back, those in 8 bits on boundaries: pieces of the one are not pieces of the other)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) at[i] = (Byte)((i & 4 ? hi : lo) >> (8 * (i & 3)));
     } else if (!EVEN) {
 #pragma unroll 1
         for (int i = col < 0 ? -col : 0; i < 8 && col + i < D; ++i) at[i] = (Byte)((i & 4 ? hi : lo) >> (8 * (i & 3)));
@@ -219,7 +249,7 @@ template <bool EVEN> __device__ __forceinline__ void store_int8(Byte* at, const 
 }
 
 // ---- teams ---------------------------------------------------------------------------------------------------------------
-// A team has a row: a power of two of a warp's threads, or whole warps of a CTA, which then has one row.
+// A team has a row: a power of two of a warp's threads, or whole warps.
 struct Teams {
     int threads, rows;  // of a team; of a CTA
 };
@@ -229,7 +259,7 @@ static_assert(pieces_of(NORM_MAX_D) <= 4 * threads_most(4) && pieces_of(NORM_MAX
 constexpr int MAX_WARPS = 32;
 // Sum and maximum over a team, in everyone's registers.  room: two of them in turn, so that one barrier a row is enough: before a thread comes to
 // write one again all have passed the other's barrier, and so have read this one.
-struct Room { float sum[2][MAX_WARPS], top[2][MAX_WARPS]; };
+struct Room { float sum[2][MAX_WARPS], top[2][MAX_WARPS]; };  // [turn][warp of the CTA]
 template <bool SUM, bool TOP> __device__ __forceinline__ void butterfly(int n, float& sum, float& top) {
 #pragma unroll
     for (int o = 16; o; o /= 2)
@@ -238,17 +268,20 @@ template <bool SUM, bool TOP> __device__ __forceinline__ void butterfly(int n, f
             if (TOP) top = max_abs(top, __shfl_xor_sync(0xffffffffu, top, o));
         }
 }
-template <bool SUM, bool TOP> __device__ __forceinline__ void reduce(int team, Room& room, int turn, float& sum, float& top) {
+// SEVERAL: a CTA has several teams of more than a warp, each with a barrier of its own.  (A kernel that names barriers by number takes all 16 of a CTA's, and an SM
+// has room for few such CTAs: teams of 64 threads, one a CTA, 65536 x 768 78 -> 116 us.)
+template <bool SUM, bool TOP, bool SEVERAL> __device__ __forceinline__ void reduce(int team, Room& room, int turn, float& sum, float& top) {
     butterfly<SUM, TOP>(team, sum, top);
     if (team <= 32) return;
-    const int warps = team / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warps = team / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, of = SEVERAL ? threadIdx.x / team : 0;
     if (lane == 0) {
         if (SUM) room.sum[turn][warp] = sum;
         if (TOP) room.top[turn][warp] = top;
     }
-    __syncthreads();
-    if (SUM) sum = lane < warps ? room.sum[turn][lane] : 0.f;
-    if (TOP) top = lane < warps ? room.top[turn][lane] : 0.f;
+    if (SEVERAL) asm volatile("barrier.sync %0, %1;" ::"r"(1 + of), "r"(team) : "memory");
+    else __syncthreads();
+    if (SUM) sum = lane < warps ? room.sum[turn][of * warps + lane] : 0.f;
+    if (TOP) top = lane < warps ? room.top[turn][of * warps + lane] : 0.f;
     butterfly<SUM, TOP>(32, sum, top);
 }
 // The rows of a team are `step` apart, a multiple of 8 wherever a team has several and rows are no multiple of 8 long: their first pieces then all begin with the same
@@ -267,13 +300,13 @@ inline Lie lie_of(const void* p, long long M, long long D, long long ld, int siz
     const bool pieces = p && al(p, size == 1 ? 8 : 16) && (M == 1 || ld == D || (D % 8 == 0 && ld % 8 == 0));
     return Lie{(const Byte*)p, pieces ? (const Byte*)p + ((M - 1) * ld + D) * size : nullptr, ld};
 }
-// teams for rows of `pieces` pieces, nv to a thread, CTAs of some 256 threads
-inline Teams teams_of(long long pieces, int nv) {
+// teams for rows of `pieces` pieces, nv to a thread; CTAs of `threads` threads at most, of one team where it has more
+inline Teams teams_of(long long pieces, int nv, int threads) {
     const long long need = (pieces + nv - 1) / nv;
     int team = 1;
     if (need <= 32) while (team < need) team *= 2;
     else team = (int)((need + 31) / 32 * 32);
-    return Teams{team, team > 32 ? 1 : 256 / team};
+    return Teams{team, team < threads ? threads / team : 1};
 }
 // CTAs for M rows: as many as SMs hold, and a multiple of 8 where a team has several rows (see first_col)
 inline long long ctas_of(long long M, const Teams& t, int sms, int threads) {

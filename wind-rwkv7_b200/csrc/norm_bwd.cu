@@ -120,7 +120,7 @@ __global__ void __launch_bounds__(threads_most(NV), bwd_ctas(NV)) norm_bwd_kerne
         }
         if (HELD) ask(row + step);
         float sum = sum_of(both), none = 0.f;
-        reduce<true, false>(team, room, turn, sum, none);
+        reduce<true, false, HELD>(team, room, turn, sum, none);
         turn ^= 1;
         if (!in) continue;
         const float c = -(sum * p.inv_d * rstd * rstd);
@@ -211,8 +211,15 @@ __global__ void __launch_bounds__(1024) norm_dw_kernel(const float* partial, flo
 namespace norm {
 // (where all is fp32 two pieces do not fit the registers)
 static int bwd_vectors(long long M, long long pieces, bool wide) { return wide && pieces <= threads_most(1) ? 1 : vectors_of(M, pieces); }
+// One CTA an SM where there are rows for as many teams, so that there are few parts of dw; else smaller ones
+static Teams bwd_teams(long long M, long long pieces, int nv) {
+    Teams t = teams_of(pieces, nv, nv == 1 ? 256 : nv == 2 ? threads_most(nv) : 1);  // (four pieces a thread: teams are CTAs)
+    while (t.rows > 1 && (t.rows - 1) * 148LL >= M && t.rows * t.threads > 32) t.rows = (t.rows + 1) / 2;
+    while (t.rows * t.threads % 32) t.rows *= 2;
+    return t;
+}
 // The parts of dw: CTAs of the backward.  Sizes and types alone decide their number, so that the sums are the same on every device.
-static int parts_of(long long M, long long pieces, int nv) { return (int)ctas_of(M, teams_of(pieces, nv), 148, bwd_threads(nv)); }
+static int parts_of(long long M, long long pieces, int nv) { return (int)ctas_of(M, bwd_teams(M, pieces, nv), 148, bwd_threads(nv)); }
 }  // namespace norm
 
 int norm_bwd_partials(long long M, long long D) {
@@ -228,7 +235,7 @@ int launch_norm_bwd(const NormBwdParams& a, cudaStream_t stream) {
     static_cast<NormBwdParams&>(p) = a;
     const long long pieces = pieces_of(p.D);
     const int nv = bwd_vectors(p.M, pieces, p.y_f32 && p.h_f32), parts = parts_of(p.M, pieces, nv);
-    p.t = teams_of(pieces, nv);
+    p.t = bwd_teams(p.M, pieces, nv);
     p.inv_d = (float)(1. / p.D);
     p.low = low_counters(p.M * p.D);
     p.at_h = lie_of(p.h, p.M, p.D, p.ldh, p.h_f32 ? 4 : 2);
@@ -238,9 +245,8 @@ int launch_norm_bwd(const NormBwdParams& a, cudaStream_t stream) {
     p.at_dr = lie_of(p.dr, p.M, p.D, p.lddr, p.h_f32 ? 4 : 2);
 #define WKV7_DROP(nv, yf, hf, even) {norm_bwd_kernel<nv, yf, hf, false, even>, norm_bwd_kernel<nv, yf, hf, true, even>}
 #define WKV7_TYPES(nv, e) {{WKV7_DROP(nv, false, false, e), WKV7_DROP(nv, false, true, e)}, {WKV7_DROP(nv, true, false, e), WKV7_DROP(nv, true, true, e)}}
-    // (rows of four pieces a thread have no EVEN form)
     static void (*const kernels[3][2][2][2][2])(BwdKernelParams) = {{WKV7_TYPES(1, false), WKV7_TYPES(1, true)}, {WKV7_TYPES(2, false), WKV7_TYPES(2, true)},
-                                                                    {WKV7_TYPES(4, false), WKV7_TYPES(4, false)}};
+                                                                    {WKV7_TYPES(4, false), WKV7_TYPES(4, true)}};
 #undef WKV7_TYPES
 #undef WKV7_DROP
     const bool even = p.D % 8 == 0 && p.at_h.end && p.at_dy.end && (!p.dh || p.at_dh.end) && (!p.dx || p.at_dx.end) && (!p.dr || p.at_dr.end);
@@ -248,7 +254,7 @@ int launch_norm_bwd(const NormBwdParams& a, cudaStream_t stream) {
     const int threads = p.t.threads * p.t.rows;
     const int smem = threads * nv * 32;  // (the rows' gradients fit, too: rows x D <= threads x 8 nv)
     static thread_local uint32_t allowed[64];
-    if (nv == 4 && !allow_smem(kern, allowed, (p.y_f32 ? 4 : 0) | (p.h_f32 ? 2 : 0) | (p.d.threshold && p.dx ? 1 : 0), threads_most(4) * 4 * 32)) return kLaunchFailed;
+    if (nv == 4 && !allow_smem(kern, allowed, (even ? 8 : 0) | (p.y_f32 ? 4 : 0) | (p.h_f32 ? 2 : 0) | (p.d.threshold && p.dx ? 1 : 0), threads_most(4) * 4 * 32)) return kLaunchFailed;
     if (!launch(kern, dim3((unsigned)parts), threads, smem, stream, p)) return kLaunchFailed;
     if (p.dw && !launch(norm_dw_kernel, dim3((unsigned)((p.D + 31) / 32)), 1024, 0, stream, (const float*)p.partial, p.dw, p.D, parts)) return kLaunchFailed;
     return kOk;

@@ -11,9 +11,8 @@
 namespace wkv7 {
 namespace norm {
 
-// CTAs of the most threads that an SM is to hold, and the threads of an SM that the grid is sized for
-constexpr int fwd_ctas(int nv) { return nv == 1 ? 4 : 1; }
-constexpr int fwd_threads(int nv) { return nv == 1 ? 1024 : nv == 2 ? 512 : 544; }
+// threads of an SM that the grid is sized for
+constexpr int fwd_threads(int nv) { return nv == 1 ? 576 : nv == 2 ? 512 : 544; }
 struct FwdKernelParams : NormFwdParams {
     Teams t;
     Lie at_x, at_r, at_y, at_h;
@@ -22,7 +21,7 @@ struct FwdKernelParams : NormFwdParams {
 };
 // RES: no residual, bf16, fp32.  Of rows that take four pieces a thread nothing is requested ahead and the weight is not held: registers.
 template <int NV, bool XF, int RES, bool DROP, bool INT8, bool EVEN>
-__global__ void __launch_bounds__(threads_most(NV), fwd_ctas(NV)) norm_fwd_kernel(const __grid_constant__ FwdKernelParams p) {
+__global__ void __launch_bounds__(threads_most(NV), 1) norm_fwd_kernel(const __grid_constant__ FwdKernelParams p) {
     constexpr bool HELD = NV < 4, RF = RES == 2;
     constexpr int XS = XF ? 4 : 2, RS = RF ? 4 : 2;
     __shared__ Room room;
@@ -103,7 +102,7 @@ __global__ void __launch_bounds__(threads_most(NV), fwd_ctas(NV)) norm_fwd_kerne
         r_at += r_step;
         if (HELD) ask(row + step < p.M);
         float sum = sum_of(sums);
-        reduce<true, INT8>(team, room, turn, sum, top);
+        reduce<true, INT8, false>(team, room, turn, sum, top);
         turn ^= 1;
         const float rstd = rsqrtf(fmaf(sum, p.inv_d, p.eps));
         if (in) {
@@ -140,7 +139,7 @@ int launch_norm_fwd(const NormFwdParams& a, cudaStream_t stream) {
     static_cast<NormFwdParams&>(p) = a;
     const long long pieces = pieces_of(p.D);
     const int nv = vectors_of(p.M, pieces);
-    p.t = teams_of(pieces, nv);
+    p.t = teams_of(pieces, nv, pieces <= 32 * nv ? 256 : 1);
     p.inv_d = (float)(1. / p.D);
     p.low = low_counters(p.M * p.D);
     const bool int8 = p.scale != nullptr, drop = p.d.threshold != 0;
@@ -148,12 +147,12 @@ int launch_norm_fwd(const NormFwdParams& a, cudaStream_t stream) {
     p.at_r = lie_of(p.residual, p.M, p.D, p.ldr, p.r_f32 ? 4 : 2);
     p.at_h = lie_of(p.h, p.M, p.D, p.ldh, p.r_f32 ? 4 : 2);
     p.at_y = lie_of(p.y, p.M, p.D, p.ldy, int8 ? 1 : p.y_f32 ? 4 : 2);
-    // (rows of four pieces a thread have no EVEN form, only a residual has dropout)
+    // (only a residual has dropout)
 #define WKV7_OUT(nv, xf, res, drop, even) {norm_fwd_kernel<nv, xf, res, drop, false, even>, norm_fwd_kernel<nv, xf, res, drop, true, even>}
 #define WKV7_RES(nv, xf, e) \
     {{WKV7_OUT(nv, xf, 0, false, e), WKV7_OUT(nv, xf, 0, false, e)}, {WKV7_OUT(nv, xf, 1, false, e), WKV7_OUT(nv, xf, 1, true, e)}, {WKV7_OUT(nv, xf, 2, false, e), WKV7_OUT(nv, xf, 2, true, e)}}
-#define WKV7_EVEN(nv, even) {{WKV7_RES(nv, false, false), WKV7_RES(nv, true, false)}, {WKV7_RES(nv, false, even), WKV7_RES(nv, true, even)}}
-    static void (*const kernels[3][2][2][3][2][2])(FwdKernelParams) = {WKV7_EVEN(1, true), WKV7_EVEN(2, true), WKV7_EVEN(4, false)};
+#define WKV7_EVEN(nv) {{WKV7_RES(nv, false, false), WKV7_RES(nv, true, false)}, {WKV7_RES(nv, false, true), WKV7_RES(nv, true, true)}}
+    static void (*const kernels[3][2][2][3][2][2])(FwdKernelParams) = {WKV7_EVEN(1), WKV7_EVEN(2), WKV7_EVEN(4)};
 #undef WKV7_EVEN
 #undef WKV7_RES
 #undef WKV7_OUT
