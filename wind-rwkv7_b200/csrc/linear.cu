@@ -78,7 +78,6 @@ template <int ACT, bool FROM_Y> __device__ __forceinline__ float act_grad(float 
 struct Epi : LinearEpilogue {
     bool vec;       // rows of y start and end on 16-byte boundaries (bulk stores clip in steps of 16 bytes), those of the residual start there
     bool bias_vec;  // so does the bias
-    bool ws_vec;    // so do the columns' scales
 };
 __device__ __forceinline__ void load8g(const void* base, bool f32, long long at, float (&f)[8]) {
     if (f32) {
@@ -139,35 +138,26 @@ template <bool I8> __device__ __forceinline__ void add_sums8(float (&f)[8], cons
     f[0] = add_sums<I8>(f[0], a.x); f[1] = add_sums<I8>(f[1], a.y); f[2] = add_sums<I8>(f[2], a.z); f[3] = add_sums<I8>(f[3], a.w);
     f[4] = add_sums<I8>(f[4], b.x); f[5] = add_sums<I8>(f[5], b.y); f[6] = add_sums<I8>(f[6], b.z); f[7] = add_sums<I8>(f[7], b.w);
 }
-__device__ __forceinline__ float scaled(float sum, float xs, float ws) { return __fmul_rn(__fmul_rn((float)__float_as_int(sum), xs), ws); }
-// eight adjacent columns' scales
-__device__ __forceinline__ void ws8(const Epi& e, long long col, float (&f)[8]) {
-    if (e.ws_vec && col + 8 <= e.cols) {
-        load8g(e.ws, true, col, f);
-    } else {
+__device__ __forceinline__ float scaled(float sum, float ps, float qs) { return __fmul_rn(__fmul_rn((float)__float_as_int(sum), ps), qs); }
+// A block of 32 sums a lane: a lane's own scale, along P, and the block's 32 along Q, in shared memory, where all lanes read the same.  (Read from global memory
+// where they are used they were waited for: 8192 x 2048 -> 8192 105 us, without any scales 87.)
+template <bool I8> __device__ __forceinline__ void scale_block(float ps, const float* qs, float (&v)[32]) {
+    if (!I8) return;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = col + i < e.cols ? e.ws[col + i] : 0.f;
+    for (int c = 0; c < 32; c += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(qs + c);
+        v[c] = scaled(v[c], ps, q.x); v[c + 1] = scaled(v[c + 1], ps, q.y); v[c + 2] = scaled(v[c + 2], ps, q.z); v[c + 3] = scaled(v[c + 3], ps, q.w);
     }
 }
-// n adjacent columns of a row
-template <bool I8, int N> __device__ __forceinline__ void scale_row(const Epi& e, long long row, long long col, float (&v)[N]) {
+// the same, qs: one each of the lanes', which go through the warp's room of 128 bytes
+template <bool I8> __device__ __forceinline__ void scale_block(float ps, float qs, float* room, int lane, float (&v)[32]) {
     if (!I8) return;
-    const float xs = row < e.rows ? e.xs[row] : 0.f;
-#pragma unroll
-    for (int c = 0; c < N; c += 8) {
-        float f[8];
-        ws8(e, col + c, f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[c + i] = scaled(v[c + i], xs, f[i]);
-    }
+    __syncwarp();
+    room[lane] = qs;
+    __syncwarp();
+    scale_block<I8>(ps, room, v);
 }
-// a column of 32 rows
-template <bool I8> __device__ __forceinline__ void scale_col(const Epi& e, long long row, long long col, float (&v)[32]) {
-    if (!I8) return;
-    const float ws = col < e.cols ? e.ws[col] : 0.f;
-#pragma unroll
-    for (int c = 0; c < 32; ++c) v[c] = scaled(v[c], row + c < e.rows ? e.xs[row + c] : 0.f, ws);
-}
+__device__ __forceinline__ float scale_at(const float* s, long long i, long long n) { return i < n ? s[i] : 0.f; }
 // eight adjacent columns of a row, from the accumulator to memory; bias already added
 template <int ACT> __device__ __forceinline__ void finish8(const Epi& e, long long row, long long col, float (&f)[8]) {
     const int live = (int)(e.cols - col < 8 ? e.cols - col : 8);
@@ -451,6 +441,7 @@ struct TileCtrl {
     uint32_t tmem_base;
     volatile int abort, zero;
     int last;
+    alignas(16) float qs[128];  // 8 bits: the tile's scales along Q
 };
 static_assert(sizeof(TileCtrl) <= 1024, "the KB ahead of the ring");
 constexpr int TILE_THREADS = 192;  // warps 0-3: accumulator rows, warp 4: copies, warp 5: products; all six: the result
@@ -501,6 +492,14 @@ template <int ACT, bool I8> __global__ void __launch_bounds__(TILE_THREADS, 3) l
     const uint32_t tmem = ctrl->tmem_base;
     if (p.splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (waited for before the first write to another CTA)
     stream_order();
+    // 8 bits: scales along P, of this lane's row or (swap) of the column that this thread finishes, and along Q
+    float ps = 0.f;
+    if (I8) {
+        const float *const along_p = p.swap ? p.e.ws : p.e.xs, *const along_q = p.swap ? p.e.xs : p.e.ws;
+        const long long np = p.swap ? p.e.cols : p.e.rows, nq = p.swap ? p.e.rows : p.e.cols;
+        if (tid < p.nt) ctrl->qs[tid] = scale_at(along_q, q0 + tid, nq);
+        ps = scale_at(along_p, p0 + (p.swap ? rank * (BM / p.splits) + tid % (BM / p.splits) : tid), np);
+    }
 
     if (warp == 4) {
         if (elect_one()) {
@@ -574,11 +573,15 @@ template <int ACT, bool I8> __global__ void __launch_bounds__(TILE_THREADS, 3) l
                         for (int i = 0; i < 32; ++i) v[i] = add_sums<I8>(v[i], u[i]);
                     }
                 };
+                auto take = [&](float (&v)[32]) {
+                    sums(v);
+                    scale_block<I8>(ps, ctrl->qs + c, v);
+                };
                 // (blocks two by two, as the pairs have them, would take 190 registers and more: one CTA an SM)
                 const int row0 = p0 + 32 * warp, col0 = q0 + c;
                 if (row0 >= e.rows || col0 >= e.cols) continue;
-                if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); scale_row<I8>(e, row0 + lane, col0, v); });
-                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); turn_block(mine, lane, v); scale_col<I8>(e, row0, col0 + lane, v); });
+                if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, take);
+                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { take(v); turn_block(mine, lane, v); });
             }
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
@@ -625,11 +628,10 @@ template <int ACT, bool I8> __global__ void __launch_bounds__(TILE_THREADS, 3) l
             for (int r = 1; r < p.splits; ++r) {
                 add_sums<I8>(x, ld4(parts + (r * rows + i) * pitch + j));
             }
-            if (I8) {
-                const float ws = e.ws[col];
-                float* const sum[4] = {&x.x, &x.y, &x.z, &x.w};
-#pragma unroll
-                for (int q = 0; q < 4; ++q) *sum[q] = scaled(*sum[q], q0 + j + q < e.rows ? e.xs[q0 + j + q] : 0.f, ws);
+            if (I8) {  // (a thread's units are in one column, unless there are all 128)
+                const float4 q = ld4(ctrl->qs + j);
+                const float ws = rows == BM ? e.ws[col] : ps;
+                x.x = scaled(x.x, q.x, ws); x.y = scaled(x.y, q.y, ws); x.z = scaled(x.z, q.z, ws); x.w = scaled(x.w, q.w, ws);
             }
             const float bias = e.bias ? load1g(e.bias, e.bias_f32, col) : 0.f;
             const float f[4] = {x.x + bias, x.y + bias, x.z + bias, x.w + bias};
@@ -694,7 +696,11 @@ template <int ACT, bool I8> __global__ void __launch_bounds__(TILE_THREADS, 3) l
             } else {
                 joined(u, f);
             }
-            scale_row<I8>(e, row, col, f);
+            if (I8) {
+                const float xs = e.xs[row];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) f[q] = scaled(f[q], xs, ctrl->qs[j + q]);
+            }
             if (e.bias) {
                 float bias[8];
                 bias8(e, col, bias);
@@ -724,13 +730,13 @@ constexpr int PAIR_STAGING = 32 * 32 * 4;  // a block of 32 x 32 in fp32, or two
 constexpr int BAND = 8;                    // tile rows of 256 that are walked together, column by column, so that concurrent tiles share operands in L2
 constexpr int PART_BLOCKS = 4;             // blocks of 32 columns a warp has of a tile at most
 constexpr int PART_F4 = 2 * 8 * PART_BLOCKS * 8 * 32;  // float4 of a unit
-struct PairCtrl {
+struct alignas(16) PairCtrl {
     uint64_t full[PAIR_STAGES], empty[PAIR_STAGES], accum_full[2], accum_empty[2], drain;
     uint32_t tmem_base;
     volatile int abort, zero;
 };
-constexpr int PAIR_SMEM = 1024 + PAIR_STAGES * PAIR_STAGE + 8 * PAIR_STAGING + (int)sizeof(PairCtrl);
-static_assert(PAIR_SMEM <= 232448, "shared memory of a CTA");
+constexpr int PAIR_SMEM = 1024 + PAIR_STAGES * PAIR_STAGE + 8 * PAIR_STAGING + (int)sizeof(PairCtrl);  // 8 bits: 1 KB more
+static_assert(PAIR_SMEM + 1024 <= 232448, "shared memory of a CTA");
 
 // the n-th piece of work of a pair
 struct PairWork {
@@ -876,6 +882,7 @@ template <int ACT, bool I8> __global__ void __cluster_dims__(2, 1, 1) __launch_b
         // Where rows of y are not aligned the block is turned there in fp32, so that a lane has a column.
         const int quarter = warp & 3, side = (warp - 4) >> 2;
         float* mine = reinterpret_cast<float*>(staging + (warp - 4) * PAIR_STAGING);
+        float* room = reinterpret_cast<float*>(ctrl + 1) + (warp - 4) * 32;
         int turn = 0;
         const Epi& e = p.e;
         const bool two = e.vec && !p.swap && !e.y_f32 && !(e.z && e.z_f32);  // blocks go two by two
@@ -890,9 +897,17 @@ template <int ACT, bool I8> __global__ void __cluster_dims__(2, 1, 1) __launch_b
                     if (row < e.rows && col < e.cols) asm volatile("prefetch.global.L2 [%0];" ::"l"((const unsigned char*)e.residual + (row * e.ldr + col) * (e.y_f32 ? 4 : 2)));
                 }
             }
+            float ps = 0.f, qs[PART_BLOCKS] = {};  // 8 bits: this lane's scale along P, and one of each block's along Q
+            if (I8) {
+                ps = scale_at(p.swap ? e.ws : e.xs, (long long)w.pi * 2 * BM + rank * BM + 32 * quarter + lane, p.swap ? e.cols : e.rows);
+#pragma unroll
+                for (int i = 0; i < PART_BLOCKS; ++i)
+                    if (b0 + i < b1) qs[i] = scale_at(p.swap ? e.xs : e.ws, (long long)w.qi * p.bn + 32 * (b0 + i) + lane, p.swap ? e.rows : e.cols);
+            }
             mbar_wait_bounded<true>(&ctrl->accum_full[buf], (n >> 1) & 1, &ctrl->abort, status, SUM_LIMIT);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (ctrl->abort) break;
+            const auto along_q = [&](int b) { const int i = b - b0; return i & 2 ? i & 1 ? qs[3] : qs[2] : i & 1 ? qs[1] : qs[0]; };
             const long long p0 = (long long)w.pi * 2 * BM + rank * BM + 32 * quarter;
             const uint32_t acc = tmem + buf * 256 + ((uint32_t)(32 * quarter) << 16);
             auto emptied = [&] {  // the accumulator may be filled again (no memory is handed over: a release would wait for all of this warp's stores, 1600 cycles)
@@ -930,8 +945,8 @@ template <int ACT, bool I8> __global__ void __cluster_dims__(2, 1, 1) __launch_b
                         tmem_ld32(acc + 32 * b, reinterpret_cast<uint32_t(&)[32]>(v[0]));
                         tmem_ld32(acc + 32 * b + 32, reinterpret_cast<uint32_t(&)[32]>(v[1]));
                         if (b + 1 == b1 - 1) emptied();
-                        scale_row<I8>(e, row0 + lane, col0, v[0]);
-                        scale_row<I8>(e, row0 + lane, col0 + 32, v[1]);
+                        scale_block<I8>(ps, along_q(b), room, lane, v[0]);
+                        scale_block<I8>(ps, along_q(b + 1), room, lane, v[1]);
                     });
                     ++b;
                     continue;
@@ -961,10 +976,10 @@ template <int ACT, bool I8> __global__ void __cluster_dims__(2, 1, 1) __launch_b
                     if (b == b1 - 1 && !parts) emptied();
                     continue;
                 }
-                const auto column = [&](float (&v)[32]) { sums(v); scale_col<I8>(e, row0, col0 + lane, v); };
-                if (p.swap) finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, column);
-                else if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); scale_row<I8>(e, row0 + lane, col0, v); });
-                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); turn_block(mine, lane, v); scale_col<I8>(e, row0, col0 + lane, v); });
+                const auto take = [&](float (&v)[32]) { sums(v); scale_block<I8>(ps, along_q(b), room, lane, v); };
+                if (p.swap) finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, take);
+                else if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, take);
+                else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { take(v); turn_block(mine, lane, v); });
             }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory must outlive the stores' reads
@@ -1200,7 +1215,8 @@ static size_t pair_ws(const PairPlan& x) { return x.splits > 1 ? (size_t)(x.tile
 static int run_pair(LinearOperand rows, LinearOperand cols, long long k, const Epi& e, const PairPlan& x, void* workspace, int* status, cudaStream_t stream) {
     const bool i8 = e.xs != nullptr;
     const auto kern = pair_kernels.k[i8][e.act];
-    if (!allow_smem(kern, smem_allowed[i8], 16 + e.act, PAIR_SMEM)) return kLaunchFailed;
+    const int smem = PAIR_SMEM + (i8 ? 1024 : 0);
+    if (!allow_smem(kern, smem_allowed[i8], 16 + e.act, smem)) return kLaunchFailed;
     PairParams p;
     memset(&p, 0, sizeof(p));
     const LinearOperand &a = x.swap ? cols : rows, &b = x.swap ? rows : cols;
@@ -1221,7 +1237,7 @@ static int run_pair(LinearOperand rows, LinearOperand cols, long long k, const E
     }
     const long long pairs = pairs_of_sms(), units = x.whole + (x.tiles - x.whole) * x.splits;
     const unsigned grid = 2 * (unsigned)(units < pairs ? units : pairs);
-    return launch_clusters(kern, dim3(grid), PAIR_THREADS, PAIR_SMEM, 1, stream, p, status) ? kOk : kLaunchFailed;
+    return launch_clusters(kern, dim3(grid), PAIR_THREADS, smem, 1, stream, p, status) ? kOk : kLaunchFailed;
 }
 
 // Which kernel, and its shape
@@ -1289,7 +1305,6 @@ int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const Lin
     const int per16 = ep.y_f32 ? 4 : 8;
     e.vec = al16(ep.y) && ep.ldy % per16 == 0 && ep.cols % per16 == 0 && (!ep.residual || (al16(ep.residual) && ep.ldr % per16 == 0));
     e.bias_vec = al16(ep.bias);
-    e.ws_vec = al16(ep.ws);
     const bool i8 = ep.xs != nullptr;
     if ((k + BK - 1) / BK > MAX_KBLOCKS) return kTooLarge;
     const Plan p = make_plan(ep.rows, ep.cols, k, rows.mn, workspace != nullptr, i8);
