@@ -13,6 +13,7 @@
 #include <cuda.h>
 #include <cstring>
 
+#include "activations.cuh"
 #include "linear.h"
 #include "mma_bf16.cuh"
 #include "wkv7_kernels.h"
@@ -27,36 +28,6 @@ constexpr int MAXSTAGES = 12;
 constexpr long long SUM_LIMIT = ACROSS_HANDOFF_LIMIT;
 constexpr int MAX_KBLOCKS = 1 << 21;
 
-// ---- activations -----------------------------------------------------------------------------------------
-constexpr float LOG2E = 1.4426950408889634f;
-__device__ __forceinline__ float sigmoid_f(float x) { return rcp_mufu(1.f + ex2_approx(-LOG2E * x)); }
-__device__ __forceinline__ float tanh_f(float x) {
-    // (1 - e) / (1 + e), e = exp(-2 |x|): relative error 2e-6 from |x| = 0.1 on; the series' first four terms below (next one: 2e-10)
-    const float t = fabsf(x), e = ex2_approx(-2.f * LOG2E * t), x2 = x * x;
-    const float big = copysignf((1.f - e) * rcp_mufu(1.f + e), x);
-    const float small = x * (1.f + x2 * (-1.f / 3.f + x2 * (2.f / 15.f - x2 * (17.f / 315.f))));
-    return t < 0.1f ? small : big;
-}
-constexpr float GELU_C = 1.5957691216057308f;  // 2 sqrt(2 / pi): gelu(x) = x sigmoid(GELU_C (x + 0.044715 x^3))
-__device__ __forceinline__ float gelu_s(float x) { return sigmoid_f(GELU_C * x * (1.f + 0.044715f * x * x)); }
-__device__ __forceinline__ float sqrt_f(float x) {  // relative error 2^-23
-    float y;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float relu_f(float x) { return x < 0.f ? 0.f : x; }  // (a NaN stays one)
-
-template <int ACT> __device__ __forceinline__ float act(float x) {
-    switch (ACT) {
-        case kActRelu: return relu_f(x);
-        case kActRelu2: { const float r = relu_f(x); return r * r; }
-        case kActTanh: return tanh_f(x);
-        case kActSigmoid: return sigmoid_f(x);
-        case kActSilu: return x * sigmoid_f(x);
-        case kActGelu: return x * gelu_s(x);
-        default: return x;
-    }
-}
 // act'(z); FROM_Y: of relu and relu2 from their values, 2 sqrt(y) for 2 relu(z)
 template <int ACT, bool FROM_Y> __device__ __forceinline__ float act_grad(float z) {
     switch (ACT) {
@@ -1306,6 +1277,7 @@ int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const Lin
     e.vec = al16(ep.y) && ep.ldy % per16 == 0 && ep.cols % per16 == 0 && (!ep.residual || (al16(ep.residual) && ep.ldr % per16 == 0));
     e.bias_vec = al16(ep.bias);
     const bool i8 = ep.xs != nullptr;
+    if (i8 && int8_rows_fit(ep.rows, ep.cols, k)) return launch_int8_rows(rows, cols, k, ep, stream);
     if ((k + BK - 1) / BK > MAX_KBLOCKS) return kTooLarge;
     const Plan p = make_plan(ep.rows, ep.cols, k, rows.mn, workspace != nullptr, i8);
     if (p.pair) return run_pair(rows, cols, k, e, p.x, workspace, status, stream);

@@ -25,10 +25,14 @@ struct LinearOperand {
     long long ld;
     bool mn;
 };
-// 8-bit operands: K-major, rows a multiple of 16 bytes apart, k < 2^17 (the sum of 2^17 products of -128 leaves 32 bits); neither bias nor z differ.
+// 8-bit operands (epilogues with scales): K-major, rows a multiple of 16 bytes apart, k < 2^17 (a sum of 2^17 products of -128 leaves 32 bits), no z.
 // workspace: linear_workspace_bytes() bytes (rows_mn: the rows' operand is [k, index]), or null: no tile is cut along k
 size_t linear_workspace_bytes(long long rows, long long cols, long long k, bool rows_mn, bool i8 = false);
 int launch_linear(LinearOperand rows, LinearOperand cols, long long k, const LinearEpilogue& e, void* workspace, int* status, cudaStream_t stream);
+
+// products in 8 bits of few rows (linear_int8.cu): whether they are done so, and the launch
+bool int8_rows_fit(long long rows, long long cols, long long k);
+int launch_int8_rows(LinearOperand x, LinearOperand w, long long k, const LinearEpilogue& e, cudaStream_t stream);
 
 // dz = dy act'(saved) as bf16 [M, ldz] (not written where dz is null) and dbias = column sums of dz (or null; then of dz before its rounding)
 struct LinearDz {
