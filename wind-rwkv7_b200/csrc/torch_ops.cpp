@@ -700,8 +700,9 @@ py::object rms_norm(const Tensor& x, const OptTensor& w_, const OptTensor& r_, d
         } else {
             at::NoGradGuard ng;
             const auto [y, h, rstd, scale] = norm_forward(x, w, r, s, NormHow{eps, p, seed < 0 ? 0 : seed, out}, false);
-            if (out == 2) o = {y.narrow(-1, 0, x.size(-1)), scale};
-            else o = {y};
+            o.reserve(3);
+            o.push_back(out == 2 && y.size(-1) != x.size(-1) ? y.narrow(-1, 0, x.size(-1)) : y);
+            if (out == 2) o.push_back(scale);
             if (r.defined()) o.push_back(h);
         }
     }

@@ -17,6 +17,7 @@ from .rwkv7_linear import rows_of
 X_F32, R_F32, W_F32, Y_F32, Y_INT8 = 1, 2, 4, 8, 16
 MAX_D = 16384
 FLOATS = (th.bfloat16, th.float32)
+OUTS = {None: -1, th.bfloat16: 0, th.float32: 1, th.int8: 2}  # of y, -1: x's
 
 
 def f32(t):
@@ -188,9 +189,12 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-5, p=0.0, seed=None, out_d
     elements counted in row-major order.  Backward for x, weight and residual.  Squares are summed in fp32: a row beyond 1e19 leaves its range and gives 0.
     Rows may lie in a wider tensor; other layouts are copied."""
     if not th.compiler.is_compiling():
-        out = _lib.ext().rms_norm(x, weight, residual, eps, p, *_seed_of(seed), {None: -1, th.bfloat16: 0, th.float32: 1, th.int8: 2}.get(out_dtype, -2))
+        number, seed_t = (-1, None) if seed is None else _seed_of(seed)
+        out = _lib.ext().rms_norm(x, weight, residual, eps, p, number, seed_t, OUTS.get(out_dtype, -2))
         if out is not None:
-            return _pair(out, residual is not None) if out_dtype == th.int8 else out
+            if out_dtype is not th.int8:
+                return out
+            return Int8(*out) if residual is None else (Int8(out[0], out[1]), out[2])
     p, number, seed_t = _check_norm(x, weight, residual, eps, p, seed, out_dtype)
     _lib.require_cuda(x, weight, residual, seed_t)
     if out_dtype == th.int8:
@@ -209,10 +213,6 @@ def _seed_of(seed):
     return (seed if isinstance(seed, int) and 0 <= seed < 1 << 63 else -1), None
 
 
-def _pair(out, stream):
-    return (Int8(out[0], out[1]), out[2]) if stream else Int8(*out)
-
-
 def dropout(x, p, seed, *, residual=None):
     """residual + x / (1 - p) where an element of x is kept, residual (0 without one) where it is dropped; p in [0, 1].
 
@@ -221,7 +221,8 @@ def dropout(x, p, seed, *, residual=None):
     of one element on x's device, which is read when the kernel runs (a captured step draws anew when the tensor was changed before its replay).  A probability
     is met to 2^-33.  Backward for x and residual; no mask is stored."""
     if not th.compiler.is_compiling():
-        out = _lib.ext().dropout(x, p, *_seed_of(seed), residual)
+        number, seed_t = _seed_of(seed)
+        out = _lib.ext().dropout(x, p, number, seed_t, residual)
         if out is not None:
             return out
     _check_floats('dropout', 'x', x)
