@@ -277,18 +277,31 @@ template <int ACT, typename Sums> __device__ __forceinline__ void finish_cols(co
     for (int half = 0; half < 32; half += 16) {
         if (e.residual) {  // (sixteen rows of it before they are stored: y may be the residual, so the compiler keeps them in order)
             float res[16];
+            if (e.y_f32) {
+                const float* r = (const float*)e.residual + (row0 + half) * e.ldr + col;
 #pragma unroll
-            for (int c = 0; c < 16; ++c) res[c] = in && half + c < rows ? load1g(e.residual, e.y_f32, (row0 + half + c) * e.ldr + col) : 0.f;
+                for (int c = 0; c < 16; ++c, r += e.ldr) res[c] = in && half + c < rows ? *r : 0.f;
+            } else {
+                const bf16* r = (const bf16*)e.residual + (row0 + half) * e.ldr + col;
+#pragma unroll
+                for (int c = 0; c < 16; ++c, r += e.ldr) res[c] = in && half + c < rows ? __bfloat162float(*r) : 0.f;
+            }
 #pragma unroll
             for (int c = 0; c < 16; ++c) v[half + c] += res[c];
         }
         if (e.vec) continue;
+        // (addresses by addition: with a 64-bit product and a look at the type for each element these stores took twice as long, 8 bits, 4096 x 512 -> 2047 32 us instead of 19)
+        if (e.y_f32) {
+            float* y = (float*)e.y + (row0 + half) * e.ldy + col;
 #pragma unroll
-        for (int c = half; c < half + 16; ++c)
-            if (in && c < rows) {
-                if (e.y_f32) ((float*)e.y)[(row0 + c) * e.ldy + col] = v[c];
-                else ((bf16*)e.y)[(row0 + c) * e.ldy + col] = __float2bfloat16_rn(v[c]);
-            }
+            for (int c = half; c < half + 16; ++c, y += e.ldy)
+                if (in && c < rows) *y = v[c];
+        } else {
+            bf16* y = (bf16*)e.y + (row0 + half) * e.ldy + col;
+#pragma unroll
+            for (int c = half; c < half + 16; ++c, y += e.ldy)
+                if (in && c < rows) *y = __float2bfloat16_rn(v[c]);
+        }
     }
     if (e.vec) bulk_store_block<true>(mine, Y, e.y_f32, mixed, v, lane, turn, col0, row0);
 }
