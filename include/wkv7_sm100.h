@@ -331,7 +331,7 @@ int wkv7_linear_int8(const void* x, const float* xs, const void* w, const float*
                      int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int act, int flags, void* workspace, void* stream);
 /*
  * Rows to 8 bits: a = max |x[m][k]|, q = rint(127 x / a) (ties to even, decided exactly for bf16 x), scale[m] = a / 127.  x [M,K] bf16, or fp32 with WKV7_X_F32, rows
- * ldx apart; q signed 8-bit [M,K], rows ldq apart; any K > 0.  A row without a magnitude above 2^-100 becomes zeros with scale 0; one that holds a NaN or an
+ * ldx apart; q signed 8-bit [M,K], rows ldq apart; 0 < K <= 2^30.  A row without a magnitude above 2^-100 becomes zeros with scale 0; one that holds a NaN or an
  * infinity zeros with a NaN for its scale, and so are its products.
  */
 #define WKV7_X_F32 1

@@ -35,6 +35,7 @@ def test_quantize_checks(lib):
     assert f(0x1000, 0x1000, 0x1000, 1, 8, 8, 7, 0, None) == f(0x1000, 0x1000, 0x1000, 1, 8, 8, 8, 2, None) == -1
     assert f(None, 0x1000, 0x1000, 1, 8, 8, 8, 0, None) == f(0x1000, None, 0x1000, 1, 8, 8, 8, 0, None) == f(0x1000, 0x1000, None, 1, 8, 8, 8, 0, None) == -6
     assert f(0x1001, 0x1000, 0x1000, 1, 8, 8, 8, 0, None) == f(0x1002, 0x1000, 0x1000, 1, 8, 8, 8, 1, None) == f(0x1000, 0x1000, 0x1002, 1, 8, 8, 8, 0, None) == -4
+    assert f(0x1000, 0x1000, 0x1000, 1, (1 << 30) + 1, 1 << 31, 1 << 31, 0, None) == -8
     assert f(None, None, None, 0, 8, 8, 8, 0, None) == 0
 
 
@@ -59,7 +60,7 @@ def refusals(linear_int8, quantize):
         linear_int8(x, w)
     with pytest.raises(TypeError, match='quantize'):
         quantize(th.zeros(4, 64).half())
-    for bad in (th.zeros(4, 0), th.zeros(())):
+    for bad in (th.zeros(4, 0), th.zeros(()), th.zeros(1).expand(2, (1 << 30) + 1)):
         with pytest.raises(ValueError, match='quantize'):
             quantize(bad)
     with pytest.raises(RuntimeError, match='CUDA'):

@@ -125,6 +125,15 @@ def test_sizes(M, D):
     compare(M, D, F32, None, F32)
 
 
+@pytest.mark.parametrize('M,D', [(300, 1), (5000, 3), (9000, 8), (3000, 9), (700, 257), (600, 2041), (400, 2047), (350, 4097), (310, 8185), (330, 8199), (500, 16383)])
+def test_teams(M, D):
+    """Two pieces a thread, several teams a CTA, rows whose first and last pieces have a part, more rows than teams."""
+    compare(M, D, BF, BF, F32, p=0.1)
+    compare(M, D, BF, F32, BF)
+    compare(M, D, F32, F32, F32, p=0.3)
+    compare(M, D, BF, None, None)
+
+
 @pytest.mark.parametrize('D', [64, 333, 2048, 4096])
 @pytest.mark.parametrize('x_t', [BF, F32])
 @pytest.mark.parametrize('r_t', [None, BF, F32])
@@ -437,3 +446,36 @@ def test_python_form_gives_the_same():
         assert all(th.equal(s, t) for s, t in zip([*a, *th.autograd.grad(a, [x, w, r], [dy, dh])], [*b, *th.autograd.grad(b, [x, w, r], [dy, dh])]))
         a, b = dropout(x, 0.3, 8, residual=r), Dropout.apply(x, r, None, 0.3, 8)
         assert all(th.equal(s, t) for s, t in zip([a, *th.autograd.grad(a, [x, r], dh)], [b, *th.autograd.grad(b, [x, r], dh)]))
+
+
+def test_a_block_in_training():
+    """As a program runs them: the stream through two norms with dropout around the channel mixer, forward and backward, against the same in 64 bits on the same masks."""
+    from wind_rwkv.rwkv7 import dropout, linear, rms_norm
+    M, D, F, p = 300, 256, 1024, 0.1
+    x, emb = rn(M, D, seed=1, dtype=BF).requires_grad_(), rn(M, D, seed=2, dtype=BF).requires_grad_()
+    w1, w2 = (1 + rn(D, seed=3, std=0.2)).requires_grad_(), (1 + rn(D, seed=4, std=0.2)).requires_grad_()
+    wk, wv = rn(F, D, seed=5, dtype=BF, std=D ** -0.5).requires_grad_(), rn(D, F, seed=6, dtype=BF, std=F ** -0.5).requires_grad_()
+    leaves = [x, emb, w1, w2, wk, wv]
+    dy = rn(M, D, seed=7, dtype=BF)
+
+    def block(x, emb, w1, w2, wk, wv, norm, drop, mix):
+        y, h = norm(x, w1, drop(emb, 1), 2)
+        y, h = norm(mix(y, wk, wv), w2, h, 3)
+        return y + h
+
+    out = block(*leaves, lambda x, w, r, s: rms_norm(x, w, residual=r, p=p, seed=s), lambda e, s: dropout(e, p, s), lambda y, a, b: linear(linear(y, a, act='relu2'), b))
+    got = th.autograd.grad(out, leaves, dy)
+    ref = [t.detach().double().requires_grad_() for t in leaves]
+
+    def mask(t, s):
+        return th.where(mask_of((M, D), p, s), t / (1 - p), 0.)
+
+    def norm(x, w, r, s):
+        h = r + mask(x, s)
+        return h / (h.square().mean(-1, keepdim=True) + 1e-5).sqrt() * w, h
+
+    want_out = block(*ref, norm, mask, lambda y, a, b: th.relu(y @ a.T).square() @ b.T)
+    want = th.autograd.grad(want_out, ref, dy.double())
+    # a dozen tensors rounded to bf16 on the way there and back: rms 2^-9 / sqrt(3) of each, relu2 doubles what comes before it
+    for g, w in zip([out.detach(), *got], [want_out.detach(), *want]):
+        assert float((g.double() - w).norm() / w.norm()) < 24 * 2.0 ** -9 / 3 ** 0.5

@@ -542,6 +542,7 @@ int wkv7_linear_int8(const void* x, const float* xs, const void* w, const float*
 
 int wkv7_quantize(const void* x, void* q, float* scale, int64_t M, int64_t K, int64_t ldx, int64_t ldq, int flags, void* stream) {
     if (M < 0 || K <= 0 || ldx < K || ldq < K || (flags & ~WKV7_X_F32)) return WKV7_ERR_SHAPE;
+    if (K > 1 << 30) return WKV7_ERR_TOO_LARGE;
     if (M == 0) return WKV7_OK;
     if (!x || !q || !scale) return WKV7_ERR_NULL;
     if ((uintptr_t)x % (flags & WKV7_X_F32 ? 4 : 2) || (uintptr_t)scale % 4) return WKV7_ERR_ALIGN;

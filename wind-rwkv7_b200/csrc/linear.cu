@@ -113,20 +113,21 @@ __device__ __forceinline__ float scaled(float sum, float ps, float qs) { return 
 // A block of 32 sums a lane: a lane's own scale, along P, and the block's 32 along Q, in shared memory, where all lanes read the same.  (Read from global memory
 // where they are used they were waited for: 8192 x 2048 -> 8192 105 us, without any scales 87.)
 template <bool I8> __device__ __forceinline__ void scale_block(float ps, const float* qs, float (&v)[32]) {
-    if (!I8) return;
+    if constexpr (I8)
 #pragma unroll
-    for (int c = 0; c < 32; c += 4) {
-        const float4 q = *reinterpret_cast<const float4*>(qs + c);
-        v[c] = scaled(v[c], ps, q.x); v[c + 1] = scaled(v[c + 1], ps, q.y); v[c + 2] = scaled(v[c + 2], ps, q.z); v[c + 3] = scaled(v[c + 3], ps, q.w);
-    }
+        for (int c = 0; c < 32; c += 4) {
+            const float4 q = *reinterpret_cast<const float4*>(qs + c);
+            v[c] = scaled(v[c], ps, q.x); v[c + 1] = scaled(v[c + 1], ps, q.y); v[c + 2] = scaled(v[c + 2], ps, q.z); v[c + 3] = scaled(v[c + 3], ps, q.w);
+        }
 }
 // the same, qs: one each of the lanes', which go through the warp's room of 128 bytes
 template <bool I8> __device__ __forceinline__ void scale_block(float ps, float qs, float* room, int lane, float (&v)[32]) {
-    if (!I8) return;
-    __syncwarp();
-    room[lane] = qs;
-    __syncwarp();
-    scale_block<I8>(ps, room, v);
+    if constexpr (I8) {
+        __syncwarp();
+        room[lane] = qs;
+        __syncwarp();
+        scale_block<I8>(ps, room, v);
+    }
 }
 __device__ __forceinline__ float scale_at(const float* s, long long i, long long n) { return i < n ? s[i] : 0.f; }
 // eight adjacent columns of a row, from the accumulator to memory; bias already added

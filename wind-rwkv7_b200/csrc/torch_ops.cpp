@@ -761,7 +761,7 @@ py::object dropout(const Tensor& x, double p, int64_t seed, const OptTensor& see
 
 py::object quantize(const Tensor& x) {
     int64_t ld;
-    if (!eager({&x}, false) || x.dim() < 1 || x.numel() == 0 || !float_type(x) || !pitched_rows(x, &ld)) return py::none();
+    if (!eager({&x}, false) || x.dim() < 1 || x.numel() == 0 || x.size(-1) > 1 << 30 || !float_type(x) || !pitched_rows(x, &ld)) return py::none();
     Tensor q, scale;
     {
         py::gil_scoped_release nogil;

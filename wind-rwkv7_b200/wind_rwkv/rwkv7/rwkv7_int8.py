@@ -83,7 +83,7 @@ _fw_op = _lib.opaque_op('linear_int8', fw_int8,
 def quantize(x):
     """Rows of x [..., K] in 8 bits: Int8(q, scale) with scale = max |row| / 127 and q = row / scale, rounded to the nearest, ties to even.
 
-    x bf16 or fp32, K up to 2^31 - 1.  A row without a magnitude above 2^-100 becomes zeros with scale 0; one that holds a NaN or an infinity becomes zeros with a NaN for
+    x bf16 or fp32, K up to 2^30.  A row without a magnitude above 2^-100 becomes zeros with scale 0; one that holds a NaN or an infinity becomes zeros with a NaN for
     its scale, so that its products are NaN.  q's rows lie on 16-byte boundaries (K rounded up to 16 apart).  No autograd: the results are constants."""
     if not th.compiler.is_compiling():
         out = _lib.ext().quantize(x)
@@ -91,8 +91,8 @@ def quantize(x):
             return Int8(*out)
     if x.dtype not in (th.bfloat16, th.float32):
         raise TypeError(f'quantize takes bfloat16 or float32, not {x.dtype}')
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f'quantize takes x [..., K] with K > 0, got {list(x.shape)}')
+    if x.dim() < 1 or not 0 < x.shape[-1] <= 1 << 30:
+        raise ValueError(f'quantize takes x [..., K] with K from 1 to 2^30, got {list(x.shape)}')
     _lib.require_cuda(x)
     q, scale = _lib.call(_rows_op, rows8, x.detach())
     return Int8(q[..., :x.shape[-1]], scale)

@@ -186,7 +186,7 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-5, p=0.0, seed=None, out_d
 
     x [..., D] bf16 or fp32, D up to 16384; weight [D] bf16 or fp32, or None; residual [..., D] bf16 or fp32, whose type h has: the stream, rounded to it, is what is normed.
     y has x's type unless out_dtype says bf16, fp32 or int8; int8 gives Int8(q, scale) for linear_int8 (see quantize), without a backward.  p, seed: of dropout(),
-    elements counted in row-major order.  Backward for x, weight and residual.  Squares are summed in fp32: a row beyond 1e19 leaves its range and gives 0.
+    elements counted in row-major order.  Backward for x, weight and residual.  Squares are summed in fp32: a row beyond 1e19 leaves its range and gives 0 (with eps = 0, one below 1e-19 infinities).
     Rows may lie in a wider tensor; other layouts are copied."""
     if not th.compiler.is_compiling():
         number, seed_t = (-1, None) if seed is None else _seed_of(seed)
