@@ -91,7 +91,8 @@ template <int NV, bool XF, bool EVEN> __global__ void __launch_bounds__(NV ? thr
 }
 
 // ---- dropout alone ---------------------------------------------------------------------------------------------------------
-// Two pieces a thread at a time; the last elements, less than a piece, are the first thread's.
+// Two pieces a thread at a time; the last elements, less than a piece, go one to a thread.
+constexpr int DROPOUT_CTAS = 8;  // of an SM, where registers leave room for as many
 template <bool XF, int RES, bool LOW> __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
     constexpr bool RF = RES == 2;
     constexpr int XS = XF ? 4 : 2, RS = RF ? 4 : 2;
@@ -99,18 +100,17 @@ template <bool XF, int RES, bool LOW> __global__ void __launch_bounds__(256) dro
     const Dropper drop(p.d);
     const int ys = p.y_f32 ? 4 : 2;
     const long long pieces = p.n >> 3, step = (long long)gridDim.x * 512;
-    auto finish = [&](const Raw<XF>& x, const Raw<RF>& r, long long n, int live) {
+    auto finish = [&](const Raw<XF>& x, const Raw<RF>& r, long long n) {
         float f[8];
         floats<XF>(x, f);
-        if (p.d.threshold) drop.template apply<LOW>(n, f);
+        drop.template apply<LOW>(n, f);
         if (RES) {
             float g[8];
             floats<RF>(r, g);
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = __fadd_rn(g[i], f[i]);
         }
-        if (live == 8) store<true>((Byte*)p.y + 8 * n * ys, nullptr, p.y_f32, 0, 8, f);
-        else store<false>((Byte*)p.y + 8 * n * ys, nullptr, p.y_f32, 0, live, f);
+        store<true>((Byte*)p.y + 8 * n * ys, nullptr, p.y_f32, 0, 8, f);
     };
     for (long long n = (long long)blockIdx.x * 512 + threadIdx.x; n < pieces; n += step) {
         Raw<XF> x[2];
@@ -123,15 +123,20 @@ template <bool XF, int RES, bool LOW> __global__ void __launch_bounds__(256) dro
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-            if (n + 256 * b < pieces) finish(x[b], r[b], n + 256 * b, 8);
+            if (n + 256 * b < pieces) finish(x[b], r[b], n + 256 * b);
     }
-    const int rest = (int)(p.n & 7);
-    if (rest && blockIdx.x == 0 && threadIdx.x == 0) {
-        Raw<XF> x;
-        Raw<RF> r;
-        complete<XF, false>(x, (const Byte*)p.x + 8 * pieces * XS, nullptr, 0, rest);
-        if (RES) complete<RF, false>(r, (const Byte*)p.residual + 8 * pieces * RS, nullptr, 0, rest);
-        finish(x, r, pieces, rest);
+    if (blockIdx.x == 0 && threadIdx.x < (p.n & 7)) {
+        const long long at = 8 * pieces + threadIdx.x;
+        uint32_t c[2][4];
+        drop.template words<LOW>(pieces, c);
+        uint32_t word = c[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) word = threadIdx.x == i ? c[i / 4][i % 4] : word;
+        float f = XF ? ((const float*)p.x)[at] : __bfloat162float(((const bf16*)p.x)[at]);
+        f = drop.keeps(word) ? __fmul_rn(f, drop.scale) : 0.f;
+        if (RES) f = __fadd_rn(RF ? ((const float*)p.residual)[at] : __bfloat162float(((const bf16*)p.residual)[at]), f);
+        if (p.y_f32) ((float*)p.y)[at] = f;
+        else ((bf16*)p.y)[at] = __float2bfloat16_rn(f);
     }
 }
 
@@ -160,7 +165,7 @@ int launch_dropout(const DropoutParams& p, cudaStream_t stream) {
 #define WKV7_LOW(xf, res) {dropout_kernel<xf, res, false>, dropout_kernel<xf, res, true>}
     static void (*const kernels[2][3][2])(DropoutParams) = {{WKV7_LOW(false, 0), WKV7_LOW(false, 1), WKV7_LOW(false, 2)}, {WKV7_LOW(true, 0), WKV7_LOW(true, 1), WKV7_LOW(true, 2)}};
 #undef WKV7_LOW
-    const long long want = (p.n + 4095) / 4096, most = (long long)sm_count() * 8;
+    const long long want = (p.n + 4095) / 4096, most = (long long)sm_count() * DROPOUT_CTAS;
     return launch(kernels[p.x_f32][p.residual ? 1 + p.r_f32 : 0][low_counters(p.n)], dim3((unsigned)(want < most ? want : most)), 256, 0, stream, p) ? kOk : kLaunchFailed;
 }
 

@@ -11,9 +11,10 @@ namespace norm {
 // Ten rounds of two 32 x 32 -> 64 products for four words.  No mask is stored: the backward forms the words again.  Its products bound dropout of bf16 elements: 36 of
 // them for a piece of eight, at four cycles each in a quarter of an SM, are 43 us for 2^26 elements, as much as their traffic.
 struct Dropper {
-    uint32_t k0, k1, below;  // kept: word > below (the threshold less one; 2^32 less one drops all)
+    uint32_t k0, k1, from;  // kept: word >= from
+    bool none;              // all dropped, the threshold is 2^32
     float scale;
-    __device__ __forceinline__ explicit Dropper(const Dropout& d) : below((uint32_t)(d.threshold - 1)), scale(d.scale) {
+    __device__ __forceinline__ explicit Dropper(const Dropout& d) : from((uint32_t)d.threshold), none(d.threshold >> 32 != 0), scale(d.scale) {
         const unsigned long long s = d.where ? *d.where : d.seed;
         k0 = __shfl_sync(0xffffffffu, (uint32_t)s, 0);  // (the same for all lanes, which the compiler cannot see)
         k1 = __shfl_sync(0xffffffffu, (uint32_t)(s >> 32), 0);
@@ -39,12 +40,13 @@ struct Dropper {
             }
         }
     }
+    __device__ __forceinline__ bool keeps(uint32_t word) const { return word >= from && !none; }
     // eight adjacent elements, of which the first is element 8 n
     template <bool LOW> __device__ __forceinline__ void apply(unsigned long long n, float (&f)[8]) const {
         uint32_t c[2][4];
         words<LOW>(n, c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = c[i / 4][i % 4] > below ? __fmul_rn(f[i], scale) : 0.f;
+        for (int i = 0; i < 8; ++i) f[i] = keeps(c[i / 4][i % 4]) ? __fmul_rn(f[i], scale) : 0.f;
     }
     __device__ __forceinline__ void apply(bool low, unsigned long long n, float (&f)[8]) const {
         if (low) apply<true>(n, f);
