@@ -277,22 +277,31 @@ template <int ACT, typename Sums> __device__ __forceinline__ void finish_cols(co
 #pragma unroll
     for (int half = 0; half < 32; half += 16) {
         if (e.residual) {  // (sixteen rows of it before they are stored: y may be the residual, so the compiler keeps them in order)
-            float res[16];
+            // (loads without conditions, behind the last row or column the last again: conditional ones went one after the other, 8 bits, 4000 x 2048 -> 4001 105 us instead of 53)
+            uint32_t res[16];
+            const long long at = (row0 + (half < rows ? half : 0)) * e.ldr + (in ? col : e.cols - 1);
             if (e.y_f32) {
-                const float* r = (const float*)e.residual + (row0 + half) * e.ldr + col;
+                const uint32_t* r = (const uint32_t*)e.residual + at;
 #pragma unroll
-                for (int c = 0; c < 16; ++c, r += e.ldr) res[c] = in && half + c < rows ? *r : 0.f;
+                for (int c = 0; c < 16; ++c) { res[c] = *r; r += half + c + 1 < rows ? e.ldr : 0; }
             } else {
-                const bf16* r = (const bf16*)e.residual + (row0 + half) * e.ldr + col;
+                const uint16_t* r = (const uint16_t*)e.residual + at;
 #pragma unroll
-                for (int c = 0; c < 16; ++c, r += e.ldr) res[c] = in && half + c < rows ? __bfloat162float(*r) : 0.f;
+                for (int c = 0; c < 16; ++c) { res[c] = *r; r += half + c + 1 < rows ? e.ldr : 0; }
             }
+            const int shift = e.y_f32 ? 0 : 16;
 #pragma unroll
-            for (int c = 0; c < 16; ++c) v[half + c] += res[c];
+            for (int c = 0; c < 16; ++c) v[half + c] += __uint_as_float(res[c] << shift);
         }
         if (e.vec) continue;
-        // (addresses by addition: with a 64-bit product and a look at the type for each element these stores took twice as long, 8 bits, 4096 x 512 -> 2047 32 us instead of 19)
-        if (e.y_f32) {
+        // (addresses by addition: with a 64-bit product and a look at the type for each element these stores took twice as long, 8 bits, 4096 x 512 -> 2047 32 us instead of 17)
+        if (!e.y_f32 && rows == 32) {
+            if (in) {
+                bf16* y = (bf16*)e.y + (row0 + half) * e.ldy + col;
+#pragma unroll
+                for (int c = half; c < half + 16; ++c, y += e.ldy) *y = __float2bfloat16_rn(v[c]);
+            }
+        } else if (e.y_f32) {
             float* y = (float*)e.y + (row0 + half) * e.ldy + col;
 #pragma unroll
             for (int c = half; c < half + 16; ++c, y += e.ldy)
