@@ -11,8 +11,9 @@
 namespace wkv7 {
 namespace norm {
 
-// threads of an SM that the grid is sized for
-constexpr int fwd_threads(int nv) { return nv == 1 ? 576 : nv == 2 ? 512 : 544; }
+// Threads of an SM, for which there are registers and the grid is sized.  Two pieces of bf16 without parts fit 96 registers (8192 x 2048 25.1 -> 23.5 us, 65536 x 768 78 -> 72);
+// the other forms would spill what they have requested (60000 x 1001 with dropout 131 -> 175).
+constexpr int fwd_threads(int nv, bool narrow) { return nv == 1 ? 576 : nv == 2 ? narrow ? 640 : 512 : 544; }
 struct FwdKernelParams : NormFwdParams {
     Teams t;
     Lie at_x, at_r, at_y, at_h;
@@ -21,7 +22,7 @@ struct FwdKernelParams : NormFwdParams {
 };
 // RES: no residual, bf16, fp32.  Of rows that take four pieces a thread nothing is requested ahead and the weight is not held: registers.
 template <int NV, bool XF, int RES, bool DROP, bool INT8, bool EVEN>
-__global__ void __launch_bounds__(threads_most(NV), 1) norm_fwd_kernel(const __grid_constant__ FwdKernelParams p) {
+__global__ void __launch_bounds__(NV == 1 ? threads_most(1) : fwd_threads(NV, EVEN && !XF && RES != 2), 1) norm_fwd_kernel(const __grid_constant__ FwdKernelParams p) {
     constexpr bool HELD = NV < 4, RF = RES == 2;
     constexpr int XS = XF ? 4 : 2, RS = RF ? 4 : 2;
     __shared__ Room room;
@@ -158,7 +159,7 @@ int launch_norm_fwd(const NormFwdParams& a, cudaStream_t stream) {
 #undef WKV7_OUT
     const bool even = p.D % 8 == 0 && p.at_x.end && (!p.residual || (p.at_r.end && p.at_h.end)) && p.at_y.end;
     const auto kern = kernels[nv / 2][even][p.x_f32][p.residual ? 1 + p.r_f32 : 0][drop][int8];
-    return launch(kern, dim3((unsigned)ctas_of(p.M, p.t, sm_count(), fwd_threads(nv))), p.t.threads * p.t.rows, 0, stream, p) ? kOk : kLaunchFailed;
+    return launch(kern, dim3((unsigned)ctas_of(p.M, p.t, sm_count(), fwd_threads(nv, even && !p.x_f32 && !(p.residual && p.r_f32)))), p.t.threads * p.t.rows, 0, stream, p) ? kOk : kLaunchFailed;
 }
 
 }  // namespace wkv7
