@@ -166,6 +166,23 @@ def test_batch_dimensions():
     assert th.equal(rms_norm(v), rms_norm(v[None])[0])
 
 
+@pytest.mark.parametrize('D', [256, 333, 9000])
+@pytest.mark.parametrize('p', [0., 0.2])
+def test_some_inputs_alone_have_gradients(D, p):
+    """What is not asked for is not formed; what is has the values of the whole."""
+    from wind_rwkv.rwkv7 import rms_norm
+    x, r, w = rn(40, D, seed=1, dtype=BF), rn(40, D, seed=2, dtype=BF), 1 + rn(D, seed=3, std=0.2)
+    dy, dh = rn(40, D, seed=4, dtype=BF), rn(40, D, seed=5, dtype=BF)
+    leaves = [t.clone().requires_grad_() for t in (x, w, r)]
+    whole = th.autograd.grad(rms_norm(leaves[0], leaves[1], residual=leaves[2], p=p, seed=3), leaves, [dy, dh])
+    for keep in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        t = [a.clone().requires_grad_() if i in keep else a for i, a in enumerate((x, w, r))]
+        got = th.autograd.grad(rms_norm(t[0], t[1], residual=t[2], p=p, seed=3), [t[i] for i in keep], [dy, dh])
+        assert all(th.equal(g, whole[i]) for g, i in zip(got, keep))
+        y, h = rms_norm(t[0], residual=t[2], p=p, seed=3)     # without a weight
+        assert (y.requires_grad and h.requires_grad) == (keep != (1,))
+
+
 def test_gradient_against_differences():
     """The formula itself: differences of the formula in 64 bits along random directions."""
     M, D, eps, p, seed = 6, 40, 1e-3, 0.3, 11
@@ -223,6 +240,10 @@ def test_layouts(D):
             want = rms_norm(x.clone(memory_format=th.contiguous_format), w, residual=r.clone(memory_format=th.contiguous_format))
             got = rms_norm(x, w, residual=r)
             assert all(th.equal(a, b) for a, b in zip(got, want))
+    flat = rn(12 * D + 8, seed=6, dtype=BF)
+    for off in (1, 3, 4, 8):  # rows back to back, at any alignment
+        x = flat[off:off + 12 * D].view(12, D)
+        assert th.equal(rms_norm(x, w), rms_norm(x.clone(), w))
     # gradients that come in other layouts
     x, r = (t[:, :D].clone().requires_grad_() for t in wide)
     y, h = rms_norm(x, w, residual=r, p=0.1, seed=5)
@@ -372,6 +393,20 @@ def test_beyond_32_bits():
         assert th.equal(part.cpu(), th.from_numpy(kept(first, part.numel(), 0.5, 21)))
 
 
+def test_counters_beyond_32_bits():
+    """Elements behind the 2^34th, whose counters leave 32 bits."""
+    from wind_rwkv.rwkv7 import dropout
+    n = (1 << 34) + 4099
+    if th.cuda.mem_get_info()[0] < 5 * n:
+        pytest.skip('two tensors of 32 GB do not fit')
+    y = dropout(th.ones(n, dtype=BF, device='cuda'), 0.5, 21)
+    for first in (0, (1 << 32) - 8, (1 << 34) - 2000, n - 4000):
+        part = y[first:first + 4000] != 0
+        assert th.equal(part.cpu(), th.from_numpy(kept(first, part.numel(), 0.5, 21)))
+    del y
+    th.cuda.empty_cache()
+
+
 def test_rows_beyond_32_bits():
     from wind_rwkv.rwkv7 import rms_norm
     M, D = 70000, 32768 + 8
@@ -432,6 +467,19 @@ def test_torch_compile():
     got = th.compile(f, backend='aot_eager', fullgraph=True)(x, r, w)
     gg = th.autograd.grad([t.float().sum() for t in got], [x, r, w])
     assert all(th.equal(a, b) for a, b in zip([*want, *wg], [*got, *gg]))
+
+
+@pytest.mark.parametrize('dynamic', [False, True])
+def test_torch_compile_without_a_residual(dynamic):
+    from wind_rwkv.rwkv7 import rms_norm
+    w = (1 + rn(333, seed=3, std=0.2)).requires_grad_()
+    th.compiler.reset()
+    f = th.compile(lambda x, w: rms_norm(x, w, out_dtype=F32) * 2, backend='aot_eager', fullgraph=True, dynamic=dynamic)
+    for M in (40, 41, 7):
+        x = rn(M, 333, seed=M, dtype=BF).requires_grad_()
+        want, got = rms_norm(x, w, out_dtype=F32) * 2, f(x, w)
+        assert th.equal(want, got)
+        assert all(th.equal(a, b) for a, b in zip(th.autograd.grad(want.sum(), [x, w]), th.autograd.grad(got.sum(), [x, w])))
 
 
 def test_python_form_gives_the_same():
