@@ -8,6 +8,7 @@
 #include <ATen/TracerMode.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/extension.h>
@@ -585,6 +586,8 @@ py::object linear(const Tensor& x, const Tensor& w, const OptTensor& bias_, cons
 }
 
 // ---- the residual stream, rows in 8 bits --------------------------------------------------------------------
+// an uninitialised tensor, without the dispatcher's share of at::empty
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) { return Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt)); }
 bool float_type(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
 bool is_f32(const Tensor& t) { return t.defined() && t.scalar_type() == at::kFloat; }
 int64_t pitch8(int64_t n) { return (n + 15) / 16 * 16; }  // bytes from row to row of a tensor in 8 bits
@@ -592,7 +595,7 @@ int64_t pitch8(int64_t n) { return (n + 15) / 16 * 16; }  // bytes from row to r
 Tensor empty8(const Tensor& like) {
     std::vector<int64_t> shape = like.sizes().vec();
     shape.back() = pitch8(like.size(-1));
-    return at::empty(shape, like.options().dtype(at::kChar));
+    return fresh(shape, at::kChar, like);
 }
 Tensor as_rows(const Tensor& t, int64_t* ld) {  // (hooks on saved tensors, and gradients, may come in other layouts)
     if (!t.defined()) return t;
@@ -612,12 +615,12 @@ std::array<Tensor, 4> norm_forward(const Tensor& x, const Tensor& w, const Tenso
     Tensor y, h, rstd, scale;
     if (n.out == 2) {
         y = empty8(x);
-        scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+        scale = fresh(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
     } else {
-        y = at::empty(x.sizes(), x.options().dtype(n.out ? at::kFloat : at::kBFloat16));
+        y = fresh(x.sizes(), n.out ? at::kFloat : at::kBFloat16, x);
     }
-    if (r.defined()) h = at::empty(x.sizes(), r.options());
-    if (save) rstd = at::empty({M}, x.options().dtype(at::kFloat));
+    if (r.defined()) h = fresh(x.sizes(), r.scalar_type(), x);
+    if (save) rstd = fresh({M}, at::kFloat, x);
     int64_t ldx = D, ldr = D;
     pitched_rows(x, &ldx);
     if (r.defined()) pitched_rows(r, &ldr);
@@ -658,11 +661,11 @@ struct RmsNormFn : public Function<RmsNormFn> {
         if (dh.defined()) dh = as_rows(dh.to(h.scalar_type()), &lddh);
         const bool one = p == 0. && x_f32 == is_f32(h);  // x and the stream have the same gradient
         Tensor dx, dr, dw, ws;
-        if (want_x && !one) dx = at::empty(h.sizes(), h.options().dtype(x_f32 ? at::kFloat : at::kBFloat16));
-        if (want_r || (want_x && one)) dr = at::empty(h.sizes(), h.options());
+        if (want_x && !one) dx = fresh(h.sizes(), x_f32 ? at::kFloat : at::kBFloat16, h);
+        if (want_r || (want_x && one)) dr = fresh(h.sizes(), h.scalar_type(), h);
         if (want_w) {
-            dw = at::empty({D}, h.options().dtype(at::kFloat));
-            ws = at::empty({wkv7_rms_norm_bwd_workspace_bytes(M, D)}, h.options().dtype(at::kByte));
+            dw = fresh({D}, at::kFloat, h);
+            ws = fresh({wkv7_rms_norm_bwd_workspace_bytes(M, D)}, at::kByte, h);
         }
         check(wkv7_rms_norm_bwd(h.data_ptr(), f32_of(rstd), ptr(w), dy.data_ptr(), ptr(dh), ptr(dx), ptr(dr), f32(dw), M, D, ldh, lddy, lddh, D, D, p, (uint64_t)how[2], ptr(seed),
                                 (x_f32 ? WKV7_X_F32 : 0) | (is_f32(h) ? WKV7_R_F32 : 0) | (is_f32(w) ? WKV7_W_F32 : 0) | (out_f32 ? WKV7_Y_F32 : 0), ptr(ws), stream()),
@@ -712,7 +715,7 @@ py::object rms_norm(const Tensor& x, const OptTensor& w_, const OptTensor& r_, d
 
 // adjacent elements from a 16-byte boundary on
 Tensor dropped(const Tensor& x, const Tensor& r, const Tensor& seed_t, double p, int64_t seed, at::ScalarType type) {
-    Tensor y = at::empty(x.sizes(), x.options().dtype(type));
+    Tensor y = fresh(x.sizes(), type, x);
     check(wkv7_dropout(x.data_ptr(), ptr(r), y.data_ptr(), x.numel(), p, (uint64_t)seed, ptr(seed_t), (is_f32(x) ? WKV7_X_F32 : 0) | (is_f32(r) ? WKV7_R_F32 : 0) | (is_f32(y) ? WKV7_Y_F32 : 0),
                        stream()), "wkv7_dropout");
     return y;
@@ -769,7 +772,7 @@ py::object quantize(const Tensor& x) {
         at::NoGradGuard ng;
         const int64_t K = x.size(-1);
         q = empty8(x);
-        scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+        scale = fresh(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
         check(wkv7_quantize(x.data_ptr(), q.data_ptr(), f32_of(scale), x.numel() / K, K, ld, q.size(-1), is_f32(x) ? WKV7_X_F32 : 0, stream()), "wkv7_quantize");
         if (q.size(-1) != K) q = q.narrow(-1, 0, K);
     }
@@ -800,9 +803,9 @@ py::object linear_int8(const Tensor& xq, const Tensor& xs, const Tensor& wq, con
         py::gil_scoped_release nogil;
         const c10::cuda::CUDAGuard guard(xq.device());
         at::NoGradGuard ng;
-        y = at::empty(shape, xs.options().dtype(out_f32 ? at::kFloat : at::kBFloat16));
+        y = fresh(shape, out_f32 ? at::kFloat : at::kBFloat16, xq);
         Tensor work;
-        if (const int64_t bytes = wkv7_linear_int8_workspace_bytes(M, N, K)) work = at::empty({bytes}, xs.options().dtype(at::kByte));
+        if (const int64_t bytes = wkv7_linear_int8_workspace_bytes(M, N, K)) work = fresh({bytes}, at::kByte, xq);
         check(wkv7_linear_int8(xq.data_ptr(), f32_of(xs), wq.data_ptr(), f32_of(ws), ptr(bias), ptr(residual), y.data_ptr(), M, N, K, ldx, ldw, ldr, N, (int)act,
                                (out_f32 ? WKV7_LINEAR_F32_OUT : 0) | (is_f32(bias) ? WKV7_LINEAR_F32_BIAS : 0), ptr(work), stream()), "wkv7_linear_int8");
     }
