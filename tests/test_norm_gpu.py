@@ -527,3 +527,34 @@ def test_a_block_in_training():
     # a dozen tensors rounded to bf16 on the way there and back: rms 2^-9 / sqrt(3) of each, relu2 doubles what comes before it
     for g, w in zip([out.detach(), *got], [want_out.detach(), *want]):
         assert float((g.double() - w).norm() / w.norm()) < 24 * 2.0 ** -9 / 3 ** 0.5
+
+
+@pytest.mark.parametrize('x_t,r_t', [(F32, None), (F32, F32), (F32, BF), (BF, F32)])
+@pytest.mark.parametrize('form', ['eager', 'python'])
+def test_second_derivatives_of_dropout(x_t, r_t, form):
+    """A penalty on the gradient: y = r + k x with k = kept / (1 - p), dx = k dy, and so through dx to dy."""
+    from wind_rwkv.rwkv7 import dropout
+    from wind_rwkv.rwkv7.rwkv7_norm import Dropout
+    shape, p, seed = (50, 77), 0.3, 19
+    x = rn(*shape, seed=1, dtype=x_t).requires_grad_()
+    r = None if r_t is None else rn(*shape, seed=2, dtype=r_t).requires_grad_()
+    leaves = [t for t in (x, r) if t is not None]
+    y = dropout(x, p, seed, residual=r) if form == 'eager' else Dropout.apply(x, r, None, p, seed)
+    first = th.autograd.grad(y.square().sum(), leaves, create_graph=True)
+    assert all(g.requires_grad for g in first) and first[0].dtype == x_t
+    u = rn(*shape, seed=3, dtype=x_t)
+    second = th.autograd.grad(first[0], leaves, u)
+    K = mask_of(shape, p, seed).double() / (1 - p)
+    X, R = x.detach().double(), 0. if r is None else r.detach().double()
+    Y = R + K * X
+    # y: three roundings of its parts and its own; 2 y is exact; dx: two and its type's.  Of the second derivative 2 k k u each product: two and its type's
+    parts = (K * X).abs() + (0. if r is None else R.abs())
+    e = 2 * K * (3 * E * parts + U[y.dtype] * (Y.abs() + 3 * E * parts))
+    check('dx', first[0], 2 * K * Y, e + (2 * E + U[x_t]) * ((2 * K * Y).abs() + e))
+    for g, want in zip(second, [2 * K * K * u.double()] + ([] if r is None else [2 * K * u.double()])):
+        check('second', g, want, (4 * E + U[y.dtype] + U[g.dtype]) * 1.01 * want.abs())
+    if form == 'eager' and x_t == r_t:  # linear in dy, whatever x is
+        v = rn(*shape, seed=4).requires_grad_()
+        dx, = th.autograd.grad(dropout(x, p, seed, residual=r), x, v, create_graph=True)
+        back, = th.autograd.grad(dx, v, u)
+        check('dv', back, K * u.double(), 4 * E * (K * u.double()).abs())

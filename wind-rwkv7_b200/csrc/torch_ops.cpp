@@ -721,24 +721,29 @@ Tensor dropped(const Tensor& x, const Tensor& r, const Tensor& seed_t, double p,
     return y;
 }
 struct DropoutFn : public Function<DropoutFn> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& r_, const OptTensor& seed_, double p, int64_t seed) {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& r_, const OptTensor& seed_, double p, int64_t seed, bool out_f32) {
         const Tensor r = r_.value_or(Tensor()), s = seed_.value_or(Tensor());
         ctx->save_for_backward({s});
         ctx->set_materialize_grads(false);
         ctx->saved_data["how"] = std::vector<int64_t>{is_f32(x) | r.defined() << 1, bits_of(p), seed};
-        return dropped(x, r, s, p, seed, r.defined() ? r.scalar_type() : x.scalar_type());
+        return dropped(x, r, s, p, seed, out_f32 ? at::kFloat : at::kBFloat16);
     }
     static variable_list backward(AutogradContext* ctx, variable_list go) {
-        variable_list g(5);
+        variable_list g(6);
         const Tensor dy = go[0];
         if (!dy.defined()) return g;
         const auto how = ctx->saved_data["how"].toIntVector();
         if (how[0] >> 1 && ctx->needs_input_grad(1)) g[1] = dy;
         if (!ctx->needs_input_grad(0)) return g;
         const c10::cuda::CUDAGuard guard(dy.device());
-        at::NoGradGuard ng;
         const Tensor s = ctx->get_saved_variables()[0];
-        g[0] = dropped(dense(dy), Tensor(), s, double_of(how[1]), how[2], how[0] & 1 ? at::kFloat : at::kBFloat16);
+        const bool x_f32 = how[0] & 1;
+        if (grad_wanted({&dy})) {  // dx is dropout of dy, and differentiated as such
+            g[0] = apply(dense(dy), OptTensor(), opt(s), double_of(how[1]), how[2], x_f32);
+        } else {
+            at::NoGradGuard ng;
+            g[0] = dropped(dense(dy), Tensor(), s, double_of(how[1]), how[2], x_f32 ? at::kFloat : at::kBFloat16);
+        }
         return g;
     }
 };
@@ -753,7 +758,7 @@ py::object dropout(const Tensor& x, double p, int64_t seed, const OptTensor& see
         if (seed < 0) seed = 0;
         const Tensor xd = dense(x), rd = dense(r);  // (with autograd: copies are part of the graph)
         if (grad_wanted({&x, &r})) {
-            y = DropoutFn::apply(xd, opt(rd), opt(s), p, seed);
+            y = DropoutFn::apply(xd, opt(rd), opt(s), p, seed, is_f32(r.defined() ? r : x));
         } else {
             at::NoGradGuard ng;
             y = dropped(xd, rd, s, p, seed, r.defined() ? r.scalar_type() : x.scalar_type());

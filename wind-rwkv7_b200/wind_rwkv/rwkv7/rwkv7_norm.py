@@ -127,16 +127,21 @@ class RmsNorm(th.autograd.Function):
 
 class Dropout(th.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, seed_t, p, seed):
+    def forward(ctx, x, residual, seed_t, p, seed, out_f32=None):
         ctx.save_for_backward(seed_t)
         ctx.how = (p, seed, x.dtype)
-        return _lib.call(_drop_op, drop, x, residual, seed_t, p, seed, f32(x if residual is None else residual))
+        return _lib.call(_drop_op, drop, x, residual, seed_t, p, seed, f32(x if residual is None else residual) if out_f32 is None else out_f32)
 
     @staticmethod
     def backward(ctx, dy):
         p, seed, x_dtype = ctx.how
-        dx = _lib.call(_drop_op, drop, dy, None, ctx.saved_tensors[0], p, seed, x_dtype == th.float32) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+        dx = None
+        if ctx.needs_input_grad[0]:
+            how = (ctx.saved_tensors[0], p, seed, x_dtype == th.float32)
+            # (where autograd records the backward dx is dropout of dy, and differentiated as such)
+            again = not th.compiler.is_compiling() and th.is_grad_enabled() and dy.requires_grad
+            dx = Dropout.apply(dy, None, *how) if again else _lib.call(_drop_op, drop, dy, None, *how)
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
 
 
 def _check_floats(name, what, t, shape=None):
@@ -219,7 +224,7 @@ def dropout(x, p, seed, *, residual=None):
     x [...] bf16 or fp32; residual of x's shape, bf16 or fp32, whose type the result then has.  Which elements are dropped is a function of the seed and of an element's
     place in row-major order: equal seeds drop equal elements, so each layer and step takes its own.  seed: an integer from 0 to 2^63 - 1, or an int64 tensor
     of one element on x's device, which is read when the kernel runs (a captured step draws anew when the tensor was changed before its replay).  A probability
-    is met to 2^-33.  Backward for x and residual; no mask is stored."""
+    is met to 2^-33.  Backward for x and residual, to any order; no mask is stored."""
     if not th.compiler.is_compiling():
         number, seed_t = _seed_of(seed)
         out = _lib.ext().dropout(x, p, number, seed_t, residual)
