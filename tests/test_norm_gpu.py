@@ -558,3 +558,42 @@ def test_second_derivatives_of_dropout(x_t, r_t, form):
         dx, = th.autograd.grad(dropout(x, p, seed, residual=r), x, v, create_graph=True)
         back, = th.autograd.grad(dx, v, u)
         check('dv', back, K * u.double(), 4 * E * (K * u.double()).abs())
+
+
+@pytest.mark.parametrize('D', [128, 333])
+@pytest.mark.parametrize('form', ['eager', 'python'])
+def test_second_derivatives_of_the_norm_are_refused(D, form):
+    """A backward that is recorded gives the same gradients; what is differentiated through them raises, whichever input or gradient it comes from, and no term is left out."""
+    from wind_rwkv.rwkv7 import rms_norm
+    from wind_rwkv.rwkv7.rwkv7_norm import RmsNorm
+    for p, r_t in ((0., BF), (0.2, F32), (0., None)):
+        x, w = rn(9, D, seed=1, dtype=BF).requires_grad_(), (1 + rn(D, seed=3, std=0.2)).requires_grad_()
+        r = None if r_t is None else rn(9, D, seed=2, dtype=r_t).requires_grad_()
+        dy, dh = rn(9, D, seed=4, dtype=BF).requires_grad_(), rn(9, D, seed=5, dtype=r_t or BF).requires_grad_()
+        leaves = [t for t in (x, w, r) if t is not None]
+
+        def call(x, w, r):
+            y, h = (rms_norm(x, w, residual=r, p=p, seed=6), None) if r is None else rms_norm(x, w, residual=r, p=p, seed=6)
+            if form == 'python':
+                y, h = RmsNorm.apply(x, w, r, None, 1e-5, p, 6, False)
+            return [y] if h is None else [y, h]
+
+        outs = call(x, w, r)
+        want = th.autograd.grad(outs, leaves, [dy, dh][:len(outs)], retain_graph=True)
+        assert not any(g.requires_grad for g in want)
+        got = th.autograd.grad(outs, leaves, [dy, dh][:len(outs)], create_graph=True)
+        assert all(th.equal(a, b) for a, b in zip(got, want))
+        for i, g in enumerate(got):
+            for of in leaves + [dy]:
+                if i == 1 and of is w:   # dw does not depend on w
+                    continue
+                with pytest.raises(RuntimeError, match='second derivative'):
+                    th.autograd.grad(g.float().sum() + outs[0].float().sum() + dy.float().sum(), of, retain_graph=True)
+        # a constant of what is asked for: there is nothing to refuse
+        outs = call(x.detach(), w, None if r is None else r.detach())
+        g, = th.autograd.grad(outs[0], w, dy.detach(), create_graph=True)
+        assert th.equal(g, th.autograd.grad(call(x.detach(), w, None if r is None else r.detach())[0], w, dy.detach())[0]) and not g.requires_grad
+        # a step that records its backward and differentiates nothing through it
+        t = [a.detach().requires_grad_() for a in leaves]
+        sum(o.float().sum() for o in call(t[0], t[1], t[2] if len(t) > 2 else None)).backward(create_graph=True)
+        assert all(a.grad is not None for a in t)

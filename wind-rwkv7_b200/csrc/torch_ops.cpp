@@ -629,8 +629,15 @@ std::array<Tensor, 4> norm_forward(const Tensor& x, const Tensor& w, const Tenso
           "wkv7_rms_norm_fwd");
     return {y, h, rstd, scale};
 }
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 int64_t bits_of(double d) { int64_t b; memcpy(&b, &d, 8); return b; }
 double double_of(int64_t b) { double d; memcpy(&d, &b, 8); return d; }
+// A gradient whose own derivative is not formed.  Where autograd records the backward, the gradient stays joined to what it depends on, and a second backward that comes this
+// way raises instead of leaving the term out.
+struct NormGradFn : public Function<NormGradFn> {
+    static Tensor forward(AutogradContext*, const Tensor& g, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&) { return g; }
+    static variable_list backward(AutogradContext*, variable_list) { throw std::runtime_error("rms_norm has no second derivative"); }
+};
 struct RmsNormFn : public Function<RmsNormFn> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w_, const OptTensor& r_, const OptTensor& seed_, double eps, double p, int64_t seed, int64_t out) {
         const Tensor w = w_.value_or(Tensor()), r = r_.value_or(Tensor()), s = seed_.value_or(Tensor());
@@ -652,6 +659,7 @@ struct RmsNormFn : public Function<RmsNormFn> {
         if ((!dy.defined() && !dh.defined()) || !(want_x || want_w || want_r)) return g;
         const variable_list s = ctx->get_saved_variables();
         const c10::cuda::CUDAGuard guard(s[0].device());
+        const bool recorded = at::GradMode::is_enabled();
         at::NoGradGuard ng;
         const int64_t D = s[0].size(-1), M = s[0].numel() / D;
         int64_t ldh = D, lddy = D, lddh = D;
@@ -673,6 +681,14 @@ struct RmsNormFn : public Function<RmsNormFn> {
         if (want_x) g[0] = one ? dr : dx;
         if (want_w) g[1] = dw.to(w.scalar_type());
         if (want_r) g[2] = dr;
+        if (recorded) {
+            const at::AutoGradMode on(true);
+            const OptTensor from_y = opt(go[0]), from_h = residual ? opt(go[1]) : OptTensor(), of_w = weight ? opt(s[2]) : OptTensor();
+            const OptTensor of_h = want_x || want_r ? opt(s[0]) : OptTensor();  // (as an output it belongs to the graph for the weight's sake alone, too)
+            for (const int i : {0, 2})
+                if (g[i].defined()) g[i] = NormGradFn::apply(g[i], from_y, from_h, of_h, of_w);
+            if (want_w) g[1] = NormGradFn::apply(g[1], from_y, OptTensor(), of_h, OptTensor());
+        }
         return g;
     }
 };
@@ -682,7 +698,6 @@ bool dropout_ok(double p, int64_t seed, const Tensor& seed_t, const Tensor& x) {
     if (seed_t.defined()) return plain(seed_t) && seed_t.scalar_type() == at::kLong && seed_t.numel() == 1 && seed_t.device() == x.device();
     return seed >= 0;
 }
-OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 py::object rms_norm(const Tensor& x, const OptTensor& w_, const OptTensor& r_, double eps, double p, int64_t seed, const OptTensor& seed_, int64_t out) {
     const Tensor w = w_.value_or(Tensor()), r = r_.value_or(Tensor()), s = seed_.value_or(Tensor());
     int64_t ld;

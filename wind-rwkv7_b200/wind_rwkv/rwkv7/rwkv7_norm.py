@@ -100,6 +100,18 @@ _drop_op = _lib.opaque_op('dropout', drop, lambda x, residual, seed_t, p, seed, 
                           '(Tensor x, Tensor? residual, Tensor? seed_t, float p, int seed, bool out_f32) -> Tensor')
 
 
+class NormGrad(th.autograd.Function):
+    """A gradient whose own derivative is not formed.  Where autograd records the backward, the gradient stays joined to what it depends on, and a second backward that comes
+    this way raises instead of leaving the term out."""
+    @staticmethod
+    def forward(ctx, g, *of):
+        return g
+
+    @staticmethod
+    def backward(ctx, dg):
+        raise RuntimeError('rms_norm has no second derivative')
+
+
 class RmsNorm(th.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, seed_t, eps, p, seed, out_f32):
@@ -118,11 +130,17 @@ class RmsNorm(th.autograd.Function):
         if (dy is None and dh is None) or not (want_x or want_w or want_r):
             return (None,) * 8
         h, rstd, weight, seed_t = ctx.saved_tensors
+        from_y, from_h = dy, dh
         dy = th.zeros(h.shape, dtype=th.float32 if out_f32 else th.bfloat16, device=h.device) if dy is None else dy.to(th.float32 if out_f32 else th.bfloat16)
         dh = None if dh is None else dh.to(h.dtype)
         one = not p and x_dtype == h.dtype  # x and the stream have the same gradient
         dx, dr, dw = _lib.call(_bw_op, bw_norm, h, rstd, weight, dy, dh, seed_t, p, seed, x_dtype == th.float32, want_x and not one, want_r or (want_x and one), want_w)
-        return (dr if one else dx) if want_x else None, dw.to(weight.dtype) if want_w else None, dr if want_r else None, None, None, None, None, None
+        dx, dw, dr = (dr if one else dx) if want_x else None, dw.to(weight.dtype) if want_w else None, dr if want_r else None
+        if not th.compiler.is_compiling() and th.is_grad_enabled():
+            h = h if want_x or want_r else None  # (as an output it belongs to the graph for the weight's sake alone, too)
+            dx, dr = (g if g is None else NormGrad.apply(g, from_y, from_h, h, weight) for g in (dx, dr))
+            dw = dw if dw is None else NormGrad.apply(dw, from_y, h)
+        return dx, dw, dr, None, None, None, None, None
 
 
 class Dropout(th.autograd.Function):
@@ -191,8 +209,8 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-5, p=0.0, seed=None, out_d
 
     x [..., D] bf16 or fp32, D up to 16384; weight [D] bf16 or fp32, or None; residual [..., D] bf16 or fp32, whose type h has: the stream, rounded to it, is what is normed.
     y has x's type unless out_dtype says bf16, fp32 or int8; int8 gives Int8(q, scale) for linear_int8 (see quantize), without a backward.  p, seed: of dropout(),
-    elements counted in row-major order.  Backward for x, weight and residual.  Squares are summed in fp32: a row beyond 1e19 leaves its range and gives 0 (with eps = 0, one below 1e-19 infinities).
-    Rows may lie in a wider tensor; other layouts are copied."""
+    elements counted in row-major order.  Backward for x, weight and residual; a second derivative is refused.  Squares are summed in fp32: a row
+    beyond 1e19 leaves its range and gives 0 (with eps = 0, one below 1e-19 infinities).  Rows may lie in a wider tensor; other layouts are copied."""
     if not th.compiler.is_compiling():
         number, seed_t = (-1, None) if seed is None else _seed_of(seed)
         out = _lib.ext().rms_norm(x, weight, residual, eps, p, number, seed_t, OUTS.get(out_dtype, -2))
