@@ -323,7 +323,7 @@ int wkv7_linear_bwd(const void* x, const void* w, const void* saved, const void*
  *   y = act((sum_k x[m][k] w[n][k]) xs[m] ws[n] + bias[n]) + residual
  * x [M,K], w [N,K] signed 8-bit integers, rows ldx, ldw elements apart (multiples of 16, both 16-byte aligned: bulk tensor copies); xs fp32 [M], ws fp32 [N] (a scale
  * a row and a channel); 0 < K < 2^17, whose sums fit 32 bits whatever the operands hold.  The sum is exact; then come one rounding to fp32, one for each scale
- * and the epilogue's, as wkv7_linear_fwd's.  y, bias, residual, act, flags (WKV7_LINEAR_F32_OUT, _F32_BIAS) and workspace as there; workspace:
+ * (ws first, whatever M, N and K) and the epilogue's, as wkv7_linear_fwd's.  y, bias, residual, act, flags (WKV7_LINEAR_F32_OUT, _F32_BIAS) and workspace as there; workspace:
  * wkv7_linear_int8_workspace_bytes(M, N, K) bytes.
  */
 int64_t wkv7_linear_int8_workspace_bytes(int64_t M, int64_t N, int64_t K);

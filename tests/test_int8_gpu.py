@@ -333,3 +333,33 @@ def test_a_block_in_8_bits():
             H = H + th.relu(Y @ W[0].T).square() @ W[1].T
         # 8 bits of y and of relu2's values: a rounding of scale / 2 in each of D and F terms; the bf16 stream's two roundings a step
         assert float((h.double() - H).norm() / H.norm()) < 2e-2
+
+
+BATCHES = (1, 2, 5, 24, 64, 70, 130, 300, 700, 1283, 4096, 8192)  # the rows' kernel, tiles along the columns and the rows, cut or whole, pairs both ways
+
+
+@pytest.mark.parametrize('N,K', [(4096, 1024), (4001, 1024), (1000, 8192)])
+def test_a_row_has_the_same_bits_in_every_batch(N, K):
+    from wind_rwkv.rwkv7 import linear_int8
+    x, w, xs, ws, b = ints(8192, K, seed=1), ints(N, K, seed=2), rn(8192, seed=3), rn(N, seed=4), rn(N, seed=5)
+    for bias in (None, b):
+        want = linear_int8((x, xs), (w, ws), bias, out_dtype=F32)
+        for M in BATCHES[:-1]:
+            assert th.equal(linear_int8((x[:M], xs[:M]), (w, ws), bias, out_dtype=F32), want[:M]), M
+
+
+@pytest.mark.parametrize('N,K', [(4096, 1024), (4001, 1024), (1000, 8192)])
+def test_rows_near_the_end_of_fp32(N, K):
+    """Scales of 1e36: sum xs is beyond fp32, the result with the weight's scales is not."""
+    from wind_rwkv.rwkv7 import linear_int8, quantize
+    w8 = quantize(rn(N, K, seed=2, std=1e-4))
+    x = rn(8192, K, seed=1)
+    x[0] *= 2e37
+    x[1] = 3e38
+    x8 = quantize(x)
+    assert float(x8.scale[1]) > 2e36
+    for M in BATCHES:
+        rows = slice(0, min(M, 3))
+        Y = (x8.q[rows].double() @ w8.q.double().T) * w8.scale.double() * x8.scale[rows].double()[:, None]  # (the sums of integers are exact)
+        assert float(Y[:1].abs().max()) > 1e33 and float(Y.abs().max()) < 2.0 ** 127
+        check('y', linear_int8((x8.q[:M], x8.scale[:M]), w8, out_dtype=F32)[rows], Y, 3.01 * E * Y.abs())

@@ -102,7 +102,8 @@ __device__ __forceinline__ void bias8(const Epi& e, long long col, float (&f)[8]
     }
 }
 // Sums of products in 8 bits are 32-bit integers, exact, and go through registers and memory as floats of the same bits.  They become numbers, times their row's
-// and their column's scale, where an epilogue takes them: one rounding in the conversion (from 2^24 on) and one for each scale.
+// and their column's scale, where an epilogue takes them: one rounding in the conversion (from 2^24 on) and one for each scale.  The column's comes first in every kernel, so
+// that a row has the same bits in every batch; rows of activations near fp32's end leave its range last so, as a weight's scale is far from 1e30.
 template <bool I8> __device__ __forceinline__ float add_sums(float a, float b) { return I8 ? __int_as_float(__float_as_int(a) + __float_as_int(b)) : a + b; }
 template <bool I8> __device__ __forceinline__ void add_sums(float4& a, const float4& b) {
     a.x = add_sums<I8>(a.x, b.x); a.y = add_sums<I8>(a.y, b.y); a.z = add_sums<I8>(a.z, b.z); a.w = add_sums<I8>(a.w, b.w);
@@ -111,24 +112,26 @@ template <bool I8> __device__ __forceinline__ void add_sums8(float (&f)[8], cons
     f[0] = add_sums<I8>(f[0], a.x); f[1] = add_sums<I8>(f[1], a.y); f[2] = add_sums<I8>(f[2], a.z); f[3] = add_sums<I8>(f[3], a.w);
     f[4] = add_sums<I8>(f[4], b.x); f[5] = add_sums<I8>(f[5], b.y); f[6] = add_sums<I8>(f[6], b.z); f[7] = add_sums<I8>(f[7], b.w);
 }
-__device__ __forceinline__ float scaled(float sum, float ps, float qs) { return __fmul_rn(__fmul_rn((float)__float_as_int(sum), ps), qs); }
+__device__ __forceinline__ float scaled(float sum, float ws, float xs) { return __fmul_rn(__fmul_rn((float)__float_as_int(sum), ws), xs); }
 // A block of 32 sums a lane: a lane's own scale, along P, and the block's 32 along Q, in shared memory, where all lanes read the same.  (Read from global memory
 // where they are used they were waited for: 8192 x 2048 -> 8192 105 us, without any scales 87.)
-template <bool I8> __device__ __forceinline__ void scale_block(float ps, const float* qs, float (&v)[32]) {
+// SWAP: P runs over the columns.
+template <bool I8, bool SWAP> __device__ __forceinline__ void scale_block(float ps, const float* qs, float (&v)[32]) {
+    const auto times = [ps](float sum, float q) { return SWAP ? scaled(sum, ps, q) : scaled(sum, q, ps); };
     if constexpr (I8)
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
             const float4 q = *reinterpret_cast<const float4*>(qs + c);
-            v[c] = scaled(v[c], ps, q.x); v[c + 1] = scaled(v[c + 1], ps, q.y); v[c + 2] = scaled(v[c + 2], ps, q.z); v[c + 3] = scaled(v[c + 3], ps, q.w);
+            v[c] = times(v[c], q.x); v[c + 1] = times(v[c + 1], q.y); v[c + 2] = times(v[c + 2], q.z); v[c + 3] = times(v[c + 3], q.w);
         }
 }
 // the same, qs: one each of the lanes', which go through the warp's room of 128 bytes
-template <bool I8> __device__ __forceinline__ void scale_block(float ps, float qs, float* room, int lane, float (&v)[32]) {
+template <bool I8, bool SWAP> __device__ __forceinline__ void scale_block(float ps, float qs, float* room, int lane, float (&v)[32]) {
     if constexpr (I8) {
         __syncwarp();
         room[lane] = qs;
         __syncwarp();
-        scale_block<I8>(ps, room, v);
+        scale_block<I8, SWAP>(ps, room, v);
     }
 }
 __device__ __forceinline__ float scale_at(const float* s, long long i, long long n) { return i < n ? s[i] : 0.f; }
@@ -571,7 +574,7 @@ template <int ACT, bool I8> __global__ void __launch_bounds__(TILE_THREADS, 3) l
                 };
                 auto take = [&](float (&v)[32]) {
                     sums(v);
-                    scale_block<I8>(ps, ctrl->qs + c, v);
+                    scale_block<I8, false>(ps, ctrl->qs + c, v);
                 };
                 // (blocks two by two, as the pairs have them, would take 190 registers and more: one CTA an SM)
                 const int row0 = p0 + 32 * warp, col0 = q0 + c;
@@ -627,7 +630,7 @@ template <int ACT, bool I8> __global__ void __launch_bounds__(TILE_THREADS, 3) l
             if (I8) {  // (a thread's units are in one column, unless there are all 128)
                 const float4 q = ld4(ctrl->qs + j);
                 const float ws = rows == BM ? e.ws[col] : ps;
-                x.x = scaled(x.x, q.x, ws); x.y = scaled(x.y, q.y, ws); x.z = scaled(x.z, q.z, ws); x.w = scaled(x.w, q.w, ws);
+                x.x = scaled(x.x, ws, q.x); x.y = scaled(x.y, ws, q.y); x.z = scaled(x.z, ws, q.z); x.w = scaled(x.w, ws, q.w);
             }
             const float bias = e.bias ? load1g(e.bias, e.bias_f32, col) : 0.f;
             const float f[4] = {x.x + bias, x.y + bias, x.z + bias, x.w + bias};
@@ -695,7 +698,7 @@ template <int ACT, bool I8> __global__ void __launch_bounds__(TILE_THREADS, 3) l
             if (I8) {
                 const float xs = e.xs[row];
 #pragma unroll
-                for (int q = 0; q < 8; ++q) f[q] = scaled(f[q], xs, ctrl->qs[j + q]);
+                for (int q = 0; q < 8; ++q) f[q] = scaled(f[q], ctrl->qs[j + q], xs);
             }
             if (e.bias) {
                 float bias[8];
@@ -941,8 +944,8 @@ template <int ACT, bool I8> __global__ void __cluster_dims__(2, 1, 1) __launch_b
                         tmem_ld32(acc + 32 * b, reinterpret_cast<uint32_t(&)[32]>(v[0]));
                         tmem_ld32(acc + 32 * b + 32, reinterpret_cast<uint32_t(&)[32]>(v[1]));
                         if (b + 1 == b1 - 1) emptied();
-                        scale_block<I8>(ps, along_q(b), room, lane, v[0]);
-                        scale_block<I8>(ps, along_q(b + 1), room, lane, v[1]);
+                        scale_block<I8, false>(ps, along_q(b), room, lane, v[0]);
+                        scale_block<I8, false>(ps, along_q(b + 1), room, lane, v[1]);
                     });
                     ++b;
                     continue;
@@ -972,8 +975,8 @@ template <int ACT, bool I8> __global__ void __cluster_dims__(2, 1, 1) __launch_b
                     if (b == b1 - 1 && !parts) emptied();
                     continue;
                 }
-                const auto take = [&](float (&v)[32]) { sums(v); scale_block<I8>(ps, along_q(b), room, lane, v); };
-                if (p.swap) finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, take);
+                const auto take = [&](float (&v)[32]) { sums(v); scale_block<I8, false>(ps, along_q(b), room, lane, v); };
+                if (p.swap) finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { sums(v); scale_block<I8, true>(ps, along_q(b), room, lane, v); });
                 else if (e.vec) finish_rows<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, take);
                 else finish_cols<ACT>(e, &p.Y, &p.Z, mine, mixed, lane, turn, row0, col0, [&](float (&v)[32]) { take(v); turn_block(mine, lane, v); });
             }

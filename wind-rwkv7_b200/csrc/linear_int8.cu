@@ -106,7 +106,7 @@ template <int MT, int STEP> __global__ void __launch_bounds__(32 * ROWS_WARPS) i
     if (m >= e.rows || m >= MT || col >= e.cols) return;
     int s = 0;
     for (int r = 0; r < warps; ++r) s += sums[r][m][i];
-    float v = __fmul_rn(__fmul_rn((float)s, e.xs[m]), e.ws[col]);
+    float v = __fmul_rn(__fmul_rn((float)s, e.ws[col]), e.xs[m]);  // (in this order in the other kernels, too)
     if (e.bias) v += e.bias_f32 ? ((const float*)e.bias)[col] : __bfloat162float(((const bf16*)e.bias)[col]);
     v = act_of(e.act, v);
     const long long at = m * e.ldy + col;

@@ -130,7 +130,7 @@ def linear_int8(x, w, bias=None, *, act=None, residual=None, out_dtype=None):
     """y = act((xq @ wq^T) xs ws + bias) + residual: x = (xq [..., K] int8, xs [...] fp32), w = (wq [N, K] int8, ws [N] fp32), as quantize and rms_norm give them.
 
     bias [N] bf16 or fp32, act and residual as linear's; y bf16, or fp32 with out_dtype=torch.float32.  K from 1 to 131071, any N.  The sum is exact (32-bit integers); behind it
-    each scale, the bias, the activation and the residual are applied in fp32 and the result is rounded once.  Rows may lie in a wider tensor, on 16-byte boundaries; other
+    ws, xs, the bias, the activation and the residual are applied in fp32, in this order, and the result is rounded once.  What must stay within fp32's range is sum ws, not sum xs.  Rows may lie in a wider tensor, on 16-byte boundaries; other
     layouts are copied.  No backward."""
     if not th.compiler.is_compiling():
         if act in ACTS and out_dtype in (None, th.bfloat16, th.float32) and isinstance(x, tuple) and isinstance(w, tuple) and len(x) == len(w) == 2:
