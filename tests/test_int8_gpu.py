@@ -363,3 +363,20 @@ def test_rows_near_the_end_of_fp32(N, K):
         Y = (x8.q[rows].double() @ w8.q.double().T) * w8.scale.double() * x8.scale[rows].double()[:, None]  # (the sums of integers are exact)
         assert float(Y[:1].abs().max()) > 1e33 and float(Y.abs().max()) < 2.0 ** 127
         check('y', linear_int8((x8.q[:M], x8.scale[:M]), w8, out_dtype=F32)[rows], Y, 3.01 * E * Y.abs())
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+    from wind_rwkv.rwkv7 import linear_int8, quantize, rms_norm
+    x8, w8, x, r = (ints(4, 64, seed=1), rn(4, seed=2)), (ints(16, 64, seed=3), rn(16, seed=4)), rn(4, 64, seed=5), rn(4, 16, seed=6, dtype=BF)
+    want = linear_int8(x8, w8, residual=r), *quantize(x), *rms_norm(x, out_dtype=th.int8)
+    with fw.dual_level(), th.no_grad():
+        def dual(t):
+            return fw.make_dual(t, th.ones_like(t))
+        for call in (lambda: linear_int8(x8, w8, residual=dual(r)), lambda: linear_int8((x8[0], dual(x8[1])), w8), lambda: linear_int8(x8, (w8[0], dual(w8[1]))),
+                     lambda: linear_int8(x8, w8, dual(rn(16, seed=7))), lambda: quantize(dual(x)), lambda: rms_norm(dual(x), out_dtype=th.int8),
+                     lambda: rms_norm(x, residual=dual(x), out_dtype=th.int8), lambda: rms_norm(x, dual(rn(64, seed=8)), out_dtype=th.int8)):
+            with pytest.raises(RuntimeError, match='tangent'):
+                call()
+        got = linear_int8(x8, w8, residual=r), *quantize(x), *rms_norm(x, out_dtype=th.int8)
+    assert all(th.equal(a, b) for a, b in zip(got, want))

@@ -96,3 +96,19 @@ def test_operands_on_16_byte_boundaries():
     for view in (t, wide[:, 1:30], t.t()):
         r, ld = operand8(view)
         assert th.equal(r, view) and ld % 16 == 0 and r.data_ptr() % 16 == 0 and r.stride(0) == ld
+
+
+def test_forward_mode_tangents_are_refused(lib):
+    import torch.autograd.forward_ad as fw
+    from wind_rwkv.rwkv7 import linear_int8, quantize, rms_norm
+    x, w = (th.zeros(4, 64, dtype=I8), th.zeros(4)), (th.zeros(16, 64, dtype=I8), th.zeros(16))
+    with fw.dual_level(), th.no_grad():
+        def dual(t):
+            return fw.make_dual(t, th.ones_like(t))
+        for call in (lambda: linear_int8(x, w, residual=dual(th.zeros(4, 16, dtype=BF))), lambda: linear_int8(x, w, dual(th.zeros(16))), lambda: linear_int8((x[0], dual(x[1])), w),
+                     lambda: linear_int8(x, (w[0], dual(w[1]))), lambda: quantize(dual(th.zeros(4, 64))), lambda: rms_norm(dual(th.zeros(4, 64)), out_dtype=I8),
+                     lambda: rms_norm(th.zeros(4, 64), dual(th.zeros(64)), out_dtype=I8), lambda: rms_norm(th.zeros(4, 64), residual=dual(th.zeros(4, 64)), out_dtype=I8)):
+            with pytest.raises(RuntimeError, match='tangent'):
+                call()
+        with pytest.raises(RuntimeError, match='CUDA'):  # (a level alone refuses nothing)
+            linear_int8(x, w)

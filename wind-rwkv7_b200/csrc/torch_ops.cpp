@@ -76,7 +76,7 @@ struct Eager {
         return !o || (THPVariable_CheckExact(o) && !(duals && t._fw_grad(0).defined()));
     }
 };
-bool eager(std::initializer_list<const Tensor*> ts, bool autograd = true) {  // autograd: the Python form has an autograd function
+bool eager(std::initializer_list<const Tensor*> ts, bool autograd = true) {  // autograd: the Python form has an autograd function, or refuses duals
     const Eager ok(autograd);
     for (const Tensor* t : ts)
         if (!ok(*t)) return false;
@@ -784,7 +784,7 @@ py::object dropout(const Tensor& x, double p, int64_t seed, const OptTensor& see
 
 py::object quantize(const Tensor& x) {
     int64_t ld;
-    if (!eager({&x}, false) || x.dim() < 1 || x.numel() == 0 || x.size(-1) > 1 << 30 || !float_type(x) || !pitched_rows(x, &ld)) return py::none();
+    if (!eager({&x}) || x.dim() < 1 || x.numel() == 0 || x.size(-1) > 1 << 30 || !float_type(x) || !pitched_rows(x, &ld)) return py::none();
     Tensor q, scale;
     {
         py::gil_scoped_release nogil;
@@ -805,7 +805,7 @@ bool operand8(const Tensor& t, int64_t* ld) {
 py::object linear_int8(const Tensor& xq, const Tensor& xs, const Tensor& wq, const Tensor& ws, const OptTensor& bias_, const OptTensor& residual_, int64_t act, bool out_f32) {
     const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
     int64_t ldx, ldw, ldr = 0;
-    if (!eager({&xq, &xs, &wq, &ws, &bias, &residual}, false) || xq.dim() < 1 || wq.dim() != 2 || !operand8(xq, &ldx) || !operand8(wq, &ldw)) return py::none();
+    if (!eager({&xq, &xs, &wq, &ws, &bias, &residual}) || xq.dim() < 1 || wq.dim() != 2 || !operand8(xq, &ldx) || !operand8(wq, &ldw)) return py::none();
     const int64_t K = xq.size(-1), N = wq.size(0), M = xq.numel() / K;
     const auto scales = [&](const Tensor& s, const Tensor& q) {
         return plain(s) && s.scalar_type() == at::kFloat && s.sizes() == q.sizes().slice(0, q.dim() - 1) && s.is_contiguous() && s.device() == xq.device();

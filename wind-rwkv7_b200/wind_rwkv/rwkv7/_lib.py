@@ -8,6 +8,7 @@ import importlib.util
 import os
 
 import torch as th
+from torch.autograd import forward_ad
 
 _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 EXT_PATH = os.path.join(_PKG_ROOT, 'lib', '_wkv7_torch.so')
@@ -195,6 +196,12 @@ def require_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise RuntimeError('wkv7 ops run on CUDA tensors only (sm_100a); there is no CPU path')
+
+
+def refuse_tangents(what, *ts):
+    """For what has no derivative: a forward-mode tangent would be left out of the result without a word."""
+    if not th.compiler.is_compiling() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f'{what} has no derivative, and an argument has a forward-mode tangent: take it off (torch.autograd.forward_ad.unpack_dual)')
 
 
 def strides4(x):

@@ -84,7 +84,8 @@ def quantize(x):
     """Rows of x [..., K] in 8 bits: Int8(q, scale) with scale = max |row| / 127 and q = row / scale, rounded to the nearest, ties to even.
 
     x bf16 or fp32, K up to 2^30.  A row without a magnitude above 2^-100 becomes zeros with scale 0; one that holds a NaN or an infinity becomes zeros with a NaN for
-    its scale, so that its products are NaN.  q's rows lie on 16-byte boundaries (K rounded up to 16 apart).  No autograd: the results are constants."""
+    its scale, so that its products are NaN.  q's rows lie on 16-byte boundaries (K rounded up to 16 apart).  No autograd: the results are constants for a
+    backward; a forward-mode tangent is refused."""
     if not th.compiler.is_compiling():
         out = _lib.ext().quantize(x)
         if out is not None:
@@ -93,6 +94,7 @@ def quantize(x):
         raise TypeError(f'quantize takes bfloat16 or float32, not {x.dtype}')
     if x.dim() < 1 or not 0 < x.shape[-1] <= 1 << 30:
         raise ValueError(f'quantize takes x [..., K] with K from 1 to 2^30, got {list(x.shape)}')
+    _lib.refuse_tangents('quantize', x)
     _lib.require_cuda(x)
     q, scale = _lib.call(_rows_op, rows8, x.detach())
     return Int8(q[..., :x.shape[-1]], scale)
@@ -124,6 +126,7 @@ def _check(x, w, bias, residual, act, out_dtype):
         raise ValueError(f'linear_int8: residual {[*xq.shape[:-1], N]} of the output\'s type {out}, got {list(residual.shape)} {residual.dtype}')
     if th.is_grad_enabled() and any(t is not None and t.requires_grad for t in (xs, ws, bias, residual)):
         raise RuntimeError('linear_int8 has no backward: call it under torch.no_grad()')
+    _lib.refuse_tangents('linear_int8', xs, ws, bias, residual)
 
 
 def linear_int8(x, w, bias=None, *, act=None, residual=None, out_dtype=None):

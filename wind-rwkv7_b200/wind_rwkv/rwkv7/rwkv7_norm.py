@@ -201,6 +201,8 @@ def _check_norm(x, weight, residual, eps, p, seed, out_dtype):
         raise ValueError('rms_norm: dropout is of what joins the residual stream; without one use dropout()')
     if out_dtype == th.int8 and th.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
         raise RuntimeError('rms_norm in 8 bits has no backward: call it under torch.no_grad()')
+    if out_dtype == th.int8:
+        _lib.refuse_tangents('rms_norm in 8 bits', x, weight, residual)
     return how
 
 
