@@ -597,3 +597,19 @@ def test_second_derivatives_of_the_norm_are_refused(D, form):
         t = [a.detach().requires_grad_() for a in leaves]
         sum(o.float().sum() for o in call(t[0], t[1], t[2] if len(t) > 2 else None)).backward(create_graph=True)
         assert all(a.grad is not None for a in t)
+
+
+def test_seeds_are_integers_whether_or_not_they_are_used():
+    import numpy as np
+    from wind_rwkv.rwkv7 import dropout, rms_norm
+    x = rn(4, 64, seed=1, dtype=BF)
+    for seed in (-1, -2, 1 << 63, 1.5, th.zeros(2, dtype=th.int64, device='cuda'), th.zeros(1, device='cuda')):
+        for p in (0., 0.5):
+            with pytest.raises(ValueError, match='rms_norm: a seed'):
+                rms_norm(x, residual=x, p=p, seed=seed)
+            with pytest.raises(ValueError, match='dropout: a seed'):
+                dropout(x, p, seed)
+    want = rms_norm(x, residual=x)
+    for seed in (0, 7, (1 << 63) - 1, np.int64(7), th.tensor([7], device='cuda')):
+        assert all(th.equal(a, b) for a, b in zip(rms_norm(x, residual=x, seed=seed), want))
+        rms_norm(x, residual=x, p=0.5, seed=seed)

@@ -109,3 +109,17 @@ def test_the_generators_words():
     assert [int(w) for w in words(0, 4, 0, counter=(0xffffffff,) * 4, key=(0xffffffff,) * 2)] == [0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd]
     assert [int(w) for w in words(0, 4, 0, counter=(0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344), key=(0xa4093822, 0x299f31d0))] == [0xd16cfe09, 0x94fdcceb, 0x5001e420, 0x24126ea1]
     assert (words(6, 3, 5) == words(0, 12, 5)[6:9]).all()
+
+
+def test_seeds_are_integers_whether_or_not_they_are_used(lib):
+    from wind_rwkv.rwkv7 import dropout, rms_norm
+    x = th.zeros(4, 64, dtype=BF)
+    for seed in (-1, -2, 1 << 63, 1.5, th.zeros(2, dtype=th.int64), th.zeros(1)):
+        for p in (0., 0.5):
+            with pytest.raises(ValueError, match='rms_norm: a seed'):
+                rms_norm(x, residual=x, p=p, seed=seed)
+            with pytest.raises(ValueError, match='dropout: a seed'):
+                dropout(x, p, seed)
+    for seed in (0, 7, (1 << 63) - 1):
+        with pytest.raises(RuntimeError, match='CUDA'):
+            rms_norm(x, residual=x, seed=seed)

@@ -692,7 +692,8 @@ struct RmsNormFn : public Function<RmsNormFn> {
         return g;
     }
 };
-// p and where the seed is; seed < 0: no number
+// p and where the seed is; seed: a number, NO_SEED where none is given, or below, what is not a seed
+constexpr int64_t NO_SEED = -1;
 bool dropout_ok(double p, int64_t seed, const Tensor& seed_t, const Tensor& x) {
     if (!(p >= 0. && p <= 1.)) return false;
     if (seed_t.defined()) return plain(seed_t) && seed_t.scalar_type() == at::kLong && seed_t.numel() == 1 && seed_t.device() == x.device();
@@ -705,7 +706,7 @@ py::object rms_norm(const Tensor& x, const OptTensor& w_, const OptTensor& r_, d
     if (w.defined() && (!plain(w) || !float_type(w) || w.dim() != 1 || w.size(0) != x.size(-1) || !w.is_contiguous() || w.device() != x.device())) return py::none();
     if (r.defined() && (!plain(r) || !float_type(r) || r.sizes() != x.sizes() || r.device() != x.device() || !pitched_rows(r, &ld))) return py::none();
     if (p != 0. && !r.defined()) return py::none();
-    if (p == 0. ? s.defined() && !dropout_ok(p, seed, s, x) : !dropout_ok(p, seed, s, x)) return py::none();
+    if (!(p == 0. && seed == NO_SEED && !s.defined()) && !dropout_ok(p, seed, s, x)) return py::none();  // (where nothing is dropped a seed may be left out)
     if (out < 0) out = is_f32(x);
     const bool grad = grad_wanted({&x, &w, &r});
     if (grad && out == 2) return py::none();

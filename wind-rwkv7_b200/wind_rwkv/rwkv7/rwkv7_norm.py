@@ -179,7 +179,7 @@ def _check_dropout(name, p, seed):
         return float(p), 0, seed.detach()
     if seed is None and p > 0:
         raise ValueError(f'{name} needs a seed where p > 0')
-    if seed is not None and not 0 <= seed < 1 << 63:
+    if seed is not None and not (0 <= seed < 1 << 63 and int(seed) == seed):
         raise ValueError(f'{name}: a seed is an integer from 0 to 2^63 - 1, got {seed}')
     return float(p), 0 if seed is None else int(seed), None
 
@@ -214,7 +214,7 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-5, p=0.0, seed=None, out_d
     elements counted in row-major order.  Backward for x, weight and residual; a second derivative is refused.  Squares are summed in fp32: a row
     beyond 1e19 leaves its range and gives 0 (with eps = 0, one below 1e-19 infinities).  Rows may lie in a wider tensor; other layouts are copied."""
     if not th.compiler.is_compiling():
-        number, seed_t = (-1, None) if seed is None else _seed_of(seed)
+        number, seed_t = _seed_of(seed)
         out = _lib.ext().rms_norm(x, weight, residual, eps, p, number, seed_t, OUTS.get(out_dtype, -2))
         if out is not None:
             if out_dtype is not th.int8:
@@ -232,10 +232,10 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-5, p=0.0, seed=None, out_d
 
 
 def _seed_of(seed):
-    """(number or -1, tensor or None) for the eager path, which leaves what it does not know to the checks."""
-    if isinstance(seed, th.Tensor):
+    """(number, tensor or None) for the eager path, which leaves what it does not know to the checks; -1: no number given, -2: not a seed."""
+    if seed is None or isinstance(seed, th.Tensor):
         return -1, seed
-    return (seed if isinstance(seed, int) and 0 <= seed < 1 << 63 else -1), None
+    return (seed if isinstance(seed, int) and 0 <= seed < 1 << 63 else -2), None
 
 
 def dropout(x, p, seed, *, residual=None):
