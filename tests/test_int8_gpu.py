@@ -380,3 +380,22 @@ def test_forward_mode_tangents_are_refused():
                 call()
         got = linear_int8(x8, w8, residual=r), *quantize(x), *rms_norm(x, out_dtype=th.int8)
     assert all(th.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('M,N,K', [(1, 77, 64), (2, 1000, 203), (24, 2048, 8192), (64, 257, 4111), (70, 1000, 8192), (130, 4096, 1024), (200, 40, 20000), (300, 4001, 8192), (700, 4096, 1024),
+                                   (700, 4001, 1024), (1283, 1000, 8192), (4096, 1000, 8192), (4096, 4001, 1024), (4096, 4096, 1024)])
+def test_y_may_be_its_own_residual(M, N, K):
+    from wind_rwkv.rwkv7 import _lib
+    L = _lib.lib()
+    x, w, xs, ws = ints(M, K, seed=1), ints(N, K, seed=2), rn(M, seed=3), rn(N, seed=4)
+    work = th.empty(max(16, L.wkv7_linear_int8_workspace_bytes(M, N, K)), dtype=th.uint8, device='cuda')
+    for f32 in (0, 1):
+        for ld in (N, N + 3, (N + 15) // 8 * 8):
+            r = rn(M, ld, seed=5, std=1e3, dtype=F32 if f32 else BF)
+            out = []
+            for y in (th.zeros_like(r), r.clone()):
+                residual = r if not out else y
+                assert L.wkv7_linear_int8(x.data_ptr(), xs.data_ptr(), w.data_ptr(), ws.data_ptr(), None, residual.data_ptr(), y.data_ptr(), M, N, K, x.stride(0), w.stride(0), ld, ld,
+                                          2, f32, work.data_ptr(), _lib.stream_of(x)) == 0
+                out.append(y)
+            assert th.equal(out[0][:, :N], out[1][:, :N]) and th.equal(out[1][:, N:], r[:, N:])

@@ -442,3 +442,23 @@ def test_compiles():
 def test_device_status_is_clean():
     from wind_rwkv.rwkv7 import _lib
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize('M,N,K', [(1, 77, 64), (24, 2048, 8192), (64, 257, 4112), (70, 1000, 8192), (130, 4096, 1024), (200, 40, 20000), (300, 4001, 8192), (700, 4096, 1024), (700, 4001, 1024),
+                                   (1283, 1000, 8192), (4096, 1000, 4096), (4096, 4001, 1024), (4096, 4096, 1024)])
+def test_y_may_be_its_own_residual(M, N, K):
+    from wind_rwkv.rwkv7 import _lib
+    L = _lib.lib()
+    gen = th.Generator(device='cuda').manual_seed(1)
+    x, w = (th.randn(n, K, generator=gen, device='cuda').bfloat16() for n in (M, N))
+    work = th.empty(max(16, L.wkv7_linear_fwd_workspace_bytes(M, N, K)), dtype=th.uint8, device='cuda')
+    for f32 in (0, 1):
+        for ld in (N, N + 3, (N + 15) // 8 * 8):
+            r = (th.randn(M, ld, generator=gen, device='cuda') * 100).to(th.float32 if f32 else th.bfloat16)
+            out = []
+            for y in (th.zeros_like(r), r.clone()):
+                residual = r if not out else y
+                assert L.wkv7_linear_fwd(x.data_ptr(), w.data_ptr(), None, residual.data_ptr(), y.data_ptr(), None, M, N, K, K, K, ld, ld, 0, 2, f32, work.data_ptr(),
+                                         _lib.stream_of(x)) == 0
+                out.append(y)
+            assert th.equal(out[0][:, :N], out[1][:, :N]) and th.equal(out[1][:, N:], r[:, N:])
