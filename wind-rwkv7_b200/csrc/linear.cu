@@ -10,8 +10,8 @@
 // linear_tile_kernel, for the rest: one tile of 128 x NT a CTA, the sum over k split over a cluster of up to eight CTAs, which add their
 // parts through distributed shared memory in a fixed order (each part is sent: fetching it, 24 x 8192 x 2048 took 32 us instead of 12).  Few rows (decoding): the
 // weight is P and the rows of x are Q, so that a CTA streams 128 weight rows against all of x.  Bound by the weight's stream: 16 x 2048 x 50001 in 37 us, 5.7 TB/s.
-// 8 bits (I8): the same kernels with tcgen05.mma.kind::i8, k blocks of 128 bytes as before, sums in 32-bit integers and the scales behind them.  8192 x 2048 -> 8192 96 us alone (2.9 POP/s; bf16
-// 179), 8192^3 333 (3.3 POP/s), 1283 x 2560 -> 10240 29.4, 16 x 2048 -> 50001 22 (4.8 TB/s), 24 x 8192 -> 2048 9.
+// 8 bits (I8): the same kernels with tcgen05.mma.kind::i8, k blocks of 128 bytes as before, sums in 32-bit integers and the scales behind them.  8192 x 2048 -> 8192 92 to 96 us alone (2.9 POP/s;
+// bf16 182), 8192^3 335 (3.3 POP/s), 1283 x 2560 -> 10240 29, 16 x 2048 -> 50001 22 (4.8 TB/s), 24 x 8192 -> 2048 8.7.  With the scales the pairs' epilogue spills 64 to 116 bytes a thread.
 #include <cuda.h>
 #include <cstring>
 

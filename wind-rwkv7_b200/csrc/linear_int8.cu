@@ -1,5 +1,5 @@
 // Products in 8 bits of a few rows (generation):  y = act((x w^T) xs ws + bias) + residual,  x [M, K], w [N, K] signed 8-bit.
-// Bound by the weight's stream.  A CTA has 16 rows of the weight and all of k, shared out over its eight warps: within 64 k a lane has 16 adjacent bytes of two weight
+// Bound by the weight's stream.  A CTA has 16 rows of the weight and all of k, shared out over its warps, one to sixteen: within 64 k a lane has 16 adjacent bytes of two weight
 // rows and of each x row, and sums their products, four an instruction.  All requests of a step are under way together.  The sums, 32-bit integers, are joined over the
 // lanes that share a weight row and through shared memory over the warps.  Figures, against the tensor-memory form of linear.cu, at int8_rows_fit().
 // (With mma.sync m16n8k32 for the products 16 x 2048 -> 50001 took 81 us instead of 22: some 200 cycles an instruction.)
@@ -117,15 +117,16 @@ template <int MT, int STEP> __global__ void __launch_bounds__(32 * ROWS_WARPS) i
 
 }  // namespace lin
 
-// us, in a graph, against the tensor-memory form: 1 x 2048 -> 8192 5.4 / 7.4 (the weight's stream alone 2.6), 2 x 2048 -> 8192 5.8 / 7.6, 1 x 8192 -> 2048 7.0 / 7.3, 1 x 768 -> 768
-// 2.1 / 3.5; but 1 x 2048 -> 50001 21.8 / 21.1, and with more rows the products of four take longer than the stream: 4 x 4096 -> 4096 8.9 / 7.8
+// us, in a graph, against the tensor-memory form: 1 x 2048 -> 8192 5.2 / 7.4 (the weight's stream alone 2.6), 1 x 8192 -> 2048 6.6 / 6.9, 1 x 768 -> 768 2.0 / 3.5.  About the cut, one row and two:
+// 4096 -> 8192 8.9 / 10.0 and 10.2 / 10.1, 8192 -> 4096 8.7 / 10.2 and 9.9 / 10.3; 8192 -> 8192 15.2 / 15.5 and 17.6 / 15.6, 4096 -> 14336 14.9 / 14.3 and 17.3 / 14.4, 2048 -> 50001 22.2 / 20.4 and
+// 25.3 / 20.5.  On the other side of it by themselves: 2560 -> 10240 10.3 / 8.9 (40 chunks for eight warps of four), 14336 -> 4096 12.6 / 14.7, 2 x 8192 -> 2048 8.0 / 7.1.  With more rows the products
+// of four take longer than the stream: 4 x 4096 -> 4096 8.9 / 7.8
 bool int8_rows_fit(long long rows, long long cols, long long k) { return rows <= lin::ROWS_MOST && cols * k <= 1LL << 25; }
 
 int launch_int8_rows(LinearOperand x, LinearOperand w, long long k, const LinearEpilogue& e, cudaStream_t stream) {
     using namespace lin;
     const RowsParams p{(const signed char*)x.p, (const signed char*)w.p, e, x.ld, w.ld, (int)k};
     const auto kern = e.rows == 1 ? int8_rows_kernel<1, 4> : int8_rows_kernel<2, 4>;
-    const unsigned ctas = (unsigned)((e.cols + ROWS_N - 1) / ROWS_N);
     // warps: a step each
     const long long chunks = (k + ROWS_CHUNK - 1) / ROWS_CHUNK;
     int warps = 1;

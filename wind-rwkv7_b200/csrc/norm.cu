@@ -1,4 +1,4 @@
-// Rows to 8 bits, and dropout by itself.  Both are bound by memory; dropout of bf16 elements as much by its generator's ten rounds.
+// Rows to 8 bits, and dropout by itself.  Both are bound by memory, dropout of bf16 elements with its generator's ten rounds only partly behind it.
 #include "norm.cuh"
 
 namespace wkv7 {
@@ -92,8 +92,8 @@ template <int NV, bool XF, bool EVEN> __global__ void __launch_bounds__(NV ? thr
 }
 
 // ---- dropout alone ---------------------------------------------------------------------------------------------------------
-// Two pieces a thread at a time; the last elements, less than a piece, go one to a thread.  us for 2^26 elements: bf16 63 (4.3 TB/s; the generator alone some 43), with a residual 69 (5.8),
-// all in fp32 126 (6.4, the copy rate).
+// Two pieces a thread at a time; the last elements, less than a piece, go one to a thread.  us for 2^26 elements: bf16 63 (4.3 TB/s; traffic alone would be 41, the
+// generator's products 32; no pipe is full, ALU 61 %, issue 55 %, heavy FMA 36 %), with a residual 69 (5.8), all in fp32 126 (6.4, the copy rate).
 constexpr int DROPOUT_CTAS = 8;  // of an SM, where registers leave room for as many
 template <bool XF, int RES, bool LOW> __global__ void __launch_bounds__(256) dropout_kernel(const __grid_constant__ DropoutParams p) {
     constexpr bool RF = RES == 2;

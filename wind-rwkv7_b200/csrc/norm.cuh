@@ -8,8 +8,8 @@ namespace wkv7 {
 namespace norm {
 
 // ---- Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3; 2011) -----------------------
-// Ten rounds of two 32 x 32 -> 64 products for four words.  No mask is stored: the backward forms the words again.  Its products bound dropout of bf16 elements: 36 of
-// them for a piece of eight, at four cycles each in a quarter of an SM, are 43 us for 2^26 elements, as much as their traffic.
+// Ten rounds of two 32 x 32 -> 64 products for four words.  No mask is stored: the backward forms the words again.  36 products
+// for a piece of eight, at four cycles each in a quarter of an SM, come to 63800 cycles for 2^26 elements: 32 us at 1965 MHz, computed, beside 41 of traffic in bf16.
 struct Dropper {
     uint32_t k0, k1, from;  // kept: word >= from
     bool none;              // all dropped, the threshold is 2^32

@@ -1,4 +1,4 @@
-// Interface between the C ABI (capi.cu) and the residual stream's kernels: norm, dropout, rows to 8 bits (norm.cu).
+// Interface between the C ABI (capi.cu) and the residual stream's kernels: norm, dropout, rows to 8 bits (norm_fwd.cu, norm_bwd.cu, norm.cu).
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>

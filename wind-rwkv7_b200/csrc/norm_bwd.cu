@@ -17,7 +17,7 @@ struct BwdKernelParams : NormBwdParams {
     bool low;     // dropout's counters are below 2^32
 };
 // HELD: the weight's gradient and the next row are in registers, the weight in shared memory (in registers, too, 100 to 400 bytes a thread would be spilled, among
-// them what has been requested, which is then waited for: 16384 x 4096 with an fp32 stream 198 -> 261 us).  Rows of four pieces a thread have the gradient in shared memory
+// them what has been requested, which is then waited for: 16384 x 4096 with an fp32 stream 185 -> 261 us).  Rows of four pieces a thread have the gradient in shared memory
 // and are read twice.
 template <int NV, bool YF, bool HF, bool DROP, bool EVEN>
 __global__ void __launch_bounds__(threads_most(NV), bwd_ctas(NV)) norm_bwd_kernel(const __grid_constant__ BwdKernelParams p) {
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(1024) norm_dw_kernel(const float* partial, flo
 }  // namespace norm
 
 namespace norm {
-// (where all is fp32 two pieces do not fit the registers)
+// (where all is fp32 two pieces do not fit the registers: such rows of more than 288 pieces spill 84 to 200 bytes a thread)
 static int bwd_vectors(long long M, long long pieces, bool wide) { return wide && pieces <= threads_most(1) ? 1 : vectors_of(M, pieces); }
 // One CTA an SM where there are rows for as many teams, so that there are few parts of dw; else smaller ones
 static Teams bwd_teams(long long M, long long pieces, int nv) {

@@ -13,7 +13,8 @@ namespace wkv7 {
 namespace norm {
 
 // Threads of an SM, for which there are registers and the grid is sized.  Two pieces of bf16 without parts fit 96 registers (8192 x 2048 25.1 -> 23.5 us, 65536 x 768 78 -> 72);
-// the other forms would spill what they have requested (60000 x 1001 with dropout 131 -> 175).
+// the other forms of two pieces would spill what they have requested (60000 x 1001 with dropout 131 -> 175).  Four pieces: 544 threads, which rows of 16378 to 16383 elements need, leave
+// 96 registers, and 39 of the 40 such forms spill, 4 to 836 bytes a thread.
 constexpr int fwd_threads(int nv, bool narrow) { return nv == 1 ? 576 : nv == 2 ? narrow ? 640 : 512 : 544; }
 struct FwdKernelParams : NormFwdParams {
     Teams t;

@@ -6,7 +6,8 @@ The reference leaves both to the model around the mixer.  A block of a model, in
     q8, h = rms_norm(mixed, weight, residual=h, out_dtype=torch.int8)     # h += mixed; q8 = Int8(q, scale)
 
 Dropout comes from a counter-based generator (Philox4x32-10): which elements are dropped is a function of the seed and of an element's place, no mask is
-stored and the backward forms it again.  Kernels: csrc/norm.cu.
+stored and the backward forms it again.  Kernels: csrc/norm_fwd.cu and norm_bwd.cu (rms_norm), norm.cu (dropout).  The norm is by the root mean square alone: no mean is taken off and no
+bias added, so that a model with LayerNorm cannot use it.
 """
 import torch as th
 
