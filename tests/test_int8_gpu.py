@@ -348,6 +348,19 @@ def test_a_row_has_the_same_bits_in_every_batch(N, K):
             assert th.equal(linear_int8((x[:M], xs[:M]), (w, ws), bias, out_dtype=F32), want[:M]), M
 
 
+@pytest.mark.parametrize('act', [a for a in F64 if a])
+@pytest.mark.parametrize('N', [4096, 4001])
+def test_a_row_has_the_same_bits_behind_the_epilogue(act, N):
+    from wind_rwkv.rwkv7 import linear_int8
+    K = 1024
+    x, w, xs, ws, b = ints(8192, K, seed=1), ints(N, K, seed=2), rn(8192, seed=3, std=1e-3), rn(N, seed=4, std=1e-2), rn(N, seed=5)
+    for out in (F32, BF):
+        r = rn(8192, N, seed=6, dtype=out)
+        want = linear_int8((x, xs), (w, ws), b, act=act, residual=r, out_dtype=out)
+        for M in BATCHES[:-1]:
+            assert th.equal(linear_int8((x[:M], xs[:M]), (w, ws), b, act=act, residual=r[:M], out_dtype=out), want[:M]), M
+
+
 @pytest.mark.parametrize('N,K', [(4096, 1024), (4001, 1024), (1000, 8192)])
 def test_rows_near_the_end_of_fp32(N, K):
     """Scales of 1e36: sum xs is beyond fp32, the result with the weight's scales is not."""

@@ -644,7 +644,7 @@ template <int ACT, bool I8> __global__ void __launch_bounds__(TILE_THREADS, 3) l
                 const long long row = q0 + j + q;
                 if (row >= e.rows) break;
                 if (e.z) store_z1(e, row, col, f[q]);
-                const float v = act<ACT>(f[q]) + res[q];
+                const float a = act<ACT>(f[q]), v = I8 ? __fadd_rn(a, res[q]) : a + res[q];  // (8 bits: not merged with the activation's last product, as nowhere else)
                 if (e.y_f32) ((float*)e.y)[row * e.ldy + col] = v;
                 else ((bf16*)e.y)[row * e.ldy + col] = __float2bfloat16_rn(v);
             }
