@@ -1,7 +1,7 @@
 """Products in 8 bits for serving: `quantize(x)` gives rows as integers with a scale each, `linear_int8(x, w, ...)` multiplies two such tensors.
 
 The weight's stream, which bounds the generation of a few sequences, is half of bf16's, and so is the tensor cores' time for a prompt.  The rows' own way to 8 bits comes on
-top.  With it large prompts and a head take 0.6 to 0.7 of `linear`'s time.  A few tokens' calls wait for the host; in a captured graph one token gains (1 x 2048 -> 8192 with its norm 7.1
+top.  With it large prompts through wide weights and a head take 0.6 to 0.7 of `linear`'s time.  A few tokens' calls wait for the host; in a captured graph one token gains (1 x 2048 -> 8192 with its norm 7.1
 us, in bf16 11.5), 24 x 8192 -> 2048 does not (12.5, 11.9).  Weights are quantized once, a scale a channel; activations row by row, by `rms_norm(..., out_dtype=torch.int8)` where a norm precedes the product and by `quantize` elsewhere:
 
     w8 = quantize(w)                                                     # once: w [N, K]
